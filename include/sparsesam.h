@@ -290,6 +290,74 @@ int ssam_layernorm_nchw(const float* x, int B, int HW, int C, const float* w, co
 int ssam_layernorm_gelu_half(const void* x, int64_t rows, int C, const void* w, const void* b, float eps, int gelu,
                              int dtype, void* out, void* stream);
 
+/* Gradients of ssam_layernorm_gelu_half for the output gradient dout [rows, C]: dx
+ * [rows, C] and the sums over the rows dw, db [C], all of x's dtype (the row's mean
+ * and variance are recomputed from x). Shapes, dtypes and alignment as there, rows >= 1;
+ * dx may be dout, and does not otherwise overlap an input. workspace:
+ * ssam_layernorm_gelu_half_bwd_workspace_size() bytes, 16-byte aligned. No
+ * counterpart in the reference, whose evaluation does not train. */
+size_t ssam_layernorm_gelu_half_bwd_workspace_size(int64_t rows, int C);
+int ssam_layernorm_gelu_half_bwd(const void* x, const void* dout, int64_t rows, int C, const void* w, const void* b,
+                                 float eps, int gelu, int dtype, void* dx, void* dw, void* db, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Group normalisation with an activation over channels-last maps x [N, HW, C]:
+ *   xh = (x - mean) * rstd,  out = act(xh * w + b)
+ * mean and rstd = 1 / sqrt(var + eps) (biased variance) are over the HW positions and
+ * the C / groups channels of each (sample, group). w, b [C].
+ *   act   : 0 none, 1 ReLU, 2 GELU (erf), 3 SiLU.
+ *   dtype : 0 fp16, 1 bf16, 2 fp32 (x, w, b, out and the gradients alike; the
+ *           arithmetic is fp32, rounded once).
+ *   mean, rstd : optional fp32 [N, groups], what the backward pass takes.
+ * ssam_groupnorm_act_bwd: dx [N, HW, C], dw and db [C] for the output gradient dout;
+ * dx may be dout. x, w, b, out, dout, dx and workspace are 16-byte aligned; C is a
+ * multiple of 8 (fp32: 4) and of groups, at most 2048 (fp32: 1024), N at most 65535
+ * (SSAM_ERR_UNSUPPORTED otherwise). workspace: ssam_groupnorm_act_workspace_size()
+ * bytes (backward 0 / 1). Sums are taken in a fixed order: equal calls give equal bits.
+ * No counterpart in the reference: the norm of the segmentation heads that follow
+ * the SAM3 encoder (convolution -> GroupNorm -> ReLU).
+ * ------------------------------------------------------------------------- */
+size_t ssam_groupnorm_act_workspace_size(int N, int64_t HW, int C, int groups, int backward);
+int ssam_groupnorm_act_fwd(const void* x, int N, int64_t HW, int C, int groups, const void* w, const void* b, float eps,
+                           int act, int dtype, void* out, float* mean, float* rstd, void* workspace,
+                           size_t workspace_bytes, void* stream);
+int ssam_groupnorm_act_bwd(const void* x, const void* dout, int N, int64_t HW, int C, int groups, const void* w,
+                           const void* b, const float* mean, const float* rstd, int act, int dtype, void* dx, void* dw,
+                           void* db, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Cross attention between token sets of different lengths (the mask decoder's
+ * token -> image and image -> token attention; SAM-HQ's decoder calls torch for it):
+ *   out[b, t, h] = softmax_j(scale <q[b, t, h], k[b, j, n]>) v[b, j, n],  n = h / (heads / kv_heads)
+ * over the keys j that are there: j < key_lens[b] (int32 [B], NULL: Tk; clamped to
+ * 0 .. Tk) and key_mask[b, j] != 0 (uint8 [B, Tk] contiguous, NULL: all). What the K and V
+ * rows of the other keys hold does not matter. A query without keys gives zeros.
+ *   q, out [B, Tq, heads, d];  k, v [B, Tk, kv_heads, d], kv_heads divides heads.
+ *   strides : HOST array of 12 element strides: (batch, token, head) of q, k, v and out
+ *             (backward: of dout in out's place); d is contiguous. A stride of 0
+ *             broadcasts an input. Strides are multiples of 8 elements (fp32: 4).
+ *   dtype   : 0 fp16, 1 bf16, 2 fp32; logits, statistics and sums are fp32.
+ *   scale   : positive and finite.
+ *   out_f32 : optional fp32 [B, Tq, heads, d] contiguous copy of the result before its
+ *             rounding, and lse, optional fp32 [B, heads, Tq] (base-2 log-sum-exp of the
+ *             logits): what the backward pass takes. For dtype 2 with a contiguous `out`
+ *             that pass takes `out` itself.
+ * ssam_cross_attn_bwd: contiguous gradients dq [B, Tq, heads, d], dk, dv [B, Tk, kv_heads, d]
+ * of x's dtype; dq, or dk and dv together, may be NULL (not computed). Keys that are not
+ * there get zero gradients. delta: fp32 [B, heads, Tq] scratch.
+ * d is a multiple of 8, at most 128; B and kv_heads at most 65535 (SSAM_ERR_UNSUPPORTED
+ * otherwise). Pointers are 16-byte aligned; outputs overlap no input. Sums are taken in a
+ * fixed order: equal calls give equal bits.
+ * ------------------------------------------------------------------------- */
+int ssam_cross_attn_fwd(const void* q, const void* k, const void* v, const int64_t* strides, int B, int Tq, int Tk,
+                        int heads, int kv_heads, int d, int dtype, float scale, const int32_t* key_lens,
+                        const uint8_t* key_mask, void* out, float* out_f32, float* lse, void* stream);
+int ssam_cross_attn_bwd(const void* q, const void* k, const void* v, const void* dout, const int64_t* strides, int B,
+                        int Tq, int Tk, int heads, int kv_heads, int d, int dtype, float scale, const int32_t* key_lens,
+                        const uint8_t* key_mask, const float* out_f32, const float* lse, float* delta, void* dq,
+                        void* dk, void* dv, void* stream);
+
 /* Row LayerNorm fp32 -> bf16 that also stores its input rows unchanged to
  * copy (fp32 [n_rows, C], 16-byte aligned). The encoder keeps its intermediate
  * embedding after a global-attention block (the token grid the SAM-HQ encoder

@@ -176,6 +176,50 @@ int ssam_layernorm_gelu_half(const void* x, int64_t rows, int C, const void* w, 
   return ssam::layernorm_half(x, rows, C, w, b, eps, gelu, dtype, out, static_cast<cudaStream_t>(stream));
 }
 
+size_t ssam_layernorm_gelu_half_bwd_workspace_size(int64_t rows, int C) {
+  return ssam::layernorm_half_bwd_workspace_size(rows, C);
+}
+
+int ssam_layernorm_gelu_half_bwd(const void* x, const void* dout, int64_t rows, int C, const void* w, const void* b,
+                                 float eps, int gelu, int dtype, void* dx, void* dw, void* db, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+  return ssam::layernorm_half_bwd(x, dout, rows, C, w, b, eps, gelu, dtype, dx, dw, db, workspace, workspace_bytes,
+                                  static_cast<cudaStream_t>(stream));
+}
+
+size_t ssam_groupnorm_act_workspace_size(int N, int64_t HW, int C, int groups, int backward) {
+  return ssam::groupnorm_workspace_size(N, HW, C, groups, backward);
+}
+
+int ssam_groupnorm_act_fwd(const void* x, int N, int64_t HW, int C, int groups, const void* w, const void* b, float eps,
+                           int act, int dtype, void* out, float* mean, float* rstd, void* workspace,
+                           size_t workspace_bytes, void* stream) {
+  return ssam::groupnorm_act_fwd(x, N, HW, C, groups, w, b, eps, act, dtype, out, mean, rstd, workspace,
+                                 workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int ssam_groupnorm_act_bwd(const void* x, const void* dout, int N, int64_t HW, int C, int groups, const void* w,
+                           const void* b, const float* mean, const float* rstd, int act, int dtype, void* dx, void* dw,
+                           void* db, void* workspace, size_t workspace_bytes, void* stream) {
+  return ssam::groupnorm_act_bwd(x, dout, N, HW, C, groups, w, b, mean, rstd, act, dtype, dx, dw, db, workspace,
+                                 workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int ssam_cross_attn_fwd(const void* q, const void* k, const void* v, const int64_t* strides, int B, int Tq, int Tk,
+                        int heads, int kv_heads, int d, int dtype, float scale, const int32_t* key_lens,
+                        const uint8_t* key_mask, void* out, float* out_f32, float* lse, void* stream) {
+  return ssam::cross_attn_fwd(q, k, v, strides, B, Tq, Tk, heads, kv_heads, d, dtype, scale, key_lens, key_mask, out,
+                              out_f32, lse, static_cast<cudaStream_t>(stream));
+}
+
+int ssam_cross_attn_bwd(const void* q, const void* k, const void* v, const void* dout, const int64_t* strides, int B,
+                        int Tq, int Tk, int heads, int kv_heads, int d, int dtype, float scale, const int32_t* key_lens,
+                        const uint8_t* key_mask, const float* out_f32, const float* lse, float* delta, void* dq,
+                        void* dk, void* dv, void* stream) {
+  return ssam::cross_attn_bwd(q, k, v, dout, strides, B, Tq, Tk, heads, kv_heads, d, dtype, scale, key_lens, key_mask,
+                              out_f32, lse, delta, dq, dk, dv, static_cast<cudaStream_t>(stream));
+}
+
 int ssam_layernorm_rows_copy(const float* x, int n_rows, int C, const float* w, const float* b, float eps,
                              void* out_bf16, float* copy, void* stream) {
   return ssam::layernorm_rows_copy(x, n_rows, C, w, b, eps, out_bf16, copy, static_cast<cudaStream_t>(stream));

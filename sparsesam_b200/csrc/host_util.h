@@ -102,6 +102,24 @@ int window_of_raster(int B, int H, int W, int ws, int32_t* win_rows, cudaStream_
 int fill_pad_rows(void* out, int64_t ld, const int32_t* rows, int n_rows, int C, const float* bias,
                   cudaStream_t stream);
 int patch_im2col_split3(const float* img, int B, int Cin, int H, int W, int p, void* out, cudaStream_t stream);
+int cross_attn_fwd(const void* q, const void* k, const void* v, const int64_t* strides, int B, int Tq, int Tk,
+                   int heads, int kv_heads, int d, int dtype, float scale, const int32_t* key_lens,
+                   const uint8_t* key_mask, void* out, float* out_f32, float* lse, cudaStream_t stream);
+int cross_attn_bwd(const void* q, const void* k, const void* v, const void* dout, const int64_t* strides, int B, int Tq,
+                   int Tk, int heads, int kv_heads, int d, int dtype, float scale, const int32_t* key_lens,
+                   const uint8_t* key_mask, const float* out_f32, const float* lse, float* delta, void* dq, void* dk,
+                   void* dv, cudaStream_t stream);
+size_t groupnorm_workspace_size(int N, int64_t HW, int C, int groups, int backward);
+int groupnorm_act_fwd(const void* x, int N, int64_t HW, int C, int groups, const void* w, const void* b, float eps,
+                      int act, int dtype, void* out, float* mean, float* rstd, void* workspace, size_t workspace_bytes,
+                      cudaStream_t stream);
+int groupnorm_act_bwd(const void* x, const void* dout, int N, int64_t HW, int C, int groups, const void* w,
+                      const void* b, const float* mean, const float* rstd, int act, int dtype, void* dx, void* dw,
+                      void* db, void* workspace, size_t workspace_bytes, cudaStream_t stream);
+size_t layernorm_half_bwd_workspace_size(int64_t rows, int C);
+int layernorm_half_bwd(const void* x, const void* dout, int64_t rows, int C, const void* w, const void* b, float eps,
+                       int gelu, int dtype, void* dx, void* dw, void* db, void* workspace, size_t workspace_bytes,
+                       cudaStream_t stream);
 size_t rc_mlp_workspace_size(int n_rows, int C, int hidden);
 int rc_mlp_fwd(float* x, int64_t ldx, const int32_t* rows, int n_rows, int C, int hidden, const float* ln_w,
                const float* ln_b, float eps, const void* w1, const float* b1, const void* w2, const float* b2,

@@ -5,5 +5,7 @@
 #include "perm.cu"
 #include "rows.cu"
 #include "attention.cu"
+#include "cross_attention.cu"
+#include "norms.cu"
 #include "capi.cu"
 #include "noalloc.cu"

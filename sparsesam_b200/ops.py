@@ -7,6 +7,10 @@ a CUDA device is rejected.
 """
 from __future__ import annotations
 
+import contextlib
+import ctypes
+import math
+
 import torch
 
 from . import _lib
@@ -45,6 +49,22 @@ def _check_cuda(*ts: torch.Tensor) -> None:
     for t in ts:
         if t is not None and not t.is_cuda:
             raise ValueError("sparsesam_b200 ops run on CUDA tensors only (no CPU fallback)")
+
+
+def _on(t: torch.Tensor):
+    """Context that makes t's device the current one (launches go to the current device's streams)."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _same_device(*ts: torch.Tensor) -> None:
+    if any(t is not None and t.device != ts[0].device for t in ts):
+        raise ValueError("all tensors of a call must be on one device")
+
+
+def _wants_grad(*ts: torch.Tensor) -> bool:
+    return torch.is_grad_enabled() and any(t.requires_grad for t in ts)
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
@@ -460,24 +480,249 @@ def layernorm_nchw(x: torch.Tensor, B: int, H: int, W: int, w: torch.Tensor, b: 
 
 
 LN_HALF_CHANNELS = (32, 64, 128, 256)
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+def _layernorm_gelu_half(x, w, b, eps, gelu):
+    out = torch.empty_like(x)
+    C = x.shape[-1]
+    if x.numel():
+        with _on(x):
+            _lib.call("ssam_layernorm_gelu_half", x.data_ptr(), x.numel() // C, C, w.data_ptr(), b.data_ptr(), eps, gelu,
+                      _DTYPES[x.dtype], out.data_ptr(), _stream(x))
+    return out
+
+
+class _LayerNormGeluHalf(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, b, eps, gelu):
+        ctx.save_for_backward(x, w, b)
+        ctx.eps, ctx.gelu = eps, gelu
+        return _layernorm_gelu_half(x, w, b, eps, gelu)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        x, w, b = ctx.saved_tensors
+        C = x.shape[-1]
+        rows = x.numel() // C
+        if rows == 0:
+            return torch.zeros_like(x), torch.zeros_like(w), torch.zeros_like(b), None, None
+        dout = _dense(dout)
+        dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty_like(b)
+        n = _lib.load().ssam_layernorm_gelu_half_bwd_workspace_size(rows, C)
+        ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+        with _on(x):
+            _lib.call("ssam_layernorm_gelu_half_bwd", x.data_ptr(), dout.data_ptr(), rows, C, w.data_ptr(), b.data_ptr(),
+                      ctx.eps, ctx.gelu, _DTYPES[x.dtype], dx.data_ptr(), dw.data_ptr(), db.data_ptr(), ws.data_ptr(), n,
+                      _stream(x))
+        return dx, dw, db, None, None
+
+
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    """t in row-major memory that vector loads can read (an incoming gradient may have any layout)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def layernorm_gelu_half(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor, eps: float,
                         gelu: bool) -> torch.Tensor:
     """Channel LayerNorm (+ exact GELU) of fp16 / bf16 channels-last rows (..., C),
-    C in LN_HALF_CHANNELS; w, b of x's dtype. Returns a new tensor of x's shape."""
+    C in LN_HALF_CHANNELS; w, b of x's dtype. Returns a new tensor of x's shape.
+    Differentiable in x, w and b (once)."""
     _check_cuda(x, w, b)
     if x.dtype not in (torch.float16, torch.bfloat16) or w.dtype != x.dtype or b.dtype != x.dtype:
         raise ValueError("x, w and b must share one half-precision dtype")
     if not x.is_contiguous() or not w.is_contiguous() or not b.is_contiguous():
         raise ValueError("x, w and b must be contiguous")
-    C = x.shape[-1]
+    if _wants_grad(x, w, b):
+        return _LayerNormGeluHalf.apply(x, w, b, float(eps), int(bool(gelu)))
+    return _layernorm_gelu_half(x, w, b, float(eps), int(bool(gelu)))
+
+
+# ---------------------------------------------------------------------------
+# GroupNorm + activation
+# ---------------------------------------------------------------------------
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+
+
+def _groupnorm_act(x, groups, w, b, eps, act, stats):
+    N, C = x.shape[0], x.shape[-1]
     out = torch.empty_like(x)
     if x.numel() == 0:
+        return out, None
+    HW = x.numel() // (N * C)
+    st = torch.empty(2, N, groups, dtype=torch.float32, device=x.device) if stats else None
+    n = _lib.load().ssam_groupnorm_act_workspace_size(N, HW, C, groups, 0)
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+    with _on(x):
+        _lib.call("ssam_groupnorm_act_fwd", x.data_ptr(), N, HW, C, groups, w.data_ptr(), b.data_ptr(), eps, act,
+                  _DTYPES[x.dtype], out.data_ptr(), st[0].data_ptr() if stats else None,
+                  st[1].data_ptr() if stats else None, ws.data_ptr(), n, _stream(x))
+    return out, st
+
+
+class _GroupNormAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, b, groups, eps, act):
+        out, st = _groupnorm_act(x, groups, w, b, eps, act, True)
+        ctx.save_for_backward(x, w, b, st)
+        ctx.groups, ctx.act = groups, act
         return out
-    _lib.call("ssam_layernorm_gelu_half", x.data_ptr(), x.numel() // C, C, w.data_ptr(), b.data_ptr(),
-              float(eps), int(bool(gelu)), 0 if x.dtype == torch.float16 else 1, out.data_ptr(), _stream(x))
-    return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        x, w, b, st = ctx.saved_tensors
+        if x.numel() == 0:
+            return torch.zeros_like(x), torch.zeros_like(w), torch.zeros_like(b), None, None, None
+        N, C = x.shape[0], x.shape[-1]
+        HW = x.numel() // (N * C)
+        dout = _dense(dout)
+        dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty_like(b)
+        n = _lib.load().ssam_groupnorm_act_workspace_size(N, HW, C, ctx.groups, 1)
+        ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+        with _on(x):
+            _lib.call("ssam_groupnorm_act_bwd", x.data_ptr(), dout.data_ptr(), N, HW, C, ctx.groups, w.data_ptr(),
+                      b.data_ptr(), st[0].data_ptr(), st[1].data_ptr(), ctx.act, _DTYPES[x.dtype], dx.data_ptr(),
+                      dw.data_ptr(), db.data_ptr(), ws.data_ptr(), n, _stream(x))
+        return dx, dw, db, None, None, None
+
+
+def groupnorm_act(x: torch.Tensor, groups: int, w: torch.Tensor, b: torch.Tensor, eps: float = 1e-5,
+                  act: str = "none") -> torch.Tensor:
+    """act(GroupNorm(x) * w + b) of channels-last maps x (N, ..., C): statistics over all
+    positions and the C / groups channels of a group, per sample. act in ACTIVATIONS (gelu is
+    the erf form). fp16, bf16 or fp32, one dtype for x, w (C,) and b (C,); C a multiple of 8
+    (fp32: 4) and of groups, at most 2048 (fp32: 1024). Returns a new tensor of x's shape.
+    Differentiable in x, w and b (once)."""
+    _check_cuda(x, w, b)
+    _same_device(x, w, b)
+    if x.dtype not in _DTYPES or w.dtype != x.dtype or b.dtype != x.dtype:
+        raise TypeError("x, w and b must share one dtype of fp16, bf16, fp32")
+    if x.dim() < 2 or w.shape != x.shape[-1:] or b.shape != x.shape[-1:]:
+        raise ValueError("x must be (N, ..., C), w and b (C,)")
+    if not x.is_contiguous() or not w.is_contiguous() or not b.is_contiguous():
+        raise ValueError("x, w and b must be contiguous (x channels-last)")
+    if groups <= 0 or x.shape[-1] % groups:
+        raise ValueError(f"groups must divide the {x.shape[-1]} channels, got {groups}")
+    if act not in ACTIVATIONS:
+        raise ValueError(f"act must be one of {tuple(ACTIVATIONS)}, got {act!r}")
+    if _wants_grad(x, w, b):
+        return _GroupNormAct.apply(x, w, b, int(groups), float(eps), ACTIVATIONS[act])
+    return _groupnorm_act(x, int(groups), w, b, float(eps), ACTIVATIONS[act], False)[0]
+
+
+# ---------------------------------------------------------------------------
+# Cross attention
+# ---------------------------------------------------------------------------
+def _strides(*ts: torch.Tensor):
+    return (ctypes.c_int64 * 12)(*(s for t in ts for s in t.stride()[:3]))
+
+
+def _cross_attn(q, k, v, scale, key_lens, key_mask, train):
+    B, Tq, H, D = q.shape
+    Tk, Hk = k.shape[1], k.shape[2]
+    out = torch.empty(B, Tq, H, D, dtype=q.dtype, device=q.device)
+    if out.numel() == 0 or Tk == 0:
+        return out.zero_(), None, None
+    lse = out32 = None
+    if train:
+        lse = torch.empty(B, H, Tq, dtype=torch.float32, device=q.device)
+        out32 = out if q.dtype == torch.float32 else torch.empty(B, Tq, H, D, dtype=torch.float32, device=q.device)
+    with _on(q):
+        _lib.call("ssam_cross_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v, out), B, Tq, Tk, H,
+                  Hk, D, _DTYPES[q.dtype], scale, _ptr(key_lens), _ptr(key_mask), out.data_ptr(),
+                  _ptr(out32) if out32 is not out else None, _ptr(lse), _stream(q))
+    return out, out32, lse
+
+
+class _CrossAttn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, scale, key_lens, key_mask):
+        out, out32, lse = _cross_attn(q, k, v, scale, key_lens, key_mask, True)
+        ctx.save_for_backward(q, k, v, out32, lse, key_lens, key_mask)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out32, lse, key_lens, key_mask = ctx.saved_tensors
+        B, Tq, H, D = q.shape
+        Tk, Hk = k.shape[1], k.shape[2]
+        need_q, need_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        dq = torch.empty(B, Tq, H, D, dtype=q.dtype, device=q.device) if need_q else None
+        dk = torch.empty(B, Tk, Hk, D, dtype=q.dtype, device=q.device) if need_kv else None
+        dv = torch.empty_like(dk) if need_kv else None
+        if lse is None:     # no queries or no keys: nothing depends on anything
+            for g in (dq, dk, dv):
+                if g is not None:
+                    g.zero_()
+            return dq, dk, dv, None, None, None
+        dout = _vector_rows(dout)
+        delta = torch.empty_like(lse)
+        with _on(q):
+            _lib.call("ssam_cross_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(),
+                      _strides(q, k, v, dout), B, Tq, Tk, H, Hk, D, _DTYPES[q.dtype], ctx.scale, _ptr(key_lens),
+                      _ptr(key_mask), out32.data_ptr(), lse.data_ptr(), delta.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv),
+                      _stream(q))
+        return dq, dk, dv, None, None, None
+
+
+def _vector_ok(t: torch.Tensor) -> bool:
+    """Whether every (batch, token, head) row of t is contiguous and starts on a 16-byte boundary."""
+    unit = 16 // t.element_size()
+    return (t.stride(3) == 1 and t.data_ptr() % 16 == 0
+            and all(s % unit == 0 for s, n in zip(t.stride()[:3], t.shape) if n > 1))
+
+
+def _vector_rows(t: torch.Tensor) -> torch.Tensor:
+    return t if _vector_ok(t) else t.clone(memory_format=torch.contiguous_format)
+
+
+CROSS_ATTN_MAX_DIM = 128
+
+
+def cross_attn_supported(heads: int, kv_heads: int, d: int, dtype: torch.dtype) -> bool:
+    """Whether cross_attn takes these heads."""
+    return dtype in _DTYPES and 0 < d <= CROSS_ATTN_MAX_DIM and d % 8 == 0 and kv_heads > 0 and heads % kv_heads == 0
+
+
+def cross_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float | None = None,
+               key_lens: torch.Tensor | None = None, key_mask: torch.Tensor | None = None) -> torch.Tensor:
+    """softmax(scale q k^T) v of queries q (B, Tq, H, D) over another token set's k, v
+    (B, Tk, Hk, D); query head h reads key head h // (H // Hk). Returns (B, Tq, H, D).
+
+    fp16, bf16 or fp32 (one dtype), D a multiple of 8 up to 128; any strides with contiguous
+    D and 16-byte aligned rows (a stride of 0 broadcasts). scale defaults to 1 / sqrt(D).
+    key_lens (int32 (B,)) and key_mask (bool (B, Tk), True: attend) say which keys are
+    there: what the others hold does not matter, and a query without keys gives zeros.
+    Differentiable in q, k and v (once)."""
+    _check_cuda(q, k, v, key_lens, key_mask)
+    _same_device(q, k, v, key_lens, key_mask)
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise ValueError(f"q (B, Tq, H, D), k and v (B, Tk, Hk, D) expected, got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("q, k and v must share one dtype of fp16, bf16, fp32")
+    B, Tk = k.shape[:2]
+    if not cross_attn_supported(q.shape[2], k.shape[2], q.shape[3], q.dtype):
+        raise ValueError(f"heads {q.shape[2]} / {k.shape[2]} of {q.shape[3]} are not supported: key heads divide query "
+                         f"heads, head size a multiple of 8 up to {CROSS_ATTN_MAX_DIM}")
+    if not (_vector_ok(q) and _vector_ok(k) and _vector_ok(v)):
+        raise ValueError("q, k and v need contiguous, 16-byte aligned head rows")
+    if key_lens is not None and (key_lens.dtype != torch.int32 or key_lens.shape != (B,) or not key_lens.is_contiguous()):
+        raise ValueError("key_lens must be contiguous int32 (B,)")
+    if key_mask is not None and (key_mask.dtype != torch.bool or key_mask.shape != (B, Tk)
+                                 or not key_mask.is_contiguous()):
+        raise ValueError("key_mask must be contiguous bool (B, Tk)")
+    scale = 1.0 / math.sqrt(q.shape[3]) if scale is None else float(scale)
+    if not 0.0 < scale < 3e38:
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if _wants_grad(q, k, v):
+        return _CrossAttn.apply(q, k, v, scale, key_lens, key_mask)
+    return _cross_attn(q, k, v, scale, key_lens, key_mask, False)[0]
 
 
 def split_bf16x2(x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
