@@ -212,6 +212,10 @@ int ssam_cross_attn_fwd(const void* q, const void* k, const void* v, const int64
                               out_f32, lse, static_cast<cudaStream_t>(stream));
 }
 
+int ssam_cross_attn_bwd_uses_out_f32(int Tk, int d, int dtype) {
+  return ssam::cross_attn_bwd_uses_out_f32(Tk, d, dtype);
+}
+
 int ssam_cross_attn_bwd(const void* q, const void* k, const void* v, const void* dout, const int64_t* strides, int B,
                         int Tq, int Tk, int heads, int kv_heads, int d, int dtype, float scale, const int32_t* key_lens,
                         const uint8_t* key_mask, const float* out_f32, const float* lse, float* delta, void* dq,

@@ -63,31 +63,31 @@ __device__ __forceinline__ float ex2f(float x) {
   return y;
 }
 
-template <class T>
-__device__ __forceinline__ float4 load4(const T* p);
-template <>
-__device__ __forceinline__ float4 load4<float>(const float* p) {
-  return __ldg(reinterpret_cast<const float4*>(p));
+template <class K>
+static int launch_cluster(K kernel, dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream,
+                          const XAttn& a, int arg) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return status_from_cuda(cudaLaunchKernelEx(&cfg, kernel, a, arg));
 }
-template <>
-__device__ __forceinline__ float4 load4<__half>(const __half* p) {
-  const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
-  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
-  const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
-  return make_float4(a.x, a.y, b.x, b.y);
-}
-template <>
-__device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p) {
-  const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
-  return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
-                     __uint_as_float(u.y & 0xffff0000u));
-}
-__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
-__device__ __forceinline__ void store1(__half* p, float v) { *p = __float2half_rn(v); }
-__device__ __forceinline__ void store1(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+}  // namespace ssam
+
+#include "cross_attention_mma.cuh"
+
+namespace ssam {
 
 // ---------------------------------------------------------------------------
-// Scalar kernels (fp32 FMAs): a thread owns DT dims of one row, TPR threads share
+// fp32 inputs: scalar kernels (fp32 FMAs). A thread owns DT dims of one row, TPR threads share
 // a row. A block holds RB rows x KS slices of the other axis (RB * KS * TPR = 128).
 // ---------------------------------------------------------------------------
 constexpr int kXThreads = 128;
@@ -119,24 +119,24 @@ __device__ __forceinline__ void row_axpy(float w, const float* b, float (&acc)[D
     acc[i + 3] = fmaf(w, v.w, acc[i + 3]);
   }
 }
-template <class T, int DT>
-__device__ __forceinline__ void load_row(const T* p, int dims, bool ok, float (&r)[DT]) {
+template <int DT>
+__device__ __forceinline__ void load_row(const float* p, int dims, bool ok, float (&r)[DT]) {
 #pragma unroll
   for (int i = 0; i < DT; i += 4) {
-    const float4 v = ok && i < dims ? load4<T>(p + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float4 v = ok && i < dims ? __ldg(reinterpret_cast<const float4*>(p + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
     r[i] = v.x, r[i + 1] = v.y, r[i + 2] = v.z, r[i + 3] = v.w;
   }
 }
 
 // Copies `n` rows (<= kXTile) of width d into sm[kXTile][LD] as floats; rows for
 // which ok(i) is false, and channels past d, are zero.
-template <class T, int DP, class P, class O>
+template <int DP, class P, class O>
 __device__ __forceinline__ void stage_rows(float* sm, int n, int d, P row, O ok) {
   constexpr int V = DP / 4, LD = DP + 4;
   for (int e = threadIdx.x; e < kXTile * V; e += kXThreads) {
     const int i = e / V, c = (e % V) * 4;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (i < n && c < d && ok(i)) v = load4<T>(static_cast<const T*>(row(i)) + c);
+    if (i < n && c < d && ok(i)) v = __ldg(reinterpret_cast<const float4*>(row(i) + c));
     *reinterpret_cast<float4*>(sm + i * LD + c) = v;
   }
 }
@@ -169,7 +169,7 @@ __device__ __forceinline__ void merge_sums(float* part, int KS, int RB, int W, E
   cluster_sync_all();
 }
 
-template <class T, int DT, int TPR>
+template <int DT, int TPR>
 __global__ void __launch_bounds__(kXThreads) xattn_fwd_scalar(const XAttn a, int RB) {
   constexpr int DP = DT * TPR, LD = DP + 4;
   extern __shared__ __align__(16) float xsm[];
@@ -185,20 +185,20 @@ __global__ void __launch_bounds__(kXThreads) xattn_fwd_scalar(const XAttn a, int
   const bool row_ok = r < rows;
   const int dims = a.d - part * DT;
   float q[DT], o[DT];
-  load_row<T, DT>(static_cast<const T*>(a.q) + b * a.qs[0] + t * a.qs[1] + h * a.qs[2] + part * DT, dims, row_ok, q);
+  load_row<DT>(static_cast<const float*>(a.q) + b * a.qs[0] + t * a.qs[1] + h * a.qs[2] + part * DT, dims, row_ok, q);
 #pragma unroll
   for (int i = 0; i < DT; ++i) o[i] = 0.f;
   float m = -INFINITY, l = 0.f;
   const int keys = xattn_keys(a, b);
-  const T* kb = static_cast<const T*>(a.k) + b * a.ks[0] + n * a.ks[2];
-  const T* vb = static_cast<const T*>(a.v) + b * a.vs[0] + n * a.vs[2];
+  const float* kb = static_cast<const float*>(a.k) + b * a.ks[0] + n * a.ks[2];
+  const float* vb = static_cast<const float*>(a.v) + b * a.vs[0] + n * a.vs[2];
   const uint8_t* mask = a.key_mask == nullptr ? nullptr : a.key_mask + static_cast<int64_t>(b) * a.Tk;
   for (int j0 = rank * kXTile; j0 < keys; j0 += cl * kXTile) {
     const int nk = min(kXTile, keys - j0);
     auto ok = [&](int i) { return mask == nullptr || __ldg(mask + j0 + i) != 0; };
     __syncthreads();
-    stage_rows<T, DP>(sk, nk, a.d, [&](int i) { return kb + (j0 + i) * a.ks[1]; }, ok);
-    stage_rows<T, DP>(sv, nk, a.d, [&](int i) { return vb + (j0 + i) * a.vs[1]; }, ok);
+    stage_rows<DP>(sk, nk, a.d, [&](int i) { return kb + (j0 + i) * a.ks[1]; }, ok);
+    stage_rows<DP>(sv, nk, a.d, [&](int i) { return vb + (j0 + i) * a.vs[1]; }, ok);
     if (threadIdx.x < kXTile) there[threadIdx.x] = threadIdx.x < nk && ok(threadIdx.x);
     __syncthreads();
     for (int j = slice; j < kXTile; j += KS) {
@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(kXThreads) xattn_fwd_scalar(const XAttn a, int
       }
     } else if (col < a.d) {
       const float y = den > 0.f ? s / den : (den == 0.f ? 0.f : s / den);
-      store1(static_cast<T*>(a.out) + b * a.os[0] + et * a.os[1] + eh * a.os[2] + col, y);
+      *(static_cast<float*>(a.out) + b * a.os[0] + et * a.os[1] + eh * a.os[2] + col) = y;
       if (a.out_f32 != nullptr)
         a.out_f32[((static_cast<int64_t>(b) * a.Tq + et) * a.heads + eh) * a.d + col] = y;
     }
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(kXThreads) xattn_fwd_scalar(const XAttn a, int
 }
 
 // dQ: the forward's loop with p from the saved statistics. Also writes D for the dK / dV kernel.
-template <class T, int DT, int TPR>
+template <int DT, int TPR>
 __global__ void __launch_bounds__(kXThreads) xattn_dq_scalar(const XAttn a, int RB) {
   constexpr int DP = DT * TPR, LD = DP + 4;
   extern __shared__ __align__(16) float xsm[];
@@ -297,12 +297,12 @@ __global__ void __launch_bounds__(kXThreads) xattn_dq_scalar(const XAttn a, int 
   const bool row_ok = r < rows;
   const int dims = a.d - part * DT;
   float q[DT], dO[DT], dq[DT];
-  load_row<T, DT>(static_cast<const T*>(a.q) + b * a.qs[0] + t * a.qs[1] + h * a.qs[2] + part * DT, dims, row_ok, q);
-  load_row<T, DT>(static_cast<const T*>(a.dout) + b * a.os[0] + t * a.os[1] + h * a.os[2] + part * DT, dims, row_ok,
+  load_row<DT>(static_cast<const float*>(a.q) + b * a.qs[0] + t * a.qs[1] + h * a.qs[2] + part * DT, dims, row_ok, q);
+  load_row<DT>(static_cast<const float*>(a.dout) + b * a.os[0] + t * a.os[1] + h * a.os[2] + part * DT, dims, row_ok,
                   dO);
   const int64_t stat = (static_cast<int64_t>(b) * a.heads + h) * a.Tq + t;
   // D in the order of dP's sum, so that a row with one key has dP - D = 0 exactly
-  load_row<float, DT>(a.out_f32 + ((static_cast<int64_t>(b) * a.Tq + t) * a.heads + h) * a.d + part * DT, dims, row_ok,
+  load_row<DT>(a.out_f32 + ((static_cast<int64_t>(b) * a.Tq + t) * a.heads + h) * a.d + part * DT, dims, row_ok,
                       dq);
   float delta = 0.f;
 #pragma unroll
@@ -315,15 +315,15 @@ __global__ void __launch_bounds__(kXThreads) xattn_dq_scalar(const XAttn a, int 
   for (int i = 0; i < DT; ++i) dq[i] = 0.f;
   if (a.dq != nullptr) {
     const int keys = xattn_keys(a, b);
-    const T* kb = static_cast<const T*>(a.k) + b * a.ks[0] + n * a.ks[2];
-    const T* vb = static_cast<const T*>(a.v) + b * a.vs[0] + n * a.vs[2];
+    const float* kb = static_cast<const float*>(a.k) + b * a.ks[0] + n * a.ks[2];
+    const float* vb = static_cast<const float*>(a.v) + b * a.vs[0] + n * a.vs[2];
     const uint8_t* mask = a.key_mask == nullptr ? nullptr : a.key_mask + static_cast<int64_t>(b) * a.Tk;
     for (int j0 = rank * kXTile; j0 < keys; j0 += cl * kXTile) {
       const int nk = min(kXTile, keys - j0);
       auto ok = [&](int i) { return mask == nullptr || __ldg(mask + j0 + i) != 0; };
       __syncthreads();
-      stage_rows<T, DP>(sk, nk, a.d, [&](int i) { return kb + (j0 + i) * a.ks[1]; }, ok);
-      stage_rows<T, DP>(sv, nk, a.d, [&](int i) { return vb + (j0 + i) * a.vs[1]; }, ok);
+      stage_rows<DP>(sk, nk, a.d, [&](int i) { return kb + (j0 + i) * a.ks[1]; }, ok);
+      stage_rows<DP>(sv, nk, a.d, [&](int i) { return vb + (j0 + i) * a.vs[1]; }, ok);
       if (threadIdx.x < kXTile) there[threadIdx.x] = threadIdx.x < nk && ok(threadIdx.x);
       __syncthreads();
       for (int j = slice; j < kXTile; j += KS) {
@@ -341,13 +341,13 @@ __global__ void __launch_bounds__(kXThreads) xattn_dq_scalar(const XAttn a, int 
       const int rr = r0 + er;
       if (rr >= rows || col >= a.d) return;
       const int eg = rr / a.Tq, et = rr - eg * a.Tq, eh = n * a.group + eg;
-      store1(static_cast<T*>(a.dq) + ((static_cast<int64_t>(b) * a.Tq + et) * a.heads + eh) * a.d + col, s * a.scale);
+      *(static_cast<float*>(a.dq) + ((static_cast<int64_t>(b) * a.Tq + et) * a.heads + eh) * a.d + col) = s * a.scale;
     });
   }
 }
 
 // dK, dV: a thread owns (part of) one key; the block's slices walk the query rows.
-template <class T, int DT, int TPR>
+template <int DT, int TPR>
 __global__ void __launch_bounds__(kXThreads) xattn_dkv_scalar(const XAttn a, int RB) {
   constexpr int DP = DT * TPR, LD = DP + 4;
   extern __shared__ __align__(16) float xsm[];
@@ -363,8 +363,8 @@ __global__ void __launch_bounds__(kXThreads) xattn_dkv_scalar(const XAttn a, int
                       (a.key_mask == nullptr || __ldg(a.key_mask + static_cast<int64_t>(b) * a.Tk + j) != 0);
   const int dims = a.d - part * DT;
   float k[DT], v[DT], dk[DT], dv[DT];
-  load_row<T, DT>(static_cast<const T*>(a.k) + b * a.ks[0] + j * a.ks[1] + n * a.ks[2] + part * DT, dims, key_ok, k);
-  load_row<T, DT>(static_cast<const T*>(a.v) + b * a.vs[0] + j * a.vs[1] + n * a.vs[2] + part * DT, dims, key_ok, v);
+  load_row<DT>(static_cast<const float*>(a.k) + b * a.ks[0] + j * a.ks[1] + n * a.ks[2] + part * DT, dims, key_ok, k);
+  load_row<DT>(static_cast<const float*>(a.v) + b * a.vs[0] + j * a.vs[1] + n * a.vs[2] + part * DT, dims, key_ok, v);
 #pragma unroll
   for (int i = 0; i < DT; ++i) dk[i] = 0.f, dv[i] = 0.f;
   for (int r0 = rank * kXTile; r0 < rows; r0 += cl * kXTile) {
@@ -375,8 +375,8 @@ __global__ void __launch_bounds__(kXThreads) xattn_dkv_scalar(const XAttn a, int
     };
     auto ok = [](int) { return true; };
     __syncthreads();
-    stage_rows<T, DP>(sq, nr, a.d, [&](int i) { return static_cast<const T*>(a.q) + at(i, a.qs); }, ok);
-    stage_rows<T, DP>(so, nr, a.d, [&](int i) { return static_cast<const T*>(a.dout) + at(i, a.os); }, ok);
+    stage_rows<DP>(sq, nr, a.d, [&](int i) { return static_cast<const float*>(a.q) + at(i, a.qs); }, ok);
+    stage_rows<DP>(so, nr, a.d, [&](int i) { return static_cast<const float*>(a.dout) + at(i, a.os); }, ok);
     if (threadIdx.x < kXTile) {
       const int i = threadIdx.x, r = r0 + i, g = r / a.Tq, t = r - g * a.Tq;
       const int64_t stat = (static_cast<int64_t>(b) * a.heads + n * a.group + g) * a.Tq + t;
@@ -402,32 +402,13 @@ __global__ void __launch_bounds__(kXThreads) xattn_dkv_scalar(const XAttn a, int
     if (jj >= a.Tk || c >= a.d) return;
     const int64_t to = ((static_cast<int64_t>(b) * a.Tk + jj) * a.kv_heads + n) * a.d + c;
     if (col < DP)
-      store1(static_cast<T*>(a.dk) + to, s * a.scale);
+      *(static_cast<float*>(a.dk) + to) = s * a.scale;
     else
-      store1(static_cast<T*>(a.dv) + to, s);
+      *(static_cast<float*>(a.dv) + to) = s;
   });
 }
 
-// ---------------------------------------------------------------------------
 // Launch
-// ---------------------------------------------------------------------------
-template <class K>
-static int launch_cluster(K kernel, dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream,
-                          const XAttn& a, int arg) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = cluster;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return status_from_cuda(cudaLaunchKernelEx(&cfg, kernel, a, arg));
-}
-
 // Rows per block (a power of two, at most 128 / tpr) and blocks per cluster for `own` rows that
 // each walk `other` entries: blocks are added along `other` until the device is filled.
 static void xattn_plan(int own, int other, int64_t pairs, int tpr, int* rb, int* cluster) {
@@ -440,7 +421,7 @@ static void xattn_plan(int own, int other, int64_t pairs, int tpr, int* rb, int*
   *cluster = c;
 }
 
-template <class T, int DT, int TPR>
+template <int DT, int TPR>
 static int xattn_scalar(const XAttn& a, bool backward, cudaStream_t stream) {
   constexpr int DP = DT * TPR;
   const size_t tiles = 2 * kXTile * (DP + 4) * sizeof(float);
@@ -450,26 +431,27 @@ static int xattn_scalar(const XAttn& a, bool backward, cudaStream_t stream) {
   if (!backward) {
     xattn_plan(rows, a.Tk, pairs, TPR, &rb, &cl);
     const size_t merge = (kXThreads + kXThreads / TPR * (DP + 1)) * sizeof(float);
-    return launch_cluster(xattn_fwd_scalar<T, DT, TPR>, dim3((rows + rb - 1) / rb * cl, a.kv_heads, a.B), kXThreads,
+    return launch_cluster(xattn_fwd_scalar<DT, TPR>, dim3((rows + rb - 1) / rb * cl, a.kv_heads, a.B), kXThreads,
                           tiles > merge ? tiles : merge, cl, stream, a, rb);
   }
   xattn_plan(rows, a.Tk, pairs, TPR, &rb, &cl);
   size_t merge = kXThreads / TPR * DP * sizeof(float);
-  int st = launch_cluster(xattn_dq_scalar<T, DT, TPR>, dim3((rows + rb - 1) / rb * cl, a.kv_heads, a.B), kXThreads,
+  int st = launch_cluster(xattn_dq_scalar<DT, TPR>, dim3((rows + rb - 1) / rb * cl, a.kv_heads, a.B), kXThreads,
                           tiles > merge ? tiles : merge, cl, stream, a, rb);
   if (st != SSAM_OK || a.dk == nullptr) return st;
   xattn_plan(a.Tk, rows, pairs, TPR, &rb, &cl);
   merge = kXThreads / TPR * 2 * DP * sizeof(float);
-  return launch_cluster(xattn_dkv_scalar<T, DT, TPR>, dim3((a.Tk + rb - 1) / rb * cl, a.kv_heads, a.B), kXThreads,
+  return launch_cluster(xattn_dkv_scalar<DT, TPR>, dim3((a.Tk + rb - 1) / rb * cl, a.kv_heads, a.B), kXThreads,
                         tiles > merge ? tiles : merge, cl, stream, a, rb);
 }
 
-template <class T>
-static int xattn_dispatch(const XAttn& a, bool backward, cudaStream_t stream) {
-  if (a.d <= 16) return xattn_scalar<T, 16, 1>(a, backward, stream);
-  if (a.d <= 32) return xattn_scalar<T, 32, 1>(a, backward, stream);
-  if (a.d <= 64) return xattn_scalar<T, 32, 2>(a, backward, stream);
-  return xattn_scalar<T, 32, 4>(a, backward, stream);
+static int xattn_dispatch(const XAttn& a, int dtype, bool backward, cudaStream_t stream) {
+  if (dtype == 0) return xattn_mma<__half>(a, backward, stream);
+  if (dtype == 1) return xattn_mma<__nv_bfloat16>(a, backward, stream);
+  if (a.d <= 16) return xattn_scalar<16, 1>(a, backward, stream);
+  if (a.d <= 32) return xattn_scalar<32, 1>(a, backward, stream);
+  if (a.d <= 64) return xattn_scalar<32, 2>(a, backward, stream);
+  return xattn_scalar<32, 4>(a, backward, stream);
 }
 
 // Checks shared by both directions; the strides and pointers are those the kernels read with
@@ -509,17 +491,17 @@ int cross_attn_fwd(const void* q, const void* k, const void* v, const int64_t* s
   const int st = xattn_check(a, dtype);
   if (st != SSAM_OK) return st;
   if (!aligned16(out) || (out_f32 != nullptr && !aligned16(out_f32))) return SSAM_ERR_ALIGN;
-  if (dtype == 0) return xattn_dispatch<__half>(a, false, stream);
-  if (dtype == 1) return xattn_dispatch<__nv_bfloat16>(a, false, stream);
-  return xattn_dispatch<float>(a, false, stream);
+  return xattn_dispatch(a, dtype, false, stream);
 }
+
+int cross_attn_bwd_uses_out_f32(int Tk, int d, int dtype) { return xattn_uses_out_f32(Tk, d, dtype) ? 1 : 0; }
 
 int cross_attn_bwd(const void* q, const void* k, const void* v, const void* dout, const int64_t* strides, int B, int Tq,
                    int Tk, int heads, int kv_heads, int d, int dtype, float scale, const int32_t* key_lens,
                    const uint8_t* key_mask, const float* out_f32, const float* lse, float* delta, void* dq, void* dk,
                    void* dv, cudaStream_t stream) {
-  if (q == nullptr || k == nullptr || v == nullptr || dout == nullptr || strides == nullptr || out_f32 == nullptr ||
-      lse == nullptr || delta == nullptr || (dk == nullptr) != (dv == nullptr))
+  if (q == nullptr || k == nullptr || v == nullptr || dout == nullptr || strides == nullptr ||
+      (out_f32 == nullptr && xattn_uses_out_f32(Tk, d, dtype)) || lse == nullptr || delta == nullptr || (dk == nullptr) != (dv == nullptr))
     return SSAM_ERR_INVALID;
   XAttn a = xattn_args(q, k, v, strides, B, Tq, Tk, heads, kv_heads, d, scale, key_lens, key_mask);
   a.dout = dout, a.out_f32 = const_cast<float*>(out_f32), a.lse = const_cast<float*>(lse), a.delta = delta;
@@ -530,9 +512,7 @@ int cross_attn_bwd(const void* q, const void* k, const void* v, const void* dout
                         static_cast<const void*>(dq), static_cast<const void*>(dk), static_cast<const void*>(dv)})
     if (!aligned16(p)) return SSAM_ERR_ALIGN;
   if (dq == nullptr && dk == nullptr) return SSAM_OK;
-  if (dtype == 0) return xattn_dispatch<__half>(a, true, stream);
-  if (dtype == 1) return xattn_dispatch<__nv_bfloat16>(a, true, stream);
-  return xattn_dispatch<float>(a, true, stream);
+  return xattn_dispatch(a, dtype, true, stream);
 }
 
 }  // namespace ssam

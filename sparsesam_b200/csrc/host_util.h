@@ -105,6 +105,7 @@ int patch_im2col_split3(const float* img, int B, int Cin, int H, int W, int p, v
 int cross_attn_fwd(const void* q, const void* k, const void* v, const int64_t* strides, int B, int Tq, int Tk,
                    int heads, int kv_heads, int d, int dtype, float scale, const int32_t* key_lens,
                    const uint8_t* key_mask, void* out, float* out_f32, float* lse, cudaStream_t stream);
+int cross_attn_bwd_uses_out_f32(int Tk, int d, int dtype);
 int cross_attn_bwd(const void* q, const void* k, const void* v, const void* dout, const int64_t* strides, int B, int Tq,
                    int Tk, int heads, int kv_heads, int d, int dtype, float scale, const int32_t* key_lens,
                    const uint8_t* key_mask, const float* out_f32, const float* lse, float* delta, void* dq, void* dk,

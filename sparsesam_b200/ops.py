@@ -629,7 +629,10 @@ def _cross_attn(q, k, v, scale, key_lens, key_mask, train):
     lse = out32 = None
     if train:
         lse = torch.empty(B, H, Tq, dtype=torch.float32, device=q.device)
-        out32 = out if q.dtype == torch.float32 else torch.empty(B, Tq, H, D, dtype=torch.float32, device=q.device)
+        if q.dtype == torch.float32:
+            out32 = out
+        elif _lib.load().ssam_cross_attn_bwd_uses_out_f32(Tk, D, _DTYPES[q.dtype]):
+            out32 = torch.empty(B, Tq, H, D, dtype=torch.float32, device=q.device)
     with _on(q):
         _lib.call("ssam_cross_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v, out), B, Tq, Tk, H,
                   Hk, D, _DTYPES[q.dtype], scale, _ptr(key_lens), _ptr(key_mask), out.data_ptr(),
@@ -665,7 +668,7 @@ class _CrossAttn(torch.autograd.Function):
         with _on(q):
             _lib.call("ssam_cross_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(),
                       _strides(q, k, v, dout), B, Tq, Tk, H, Hk, D, _DTYPES[q.dtype], ctx.scale, _ptr(key_lens),
-                      _ptr(key_mask), out32.data_ptr(), lse.data_ptr(), delta.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv),
+                      _ptr(key_mask), _ptr(out32), lse.data_ptr(), delta.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv),
                       _stream(q))
         return dq, dk, dv, None, None, None
 
