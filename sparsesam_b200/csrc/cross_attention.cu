@@ -22,6 +22,8 @@
 // order, so results do not depend on scheduling and no workspace is needed.
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "common.cuh"
 #include "host_util.h"
 

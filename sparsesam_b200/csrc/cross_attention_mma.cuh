@@ -33,6 +33,11 @@ struct Mma<__half> {
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   }
+  static __device__ __forceinline__ void run8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(b0));
+  }
   static __device__ __forceinline__ uint32_t pack(float x, float y) {
     const __half2 h = __floats2half2_rn(x, y);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -48,11 +53,19 @@ struct Mma<__nv_bfloat16> {
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   }
+  static __device__ __forceinline__ void run8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(b0));
+  }
   static __device__ __forceinline__ uint32_t pack(float x, float y) { return pack_bf16x2(x, y); }
   static __device__ __forceinline__ float2 unpack(uint32_t u) {
     return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
   }
 };
+
+__device__ __forceinline__ void store1(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void store1(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
 __device__ __forceinline__ uint32_t movm(uint32_t x) {
   uint32_t y;
@@ -383,33 +396,356 @@ __global__ void __launch_bounds__(kXmThreads) xattn_fwd_mma(const XAttn a, int s
 }
 
 // ---------------------------------------------------------------------------
-// Backward. A warp owns 16 M entries of one token set (OWN_ROWS: query rows, with
-// x1 = q, x2 = dout; else keys, with x1 = k, x2 = v) and walks the other set
-// 16 entries at a time (y1 = k or q, y2 = v or dout):
-//   s = x1 y1^T, dp = x2 y2^T, p = 2^(c s - lse), ds = p (dp - D)      (own x other)
-//   own rows:  dq += ds k              own keys:  dk += ds q,  dv += p dout
-// FUSED: the owned entries are all there are on that side, so the other side's
-// gradients of a step are complete as well and leave at once, from the turned blocks:
-//   own rows:  dk = ds^T q, dv = p^T dout        own keys:  dq = ds^T k
-// Owned sums of the block's 8 warps and the cluster are joined at the end.
+// Forward, few query rows (8 NQ per block) on many keys. The short side is the column
+// side, S^T = K Q^T (16 keys x 8 queries per instruction: no padding rows for the
+// decoder's 8 tokens), and O^T = V^T P^T. The keys are split over the block's warps and
+// the cluster; nothing passes between warps until the end.
 //
-// fp16: dS has no fixed scale (it follows the loss), so its products run in bf16, which
-// has fp32's range: dS as two bf16 terms, the fp16 factor as two bf16 terms (exact,
-// 11 = 8 + 3 bits), without the product of the two remainders. P lies in [0, 1] and
-// is scaled by 2^12, so that its fp16 remainder keeps digits down to 2^-36.
+// The reference point of the exponentials is renewed only when a logit exceeds it by
+// 2^8 (as in attention.cu), so the cross-lane maximum is not taken every step.
+// ---------------------------------------------------------------------------
+constexpr float kXmNone = -1e30f;           // reference before the first key
+constexpr float kXmSlack = 8.f;
+
+template <class T, int DP, int NQ>
+__global__ void __launch_bounds__(kXmThreads) xattn_fwd_few_rows(const XAttn a, int) {
+  constexpr int NR = DP / 8, NU = NR / 2;    // 8- and 16-channel blocks
+  constexpr int KM = DP <= 32 ? 2 : 1;       // 16-key tiles per step
+  extern __shared__ __align__(16) float xsm[];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+  const int b = blockIdx.z, n = blockIdx.y;
+  const int cl = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
+  const int rows = a.group * a.Tq;
+  const int r0 = static_cast<int>(blockIdx.x) / cl * 8 * NQ;
+  const int keys = xattn_keys(a, b);
+  const int steps = (keys + 16 * KM - 1) / (16 * KM), ns = kXmWarps * cl;
+  const int per = (steps + ns - 1) / ns * (16 * KM);
+  const int j_begin = min(keys, (rank * kXmWarps + warp) * per), j_end = min(keys, j_begin + per);
+  const T* kb = static_cast<const T*>(a.k) + b * a.ks[0] + n * a.ks[2];
+  const T* vb = static_cast<const T*>(a.v) + b * a.vs[0] + n * a.vs[2];
+  const uint8_t* mask = a.key_mask == nullptr ? nullptr : a.key_mask + static_cast<int64_t>(b) * a.Tk;
+
+  uint32_t k[KM][2][NR], v[KM][2][NR];
+  float bias[KM][2];                         // 0, or -infinity for a key that is not there
+  auto load = [&](int j0) {
+#pragma unroll
+    for (int i = 0; i < KM; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int j = j0 + i * 16 + h * 8 + g;
+        const bool ok = j < j_end && (mask == nullptr || __ldg(mask + j) != 0);
+        bias[i][h] = ok ? 0.f : -INFINITY;
+        load_frag<T, DP>(kb + j * a.ks[1], t, a.d, ok, k[i][h]);
+        load_frag<T, DP>(vb + j * a.vs[1], t, a.d, ok, v[i][h]);
+      }
+  };
+  load(j_begin);
+  uint32_t q[NQ][NR];
+#pragma unroll
+  for (int i = 0; i < NQ; ++i) {
+    const int r = r0 + i * 8 + g;
+    load_frag<T, DP>(static_cast<const T*>(a.q) + row_offset(a, a.qs, b, n, min(r, rows - 1)), t, a.d, r < rows, q[i]);
+  }
+  float o[NQ][NU][4], ref[NQ][2], l[NQ][2];
+#pragma unroll
+  for (int i = 0; i < NQ; ++i) {
+    ref[i][0] = ref[i][1] = kXmNone, l[i][0] = l[i][1] = 0.f;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) o[i][u][0] = o[i][u][1] = o[i][u][2] = o[i][u][3] = 0.f;
+  }
+
+  for (int j0 = j_begin; j0 < j_end; j0 += 16 * KM) {
+    float s[NQ][KM][4];
+    uint32_t vt[KM][2][NR];
+    bool renew = false;
+#pragma unroll
+    for (int x = 0; x < KM; ++x) {
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        s[i][x][0] = s[i][x][1] = s[i][x][2] = s[i][x][3] = 0.f;
+#pragma unroll
+        for (int c = 0; c < NR; c += 2)
+          Mma<T>::run(s[i][x], k[x][0][c], k[x][1][c], k[x][0][c + 1], k[x][1][c + 1], q[i][c], q[i][c + 1]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[i][x][e] = fmaf(s[i][x][e], a.c, bias[x][e >> 1]);
+          renew |= s[i][x][e] > ref[i][e & 1] + kXmSlack;
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int c = 0; c < NR; ++c) vt[x][h][c] = movm(v[x][h][c]);
+    }
+    if (j0 + 16 * KM < j_end) load(j0 + 16 * KM);     // the next step's, under this one's arithmetic
+    if (__any_sync(0xffffffffu, renew)) {
+#pragma unroll
+      for (int i = 0; i < NQ; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float m = ref[i][e];
+#pragma unroll
+          for (int x = 0; x < KM; ++x) m = fmaxf(m, fmaxf(s[i][x][e], s[i][x][e + 2]));
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+          const float f = ex2f(ref[i][e] - m);
+          ref[i][e] = m;
+          l[i][e] *= f;
+#pragma unroll
+          for (int u = 0; u < NU; ++u) o[i][u][e] *= f, o[i][u][e + 2] *= f;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NQ; ++i)
+#pragma unroll
+      for (int x = 0; x < KM; ++x) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[i][x][e] = ex2f(s[i][x][e] - ref[i][e & 1]);
+          l[i][e & 1] += s[i][x][e];
+        }
+        uint32_t h0, l0, h1, l1;
+        split2<T>(s[i][x][0], s[i][x][1], h0, l0);
+        split2<T>(s[i][x][2], s[i][x][3], h1, l1);
+        h0 = movm(h0), h1 = movm(h1), l0 = movm(l0), l1 = movm(l1);
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+          Mma<T>::run(o[i][u], vt[x][0][2 * u], vt[x][0][2 * u + 1], vt[x][1][2 * u], vt[x][1][2 * u + 1], h0, h1);
+          Mma<T>::run(o[i][u], vt[x][0][2 * u], vt[x][0][2 * u + 1], vt[x][1][2 * u], vt[x][1][2 * u + 1], l0, l1);
+        }
+      }
+  }
+
+  // Join: the highest reference of the warps, then of the cluster's blocks; every warp rescales
+  // its share to it, the shares are summed in a fixed order and divided on the way out.
+  constexpr int PER = NU * 4 + 2, NREG = NQ * PER, ROWS = 8 * NQ;
+  float* s_top = xsm;                        // [8][ROWS]
+  float* s_acc = xsm + kXmWarps * ROWS;      // [4][NREG][32]
+#pragma unroll
+  for (int i = 0; i < NQ; ++i)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int w = 4; w < 32; w <<= 1) l[i][e] += __shfl_xor_sync(0xffffffffu, l[i][e], w);
+      if (g == 0) s_top[warp * ROWS + i * 8 + 2 * t + e] = ref[i][e];
+    }
+  __syncthreads();
+  float top[NQ][2];
+#pragma unroll
+  for (int i = 0; i < NQ; ++i)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float m = kXmNone;
+#pragma unroll
+      for (int w = 0; w < kXmWarps; ++w) m = fmaxf(m, s_top[w * ROWS + i * 8 + 2 * t + e]);
+      top[i][e] = m;
+    }
+  __syncthreads();
+  if (warp == 0 && g == 0) {
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) s_top[i * 8 + 2 * t] = top[i][0], s_top[i * 8 + 2 * t + 1] = top[i][1];
+  }
+  if (cl > 1) {
+    cluster_sync_all();
+#pragma unroll
+    for (int i = 0; i < NQ; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t at = smem_u32(s_top + i * 8 + 2 * t + e);
+        for (int w = 0; w < cl; ++w) top[i][e] = fmaxf(top[i][e], ld_dsmem(mapa_shared(at, w)));
+      }
+  }
+  float acc[NREG];
+#pragma unroll
+  for (int i = 0; i < NQ; ++i)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float f = ex2f(ref[i][e] - top[i][e]);
+      acc[i * PER + NU * 4 + e] = l[i][e] * f;
+#pragma unroll
+      for (int u = 0; u < NU; ++u) acc[i * PER + u * 4 + e] = o[i][u][e] * f, acc[i * PER + u * 4 + e + 2] = o[i][u][e + 2] * f;
+    }
+  warp_tree_sum<NREG>(acc, s_acc, warp, lane);
+  __syncthreads();
+  if (warp == 0) {
+#pragma unroll
+    for (int i = 0; i < NREG; ++i) s_acc[i * 32 + lane] = acc[i];
+  }
+  if (cl > 1) cluster_sync_all(); else __syncthreads();
+  const uint32_t base = smem_u32(s_acc) + lane * 4;
+  const int64_t stat0 = (static_cast<int64_t>(b) * a.heads + n * a.group) * a.Tq;
+  for (int w = rank * kXmWarps + warp; w < 2 * NQ * NU; w += cl * kXmWarps) {
+    const int e = w % 2, u = w / 2 % NU, i = w / 2 / NU, ro = i * 8 + 2 * t + e, r = r0 + ro;
+    float x = 0.f, y = 0.f, den = 0.f, m = kXmNone;
+    for (int z = 0; z < cl; ++z) {
+      const uint32_t from = mapa_shared(base, z);
+      x += ld_dsmem(from + (i * PER + u * 4 + e) * 128);
+      y += ld_dsmem(from + (i * PER + u * 4 + e + 2) * 128);
+      den += ld_dsmem(from + (i * PER + NU * 4 + e) * 128);
+      m = fmaxf(m, ld_dsmem(mapa_shared(smem_u32(s_top + ro), z)));
+    }
+    if (r >= rows) continue;
+    const float inv = den == 0.f ? 0.f : 1.f / den;
+    const int ch = g / 2 * (DP / 4) + 4 * u + g % 2;   // and ch + 2
+    T* to = static_cast<T*>(a.out) + row_offset(a, a.os, b, n, r);
+    float* to32 = a.out_f32 == nullptr ? nullptr : a.out_f32 + row_dense(a, b, n, r);
+    if (ch < a.d) {
+      store1(to + ch, x * inv);
+      if (to32 != nullptr) to32[ch] = x * inv;
+    }
+    if (ch + 2 < a.d) {
+      store1(to + ch + 2, y * inv);
+      if (to32 != nullptr) to32[ch + 2] = y * inv;
+    }
+    if (a.lse != nullptr && u == 0 && g == 0) a.lse[stat0 + r] = den == 0.f ? INFINITY : m + log2f(den);
+  }
+  if (cl > 1) cluster_sync_all();
+}
+
+// ---------------------------------------------------------------------------
+// Forward, many query rows on few keys (at most 8 NK): a warp keeps the K and turned V
+// fragments of one (image, key head) and walks its share of the rows 16 at a time, the
+// next rows in flight. Bound by the bytes of q and out; neighbouring warps hold
+// neighbouring heads, so a block touches whole rows.
+// ---------------------------------------------------------------------------
+template <class T, int DP, int NK>
+__global__ void __launch_bounds__(kXmThreads) xattn_fwd_few_keys(const XAttn a, int chunks) {
+  constexpr int NR = DP / 8;
+  const int lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+  const int64_t w = static_cast<int64_t>(blockIdx.x) * kXmWarps + threadIdx.x / 32;
+  const int n = static_cast<int>(w % a.kv_heads), chunk = static_cast<int>(w / a.kv_heads % chunks);
+  const int64_t bb = w / a.kv_heads / chunks;
+  if (bb >= a.B) return;
+  const int b = static_cast<int>(bb);
+  const int rows = a.group * a.Tq, tiles = (rows + 15) / 16, per = (tiles + chunks - 1) / chunks;
+  const int r_begin = min(rows, chunk * per * 16), r_end = min(rows, r_begin + per * 16);
+  if (r_begin >= r_end) return;
+  const int keys = xattn_keys(a, b);
+  const T* kb = static_cast<const T*>(a.k) + b * a.ks[0] + n * a.ks[2];
+  const T* vb = static_cast<const T*>(a.v) + b * a.vs[0] + n * a.vs[2];
+  const T* qb = static_cast<const T*>(a.q);
+  const uint8_t* mask = a.key_mask == nullptr ? nullptr : a.key_mask + static_cast<int64_t>(b) * a.Tk;
+  const int64_t stat0 = (static_cast<int64_t>(b) * a.heads + n * a.group) * a.Tq;
+
+  uint32_t k[NK][NR], v[NK][NR], q[2][NR];
+  float bias[NK][2];                         // of keys 8 i + 2t + e
+  auto load_q = [&](int r) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      load_frag<T, DP>(qb + row_offset(a, a.qs, b, n, min(r + h * 8 + g, rows - 1)), t, a.d, r + h * 8 + g < r_end, q[h]);
+  };
+  load_q(r_begin);
+#pragma unroll
+  for (int i = 0; i < NK; ++i) {
+    const int j = i * 8 + g;
+    const bool ok = j < keys && (mask == nullptr || __ldg(mask + j) != 0);
+    load_frag<T, DP>(kb + j * a.ks[1], t, a.d, ok, k[i]);
+    load_frag<T, DP>(vb + j * a.vs[1], t, a.d, ok, v[i]);
+    const float mine = ok ? 0.f : -INFINITY;
+    bias[i][0] = __shfl_sync(0xffffffffu, mine, 8 * t);
+    bias[i][1] = __shfl_sync(0xffffffffu, mine, 8 * t + 4);
+#pragma unroll
+    for (int c = 0; c < NR; ++c) v[i][c] = movm(v[i][c]);
+  }
+
+  for (int r0 = r_begin; r0 < r_end; r0 += 16) {
+    float s[NK][4];
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+      s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+#pragma unroll
+      for (int c = 0; c < NR; c += 2) Mma<T>::run(s[i], q[0][c], q[1][c], q[0][c + 1], q[1][c + 1], k[i][c], k[i][c + 1]);
+    }
+    if (r0 + 16 < r_end) load_q(r0 + 16);
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, inv[2];
+#pragma unroll
+    for (int i = 0; i < NK; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[i][e] = fmaf(s[i][e], a.c, bias[i][e & 1]);
+        m[e >> 1] = fmaxf(m[e >> 1], s[i][e]);
+      }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      m[h] = fmaxf(m[h], __shfl_xor_sync(0xffffffffu, m[h], 1));
+      m[h] = fmaxf(m[h], __shfl_xor_sync(0xffffffffu, m[h], 2));
+      m[h] = fmaxf(m[h], kXmNone);           // a row without keys: 2^(-inf + 1e30) = 0
+    }
+#pragma unroll
+    for (int i = 0; i < NK; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[i][e] = ex2f(s[i][e] - m[e >> 1]);
+        l[e >> 1] += s[i][e];
+      }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+      inv[h] = l[h] == 0.f ? 0.f : 1.f / l[h];
+    }
+    float o[NR][4];
+#pragma unroll
+    for (int c = 0; c < NR; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NK; i += 2) {
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int x = 0; x < (NK > 1 ? 2 : 1); ++x) {
+        split2<T>(s[i + x][0] * inv[0], s[i + x][1] * inv[0], hi[2 * x], lo[2 * x]);
+        split2<T>(s[i + x][2] * inv[1], s[i + x][3] * inv[1], hi[2 * x + 1], lo[2 * x + 1]);
+      }
+#pragma unroll
+      for (int c = 0; c < NR; ++c) {
+        if constexpr (NK == 1) {
+          Mma<T>::run8(o[c], hi[0], hi[1], v[0][c]);
+          Mma<T>::run8(o[c], lo[0], lo[1], v[0][c]);
+        } else {
+          Mma<T>::run(o[c], hi[0], hi[1], hi[2], hi[3], v[i][c], v[i + 1][c]);
+          Mma<T>::run(o[c], lo[0], lo[1], lo[2], lo[3], v[i][c], v[i + 1][c]);
+        }
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = r0 + h * 8 + g;
+      if (r >= r_end) continue;
+      uint32_t y[NR];
+#pragma unroll
+      for (int c = 0; c < NR; ++c) y[c] = Mma<T>::pack(o[c][2 * h], o[c][2 * h + 1]);
+      store_frag<T, DP>(static_cast<T*>(a.out) + row_offset(a, a.os, b, n, r), t, a.d, y);
+      if (a.lse != nullptr && t == 0) a.lse[stat0 + r] = l[h] == 0.f ? INFINITY : m[h] + log2f(l[h]);
+      if (a.out_f32 != nullptr) {
+        float* f = a.out_f32 + row_dense(a, b, n, r) + t * (DP / 4);
+#pragma unroll
+        for (int c = 0; c < NR; ++c)
+          if (t * (DP / 4) + 2 * c < a.d) *reinterpret_cast<float2*>(f + 2 * c) = make_float2(o[c][2 * h], o[c][2 * h + 1]);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Backward. With p = 2^(c s - lse) and ds = p (dp - D), fp16 needs care: dS has no fixed
+// scale (it follows the loss), so its products run in bf16, which has fp32's range: dS as
+// two bf16 terms, the fp16 factor as two bf16 terms (exact, 11 = 8 + 3 bits), without the
+// product of the two remainders. P lies in [0, 1] and is scaled by 2^12, so that its fp16
+// remainder keeps digits down to 2^-36.
 // ---------------------------------------------------------------------------
 template <class T>
 constexpr bool kIsHalf = false;
 template <>
 constexpr bool kIsHalf<__half> = true;
+template <class T>
+constexpr float kPScale = kIsHalf<T> ? 4096.f : 1.f;
 
-// B operand (tokens as k) of one 16-token tile: turned blocks, as bf16 for the dS products
-template <class T, int NR>
+// Turned blocks of N fragments of 8 tokens (tokens become the k axis), as bf16 for the dS products
+template <class T, int N, int NR>
 struct Turned {
-  uint32_t hi[2][NR], lo[2][kIsHalf<T> ? NR : 1];
-  __device__ __forceinline__ void make(const uint32_t (&x)[2][NR]) {
+  uint32_t hi[N][NR], lo[kIsHalf<T> ? N : 1][kIsHalf<T> ? NR : 1];
+  __device__ __forceinline__ void make(const uint32_t (&x)[N][NR]) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < N; ++h)
 #pragma unroll
       for (int c = 0; c < NR; ++c) {
         if constexpr (kIsHalf<T>) {
@@ -423,22 +759,289 @@ struct Turned {
       }
   }
 };
-template <class T, int NR>
+// acc[c] += (hi + lo)[16 x 16] y[16 x 8 NR], y = tiles y0, y0 + 1
+template <class T, int N, int NR>
 __device__ __forceinline__ void ds_product(float (&acc)[NR][4], const uint32_t (&hi)[4], const uint32_t (&lo)[4],
-                                           const Turned<T, NR>& y) {
+                                           const Turned<T, N, NR>& y, int y0) {
   using B = Mma<__nv_bfloat16>;
 #pragma unroll
   for (int c = 0; c < NR; ++c) {
-    B::run(acc[c], hi[0], hi[1], hi[2], hi[3], y.hi[0][c], y.hi[1][c]);
-    B::run(acc[c], lo[0], lo[1], lo[2], lo[3], y.hi[0][c], y.hi[1][c]);
-    if constexpr (kIsHalf<T>) B::run(acc[c], hi[0], hi[1], hi[2], hi[3], y.lo[0][c], y.lo[1][c]);
+    B::run(acc[c], hi[0], hi[1], hi[2], hi[3], y.hi[y0][c], y.hi[y0 + 1][c]);
+    B::run(acc[c], lo[0], lo[1], lo[2], lo[3], y.hi[y0][c], y.hi[y0 + 1][c]);
+    if constexpr (kIsHalf<T>) B::run(acc[c], hi[0], hi[1], hi[2], hi[3], y.lo[y0][c], y.lo[y0 + 1][c]);
   }
 }
 
-template <class T, int DP, int M, bool OWN_ROWS, bool FUSED>
-__global__ void __launch_bounds__(kXmThreads) xattn_bwd_mma(const XAttn a, int) {
+// Sum over a row's channels of dout * out (fp32), for the row of this lane's fragment; all t lanes get it.
+template <class T, int DP>
+__device__ __forceinline__ float row_delta(const float* o32, const uint32_t (&x)[DP / 8], int t, int d, bool ok) {
+  float f = 0.f;
+  if (ok) {
+#pragma unroll
+    for (int c = 0; c < DP / 8; ++c) {
+      if (t * (DP / 4) + 2 * c >= d) break;
+      const float2 o = __ldg(reinterpret_cast<const float2*>(o32 + t * (DP / 4) + 2 * c)), y = Mma<T>::unpack(x[c]);
+      f = fmaf(o.x, y.x, f);
+      f = fmaf(o.y, y.y, f);
+    }
+  }
+  f += __shfl_xor_sync(0xffffffffu, f, 1);
+  return f + __shfl_xor_sync(0xffffffffu, f, 2);
+}
+
+// One short side: its 8 NF entries ("few") are all of it, the columns of every tile, and stay in
+// registers with their gradient sums; warps and cluster share the long side, 16 entries at a time,
+// whose gradients are complete at once and leave at once. One pass over all inputs.
+//   few = query rows (FEW_ROWS): x = k, v;  y = q, dout.  dk = ds y1, dv = p y2 leave;  dq^T += k^T ds stays
+//   few = keys:                  x = q, dout;  y = k, v.  dq = ds y1 leaves;  dk^T += q^T ds, dv^T += dout^T p stay
+template <class T, int DP, int NF, bool FEW_ROWS>
+__global__ void __launch_bounds__(kXmThreads) xattn_bwd_few(const XAttn a, int) {
+  constexpr int NR = DP / 8, NU = NR / 2;
+  constexpr float kP = kPScale<T>;
+  using B16 = Mma<__nv_bfloat16>;
+  extern __shared__ __align__(16) float xsm[];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+  const int b = blockIdx.z, n = blockIdx.y;
+  const int cl = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
+  const int rows = a.group * a.Tq, keys = xattn_keys(a, b);
+  const T* qb = static_cast<const T*>(a.q);
+  const T* ob = static_cast<const T*>(a.dout);
+  const T* kb = static_cast<const T*>(a.k) + b * a.ks[0] + n * a.ks[2];
+  const T* vb = static_cast<const T*>(a.v) + b * a.vs[0] + n * a.vs[2];
+  const uint8_t* mask = a.key_mask == nullptr ? nullptr : a.key_mask + static_cast<int64_t>(b) * a.Tk;
+  const int64_t stat0 = (static_cast<int64_t>(b) * a.heads + n * a.group) * a.Tq;
+  auto key_ok = [&](int j) { return j < keys && (mask == nullptr || __ldg(mask + j) != 0); };
+  auto load_row = [&](int r, int end, uint32_t(&x1)[NR], uint32_t(&x2)[NR]) {
+    const int rr = min(r, rows - 1);
+    load_frag<T, DP>(qb + row_offset(a, a.qs, b, n, rr), t, a.d, r < end, x1);
+    load_frag<T, DP>(ob + row_offset(a, a.os, b, n, rr), t, a.d, r < end, x2);
+  };
+  auto load_key = [&](int j, bool ok, uint32_t(&x1)[NR], uint32_t(&x2)[NR]) {
+    load_frag<T, DP>(kb + j * a.ks[1], t, a.d, ok, x1);
+    load_frag<T, DP>(vb + j * a.vs[1], t, a.d, ok, x2);
+  };
+
+  // few = rows: every key's gradient is written, the zeros of those that are not there too
+  const int total = FEW_ROWS ? a.Tk : rows;
+  const int steps = (total + 15) / 16, ns = kXmWarps * cl, per = (steps + ns - 1) / ns * 16;
+  const int begin = min(total, (rank * kXmWarps + warp) * per), end = min(total, begin + per);
+  uint32_t x1[2][NR], x2[2][NR];
+  float xs[2], xd[2];                        // long keys: bias of the key; long rows: lse (and D, found below)
+  auto load_long = [&](int i0) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int i = i0 + h * 8 + g;
+      if constexpr (FEW_ROWS) {
+        const bool ok = i < end && key_ok(i);
+        load_key(i, ok, x1[h], x2[h]);
+        xs[h] = ok ? 0.f : -INFINITY;
+      } else {
+        load_row(i, end, x1[h], x2[h]);
+        xs[h] = i < end ? __ldg(a.lse + stat0 + i) : INFINITY;
+      }
+    }
+  };
+  load_long(begin);
+
+  uint32_t y1[NF][NR], y2[NF][NR];
+  float fs[NF][2], fd[NF][2];                // of few entries 8 i + 2t + e: lse and D of rows; bias of keys
+#pragma unroll
+  for (int i = 0; i < NF; ++i) {
+    const int f = i * 8 + g;
+    float mine, del = 0.f;
+    if constexpr (FEW_ROWS) {
+      load_row(f, rows, y1[i], y2[i]);
+      mine = f < rows ? __ldg(a.lse + stat0 + f) : INFINITY;
+      del = row_delta<T, DP>(a.out_f32 + row_dense(a, b, n, min(f, rows - 1)), y2[i], t, a.d, f < rows);
+    } else {
+      const bool ok = key_ok(f);
+      load_key(f, ok, y1[i], y2[i]);
+      mine = ok ? 0.f : -INFINITY;
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      fs[i][e] = __shfl_sync(0xffffffffu, mine, 8 * t + 4 * e);
+      fd[i][e] = __shfl_sync(0xffffffffu, del, 8 * t + 4 * e);
+    }
+  }
+  Turned<T, NF, NR> y1t;
+  y1t.make(y1);
+  uint32_t y2t[FEW_ROWS ? NF : 1][NR];
+  float acc1[NF][NU][4], acc2[FEW_ROWS ? 1 : NF][NU][4];
+#pragma unroll
+  for (int i = 0; i < NF; ++i) {
+    if constexpr (FEW_ROWS) {
+#pragma unroll
+      for (int c = 0; c < NR; ++c) y2t[i][c] = movm(y2[i][c]);
+    }
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        acc1[i][u][e] = 0.f;
+        if constexpr (!FEW_ROWS) acc2[i][u][e] = 0.f;
+      }
+  }
+
+  for (int i0 = begin; i0 < end; i0 += 16) {
+    float p[NF][4], ds[NF][4];
+#pragma unroll
+    for (int i = 0; i < NF; ++i) {
+      float s[4] = {0.f, 0.f, 0.f, 0.f};
+      ds[i][0] = ds[i][1] = ds[i][2] = ds[i][3] = 0.f;
+#pragma unroll
+      for (int c = 0; c < NR; c += 2) {
+        Mma<T>::run(s, x1[0][c], x1[1][c], x1[0][c + 1], x1[1][c + 1], y1[i][c], y1[i][c + 1]);
+        Mma<T>::run(ds[i], x2[0][c], x2[1][c], x2[0][c + 1], x2[1][c + 1], y2[i][c], y2[i][c + 1]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        p[i][e] = ex2f(fmaf(s[e], a.c, FEW_ROWS ? xs[e >> 1] : fs[i][e & 1]) - (FEW_ROWS ? fs[i][e & 1] : xs[e >> 1]));
+    }
+    if constexpr (!FEW_ROWS) {
+      // all keys are here: D from p and dp themselves, so that a query with one key has dS = 0 exactly
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float f = 0.f;
+#pragma unroll
+        for (int i = 0; i < NF; ++i) f = fmaf(p[i][2 * h], ds[i][2 * h], fmaf(p[i][2 * h + 1], ds[i][2 * h + 1], f));
+        f += __shfl_xor_sync(0xffffffffu, f, 1);
+        xd[h] = f + __shfl_xor_sync(0xffffffffu, f, 2);
+      }
+    }
+    Turned<T, 2, NR> x1t;
+    x1t.make(x1);
+    uint32_t x2t[2][FEW_ROWS ? 1 : NR];
+    if constexpr (!FEW_ROWS) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int c = 0; c < NR; ++c) x2t[h][c] = movm(x2[h][c]);
+    }
+    if (i0 + 16 < end) load_long(i0 + 16);   // the next step's, under this one's arithmetic
+    float e1[NR][4], e2[FEW_ROWS ? NR : 1][4];
+#pragma unroll
+    for (int c = 0; c < NR; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        e1[c][e] = 0.f;
+        if constexpr (FEW_ROWS) e2[c][e] = 0.f;
+      }
+    constexpr int PAIR = NF > 1 ? 2 : 1;
+#pragma unroll
+    for (int i = 0; i < NF; i += PAIR) {
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int x = 0; x < PAIR; ++x) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ds[i + x][e] = p[i + x][e] * (ds[i + x][e] - (FEW_ROWS ? fd[i + x][e & 1] : xd[e >> 1]));
+        split2<__nv_bfloat16>(ds[i + x][0], ds[i + x][1], hi[2 * x], lo[2 * x]);
+        split2<__nv_bfloat16>(ds[i + x][2], ds[i + x][3], hi[2 * x + 1], lo[2 * x + 1]);
+        const uint32_t h0 = movm(hi[2 * x]), h1 = movm(hi[2 * x + 1]), l0 = movm(lo[2 * x]), l1 = movm(lo[2 * x + 1]);
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+          float(&c)[4] = acc1[i + x][u];
+          B16::run(c, x1t.hi[0][2 * u], x1t.hi[0][2 * u + 1], x1t.hi[1][2 * u], x1t.hi[1][2 * u + 1], h0, h1);
+          B16::run(c, x1t.hi[0][2 * u], x1t.hi[0][2 * u + 1], x1t.hi[1][2 * u], x1t.hi[1][2 * u + 1], l0, l1);
+          if constexpr (kIsHalf<T>)
+            B16::run(c, x1t.lo[0][2 * u], x1t.lo[0][2 * u + 1], x1t.lo[1][2 * u], x1t.lo[1][2 * u + 1], h0, h1);
+        }
+      }
+      if constexpr (PAIR == 2) {
+        ds_product<T, NF, NR>(e1, hi, lo, y1t, i);
+      } else {
+#pragma unroll
+        for (int c = 0; c < NR; ++c) {
+          B16::run8(e1[c], hi[0], hi[1], y1t.hi[0][c]);
+          B16::run8(e1[c], lo[0], lo[1], y1t.hi[0][c]);
+          if constexpr (kIsHalf<T>) B16::run8(e1[c], hi[0], hi[1], y1t.lo[0][c]);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < PAIR; ++x) {
+        split2<T>(p[i + x][0] * kP, p[i + x][1] * kP, hi[2 * x], lo[2 * x]);
+        split2<T>(p[i + x][2] * kP, p[i + x][3] * kP, hi[2 * x + 1], lo[2 * x + 1]);
+        if constexpr (!FEW_ROWS) {
+          const uint32_t h0 = movm(hi[2 * x]), h1 = movm(hi[2 * x + 1]), l0 = movm(lo[2 * x]), l1 = movm(lo[2 * x + 1]);
+#pragma unroll
+          for (int u = 0; u < NU; ++u) {
+            float(&c)[4] = acc2[i + x][u];
+            Mma<T>::run(c, x2t[0][2 * u], x2t[0][2 * u + 1], x2t[1][2 * u], x2t[1][2 * u + 1], h0, h1);
+            Mma<T>::run(c, x2t[0][2 * u], x2t[0][2 * u + 1], x2t[1][2 * u], x2t[1][2 * u + 1], l0, l1);
+          }
+        }
+      }
+      if constexpr (FEW_ROWS) {
+#pragma unroll
+        for (int c = 0; c < NR; ++c) {
+          if constexpr (PAIR == 2) {
+            Mma<T>::run(e2[c], hi[0], hi[1], hi[2], hi[3], y2t[i][c], y2t[i + 1][c]);
+            Mma<T>::run(e2[c], lo[0], lo[1], lo[2], lo[3], y2t[i][c], y2t[i + 1][c]);
+          } else {
+            Mma<T>::run8(e2[c], hi[0], hi[1], y2t[0][c]);
+            Mma<T>::run8(e2[c], lo[0], lo[1], y2t[0][c]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int i = i0 + h * 8 + g;
+      if (i >= end) continue;
+      uint32_t y[NR];
+#pragma unroll
+      for (int c = 0; c < NR; ++c) y[c] = Mma<T>::pack(e1[c][2 * h] * a.scale, e1[c][2 * h + 1] * a.scale);
+      if constexpr (FEW_ROWS) {
+        if (a.dk != nullptr) {
+          const int64_t to = ((static_cast<int64_t>(b) * a.Tk + i) * a.kv_heads + n) * a.d;
+          store_frag<T, DP>(static_cast<T*>(a.dk) + to, t, a.d, y);
+#pragma unroll
+          for (int c = 0; c < NR; ++c) y[c] = Mma<T>::pack(e2[c][2 * h] * (1.f / kP), e2[c][2 * h + 1] * (1.f / kP));
+          store_frag<T, DP>(static_cast<T*>(a.dv) + to, t, a.d, y);
+        }
+      } else if (a.dq != nullptr) {
+        store_frag<T, DP>(static_cast<T*>(a.dq) + row_dense(a, b, n, i), t, a.d, y);
+      }
+    }
+  }
+
+  // join the few side's sums of the warps and the cluster
+  auto join = [&](float* acc, void* to_v, float factor, bool first) {
+    constexpr int NREG = NF * NU * 4;
+    if (cl > 1 && !first) cluster_sync_all();          // everybody has read the previous sums
+    warp_tree_sum<NREG>(acc, xsm, warp, lane);
+    __syncthreads();
+    if (warp == 0) {
+#pragma unroll
+      for (int i = 0; i < NREG; ++i) xsm[i * 32 + lane] = acc[i];
+    }
+    if (cl > 1) cluster_sync_all(); else __syncthreads();
+    const uint32_t base = smem_u32(xsm) + lane * 4;
+    for (int w = rank * kXmWarps + warp; w < NREG; w += cl * kXmWarps) {
+      const int e = w % 4, u = w / 4 % NU, f = w / 4 / NU * 8 + 2 * t + (e & 1);
+      float x = 0.f;
+      for (int z = 0; z < cl; ++z) x += ld_dsmem(mapa_shared(base, z) + w * 128);
+      const int ch = g / 2 * (DP / 4) + 4 * u + g % 2 + (e & 2);
+      if (f < (FEW_ROWS ? rows : a.Tk) && ch < a.d && to_v != nullptr) {
+        const int64_t to = FEW_ROWS ? row_dense(a, b, n, f) : ((static_cast<int64_t>(b) * a.Tk + f) * a.kv_heads + n) * a.d;
+        store1(static_cast<T*>(to_v) + to + ch, x * factor);
+      }
+    }
+  };
+  join(&acc1[0][0][0], FEW_ROWS ? a.dq : a.dk, a.scale, true);
+  if constexpr (!FEW_ROWS) join(&acc2[0][0][0], a.dv, 1.f / kP, false);
+  if (cl > 1) cluster_sync_all();
+}
+
+// Two long sides, one kernel per side. A warp owns 16 M entries of one (OWN_ROWS: query rows, x = q, dout;
+// else keys, x = k, v) and walks the other 16 entries at a time (y):
+//   own rows:  dq += ds k              own keys:  dk += ds q,  dv += p dout
+// The other side is shared by the block's warps and the cluster. The rows' kernel comes first and
+// leaves D for the keys'.
+template <class T, int DP, int M, bool OWN_ROWS>
+__global__ void __launch_bounds__(kXmThreads) xattn_bwd_long(const XAttn a, int) {
   constexpr int NR = DP / 8;
-  constexpr float kP = kIsHalf<T> ? 4096.f : 1.f;
+  constexpr float kP = kPScale<T>;
   extern __shared__ __align__(16) float xsm[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   const int b = blockIdx.z, n = blockIdx.y;
@@ -464,8 +1067,7 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_mma(const XAttn a, int) 
   };
 
   uint32_t x1[M][2][NR], x2[M][2][NR];
-  float lse_own[M][2], delta_own[M][2];      // own rows
-  bool ok_own[M][2];                         // own keys
+  float own_s[M][2], own_d[M][2];            // own rows: lse, D; own keys: bias
 #pragma unroll
   for (int mt = 0; mt < M; ++mt)
 #pragma unroll
@@ -473,28 +1075,15 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_mma(const XAttn a, int) 
       const int i = own0 + mt * 16 + h * 8 + g;
       if constexpr (OWN_ROWS) {
         load_row(i, x1[mt][h], x2[mt][h]);
-        lse_own[mt][h] = i < rows ? __ldg(a.lse + stat0 + i) : INFINITY;
-        float f = 0.f;
-        if (i < rows) {
-          const float* o32 = a.out_f32 + row_dense(a, b, n, i) + t * (DP / 4);
-#pragma unroll
-          for (int c = 0; c < NR; ++c) {
-            if (t * (DP / 4) + 2 * c >= a.d) break;
-            const float2 o = __ldg(reinterpret_cast<const float2*>(o32 + 2 * c)), x = Mma<T>::unpack(x2[mt][h][c]);
-            f = fmaf(o.x, x.x, f);
-            f = fmaf(o.y, x.y, f);
-          }
-        }
-        f += __shfl_xor_sync(0xffffffffu, f, 1);
-        f += __shfl_xor_sync(0xffffffffu, f, 2);
-        delta_own[mt][h] = f;
-        if (!FUSED && rank == 0 && warp == 0 && t == 0 && i < rows) a.delta[stat0 + i] = f;
+        own_s[mt][h] = i < rows ? __ldg(a.lse + stat0 + i) : INFINITY;
+        own_d[mt][h] = row_delta<T, DP>(a.out_f32 + row_dense(a, b, n, min(i, rows - 1)), x2[mt][h], t, a.d, i < rows);
+        if (rank == 0 && warp == 0 && t == 0 && i < rows) a.delta[stat0 + i] = own_d[mt][h];
       } else {
         load_key(i, x1[mt][h], x2[mt][h]);
-        ok_own[mt][h] = key_ok(i);
+        own_s[mt][h] = key_ok(i) ? 0.f : -INFINITY;
       }
     }
-  if (OWN_ROWS && !FUSED && a.dq == nullptr) return;
+  if (OWN_ROWS && a.dq == nullptr) return;   // only D was wanted
 
   float acc1[M][NR][4];                                // dq or dk
   float acc2[OWN_ROWS ? 1 : M][NR][4];                 // dv
@@ -507,23 +1096,7 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_mma(const XAttn a, int) 
         acc1[mt][c][e] = 0.f;
         if constexpr (!OWN_ROWS) acc2[mt][c][e] = 0.f;
       }
-  Turned<T, NR> x1t[FUSED ? M : 1];
-  uint32_t x2t[FUSED && OWN_ROWS ? M : 1][2][NR];
-  if constexpr (FUSED) {
-#pragma unroll
-    for (int mt = 0; mt < M; ++mt) {
-      x1t[mt].make(x1[mt]);
-      if constexpr (OWN_ROWS) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int c = 0; c < NR; ++c) x2t[mt][h][c] = movm(x2[mt][h][c]);
-      }
-    }
-  }
-
-  // own rows, fused: the zero gradients of the keys behind keys are written too
-  const int total = OWN_ROWS ? (FUSED ? a.Tk : keys) : (FUSED || own0 < keys ? rows : 0);
+  const int total = OWN_ROWS ? keys : (own0 < keys ? rows : 0);
   const int steps = (total + 15) / 16, ns = kXmWarps * cl;
   const int per = (steps + ns - 1) / ns * 16;
   const int begin = min(total, (rank * kXmWarps + warp) * per), end = min(total, begin + per);
@@ -536,21 +1109,20 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_mma(const XAttn a, int) 
       else
         load_row(i0 + h * 8 + g, y1[h], y2[h]);
     }
-    float lse[2][2], delta[2][2];            // of other entries i0 + 8 nt + 2t + e (own keys)
-    bool ok[2][2];                           // (own rows)
+    float ys[2][2], yd[2][2];                // of entries i0 + 8 nt + 2t + e: bias of keys; lse, D of rows
 #pragma unroll
     for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int i = i0 + nt * 8 + 2 * t + e;
         if constexpr (OWN_ROWS) {
-          ok[nt][e] = key_ok(i);
+          ys[nt][e] = key_ok(i) ? 0.f : -INFINITY;
         } else {
-          lse[nt][e] = i < rows ? __ldg(a.lse + stat0 + i) : INFINITY;
-          delta[nt][e] = FUSED || i >= rows ? 0.f : __ldg(a.delta + stat0 + i);
+          ys[nt][e] = i < rows ? __ldg(a.lse + stat0 + i) : INFINITY;
+          yd[nt][e] = i < rows ? __ldg(a.delta + stat0 + i) : 0.f;
         }
       }
-    Turned<T, NR> y1t;
+    Turned<T, 2, NR> y1t;
     uint32_t y2t[OWN_ROWS ? 1 : 2][NR];
     y1t.make(y1);
     if constexpr (!OWN_ROWS) {
@@ -559,116 +1131,40 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_mma(const XAttn a, int) 
 #pragma unroll
         for (int c = 0; c < NR; ++c) y2t[h][c] = movm(y2[h][c]);
     }
-    float p[M][2][4], dp[M][2][4];
 #pragma unroll
-    for (int mt = 0; mt < M; ++mt)
+    for (int mt = 0; mt < M; ++mt) {
+      float p[2][4], ds[2][4];
+      uint32_t hi[4], lo[4];
 #pragma unroll
       for (int nt = 0; nt < 2; ++nt) {
         float s[4] = {0.f, 0.f, 0.f, 0.f};
-        dp[mt][nt][0] = dp[mt][nt][1] = dp[mt][nt][2] = dp[mt][nt][3] = 0.f;
+        ds[nt][0] = ds[nt][1] = ds[nt][2] = ds[nt][3] = 0.f;
 #pragma unroll
         for (int c = 0; c < NR; c += 2) {
           Mma<T>::run(s, x1[mt][0][c], x1[mt][1][c], x1[mt][0][c + 1], x1[mt][1][c + 1], y1[nt][c], y1[nt][c + 1]);
-          Mma<T>::run(dp[mt][nt], x2[mt][0][c], x2[mt][1][c], x2[mt][0][c + 1], x2[mt][1][c + 1], y2[nt][c],
-                      y2[nt][c + 1]);
+          Mma<T>::run(ds[nt], x2[mt][0][c], x2[mt][1][c], x2[mt][0][c + 1], x2[mt][1][c + 1], y2[nt][c], y2[nt][c + 1]);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const bool valid = OWN_ROWS ? ok[nt][e & 1] : ok_own[mt][e >> 1];
-          const float st = OWN_ROWS ? lse_own[mt][e >> 1] : lse[nt][e & 1];
-          p[mt][nt][e] = valid ? ex2f(__fsub_rn(__fmul_rn(s[e], a.c), st)) : 0.f;
+          const float bias = OWN_ROWS ? ys[nt][e & 1] : own_s[mt][e >> 1];
+          const float lse = OWN_ROWS ? own_s[mt][e >> 1] : ys[nt][e & 1];
+          p[nt][e] = ex2f(fmaf(s[e], a.c, bias) - lse);
+          ds[nt][e] = p[nt][e] * (ds[nt][e] - (OWN_ROWS ? own_d[mt][e >> 1] : yd[nt][e & 1]));
         }
-      }
-    if constexpr (!OWN_ROWS && FUSED) {
-      // all keys are here: D from p and dp themselves, so a query with one key has dS = 0 exactly
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float f = 0.f;
-#pragma unroll
-          for (int mt = 0; mt < M; ++mt) {
-            f = fmaf(p[mt][nt][e], dp[mt][nt][e], f);
-            f = fmaf(p[mt][nt][e + 2], dp[mt][nt][e + 2], f);
-          }
-          f += __shfl_xor_sync(0xffffffffu, f, 4);
-          f += __shfl_xor_sync(0xffffffffu, f, 8);
-          f += __shfl_xor_sync(0xffffffffu, f, 16);
-          delta[nt][e] = f;
-        }
-    }
-    float e1[FUSED ? NR : 1][4], e2[FUSED && OWN_ROWS ? NR : 1][4];   // the other side's gradients
-    if constexpr (FUSED) {
-#pragma unroll
-      for (int c = 0; c < NR; ++c)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          e1[c][e] = 0.f;
-          if constexpr (OWN_ROWS) e2[c][e] = 0.f;
-        }
-    }
-#pragma unroll
-    for (int mt = 0; mt < M; ++mt) {
-      uint32_t hi[4], lo[4];
-      float ds[2][4];
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float dl = OWN_ROWS ? delta_own[mt][e >> 1] : delta[nt][e & 1];
-          ds[nt][e] = p[mt][nt][e] * (dp[mt][nt][e] - dl);
-        }
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
         split2<__nv_bfloat16>(ds[nt][0], ds[nt][1], hi[2 * nt], lo[2 * nt]);
         split2<__nv_bfloat16>(ds[nt][2], ds[nt][3], hi[2 * nt + 1], lo[2 * nt + 1]);
       }
-      ds_product<T, NR>(acc1[mt], hi, lo, y1t);
-      if constexpr (FUSED) {
-        const uint32_t th[4] = {movm(hi[0]), movm(hi[2]), movm(hi[1]), movm(hi[3])};
-        const uint32_t tl[4] = {movm(lo[0]), movm(lo[2]), movm(lo[1]), movm(lo[3])};
-        ds_product<T, NR>(e1, th, tl, x1t[mt]);
-      }
-      if constexpr (!OWN_ROWS || FUSED) {
+      ds_product<T, 2, NR>(acc1[mt], hi, lo, y1t, 0);
+      if constexpr (!OWN_ROWS) {
 #pragma unroll
         for (int nt = 0; nt < 2; ++nt) {
-          split2<T>(p[mt][nt][0] * kP, p[mt][nt][1] * kP, hi[2 * nt], lo[2 * nt]);
-          split2<T>(p[mt][nt][2] * kP, p[mt][nt][3] * kP, hi[2 * nt + 1], lo[2 * nt + 1]);
+          split2<T>(p[nt][0] * kP, p[nt][1] * kP, hi[2 * nt], lo[2 * nt]);
+          split2<T>(p[nt][2] * kP, p[nt][3] * kP, hi[2 * nt + 1], lo[2 * nt + 1]);
         }
-        if constexpr (!OWN_ROWS) {
 #pragma unroll
-          for (int c = 0; c < NR; ++c) {
-            Mma<T>::run(acc2[mt][c], hi[0], hi[1], hi[2], hi[3], y2t[0][c], y2t[1][c]);
-            Mma<T>::run(acc2[mt][c], lo[0], lo[1], lo[2], lo[3], y2t[0][c], y2t[1][c]);
-          }
-        } else {
-          const uint32_t th[4] = {movm(hi[0]), movm(hi[2]), movm(hi[1]), movm(hi[3])};
-          const uint32_t tl[4] = {movm(lo[0]), movm(lo[2]), movm(lo[1]), movm(lo[3])};
-#pragma unroll
-          for (int c = 0; c < NR; ++c) {
-            Mma<T>::run(e2[c], th[0], th[1], th[2], th[3], x2t[mt][0][c], x2t[mt][1][c]);
-            Mma<T>::run(e2[c], tl[0], tl[1], tl[2], tl[3], x2t[mt][0][c], x2t[mt][1][c]);
-          }
-        }
-      }
-    }
-    if constexpr (FUSED) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int i = i0 + h * 8 + g;
-        uint32_t y[NR];
-#pragma unroll
-        for (int c = 0; c < NR; ++c) y[c] = Mma<T>::pack(e1[c][2 * h] * a.scale, e1[c][2 * h + 1] * a.scale);
-        if constexpr (OWN_ROWS) {
-          if (i < a.Tk && a.dk != nullptr) {
-            const int64_t to = ((static_cast<int64_t>(b) * a.Tk + i) * a.kv_heads + n) * a.d;
-            store_frag<T, DP>(static_cast<T*>(a.dk) + to, t, a.d, y);
-#pragma unroll
-            for (int c = 0; c < NR; ++c) y[c] = Mma<T>::pack(e2[c][2 * h] * (1.f / kP), e2[c][2 * h + 1] * (1.f / kP));
-            store_frag<T, DP>(static_cast<T*>(a.dv) + to, t, a.d, y);
-          }
-        } else if (i < rows && a.dq != nullptr) {
-          store_frag<T, DP>(static_cast<T*>(a.dq) + row_dense(a, b, n, i), t, a.d, y);
+        for (int c = 0; c < NR; ++c) {
+          Mma<T>::run(acc2[mt][c], hi[0], hi[1], hi[2], hi[3], y2t[0][c], y2t[1][c]);
+          Mma<T>::run(acc2[mt][c], lo[0], lo[1], lo[2], lo[3], y2t[0][c], y2t[1][c]);
         }
       }
     }
@@ -711,12 +1207,12 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_mma(const XAttn a, int) 
 // ---------------------------------------------------------------------------
 // Launch rules
 // ---------------------------------------------------------------------------
-// Owned tiles (of 16) of the fused backward kernels: what fits the register file beside
-// the turned copies.
+// Entries of a short side that stay in registers: 8-entry tiles of the backward kernel (about
+// 6 DP / 8 registers each) and of the forward kernel's keys (2 DP / 8 registers each).
 template <int DP>
-constexpr int kXmFusedRows = DP == 16 ? 4 : DP == 32 ? 2 : DP == 64 ? 1 : 0;
+constexpr int kXmFewTiles = 128 / DP;
 template <int DP>
-constexpr int kXmFusedKeys = DP == 16 ? 4 : DP == 32 ? 2 : DP == 64 ? 1 : 0;
+constexpr int kXmKeyTiles = DP <= 32 ? 8 : 256 / DP;
 
 // Blocks per cluster: enough blocks for two per SM, each warp with at least one step.
 static int xattn_cluster(int64_t blocks, int other, int step) {
@@ -731,7 +1227,7 @@ static int xattn_fwd_mma_launch(const XAttn& a, cudaStream_t stream) {
   const int64_t pairs = static_cast<int64_t>(a.B) * a.kv_heads;
   constexpr int CK = DP <= 32 ? 32 : 16;
   const int64_t whole = pairs * ((tiles + kXmWarps - 1) / kXmWarps);
-  if (a.Tk <= 2 * CK || whole >= 2 * 148)
+  if (a.Tk <= 2 * CK || (tiles >= kXmWarps && whole >= 2 * 148))
     return launch_cluster(xattn_fwd_mma<T, DP, MT>, dim3((tiles + kXmWarps - 1) / kXmWarps, a.kv_heads, a.B),
                           kXmThreads, 0, 1, stream, a, 0);
   const int cl = xattn_cluster(pairs * tiles, a.Tk, CK);
@@ -740,47 +1236,86 @@ static int xattn_fwd_mma_launch(const XAttn& a, cudaStream_t stream) {
                         1);
 }
 
-template <class T, int DP, int M, bool OWN_ROWS, bool FUSED>
-static int xattn_bwd_mma_launch(const XAttn& a, cudaStream_t stream) {
+template <class T, int DP, int NQ>
+static int xattn_few_rows_launch(const XAttn& a, cudaStream_t stream) {
+  const int rows = a.group * a.Tq, tiles = (rows + 8 * NQ - 1) / (8 * NQ);
+  const int cl = xattn_cluster(static_cast<int64_t>(a.B) * a.kv_heads * tiles, a.Tk, DP <= 32 ? 32 : 16);
+  const size_t smem = (kXmWarps * 8 * NQ + 4 * NQ * (DP / 4 + 2) * 32) * sizeof(float);
+  return launch_cluster(xattn_fwd_few_rows<T, DP, NQ>, dim3(tiles * cl, a.kv_heads, a.B), kXmThreads, smem, cl, stream,
+                        a, 0);
+}
+
+template <class T, int DP, int NK>
+static int xattn_few_keys_launch(const XAttn& a, cudaStream_t stream) {
+  const int rows = a.group * a.Tq, tiles = (rows + 15) / 16;
+  const int64_t pairs = static_cast<int64_t>(a.B) * a.kv_heads;
+  // row shares: at least 4 tiles each (the K, V fragments are loaded once per share), about 64 warps per SM
+  const int64_t want = (148 * 64 + pairs - 1) / pairs;
+  const int chunks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, (tiles + 3) / 4)));
+  const int64_t blocks = (pairs * chunks + kXmWarps - 1) / kXmWarps;
+  return launch_cluster(xattn_fwd_few_keys<T, DP, NK>, dim3(static_cast<unsigned>(blocks)), kXmThreads, 0, 1, stream, a,
+                        chunks);
+}
+
+template <class T, int DP, int NF, bool FEW_ROWS>
+static int xattn_bwd_few_launch(const XAttn& a, cudaStream_t stream) {
+  const int cl = xattn_cluster(static_cast<int64_t>(a.B) * a.kv_heads, FEW_ROWS ? a.Tk : a.group * a.Tq, 16);
+  return launch_cluster(xattn_bwd_few<T, DP, NF, FEW_ROWS>, dim3(cl, a.kv_heads, a.B), kXmThreads,
+                        4 * NF * (DP / 4) * 32 * sizeof(float), cl, stream, a, 0);
+}
+// the smallest instance that holds `few` entries
+template <class T, int DP, bool FEW_ROWS>
+static int xattn_bwd_few_pick(const XAttn& a, int few, cudaStream_t stream) {
+  if constexpr (kXmFewTiles<DP> >= 8) {
+    if (few > 32) return xattn_bwd_few_launch<T, DP, 8, FEW_ROWS>(a, stream);
+  }
+  if constexpr (kXmFewTiles<DP> >= 4) {
+    if (few > 16) return xattn_bwd_few_launch<T, DP, 4, FEW_ROWS>(a, stream);
+  }
+  if constexpr (kXmFewTiles<DP> >= 2) {
+    if (few > 8) return xattn_bwd_few_launch<T, DP, 2, FEW_ROWS>(a, stream);
+  }
+  return xattn_bwd_few_launch<T, DP, 1, FEW_ROWS>(a, stream);
+}
+
+template <class T, int DP, int M, bool OWN_ROWS>
+static int xattn_bwd_long_launch(const XAttn& a, cudaStream_t stream) {
   const int rows = a.group * a.Tq, own = OWN_ROWS ? rows : a.Tk, other = OWN_ROWS ? a.Tk : rows;
   const int tiles = (own + 16 * M - 1) / (16 * M);
   const int cl = xattn_cluster(static_cast<int64_t>(a.B) * a.kv_heads * tiles, other, 16);
   const size_t smem = 4 * M * (DP / 2) * 32 * sizeof(float);
-  return launch_cluster(xattn_bwd_mma<T, DP, M, OWN_ROWS, FUSED>, dim3(tiles * cl, a.kv_heads, a.B), kXmThreads, smem,
-                        cl, stream, a, 0);
+  return launch_cluster(xattn_bwd_long<T, DP, M, OWN_ROWS>, dim3(tiles * cl, a.kv_heads, a.B), kXmThreads, smem, cl,
+                        stream, a, 0);
 }
 
 template <class T, int DP>
 static int xattn_mma_dp(const XAttn& a, bool backward, cudaStream_t stream) {
   const int rows = a.group * a.Tq;
   if (!backward) {
-    if constexpr (DP <= 64) {
-      if (rows > 16) return xattn_fwd_mma_launch<T, DP, 2>(a, stream);
+    if (a.Tk <= 8) return xattn_few_keys_launch<T, DP, 1>(a, stream);
+    if (a.Tk <= 16) return xattn_few_keys_launch<T, DP, 2>(a, stream);
+    if constexpr (kXmKeyTiles<DP> >= 4) {
+      if (a.Tk <= 32) return xattn_few_keys_launch<T, DP, 4>(a, stream);
     }
-    return xattn_fwd_mma_launch<T, DP, 1>(a, stream);
+    if constexpr (kXmKeyTiles<DP> >= 8) {
+      if (a.Tk <= 64) return xattn_few_keys_launch<T, DP, 8>(a, stream);
+    }
+    if (rows <= 8) return xattn_few_rows_launch<T, DP, 1>(a, stream);
+    if (rows <= 16) return xattn_few_rows_launch<T, DP, 2>(a, stream);
+    if constexpr (DP <= 64) {
+      if (rows <= 24 || (rows > 32 && rows <= 48)) return xattn_few_rows_launch<T, DP, 3>(a, stream);
+      if (rows <= 64) return xattn_few_rows_launch<T, DP, 4>(a, stream);
+      return xattn_fwd_mma_launch<T, DP, 2>(a, stream);
+    } else {
+      return xattn_fwd_mma_launch<T, DP, 1>(a, stream);
+    }
   }
-  if constexpr (kXmFusedKeys<DP> >= 1) {
-    if (a.Tk <= 16) return xattn_bwd_mma_launch<T, DP, 1, false, true>(a, stream);
-  }
-  if constexpr (kXmFusedKeys<DP> >= 2) {
-    if (a.Tk <= 32) return xattn_bwd_mma_launch<T, DP, 2, false, true>(a, stream);
-  }
-  if constexpr (kXmFusedKeys<DP> >= 4) {
-    if (a.Tk <= 64) return xattn_bwd_mma_launch<T, DP, 4, false, true>(a, stream);
-  }
-  if constexpr (kXmFusedRows<DP> >= 1) {
-    if (rows <= 16) return xattn_bwd_mma_launch<T, DP, 1, true, true>(a, stream);
-  }
-  if constexpr (kXmFusedRows<DP> >= 2) {
-    if (rows <= 32) return xattn_bwd_mma_launch<T, DP, 2, true, true>(a, stream);
-  }
-  if constexpr (kXmFusedRows<DP> >= 4) {
-    if (rows <= 64) return xattn_bwd_mma_launch<T, DP, 4, true, true>(a, stream);
-  }
+  if (a.Tk <= 8 * kXmFewTiles<DP>) return xattn_bwd_few_pick<T, DP, false>(a, a.Tk, stream);
+  if (rows <= 8 * kXmFewTiles<DP>) return xattn_bwd_few_pick<T, DP, true>(a, rows, stream);
   constexpr int M = DP <= 32 ? 2 : 1;
-  const int st = xattn_bwd_mma_launch<T, DP, M, true, false>(a, stream);
+  const int st = xattn_bwd_long_launch<T, DP, M, true>(a, stream);
   if (st != SSAM_OK || a.dk == nullptr) return st;
-  return xattn_bwd_mma_launch<T, DP, M, false, false>(a, stream);
+  return xattn_bwd_long_launch<T, DP, M, false>(a, stream);
 }
 
 template <class T>
@@ -791,11 +1326,10 @@ static int xattn_mma(const XAttn& a, bool backward, cudaStream_t stream) {
   return xattn_mma_dp<T, 128>(a, backward, stream);
 }
 
-// Whether the backward pass reads out_f32 (else D comes from P and dP, see above).
+// Whether the backward pass reads out_f32 (else D comes from P and dP, see xattn_bwd_few).
 static bool xattn_uses_out_f32(int Tk, int d, int dtype) {
-  const int most = dtype == 2 ? 0 : d <= 16 ? 16 * kXmFusedKeys<16> : d <= 32 ? 16 * kXmFusedKeys<32>
-                                  : d <= 64 ? 16 * kXmFusedKeys<64> : 0;
-  return Tk > most;
+  const int dp = d <= 16 ? 16 : d <= 32 ? 32 : d <= 64 ? 64 : 128;
+  return dtype == 2 || Tk > 8 * (128 / dp);
 }
 
 }  // namespace ssam

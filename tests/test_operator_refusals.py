@@ -40,7 +40,7 @@ def test_cross_attention_abi():
     assert bwd(delta=None) == INV and bwd(dk=None) == INV and bwd(dv=None) == INV
     assert bwd(dout=8) == ALIGN and bwd(dq=8) == ALIGN and bwd(d=20) == UNSUP and bwd(st=strides(4)) == ALIGN
     uses = _lib.load().ssam_cross_attn_bwd_uses_out_f32
-    assert uses(64, 16, 0) == 0 and uses(65, 16, 1) == 1 and uses(1, 16, 2) == 1 and uses(1, 72, 0) == 1
+    assert uses(64, 16, 0) == 0 and uses(65, 16, 1) == 1 and uses(1, 16, 2) == 1 and uses(9, 72, 0) == 1 and uses(8, 128, 1) == 0
     assert bwd(dq=None, dk=None, dv=None) == 0          # nothing asked for: nothing launched
 
 
