@@ -314,11 +314,11 @@ int ssam_layernorm_gelu_half_bwd(const void* x, const void* dout, int64_t rows, 
  * dx may be dout. x, w, b, out, dout, dx and workspace are 16-byte aligned; C is a
  * multiple of 8 (fp32: 4) and of groups, at most 2048 (fp32: 1024), N at most 65535
  * (SSAM_ERR_UNSUPPORTED otherwise). workspace: ssam_groupnorm_act_workspace_size()
- * bytes (backward 0 / 1). Sums are taken in a fixed order: equal calls give equal bits.
+ * bytes (backward 0 / 1; 0 bytes: workspace may be NULL). Sums are taken in a fixed order: equal calls give equal bits.
  * No counterpart in the reference: the norm of the segmentation heads that follow
  * the SAM3 encoder (convolution -> GroupNorm -> ReLU).
  * ------------------------------------------------------------------------- */
-size_t ssam_groupnorm_act_workspace_size(int N, int64_t HW, int C, int groups, int backward);
+size_t ssam_groupnorm_act_workspace_size(int N, int64_t HW, int C, int groups, int dtype, int backward);
 int ssam_groupnorm_act_fwd(const void* x, int N, int64_t HW, int C, int groups, const void* w, const void* b, float eps,
                            int act, int dtype, void* out, float* mean, float* rstd, void* workspace,
                            size_t workspace_bytes, void* stream);

@@ -58,7 +58,7 @@ SIGNATURES: dict[str, tuple] = {
     "ssam_layernorm_gelu_half_bwd_workspace_size": (c_size, [c_i64, c_int]),
     "ssam_layernorm_gelu_half_bwd": (c_int, [c_ptr, c_ptr, c_i64, c_int, c_ptr, c_ptr, c_f32, c_int, c_int, c_ptr,
                                              c_ptr, c_ptr, c_ptr, c_size, c_ptr]),
-    "ssam_groupnorm_act_workspace_size": (c_size, [c_int, c_i64, c_int, c_int, c_int]),
+    "ssam_groupnorm_act_workspace_size": (c_size, [c_int, c_i64, c_int, c_int, c_int, c_int]),
     "ssam_groupnorm_act_fwd": (c_int, [c_ptr, c_int, c_i64, c_int, c_int, c_ptr, c_ptr, c_f32, c_int, c_int, c_ptr,
                                        c_ptr, c_ptr, c_ptr, c_size, c_ptr]),
     "ssam_groupnorm_act_bwd": (c_int, [c_ptr, c_ptr, c_int, c_i64, c_int, c_int, c_ptr, c_ptr, c_ptr, c_ptr, c_int,

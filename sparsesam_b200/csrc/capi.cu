@@ -187,8 +187,8 @@ int ssam_layernorm_gelu_half_bwd(const void* x, const void* dout, int64_t rows, 
                                   static_cast<cudaStream_t>(stream));
 }
 
-size_t ssam_groupnorm_act_workspace_size(int N, int64_t HW, int C, int groups, int backward) {
-  return ssam::groupnorm_workspace_size(N, HW, C, groups, backward);
+size_t ssam_groupnorm_act_workspace_size(int N, int64_t HW, int C, int groups, int dtype, int backward) {
+  return ssam::groupnorm_workspace_size(N, HW, C, groups, dtype, backward);
 }
 
 int ssam_groupnorm_act_fwd(const void* x, int N, int64_t HW, int C, int groups, const void* w, const void* b, float eps,

@@ -110,7 +110,7 @@ int cross_attn_bwd(const void* q, const void* k, const void* v, const void* dout
                    int Tk, int heads, int kv_heads, int d, int dtype, float scale, const int32_t* key_lens,
                    const uint8_t* key_mask, const float* out_f32, const float* lse, float* delta, void* dq, void* dk,
                    void* dv, cudaStream_t stream);
-size_t groupnorm_workspace_size(int N, int64_t HW, int C, int groups, int backward);
+size_t groupnorm_workspace_size(int N, int64_t HW, int C, int groups, int dtype, int backward);
 int groupnorm_act_fwd(const void* x, int N, int64_t HW, int C, int groups, const void* w, const void* b, float eps,
                       int act, int dtype, void* out, float* mean, float* rstd, void* workspace, size_t workspace_bytes,
                       cudaStream_t stream);

@@ -553,12 +553,12 @@ def _groupnorm_act(x, groups, w, b, eps, act, stats):
         return out, None
     HW = x.numel() // (N * C)
     st = torch.empty(2, N, groups, dtype=torch.float32, device=x.device) if stats else None
-    n = _lib.load().ssam_groupnorm_act_workspace_size(N, HW, C, groups, 0)
-    ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+    n = _lib.load().ssam_groupnorm_act_workspace_size(N, HW, C, groups, _DTYPES[x.dtype], 0)
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
     with _on(x):
         _lib.call("ssam_groupnorm_act_fwd", x.data_ptr(), N, HW, C, groups, w.data_ptr(), b.data_ptr(), eps, act,
                   _DTYPES[x.dtype], out.data_ptr(), st[0].data_ptr() if stats else None,
-                  st[1].data_ptr() if stats else None, ws.data_ptr(), n, _stream(x))
+                  st[1].data_ptr() if stats else None, _ptr(ws), n, _stream(x))
     return out, st
 
 
@@ -580,7 +580,7 @@ class _GroupNormAct(torch.autograd.Function):
         HW = x.numel() // (N * C)
         dout = _dense(dout)
         dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty_like(b)
-        n = _lib.load().ssam_groupnorm_act_workspace_size(N, HW, C, ctx.groups, 1)
+        n = _lib.load().ssam_groupnorm_act_workspace_size(N, HW, C, ctx.groups, _DTYPES[x.dtype], 1)
         ws = torch.empty(n, dtype=torch.uint8, device=x.device)
         with _on(x):
             _lib.call("ssam_groupnorm_act_bwd", x.data_ptr(), dout.data_ptr(), N, HW, C, ctx.groups, w.data_ptr(),

@@ -56,9 +56,12 @@ def test_groupnorm_abi():
     assert gn(C=16, G=3) == INV and gn(act=4) == INV and gn(dtype=3) == INV
     assert gn(C=12, G=2) == UNSUP and gn(C=2056, G=1) == UNSUP and gn(C=1028, G=1, dtype=2) == UNSUP
     assert gn(N=65536) == UNSUP
-    assert gn(ws=None) == INV and gn(n=lib.ssam_groupnorm_act_workspace_size(1, 4, 16, 2, 0) - 1) == INV
+    big = dict(HW=1 << 22, C=64)                # too large for one cluster: the chunks' moments need a workspace
+    need = lib.ssam_groupnorm_act_workspace_size(1, 1 << 22, 64, 2, 0, 0)
+    assert need > 0 and lib.ssam_groupnorm_act_workspace_size(1, 4, 16, 2, 0, 0) == 0
+    assert gn(ws=None, **big) == INV and gn(n=need - 1, **big) == INV
     assert gn(x=8) == ALIGN and gn(out=8) == ALIGN and gn(ws=8) == ALIGN
-    assert lib.ssam_groupnorm_act_workspace_size(0, 4, 16, 2, 0) == 0
+    assert lib.ssam_groupnorm_act_workspace_size(0, 4, 16, 2, 0, 0) == 0
     args = [16, 16, 1, 4, 16, 2, 16, 16, 16, 16, 0, 0, 16, 16, 16, 16, 1 << 20, None]
     for i in (0, 1, 6, 7, 8, 9, 12, 13, 14, 15):
         assert lib.ssam_groupnorm_act_bwd(*args[:i], None, *args[i + 1:]) == INV
