@@ -27,91 +27,180 @@ enum { kActNone = 0, kActRelu = 1, kActGelu = 2, kActSilu = 3 };
 // exponential of erf is the one of GELU's slope) and the approximate exponential and
 // division: a thousandth of the output's rounding, and 2 to 3 times fewer instructions,
 // which is what bounded these kernels (GELU apply of 16 x 256 x 256 x 64: 108 us exact).
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 1 / (1 + p u) of a pair from one reciprocal of the product (both factors are at least 1): the
+// reciprocals and exponentials (MUFU, a quarter of the FMA rate) are what GELU waits for.
+__device__ __forceinline__ float2 erf_t2(float2 u) {
+  const float2 d = fma2(both(0.3275911f), u, both(1.0f));
+  const float r = rcp_approx(d.x * d.y);
+  return mul2(both(r), make_float2(d.y, d.x));
+}
+// h = q / 2 of 7.1.26 without its exponential, e = exp(-u^2)
+__device__ __forceinline__ void erf_terms2(float2 z, float2& u, float2& h, float2& e) {
+  u = mul2(make_float2(fabsf(z.x), fabsf(z.y)), both(0.70710678118654752440f));
+  const float2 t = erf_t2(u);
+  h = fma2(both(0.5307027145f), t, both(-0.7265760135f));
+  h = fma2(h, t, both(0.7107068705f));
+  h = fma2(h, t, both(-0.142248368f));
+  h = fma2(h, t, both(0.127414796f));
+  h = mul2(h, t);
+  const float2 arg = mul2(mul2(u, u), both(-1.4426950408889634f));
+  e = make_float2(ex2f(arg.x), ex2f(arg.y));
+}
+// GELU(z) = max(z, 0) - |z| h e
+__device__ __forceinline__ float2 gelu2(float2 z) {
+  float2 u, h, e;
+  erf_terms2(z, u, h, e);
+  return fma2(mul2(u, both(-1.41421356237309504880f)), mul2(h, e), make_float2(fmaxf(z.x, 0.f), fmaxf(z.y, 0.f)));
+}
+// GELU'(z) = Phi(z) + z phi(z), Phi = 1/2 + sign(z) (1/2 - h e)
+__device__ __forceinline__ float2 gelu_slope2(float2 z) {
+  float2 u, h, e;
+  erf_terms2(z, u, h, e);
+  const float2 half = fma2(h, make_float2(-e.x, -e.y), both(0.5f));
+  const float2 phi = make_float2(copysignf(half.x, z.x), copysignf(half.y, z.y));
+  return add2(fma2(mul2(z, both(0.39894228040143267794f)), e, phi), both(0.5f));
+}
 template <int ACT, bool EXACT>
-__device__ __forceinline__ float act_value(float z) {
-  if (ACT == kActRelu) return z < 0.f ? 0.f : z;  // NaN stays NaN
-  if (ACT == kActGelu) return EXACT ? 0.5f * z * (1.f + erff(z * 0.70710678118654752440f)) : gelu_exact(z);
-  if (ACT == kActSilu) return EXACT ? z / (1.f + expf(-z)) : __fdividef(z, 1.f + __expf(-z));
+__device__ __forceinline__ float2 act_value(float2 z) {
+  if constexpr (ACT == kActRelu) return make_float2(z.x < 0.f ? 0.f : z.x, z.y < 0.f ? 0.f : z.y);  // NaN stays NaN
+  if constexpr (ACT == kActGelu) {
+    if constexpr (!EXACT) return gelu2(z);
+    return make_float2(0.5f * z.x * (1.f + erff(z.x * 0.70710678118654752440f)),
+                       0.5f * z.y * (1.f + erff(z.y * 0.70710678118654752440f)));
+  }
+  if constexpr (ACT == kActSilu) {
+    if constexpr (EXACT) return make_float2(z.x / (1.f + expf(-z.x)), z.y / (1.f + expf(-z.y)));
+    return make_float2(__fdividef(z.x, 1.f + __expf(-z.x)), __fdividef(z.y, 1.f + __expf(-z.y)));
+  }
   return z;
 }
-// GELU'(z) = Phi(z) + z phi(z); with u = |z| / sqrt 2 and q the polynomial part of 7.1.26,
-// Phi = 1/2 + sign(z) (1/2 - q exp(-u^2) / 2).
-__device__ __forceinline__ float gelu_slope_fast(float z) {
-  const float u = fabsf(z) * 0.70710678118654752440f;
-  float t, e;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(0.3275911f, u, 1.0f)));
-  const float half_q =
-      fmaf(fmaf(fmaf(fmaf(0.5307027145f, t, -0.7265760135f), t, 0.7107068705f), t, -0.142248368f), t, 0.127414796f) * t;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(u * u * -1.4426950408889634f));
-  const float tail = half_q * e;
-  return fmaf(z * 0.39894228040143267794f, e, z >= 0.f ? 1.f - tail : tail);
+template <bool EXACT>
+__device__ __forceinline__ float silu_slope(float z) {
+  const float s = EXACT ? 1.f / (1.f + expf(-z)) : rcp_approx(1.f + __expf(-z));
+  return s * (1.f + z * (1.f - s));
+}
+__device__ __forceinline__ float gelu_slope_exact(float z) {
+  return 0.5f * (1.f + erff(z * 0.70710678118654752440f)) + z * expf(-0.5f * z * z) * 0.39894228040143267794f;
 }
 template <int ACT, bool EXACT>
-__device__ __forceinline__ float act_slope(float z) {
-  if (ACT == kActRelu) return z > 0.f ? 1.f : 0.f;
-  if (ACT == kActGelu)
-    return EXACT ? 0.5f * (1.f + erff(z * 0.70710678118654752440f)) + z * expf(-0.5f * z * z) * 0.39894228040143267794f
-                 : gelu_slope_fast(z);
-  if (ACT == kActSilu) {
-    const float s = EXACT ? 1.f / (1.f + expf(-z)) : __fdividef(1.f, 1.f + __expf(-z));
-    return s * (1.f + z * (1.f - s));
+__device__ __forceinline__ float2 act_slope(float2 z) {
+  if constexpr (ACT == kActRelu) return make_float2(z.x > 0.f ? 1.f : 0.f, z.y > 0.f ? 1.f : 0.f);
+  if constexpr (ACT == kActGelu) {
+    if constexpr (EXACT) return make_float2(gelu_slope_exact(z.x), gelu_slope_exact(z.y));
+    return gelu_slope2(z);
   }
-  return 1.f;
+  if constexpr (ACT == kActSilu) return make_float2(silu_slope<EXACT>(z.x), silu_slope<EXACT>(z.y));
+  return both(1.f);
 }
 
-// V consecutive channels (16 bytes) of a row as floats.
+// V consecutive channels (16 bytes) of a row as V / 2 pairs of floats.
 template <class T>
 struct Vec;
 template <>
 struct Vec<float> {
   static constexpr int V = 4;
   static constexpr bool exact = true;
-  static __device__ __forceinline__ void load(const float* p, float (&f)[4]) {
-    const float4 v = *reinterpret_cast<const float4*>(p);
-    f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
+  static __device__ __forceinline__ void unpack(const uint4& u, float2 (&f)[2]) {
+    f[0] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+    f[1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
   }
-  static __device__ __forceinline__ void store(float* p, const float (&f)[4]) {
-    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+  static __device__ __forceinline__ uint4 pack(const float2 (&f)[2]) {
+    return make_uint4(__float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x), __float_as_uint(f[1].y));
   }
 };
 template <>
 struct Vec<__half> {
   static constexpr int V = 8;
   static constexpr bool exact = false;
-  static __device__ __forceinline__ void load(const __half* p, float (&f)[8]) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
+  static __device__ __forceinline__ void unpack(const uint4& u, float2 (&f)[4]) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      f[2 * i] = v.x, f[2 * i + 1] = v.y;
-    }
+    for (int i = 0; i < 4; ++i) f[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
   }
-  static __device__ __forceinline__ void store(__half* p, const float (&f)[8]) {
+  static __device__ __forceinline__ uint4 pack(const float2 (&f)[4]) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      const __half2 h = __floats2half2_rn(f[i].x, f[i].y);
       w[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
 };
 template <>
 struct Vec<__nv_bfloat16> {
   static constexpr int V = 8;
   static constexpr bool exact = false;
-  static __device__ __forceinline__ void load(const __nv_bfloat16* p, float (&f)[8]) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
+  static __device__ __forceinline__ void unpack(const uint4& u, float2 (&f)[4]) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(w[i] << 16), f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    for (int i = 0; i < 4; ++i) f[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
   }
-  static __device__ __forceinline__ void store(__nv_bfloat16* p, const float (&f)[8]) {
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
-                                              pack_bf16x2(f[6], f[7]));
+  static __device__ __forceinline__ uint4 pack(const float2 (&f)[4]) {
+    return make_uint4(pack_bf16x2(f[0].x, f[0].y), pack_bf16x2(f[1].x, f[1].y), pack_bf16x2(f[2].x, f[2].y),
+                      pack_bf16x2(f[3].x, f[3].y));
   }
 };
+template <class T>
+__device__ __forceinline__ uint4 ld_raw(const T* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+template <class T>
+__device__ __forceinline__ void st_raw(T* p, const uint4& u) { *reinterpret_cast<uint4*>(p) = u; }
+template <class T>
+__device__ __forceinline__ void load_pairs(const T* p, float2 (&f)[Vec<T>::V / 2]) { Vec<T>::unpack(ld_raw(p), f); }
+
+// A thread's private ring of D slots of S 16-byte vectors in shared memory, filled by cp.async: loads stay in
+// flight under the arithmetic without holding registers. Nothing is shared between threads, so a thread waits
+// for its own copies only.
+template <int D, int S, int THREADS>
+struct Ring {
+  uint32_t base;
+  __device__ __forceinline__ explicit Ring(const void* smem) : base(smem_u32(smem) + threadIdx.x * 16) {}
+  static constexpr int bytes = D * S * THREADS * 16;
+  __device__ __forceinline__ void fetch(int slot, int s, const void* src) const {
+    cp_async16(base + (slot * S + s) * THREADS * 16, src, 16);
+  }
+  static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+  static __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory"); }
+  __device__ __forceinline__ uint4 get(int slot, int s) const {
+    uint4 u;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                 : "r"(base + (slot * S + s) * THREADS * 16)
+                 : "memory");
+    return u;
+  }
+  // body(p, raw0[, raw1]) for p = first, first + step, .. < len; vector s of position p is at src_s + p * stride
+  template <class T, class B>
+  __device__ __forceinline__ void walk(const T* src0, const T* src1, int first, int step, int len, int stride, B body) const {
+    auto request = [&](int slot, int p) {
+      if (p < len) {
+        fetch(slot, 0, src0 + static_cast<int64_t>(p) * stride);
+        if (S == 2) fetch(slot, 1, src1 + static_cast<int64_t>(p) * stride);
+      }
+      commit();
+    };
+#pragma unroll
+    for (int i = 0; i < D; ++i) request(i, first + i * step);
+    for (int p = first; p < len; p += D * step) {
+#pragma unroll
+      for (int i = 0; i < D; ++i) {
+        const int at = p + i * step;
+        if (at >= len) break;
+        wait();
+        const uint4 u0 = get(i, 0);
+        body(at, u0, S == 2 ? get(i, 1) : u0);
+        request(i, at + D * step);           // the slot's values have been used
+      }
+    }
+  }
+};
+
 __device__ __forceinline__ void norm_store1(float* p, float v) { *p = v; }
 __device__ __forceinline__ void norm_store1(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void norm_store1(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
@@ -162,31 +251,64 @@ __device__ __forceinline__ float sum_parts(const float* red, int g, int parts) {
 // A thread's running per-channel moments of n positions.
 template <int V>
 struct Running {
-  float n = 0.f, mean[V], m2[V];
+  static constexpr int P = V / 2;
+  float n = 0.f;
+  float2 mean[P], m2[P];
   __device__ __forceinline__ Running() {
 #pragma unroll
-    for (int i = 0; i < V; ++i) mean[i] = 0.f, m2[i] = 0.f;
+    for (int i = 0; i < P; ++i) mean[i] = m2[i] = both(0.f);
   }
-  // K loaded positions of which the first k >= 1 count (the others are zeros)
   template <int K>
-  __device__ __forceinline__ void add(const float (&f)[K][V], int k) {
-    const float kf = static_cast<float>(k), inv = __frcp_rn(kf), nn = n + kf, w = __fdividef(kf, nn), cw = n * w;
+  __device__ __forceinline__ void add(const float2 (&f)[K][P]) {
+    const float nn = n + K, w = __fdividef(static_cast<float>(K), nn), cw = n * w;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      float s = 0.f, q = 0.f;
+    for (int i = 0; i < P; ++i) {
+      float2 s = f[0][i], q = both(0.f);
 #pragma unroll
-      for (int j = 0; j < K; ++j) s += f[j][i];
-      s *= inv;
+      for (int j = 1; j < K; ++j) s = add2(s, f[j][i]);
+      if (K > 1) {
+        s = mul2(s, both(-1.f / K));
 #pragma unroll
-      for (int j = 0; j < K; ++j) {
-        const float d = j < k ? f[j][i] - s : 0.f;
-        q = fmaf(d, d, q);
+        for (int j = 0; j < K; ++j) {
+          const float2 d = add2(f[j][i], s);
+          q = fma2(d, d, q);
+        }
+        s = mul2(s, both(-1.f));
       }
-      const float d = s - mean[i];
-      mean[i] = fmaf(d, w, mean[i]);
-      m2[i] += fmaf(d * d, cw, q);
+      const float2 d = fma2(mean[i], both(-1.f), s);
+      mean[i] = fma2(d, both(w), mean[i]);
+      m2[i] = add2(m2[i], fma2(mul2(d, d), both(cw), q));
     }
     n = nn;
+  }
+  // positions lane, lane + lanes, .. < len of x (stride C); keep(p, raw) sees each of them
+  template <class T, class Keep>
+  __device__ __forceinline__ void walk(const T* x, int lane, int lanes, int len, int C, Keep keep) {
+    int p = lane;
+    for (; p + (kGnBatch - 1) * lanes < len; p += lanes * kGnBatch) {
+      uint4 u[kGnBatch];
+      float2 f[kGnBatch][P];
+#pragma unroll
+      for (int j = 0; j < kGnBatch; ++j) u[j] = ld_raw(x + static_cast<int64_t>(p + j * lanes) * C);
+#pragma unroll
+      for (int j = 0; j < kGnBatch; ++j) {
+        keep(p + j * lanes, u[j]);
+        Vec<T>::unpack(u[j], f[j]);
+      }
+      add(f);
+    }
+    uint4 u[kGnBatch - 1];
+#pragma unroll
+    for (int j = 0; j < kGnBatch - 1; ++j)
+      if (p + j * lanes < len) u[j] = ld_raw(x + static_cast<int64_t>(p + j * lanes) * C);
+#pragma unroll
+    for (int j = 0; j < kGnBatch - 1; ++j)
+      if (p + j * lanes < len) {
+        float2 f[1][P];
+        keep(p + j * lanes, u[j]);
+        Vec<T>::unpack(u[j], f[0]);
+        add(f);
+      }
   }
 };
 
@@ -197,7 +319,10 @@ __device__ __forceinline__ void block_moments(const Running<V>& r, bool active, 
                                               float len, float* vals, float* red, float* s_mean, float* s_m2) {
   if (active) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) vals[lane * C + col * V + i] = r.n * r.mean[i];
+    for (int i = 0; i < V / 2; ++i) {
+      vals[lane * C + col * V + 2 * i] = r.n * r.mean[i].x;
+      vals[lane * C + col * V + 2 * i + 1] = r.n * r.mean[i].y;
+    }
   }
   int parts = group_sums(vals, lanes, C, cg, red);
   for (int g = threadIdx.x; g < C / cg; g += kGnThreads) s_mean[g] = sum_parts(red, g, parts) / (len * cg);
@@ -205,8 +330,8 @@ __device__ __forceinline__ void block_moments(const Running<V>& r, bool active, 
   if (active) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float d = r.mean[i] - s_mean[(col * V + i) / cg];
-      vals[lane * C + col * V + i] = fmaf(r.n * d, d, r.m2[i]);
+      const float d = (i & 1 ? r.mean[i / 2].y : r.mean[i / 2].x) - s_mean[(col * V + i) / cg];
+      vals[lane * C + col * V + i] = fmaf(r.n * d, d, i & 1 ? r.m2[i / 2].y : r.m2[i / 2].x);
     }
   }
   parts = group_sums(vals, lanes, C, cg, red);
@@ -228,19 +353,31 @@ struct GnArgs {
   float* sums;         // [N][2][C] totals of g and g xh
 };
 
-template <class T>
-__device__ __forceinline__ uint4 ld_raw(const T* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
-template <class T>
-__device__ __forceinline__ void as_floats(const uint4& u, float (&f)[Vec<T>::V]) { Vec<T>::load(reinterpret_cast<const T*>(&u), f); }
+using GnRing1 = Ring<8, 1, kGnThreads>;    // forward: 32 KB a block, four blocks per SM
+using GnRing2 = Ring<6, 2, kGnThreads>;    // backward (x, dout): 48 KB a block, two blocks per SM
 
-// Parameters of a thread's channels
-template <class T>
-struct Affine {
-  static constexpr int V = Vec<T>::V;
-  float w[V], b[V];
-  __device__ __forceinline__ Affine(const GnArgs& a, int ch) {
-    Vec<T>::load(static_cast<const T*>(a.w) + ch, w);
-    Vec<T>::load(static_cast<const T*>(a.b) + ch, b);
+// What a thread does with a position in the forward pass: y = act((x - mu) (rstd w) + b). x - mu comes
+// first: folded into the offset, the mean of a map of little variance would cost digits.
+template <class T, int ACT>
+struct Apply {
+  static constexpr int V = Vec<T>::V, P = V / 2;
+  float2 A[P], b[P], mu[P];
+  __device__ __forceinline__ Apply(const GnArgs& a, int ch, const float* s_mu, const float* s_rs, int g0) {
+    load_pairs(static_cast<const T*>(a.w) + ch, A);
+    load_pairs(static_cast<const T*>(a.b) + ch, b);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const int g1 = (ch + 2 * i) / a.cg - g0, g2 = (ch + 2 * i + 1) / a.cg - g0;
+      mu[i] = make_float2(-s_mu[g1], -s_mu[g2]);
+      A[i] = mul2(A[i], make_float2(s_rs[g1], s_rs[g2]));
+    }
+  }
+  __device__ __forceinline__ void operator()(const uint4& u, T* to) const {
+    float2 f[P];
+    Vec<T>::unpack(u, f);
+#pragma unroll
+    for (int i = 0; i < P; ++i) f[i] = act_value<ACT, Vec<T>::exact>(fma2(add2(f[i], mu[i]), A[i], b[i]));
+    st_raw(to, Vec<T>::pack(f));
   }
 };
 
@@ -262,24 +399,7 @@ __global__ void __launch_bounds__(kGnThreads) groupnorm_resident_kernel(const Gn
   const T* x = static_cast<const T*>(a.x) + base;
   const int len = static_cast<int>(p1 - p0);
   Running<V> r;
-  if (active) {
-    for (int p = lane; p < len; p += lanes * kGnBatch) {
-      float f[kGnBatch][V];
-      uint4 u[kGnBatch];
-      int k = 0;
-#pragma unroll
-      for (int j = 0; j < kGnBatch; ++j) {
-        u[j] = make_uint4(0u, 0u, 0u, 0u);
-        if (p + j * lanes < len) u[j] = ld_raw(x + static_cast<int64_t>(p + j * lanes) * a.C), k = j + 1;
-      }
-#pragma unroll
-      for (int j = 0; j < kGnBatch; ++j) {
-        if (p + j * lanes < len) keep[(p + j * lanes) * cols + col] = u[j];
-        as_floats<T>(u[j], f[j]);
-      }
-      r.add(f, k);
-    }
-  }
+  if (active) r.walk(x, lane, lanes, len, a.C, [&](int p, const uint4& u) { keep[p * cols + col] = u; });
   block_moments<V>(r, active, lane, col, lanes, a.slab, a.cg, static_cast<float>(max(len, 1)), vals, red, s_mean,
                    s_mean + G);
   if (cl > 1) cluster_sync_all();
@@ -307,21 +427,9 @@ __global__ void __launch_bounds__(kGnThreads) groupnorm_resident_kernel(const Gn
   }
   if (cl > 1) cluster_sync_all(); else __syncthreads();
   if (!active) return;
-  const Affine<T> pr(a, c0 + col * V);
-  float mu[V], rs[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int g = (col * V + i) / a.cg;
-    mu[i] = s_out[g], rs[i] = s_out[G + g];
-  }
+  const Apply<T, ACT> apply(a, c0 + col * V, s_out, s_out + G, c0 / a.cg);
   T* out = static_cast<T*>(a.out) + base;
-  for (int p = lane; p < len; p += lanes) {
-    float f[V];
-    as_floats<T>(keep[p * cols + col], f);
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = act_value<ACT, Vec<T>::exact>(fmaf((f[i] - mu[i]) * rs[i], pr.w[i], pr.b[i]));
-    Vec<T>::store(out + static_cast<int64_t>(p) * a.C, f);
-  }
+  for (int p = lane; p < len; p += lanes) apply(keep[p * cols + col], out + static_cast<int64_t>(p) * a.C);
 }
 
 // Sums of g and g xh of a thread's channels -> vals [2][lanes][C] -> per-channel totals tot[2][C] of the block
@@ -338,43 +446,73 @@ __device__ __forceinline__ void channel_totals(const float* vals, int lanes, int
   __syncthreads();
 }
 
+// The same in the backward pass: xh = (x - mu) rstd, g = dy act'(xh w + b).
 template <class T, int ACT>
 struct Grad {
-  static constexpr int V = Vec<T>::V;
-  float mu[V], rs[V];
+  static constexpr int V = Vec<T>::V, P = V / 2;
+  float2 w[P], b[P], mu[P], rs[P];
   __device__ __forceinline__ Grad(const GnArgs& a, int n, int ch) {
+    load_pairs(static_cast<const T*>(a.w) + ch, w);
+    load_pairs(static_cast<const T*>(a.b) + ch, b);
+    const int64_t g0 = static_cast<int64_t>(n) * (a.C / a.cg);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int64_t g = static_cast<int64_t>(n) * (a.C / a.cg) + (ch + i) / a.cg;
-      mu[i] = __ldg(a.mean + g), rs[i] = __ldg(a.rstd + g);
+    for (int i = 0; i < P; ++i) {
+      const int64_t g1 = g0 + (ch + 2 * i) / a.cg, g2 = g0 + (ch + 2 * i + 1) / a.cg;
+      rs[i] = make_float2(__ldg(a.rstd + g1), __ldg(a.rstd + g2));
+      mu[i] = make_float2(-__ldg(a.mean + g1), -__ldg(a.mean + g2));
     }
   }
-  __device__ __forceinline__ void sums(const Affine<T>& pr, const uint4& xu, const uint4& du, float (&sg)[V], float (&sx)[V]) const {
-    float f[V], d[V];
-    as_floats<T>(xu, f);
-    as_floats<T>(du, d);
+  __device__ __forceinline__ void both_terms(int i, const float2& x, const float2& d, float2& xh, float2& g) const {
+    xh = mul2(add2(x, mu[i]), rs[i]);
+    g = mul2(d, act_slope<ACT, Vec<T>::exact>(fma2(xh, w[i], b[i])));
+  }
+  __device__ __forceinline__ void sums(const uint4& xu, const uint4& du, float2 (&sg)[P], float2 (&sx)[P]) const {
+    float2 f[P], d[P];
+    Vec<T>::unpack(xu, f);
+    Vec<T>::unpack(du, d);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float xh = (f[i] - mu[i]) * rs[i];
-      const float g = d[i] * act_slope<ACT, Vec<T>::exact>(fmaf(xh, pr.w[i], pr.b[i]));
-      sg[i] += g;
-      sx[i] = fmaf(g, xh, sx[i]);
+    for (int i = 0; i < P; ++i) {
+      float2 xh, g;
+      both_terms(i, f[i], d[i], xh, g);
+      sg[i] = add2(sg[i], g);
+      sx[i] = fma2(g, xh, sx[i]);
     }
   }
-  __device__ __forceinline__ void dx(const Affine<T>& pr, const float (&m1)[V], const float (&m2)[V], const uint4& xu,
-                                     const uint4& du, T* to) const {
-    float f[V], d[V];
-    as_floats<T>(xu, f);
-    as_floats<T>(du, d);
+  // dx = g (w rstd) + (xh (-rstd m2) + (-rstd m1))
+  struct Means {
+    float2 k[P], c[P], wr[P];
+    __device__ __forceinline__ Means(const Grad& gr, const float* m1, const float* m2, int ch, int cg, int g0) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float xh = (f[i] - mu[i]) * rs[i];
-      const float gw = d[i] * act_slope<ACT, Vec<T>::exact>(fmaf(xh, pr.w[i], pr.b[i])) * pr.w[i];
-      f[i] = rs[i] * (gw - m1[i] - xh * m2[i]);
+      for (int i = 0; i < P; ++i) {
+        const int g1 = (ch + 2 * i) / cg - g0, g2 = (ch + 2 * i + 1) / cg - g0;
+        k[i] = mul2(gr.rs[i], make_float2(-m2[g1], -m2[g2]));
+        c[i] = mul2(gr.rs[i], make_float2(-m1[g1], -m1[g2]));
+        wr[i] = mul2(gr.rs[i], gr.w[i]);
+      }
     }
-    Vec<T>::store(to, f);
+  };
+  __device__ __forceinline__ void dx(const Means& m, const uint4& xu, const uint4& du, T* to) const {
+    float2 f[P], d[P];
+    Vec<T>::unpack(xu, f);
+    Vec<T>::unpack(du, d);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      float2 xh, g;
+      both_terms(i, f[i], d[i], xh, g);
+      f[i] = fma2(g, m.wr[i], fma2(xh, m.k[i], m.c[i]));
+    }
+    st_raw(to, Vec<T>::pack(f));
   }
 };
+// a thread's sums into vals [2][lanes][C]
+template <int P>
+__device__ __forceinline__ void put_sums(float* vals, int lane, int lanes, int C, int ch, const float2 (&sg)[P], const float2 (&sx)[P]) {
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    *reinterpret_cast<float2*>(vals + lane * C + ch + 2 * i) = sg[i];
+    *reinterpret_cast<float2*>(vals + (lanes + lane) * C + ch + 2 * i) = sx[i];
+  }
+}
 
 template <class T, int ACT>
 __global__ void __launch_bounds__(kGnThreads) groupnorm_bwd_resident_kernel(const GnArgs a) {
@@ -391,12 +529,11 @@ __global__ void __launch_bounds__(kGnThreads) groupnorm_bwd_resident_kernel(cons
   float* tot = vals + 2 * lanes * S;                                 // [2][S]
   const int64_t base = (static_cast<int64_t>(n) * a.HW + p0) * a.C + c0 + col * V;
   const int len = static_cast<int>(p1 - p0);
-  const Affine<T> pr(a, c0 + col * V);
   const Grad<T, ACT> gr(a, n, c0 + col * V);
   if (active) {
-    float sg[V], sx[V];
+    float2 sg[V / 2], sx[V / 2];
 #pragma unroll
-    for (int i = 0; i < V; ++i) sg[i] = 0.f, sx[i] = 0.f;
+    for (int i = 0; i < V / 2; ++i) sg[i] = sx[i] = both(0.f);
     const T *x = static_cast<const T*>(a.x) + base, *d = static_cast<const T*>(a.dout) + base;
     for (int p = lane; p < len; p += lanes * 2) {
       const bool two = p + lanes < len;
@@ -404,17 +541,13 @@ __global__ void __launch_bounds__(kGnThreads) groupnorm_bwd_resident_kernel(cons
       uint4 x0 = ld_raw(x + o0), d0 = ld_raw(d + o0), x1, d1;
       if (two) x1 = ld_raw(x + o1), d1 = ld_raw(d + o1);
       keep[p * cols + col] = x0, keep[(a.span + p) * cols + col] = d0;
-      gr.sums(pr, x0, d0, sg, sx);
+      gr.sums(x0, d0, sg, sx);
       if (two) {
         keep[(p + lanes) * cols + col] = x1, keep[(a.span + p + lanes) * cols + col] = d1;
-        gr.sums(pr, x1, d1, sg, sx);
+        gr.sums(x1, d1, sg, sx);
       }
     }
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      vals[lane * S + col * V + i] = sg[i];
-      vals[(lanes + lane) * S + col * V + i] = sx[i];
-    }
+    put_sums(vals, lane, lanes, S, col * V, sg, sx);
   }
   channel_totals(vals, lanes, S, tot);
   if (cl > 1) cluster_sync_all();
@@ -433,15 +566,10 @@ __global__ void __launch_bounds__(kGnThreads) groupnorm_bwd_resident_kernel(cons
   }
   __syncthreads();
   if (!active) return;
-  float m1[V], m2[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int g = (col * V + i) / a.cg;
-    m1[i] = all[2 * S + g], m2[i] = all[2 * S + G + g];
-  }
+  const typename Grad<T, ACT>::Means m(gr, all + 2 * S, all + 2 * S + G, c0 + col * V, a.cg, c0 / a.cg);
   T* dx = static_cast<T*>(a.out) + base;
   for (int p = lane; p < len; p += lanes)
-    gr.dx(pr, m1, m2, keep[p * cols + col], keep[(a.span + p) * cols + col], dx + static_cast<int64_t>(p) * a.C);
+    gr.dx(m, keep[p * cols + col], keep[(a.span + p) * cols + col], dx + static_cast<int64_t>(p) * a.C);
 }
 
 // part[n][chunk][g] = mean, squared deviations of the group over the chunk's positions
@@ -457,20 +585,7 @@ __global__ void __launch_bounds__(kGnThreads, 4) groupnorm_moments_kernel(const 
   Running<V> r;
   if (lane < lanes) {
     const T* x = static_cast<const T*>(a.x) + (static_cast<int64_t>(n) * a.HW + p0) * a.C + col * V;
-    const int len = static_cast<int>(p1 - p0);
-    for (int p = lane; p < len; p += lanes * kGnBatch) {
-      float f[kGnBatch][V];
-      uint4 u[kGnBatch];
-      int k = 0;
-#pragma unroll
-      for (int j = 0; j < kGnBatch; ++j) {
-        u[j] = make_uint4(0u, 0u, 0u, 0u);
-        if (p + j * lanes < len) u[j] = ld_raw(x + static_cast<int64_t>(p + j * lanes) * a.C), k = j + 1;
-      }
-#pragma unroll
-      for (int j = 0; j < kGnBatch; ++j) as_floats<T>(u[j], f[j]);
-      r.add(f, k);
-    }
+    r.walk(x, lane, lanes, static_cast<int>(p1 - p0), a.C, [](int, const uint4&) {});
   }
   block_moments<V>(r, lane < lanes, lane, col, lanes, a.C, a.cg, static_cast<float>(p1 - p0), vals, red, s_mean, s_mean + G);
   for (int g = threadIdx.x; g < G; g += kGnThreads) {
@@ -512,33 +627,15 @@ __global__ void __launch_bounds__(kGnThreads, 4) groupnorm_apply_kernel(const Gn
   const int cols = a.C / V, lanes = kGnThreads / cols;
   const int col = threadIdx.x % cols, lane = threadIdx.x / cols;
   if (lane >= lanes) return;
-  const Affine<T> pr(a, col * V);
-  float mu[V], rs[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int g = (col * V + i) / a.cg;
-    mu[i] = gsm[g], rs[i] = gsm[G + g];
-  }
+  const Apply<T, ACT> apply(a, col * V, gsm, gsm + G, 0);
   const int64_t p0 = static_cast<int64_t>(blockIdx.x) * a.span;
   const int len = static_cast<int>(min(a.HW, p0 + a.span) - p0);
   const int64_t base = (static_cast<int64_t>(n) * a.HW + p0) * a.C + col * V;
   const T* x = static_cast<const T*>(a.x) + base;
   T* out = static_cast<T*>(a.out) + base;
-  auto one = [&](const uint4& u, int p) {
-    float f[V];
-    as_floats<T>(u, f);
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = act_value<ACT, Vec<T>::exact>(fmaf((f[i] - mu[i]) * rs[i], pr.w[i], pr.b[i]));
-    Vec<T>::store(out + static_cast<int64_t>(p) * a.C, f);
-  };
-  for (int p = lane; p < len; p += lanes * 2) {
-    const bool two = p + lanes < len;
-    const uint4 u0 = ld_raw(x + static_cast<int64_t>(p) * a.C);
-    uint4 u1;
-    if (two) u1 = ld_raw(x + static_cast<int64_t>(p + lanes) * a.C);
-    one(u0, p);
-    if (two) one(u1, p + lanes);
-  }
+  GnRing1(gsm + (2 * G + 3) / 4 * 4).walk(x, x, lane, lanes, len, a.C, [&](int p, const uint4& u, const uint4&) {
+    apply(u, out + static_cast<int64_t>(p) * a.C);
+  });
 }
 
 // part[n][chunk][0 | 1][c] = sums over the chunk's positions of g and of g xh
@@ -552,27 +649,16 @@ __global__ void __launch_bounds__(kGnThreads, 2) groupnorm_bwd_sums_kernel(const
   const int64_t p0 = static_cast<int64_t>(blockIdx.x) * a.span;
   if (lane < lanes) {
     const int len = static_cast<int>(min(a.HW, p0 + a.span) - p0);
-    const Affine<T> pr(a, col * V);
     const Grad<T, ACT> gr(a, n, col * V);
-    float sg[V], sx[V];
+    float2 sg[V / 2], sx[V / 2];
 #pragma unroll
-    for (int i = 0; i < V; ++i) sg[i] = 0.f, sx[i] = 0.f;
+    for (int i = 0; i < V / 2; ++i) sg[i] = sx[i] = both(0.f);
     const int64_t base = (static_cast<int64_t>(n) * a.HW + p0) * a.C + col * V;
     const T *x = static_cast<const T*>(a.x) + base, *d = static_cast<const T*>(a.dout) + base;
-    for (int p = lane; p < len; p += lanes * 2) {
-      const bool two = p + lanes < len;
-      const int64_t o0 = static_cast<int64_t>(p) * a.C, o1 = static_cast<int64_t>(p + lanes) * a.C;
-      const uint4 x0 = ld_raw(x + o0), d0 = ld_raw(d + o0);
-      uint4 x1, d1;
-      if (two) x1 = ld_raw(x + o1), d1 = ld_raw(d + o1);
-      gr.sums(pr, x0, d0, sg, sx);
-      if (two) gr.sums(pr, x1, d1, sg, sx);
-    }
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      gsm[lane * a.C + col * V + i] = sg[i];
-      gsm[(lanes + lane) * a.C + col * V + i] = sx[i];
-    }
+    GnRing2(gsm + (2 * lanes + 2) * a.C).walk(x, d, lane, lanes, len, a.C, [&](int, const uint4& xu, const uint4& du) {
+      gr.sums(xu, du, sg, sx);
+    });
+    put_sums(gsm, lane, lanes, a.C, col * V, sg, sx);
   }
   float* tot = gsm + 2 * lanes * a.C;
   channel_totals(gsm, lanes, a.C, tot);
@@ -613,28 +699,16 @@ __global__ void __launch_bounds__(kGnThreads, 2) groupnorm_bwd_dx_kernel(const G
   const int cols = a.C / V, lanes = kGnThreads / cols;
   const int col = threadIdx.x % cols, lane = threadIdx.x / cols;
   if (lane >= lanes) return;
-  const Affine<T> pr(a, col * V);
   const Grad<T, ACT> gr(a, n, col * V);
-  float m1[V], m2[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int g = (col * V + i) / a.cg;
-    m1[i] = gsm[2 * a.C + g], m2[i] = gsm[2 * a.C + G + g];
-  }
+  const typename Grad<T, ACT>::Means m(gr, gsm + 2 * a.C, gsm + 2 * a.C + G, col * V, a.cg, 0);
   const int64_t p0 = static_cast<int64_t>(blockIdx.x) * a.span;
   const int len = static_cast<int>(min(a.HW, p0 + a.span) - p0);
   const int64_t base = (static_cast<int64_t>(n) * a.HW + p0) * a.C + col * V;
   const T *x = static_cast<const T*>(a.x) + base, *d = static_cast<const T*>(a.dout) + base;
   T* dx = static_cast<T*>(a.out) + base;
-  for (int p = lane; p < len; p += lanes * 2) {
-    const bool two = p + lanes < len;
-    const int64_t o0 = static_cast<int64_t>(p) * a.C, o1 = static_cast<int64_t>(p + lanes) * a.C;
-    const uint4 x0 = ld_raw(x + o0), d0 = ld_raw(d + o0);
-    uint4 x1, d1;
-    if (two) x1 = ld_raw(x + o1), d1 = ld_raw(d + o1);
-    gr.dx(pr, m1, m2, x0, d0, dx + o0);
-    if (two) gr.dx(pr, m1, m2, x1, d1, dx + o1);
-  }
+  GnRing2(gsm + (2 * (a.C + G) + 3) / 4 * 4).walk(x, d, lane, lanes, len, a.C, [&](int p, const uint4& xu, const uint4& du) {
+    gr.dx(m, xu, du, dx + static_cast<int64_t>(p) * a.C);
+  });
 }
 
 // db[c] = sum over the P partials of sums[p][0][c], dw[c] of sums[p][1][c]
@@ -645,7 +719,7 @@ __global__ void __launch_bounds__(1024) norm_param_grad_kernel(const float* __re
   const int e = blockIdx.x * 32 + threadIdx.x;
   float s = 0.f;
   if (e < 2 * C) {
-#pragma unroll 4
+#pragma unroll 8
     for (int p = threadIdx.y; p < P; p += 32) s += sums[static_cast<int64_t>(p) * 2 * C + e];
   }
   sm[threadIdx.y][threadIdx.x] = s;
@@ -699,7 +773,7 @@ static GnPlan groupnorm_plan(int N, int64_t HW, int C, int groups, int elem, boo
   const int64_t sample = HW * C * elem * (backward ? 2 : 1);
   p.batch = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(N, kGnL2 / sample)));
   const int per_sm = backward ? 2 : 4;
-  const int64_t want = std::max<int64_t>(1, (148 * per_sm + p.batch - 1) / p.batch);
+  const int64_t want = std::max<int64_t>(1, 148 * per_sm / p.batch);   // one wave: a block more would be a second
   p.span = static_cast<int>(std::max<int64_t>(32, (HW + want - 1) / want));
   p.chunks = static_cast<int>((HW + p.span - 1) / p.span);
   return p;
@@ -725,12 +799,16 @@ static int groupnorm_check(int N, int64_t HW, int C, int G, int act, int dtype, 
 }
 
 template <class K>
-static int launch_gn_cluster(K kernel, PerDeviceOnce& once, dim3 grid, size_t smem, int cluster, cudaStream_t stream,
-                             const GnArgs& a) {
-  const int st = once.run(current_device(), [&] {
-    return status_from_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 static_cast<int>(kGnResident)));
+static int allow_smem(PerDeviceOnce& once, K kernel, int64_t bytes) {
+  return once.run(current_device(), [&] {
+    return status_from_cuda(
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
   });
+}
+template <class K>
+static int launch_gn(K kernel, PerDeviceOnce& once, dim3 grid, size_t smem, int cluster, cudaStream_t stream,
+                     const GnArgs& a) {
+  const int st = allow_smem(once, kernel, kGnResident);
   if (st != SSAM_OK) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
@@ -745,21 +823,23 @@ static int launch_gn_cluster(K kernel, PerDeviceOnce& once, dim3 grid, size_t sm
   cfg.numAttrs = 1;
   return status_from_cuda(cudaLaunchKernelEx(&cfg, kernel, a));
 }
+static size_t gn_floats(size_t n) { return (n + 3) / 4 * 16; }
 
 template <class T, int ACT>
 static int groupnorm_fwd_t(GnArgs a, int N, int G, float* ws, cudaStream_t stream) {
-  static PerDeviceOnce once;
+  static PerDeviceOnce resident, moments, apply;
   const GnPlan p = groupnorm_plan(N, a.HW, a.C, G, sizeof(T), false);
   a.span = p.span, a.slab = p.slab, a.part = ws;
   if (p.cluster)
-    return launch_gn_cluster(groupnorm_resident_kernel<T, ACT>, once, dim3(p.cluster, a.C / p.slab, N), p.smem, p.cluster,
-                             stream, a);
+    return launch_gn(groupnorm_resident_kernel<T, ACT>, resident, dim3(p.cluster, a.C / p.slab, N), p.smem, p.cluster,
+                     stream, a);
   const int lanes = kGnThreads / (a.C / Vec<T>::V);
   for (a.n0 = 0; a.n0 < N; a.n0 += p.batch) {
     const dim3 grid(p.chunks, std::min(p.batch, N - a.n0));
-    groupnorm_moments_kernel<T><<<grid, kGnThreads, (lanes * a.C + std::max(G, kGnWarps) + 2 * G) * sizeof(float), stream>>>(a);
-    groupnorm_apply_kernel<T, ACT><<<grid, kGnThreads, 2 * G * sizeof(float), stream>>>(a);
-    const int st = status_from_cuda(cudaGetLastError());
+    int st = launch_gn(groupnorm_moments_kernel<T>, moments, grid,
+                       gn_floats(lanes * a.C + std::max(G, kGnWarps) + 2 * G), 1, stream, a);
+    if (st == SSAM_OK)
+      st = launch_gn(groupnorm_apply_kernel<T, ACT>, apply, grid, gn_floats(2 * G) + GnRing1::bytes, 1, stream, a);
     if (st != SSAM_OK) return st;
   }
   return SSAM_OK;
@@ -767,23 +847,26 @@ static int groupnorm_fwd_t(GnArgs a, int N, int G, float* ws, cudaStream_t strea
 
 template <class T, int ACT>
 static int groupnorm_bwd_t(GnArgs a, int N, int G, void* dw, void* db, float* ws, cudaStream_t stream) {
-  static PerDeviceOnce once;
+  static PerDeviceOnce resident, sums, dx;
   const GnPlan p = groupnorm_plan(N, a.HW, a.C, G, sizeof(T), true);
   a.span = p.span, a.slab = p.slab, a.sums = ws;
   a.part = ws + gn_align(static_cast<size_t>(N) * 2 * a.C * sizeof(float)) / sizeof(float);
   int st;
   if (p.cluster) {
-    st = launch_gn_cluster(groupnorm_bwd_resident_kernel<T, ACT>, once, dim3(p.cluster, a.C / p.slab, N), p.smem, p.cluster,
-                           stream, a);
+    st = launch_gn(groupnorm_bwd_resident_kernel<T, ACT>, resident, dim3(p.cluster, a.C / p.slab, N), p.smem, p.cluster,
+                   stream, a);
     if (st != SSAM_OK) return st;
   } else {
     const int lanes = kGnThreads / (a.C / Vec<T>::V);
     for (a.n0 = 0; a.n0 < N; a.n0 += p.batch) {
       const dim3 grid(p.chunks, std::min(p.batch, N - a.n0));
-      groupnorm_bwd_sums_kernel<T, ACT><<<grid, kGnThreads, (2 * lanes * a.C + 2 * a.C) * sizeof(float), stream>>>(a);
+      st = launch_gn(groupnorm_bwd_sums_kernel<T, ACT>, sums, grid, gn_floats((2 * lanes + 2) * a.C) + GnRing2::bytes, 1,
+                     stream, a);
+      if (st != SSAM_OK) return st;
       groupnorm_bwd_totals_kernel<<<dim3((2 * a.C + 31) / 32, grid.y), dim3(32, 32), 0, stream>>>(a.part, a.n0, p.chunks, a.C, a.sums);
-      groupnorm_bwd_dx_kernel<T, ACT><<<grid, kGnThreads, 2 * static_cast<size_t>(a.C + G) * sizeof(float), stream>>>(a);
       st = status_from_cuda(cudaGetLastError());
+      if (st == SSAM_OK)
+        st = launch_gn(groupnorm_bwd_dx_kernel<T, ACT>, dx, grid, gn_floats(2 * (a.C + G)) + GnRing2::bytes, 1, stream, a);
       if (st != SSAM_OK) return st;
     }
   }
@@ -844,68 +927,82 @@ int groupnorm_act_bwd(const void* x, const void* dout, int N, int64_t HW, int C,
 // the row's moments are recomputed from x (it is read anyway). Each block sums its
 // rows' parameter gradients into one partial.
 // ---------------------------------------------------------------------------
+constexpr int kLnRing = 3;
+using LnRing = Ring<kLnRing, 2, 256>;      // 24 KB a block
+
 template <class T, int C, bool GELU>
 __global__ void __launch_bounds__(256) layernorm_half_bwd_kernel(const T* __restrict__ x, const T* __restrict__ dout,
                                                                  int64_t rows, const T* __restrict__ w,
                                                                  const T* __restrict__ b, float eps, T* __restrict__ dx,
                                                                  float* __restrict__ sums) {
   constexpr int TPR = C / 8, RPB = 256 / TPR;
-  __shared__ float part[RPB][2][C];
+  __shared__ __align__(16) float part[2][RPB][C];
   const int t = threadIdx.x % TPR, lr = threadIdx.x / TPR;
-  float wf[8], bf[8], sg[8], sx[8];
-  Vec<T>::load(w + t * 8, wf);
-  Vec<T>::load(b + t * 8, bf);
+  float2 wf[4], bf[4], sg[4], sx[4];
+  load_pairs(w + t * 8, wf);
+  load_pairs(b + t * 8, bf);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) sg[i] = 0.f, sx[i] = 0.f;
-  auto row_sum = [](float v) {
+  for (int i = 0; i < 4; ++i) sg[i] = sx[i] = both(0.f);
+  auto row_sum = [](float2 p) {
+    float v = p.x + p.y;
 #pragma unroll
     for (int o = 1; o < TPR; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+    return v * (1.f / C);
   };
-  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * RPB; r0 < rows; r0 += static_cast<int64_t>(gridDim.x) * RPB) {
-    const int64_t r = r0 + lr;
-    const bool ok = r < rows;
-    float f[8], d[8];
-    if (ok) {
-      Vec<T>::load(x + r * C + t * 8, f);
-      Vec<T>::load(dout + r * C + t * 8, d);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = 0.f, d[i] = 0.f;
+  __shared__ __align__(16) uint4 ring_mem[LnRing::bytes / 16];
+  const LnRing ring(ring_mem);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * RPB;
+  auto request = [&](int slot, int64_t row) {
+    if (row < rows) {
+      ring.fetch(slot, 0, x + row * C + t * 8);
+      ring.fetch(slot, 1, dout + row * C + t * 8);
     }
-    float s = 0.f;
+    LnRing::commit();
+  };
+  int64_t r = static_cast<int64_t>(blockIdx.x) * RPB + lr;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s += f[i];
-    const float mu = row_sum(s) * (1.f / C);
-    s = 0.f;
+  for (int i = 0; i < kLnRing; ++i) request(i, r + i * step);
+  int slot = 0;
+  // a warp's lanes hold whole rows: all of a row's lanes are behind the end together, and the others go on
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * RPB; r0 < rows; r0 += step, r += step) {
+    float2 f[4], d[4], s = both(0.f);
+    LnRing::wait();
+    const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+    Vec<T>::unpack(r < rows ? ring.get(slot, 0) : none, f);
+    Vec<T>::unpack(r < rows ? ring.get(slot, 1) : none, d);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] -= mu, s = fmaf(f[i], f[i], s);
-    const float rs = rsqrtf(row_sum(s) * (1.f / C) + eps);
-    float s1 = 0.f, s2 = 0.f;
+    for (int i = 0; i < 4; ++i) s = add2(s, f[i]);
+    const float mu = row_sum(s);
+    s = both(0.f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      f[i] *= rs;
-      const float g = GELU ? d[i] * act_slope<kActGelu, false>(fmaf(f[i], wf[i], bf[i])) : d[i];
-      sg[i] += g;
-      sx[i] = fmaf(g, f[i], sx[i]);
-      d[i] = g * wf[i];
-      s1 += d[i];
-      s2 = fmaf(d[i], f[i], s2);
+    for (int i = 0; i < 4; ++i) f[i] = add2(f[i], both(-mu)), s = fma2(f[i], f[i], s);
+    const float rs = rsqrtf(row_sum(s) + eps);
+    float2 s1 = both(0.f), s2 = both(0.f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[i] = mul2(f[i], both(rs));
+      if (GELU) d[i] = mul2(d[i], gelu_slope2(fma2(f[i], wf[i], bf[i])));
+      sg[i] = add2(sg[i], d[i]);
+      sx[i] = fma2(d[i], f[i], sx[i]);
+      d[i] = mul2(d[i], wf[i]);
+      s1 = add2(s1, d[i]);
+      s2 = fma2(d[i], f[i], s2);
     }
-    s1 = row_sum(s1) * (1.f / C);
-    s2 = row_sum(s2) * (1.f / C);
-    if (ok) {
+    const float m1 = -rs * row_sum(s1), m2 = -rs * row_sum(s2);
+    if (r < rows) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) d[i] = rs * (d[i] - s1 - f[i] * s2);
-      Vec<T>::store(dx + r * C + t * 8, d);
+      for (int i = 0; i < 4; ++i) d[i] = fma2(d[i], both(rs), fma2(f[i], both(m2), both(m1)));
+      st_raw(dx + r * C + t * 8, Vec<T>::pack(d));
     }
+    request(slot, r + kLnRing * step);
+    slot = slot + 1 == kLnRing ? 0 : slot + 1;
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) part[lr][0][t * 8 + i] = sg[i], part[lr][1][t * 8 + i] = sx[i];
+  put_sums(&part[0][0][0], lr, RPB, C, t * 8, sg, sx);
   __syncthreads();
   for (int c = threadIdx.x; c < 2 * C; c += 256) {
     float s = 0.f;
-    for (int k = 0; k < RPB; ++k) s += part[k][c / C][c % C];
+#pragma unroll 8
+    for (int k = 0; k < RPB; ++k) s += part[c / C][k][c % C];
     sums[static_cast<int64_t>(blockIdx.x) * 2 * C + c] = s;
   }
 }
