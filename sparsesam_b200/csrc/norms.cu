@@ -215,15 +215,15 @@ __device__ __forceinline__ void norm_store1(__nv_bfloat16* p, float v) { *p = __
 //    one slab of whole groups in shared memory, reduces through distributed shared memory
 //    and writes the result. A slab is at least 64 bytes wide, so that sectors are whole.
 //  * Streamed (samples too large for that): a moments / sums kernel, then an apply kernel,
-//    launched for as many samples at a time as stay in L2 between the two (48 MB), so
-//    that HBM still sees x once. 16 x 256 x 256 x 64 bf16 GELU with gradients: 567 us when
-//    both kernels ran over the whole batch, with the exact functions.
+//    launched for as many samples at a time as stay in L2 between the two (72 MB; 48 MB
+//    measured 301 us, 72 MB 274, 100 MB 280 on 16 x 256 x 256 x 64 bf16 GELU with gradients),
+//    so that HBM still sees x about once.
 // ---------------------------------------------------------------------------
 constexpr int kGnThreads = 256;
 constexpr int kGnWarps = kGnThreads / 32;
 constexpr int kGnBatch = 4;                     // positions loaded ahead; their moments are exact, then merged
 constexpr int64_t kGnResident = 96 << 10;       // shared-memory bytes a resident block may hold (two blocks per SM)
-constexpr int64_t kGnL2 = 48 << 20;             // bytes of a streamed batch of samples
+constexpr int64_t kGnL2 = 72 << 20;             // bytes of a streamed batch of samples
 
 // red[g * parts + i], i < parts: partial sums of vals[lane][C] over the lanes and the cg channels of
 // group g. Ends with the block synchronised; the return value is `parts`. vals may be reused after it.
@@ -771,7 +771,8 @@ static GnPlan groupnorm_plan(int N, int64_t HW, int C, int groups, int elem, boo
     return p;
   }
   const int64_t sample = HW * C * elem * (backward ? 2 : 1);
-  p.batch = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(N, kGnL2 / sample)));
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(N, kGnL2 / sample)), launches = (N + most - 1) / most;
+  p.batch = static_cast<int>((N + launches - 1) / launches);             // launches of about equal size
   const int per_sm = backward ? 2 : 4;
   const int64_t want = std::max<int64_t>(1, 148 * per_sm / p.batch);   // one wave: a block more would be a second
   p.span = static_cast<int>(std::max<int64_t>(32, (HW + want - 1) / want));

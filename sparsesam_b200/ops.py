@@ -7,7 +7,6 @@ a CUDA device is rejected.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 
@@ -51,11 +50,25 @@ def _check_cuda(*ts: torch.Tensor) -> None:
             raise ValueError("sparsesam_b200 ops run on CUDA tensors only (no CPU fallback)")
 
 
-def _on(t: torch.Tensor):
-    """Context that makes t's device the current one (launches go to the current device's streams)."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+def _launch(name: str, t: torch.Tensor, *args) -> None:
+    """Call an entry point on t's device and that device's current torch stream (the last argument)."""
+    dev = t.get_device()
+    if dev == torch._C._cuda_getDevice():
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+
+
+def _twice_guarded(backward):
+    """A Function's backward that autograd may differentiate no further. The guard of once_differentiable costs
+    a few microseconds and matters only where a graph of the backward pass is recorded."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, dout):
+        return (guarded if torch.is_grad_enabled() else backward)(ctx, dout)
+
+    return staticmethod(run)
 
 
 def _same_device(*ts: torch.Tensor) -> None:
@@ -487,9 +500,8 @@ def _layernorm_gelu_half(x, w, b, eps, gelu):
     out = torch.empty_like(x)
     C = x.shape[-1]
     if x.numel():
-        with _on(x):
-            _lib.call("ssam_layernorm_gelu_half", x.data_ptr(), x.numel() // C, C, w.data_ptr(), b.data_ptr(), eps, gelu,
-                      _DTYPES[x.dtype], out.data_ptr(), _stream(x))
+        _launch("ssam_layernorm_gelu_half", x, x.data_ptr(), x.numel() // C, C, w.data_ptr(), b.data_ptr(), eps, gelu,
+                _DTYPES[x.dtype], out.data_ptr())
     return out
 
 
@@ -500,8 +512,7 @@ class _LayerNormGeluHalf(torch.autograd.Function):
         ctx.eps, ctx.gelu = eps, gelu
         return _layernorm_gelu_half(x, w, b, eps, gelu)
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_twice_guarded
     def backward(ctx, dout):
         x, w, b = ctx.saved_tensors
         C = x.shape[-1]
@@ -512,10 +523,8 @@ class _LayerNormGeluHalf(torch.autograd.Function):
         dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty_like(b)
         n = _lib.load().ssam_layernorm_gelu_half_bwd_workspace_size(rows, C)
         ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-        with _on(x):
-            _lib.call("ssam_layernorm_gelu_half_bwd", x.data_ptr(), dout.data_ptr(), rows, C, w.data_ptr(), b.data_ptr(),
-                      ctx.eps, ctx.gelu, _DTYPES[x.dtype], dx.data_ptr(), dw.data_ptr(), db.data_ptr(), ws.data_ptr(), n,
-                      _stream(x))
+        _launch("ssam_layernorm_gelu_half_bwd", x, x.data_ptr(), dout.data_ptr(), rows, C, w.data_ptr(), b.data_ptr(),
+                ctx.eps, ctx.gelu, _DTYPES[x.dtype], dx.data_ptr(), dw.data_ptr(), db.data_ptr(), ws.data_ptr(), n)
         return dx, dw, db, None, None
 
 
@@ -552,13 +561,12 @@ def _groupnorm_act(x, groups, w, b, eps, act, stats):
     if x.numel() == 0:
         return out, None
     HW = x.numel() // (N * C)
-    st = torch.empty(2, N, groups, dtype=torch.float32, device=x.device) if stats else None
+    st = torch.empty(2, N, groups, dtype=torch.float32, device=x.device) if stats else None    # mean, rstd
     n = _lib.load().ssam_groupnorm_act_workspace_size(N, HW, C, groups, _DTYPES[x.dtype], 0)
     ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-    with _on(x):
-        _lib.call("ssam_groupnorm_act_fwd", x.data_ptr(), N, HW, C, groups, w.data_ptr(), b.data_ptr(), eps, act,
-                  _DTYPES[x.dtype], out.data_ptr(), st[0].data_ptr() if stats else None,
-                  st[1].data_ptr() if stats else None, _ptr(ws), n, _stream(x))
+    mean = st.data_ptr() if stats else None
+    _launch("ssam_groupnorm_act_fwd", x, x.data_ptr(), N, HW, C, groups, w.data_ptr(), b.data_ptr(), eps, act,
+            _DTYPES[x.dtype], out.data_ptr(), mean, mean + 4 * N * groups if stats else None, _ptr(ws), n)
     return out, st
 
 
@@ -570,8 +578,7 @@ class _GroupNormAct(torch.autograd.Function):
         ctx.groups, ctx.act = groups, act
         return out
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_twice_guarded
     def backward(ctx, dout):
         x, w, b, st = ctx.saved_tensors
         if x.numel() == 0:
@@ -582,10 +589,10 @@ class _GroupNormAct(torch.autograd.Function):
         dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty_like(b)
         n = _lib.load().ssam_groupnorm_act_workspace_size(N, HW, C, ctx.groups, _DTYPES[x.dtype], 1)
         ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-        with _on(x):
-            _lib.call("ssam_groupnorm_act_bwd", x.data_ptr(), dout.data_ptr(), N, HW, C, ctx.groups, w.data_ptr(),
-                      b.data_ptr(), st[0].data_ptr(), st[1].data_ptr(), ctx.act, _DTYPES[x.dtype], dx.data_ptr(),
-                      dw.data_ptr(), db.data_ptr(), ws.data_ptr(), n, _stream(x))
+        mean = st.data_ptr()
+        _launch("ssam_groupnorm_act_bwd", x, x.data_ptr(), dout.data_ptr(), N, HW, C, ctx.groups, w.data_ptr(),
+                b.data_ptr(), mean, mean + 4 * N * ctx.groups, ctx.act, _DTYPES[x.dtype], dx.data_ptr(), dw.data_ptr(),
+                db.data_ptr(), ws.data_ptr(), n)
         return dx, dw, db, None, None, None
 
 
@@ -616,68 +623,74 @@ def groupnorm_act(x: torch.Tensor, groups: int, w: torch.Tensor, b: torch.Tensor
 # ---------------------------------------------------------------------------
 # Cross attention
 # ---------------------------------------------------------------------------
-def _strides(*ts: torch.Tensor):
-    return (ctypes.c_int64 * 12)(*(s for t in ts for s in t.stride()[:3]))
+_I64x12 = ctypes.c_int64 * 12
+
+
+def _strides(a: torch.Tensor, b: torch.Tensor, c: torch.Tensor, d: torch.Tensor):
+    return _I64x12(*a.stride()[:3], *b.stride()[:3], *c.stride()[:3], *d.stride()[:3])
 
 
 def _cross_attn(q, k, v, scale, key_lens, key_mask, train):
+    """(out, out in fp32 or None, [lse, D] statistics); the last two only for training."""
     B, Tq, H, D = q.shape
     Tk, Hk = k.shape[1], k.shape[2]
     out = torch.empty(B, Tq, H, D, dtype=q.dtype, device=q.device)
     if out.numel() == 0 or Tk == 0:
         return out.zero_(), None, None
-    lse = out32 = None
+    dt = _DTYPES[q.dtype]
+    stats = out32 = None
     if train:
-        lse = torch.empty(B, H, Tq, dtype=torch.float32, device=q.device)
-        if q.dtype == torch.float32:
+        stats = torch.empty(2, B, H, Tq, dtype=torch.float32, device=q.device)
+        if dt == 2:
             out32 = out
-        elif _lib.load().ssam_cross_attn_bwd_uses_out_f32(Tk, D, _DTYPES[q.dtype]):
+        elif _lib.load().ssam_cross_attn_bwd_uses_out_f32(Tk, D, dt):
             out32 = torch.empty(B, Tq, H, D, dtype=torch.float32, device=q.device)
-    with _on(q):
-        _lib.call("ssam_cross_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v, out), B, Tq, Tk, H,
-                  Hk, D, _DTYPES[q.dtype], scale, _ptr(key_lens), _ptr(key_mask), out.data_ptr(),
-                  _ptr(out32) if out32 is not out else None, _ptr(lse), _stream(q))
-    return out, out32, lse
+    _launch("ssam_cross_attn_fwd", q, q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v, out), B, Tq, Tk, H, Hk,
+            D, dt, scale, _ptr(key_lens), _ptr(key_mask), out.data_ptr(), None if out32 is out else _ptr(out32),
+            _ptr(stats))
+    return out, out32, stats
 
 
 class _CrossAttn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, scale, key_lens, key_mask):
-        out, out32, lse = _cross_attn(q, k, v, scale, key_lens, key_mask, True)
-        ctx.save_for_backward(q, k, v, out32, lse, key_lens, key_mask)
+        out, out32, stats = _cross_attn(q, k, v, scale, key_lens, key_mask, True)
+        ctx.save_for_backward(q, k, v, out32, stats, key_lens, key_mask)
         ctx.scale = scale
         return out
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_twice_guarded
     def backward(ctx, dout):
-        q, k, v, out32, lse, key_lens, key_mask = ctx.saved_tensors
+        q, k, v, out32, stats, key_lens, key_mask = ctx.saved_tensors
         B, Tq, H, D = q.shape
         Tk, Hk = k.shape[1], k.shape[2]
-        need_q, need_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        dq = torch.empty(B, Tq, H, D, dtype=q.dtype, device=q.device) if need_q else None
-        dk = torch.empty(B, Tk, Hk, D, dtype=q.dtype, device=q.device) if need_kv else None
-        dv = torch.empty_like(dk) if need_kv else None
-        if lse is None:     # no queries or no keys: nothing depends on anything
+        need = ctx.needs_input_grad
+        dq = torch.empty(B, Tq, H, D, dtype=q.dtype, device=q.device) if need[0] else None
+        dk = dv = None
+        if need[1] or need[2]:
+            dk = torch.empty(B, Tk, Hk, D, dtype=q.dtype, device=q.device)
+            dv = torch.empty(B, Tk, Hk, D, dtype=q.dtype, device=q.device)
+        if stats is None:     # no queries or no keys: nothing depends on anything
             for g in (dq, dk, dv):
                 if g is not None:
                     g.zero_()
             return dq, dk, dv, None, None, None
         dout = _vector_rows(dout)
-        delta = torch.empty_like(lse)
-        with _on(q):
-            _lib.call("ssam_cross_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(),
-                      _strides(q, k, v, dout), B, Tq, Tk, H, Hk, D, _DTYPES[q.dtype], ctx.scale, _ptr(key_lens),
-                      _ptr(key_mask), _ptr(out32), lse.data_ptr(), delta.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv),
-                      _stream(q))
+        lse = stats.data_ptr()
+        _launch("ssam_cross_attn_bwd", q, q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(),
+                _strides(q, k, v, dout), B, Tq, Tk, H, Hk, D, _DTYPES[q.dtype], ctx.scale, _ptr(key_lens), _ptr(key_mask),
+                _ptr(out32), lse, lse + 4 * B * H * Tq, _ptr(dq), _ptr(dk), _ptr(dv))
         return dq, dk, dv, None, None, None
 
 
 def _vector_ok(t: torch.Tensor) -> bool:
     """Whether every (batch, token, head) row of t is contiguous and starts on a 16-byte boundary."""
+    if t.data_ptr() % 16:
+        return False
+    if t.is_contiguous():
+        return t.shape[3] * t.element_size() % 16 == 0
     unit = 16 // t.element_size()
-    return (t.stride(3) == 1 and t.data_ptr() % 16 == 0
-            and all(s % unit == 0 for s, n in zip(t.stride()[:3], t.shape) if n > 1))
+    return t.stride(3) == 1 and all(s % unit == 0 for s, n in zip(t.stride()[:3], t.shape) if n > 1)
 
 
 def _vector_rows(t: torch.Tensor) -> torch.Tensor:
@@ -702,25 +715,32 @@ def cross_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: floa
     key_lens (int32 (B,)) and key_mask (bool (B, Tk), True: attend) say which keys are
     there: what the others hold does not matter, and a query without keys gives zeros.
     Differentiable in q, k and v (once)."""
-    _check_cuda(q, k, v, key_lens, key_mask)
-    _same_device(q, k, v, key_lens, key_mask)
-    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
-        raise ValueError(f"q (B, Tq, H, D), k and v (B, Tk, Hk, D) expected, got {tuple(q.shape)}, "
-                         f"{tuple(k.shape)}, {tuple(v.shape)}")
-    if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+    dev, dt, qs, ks = q.device, q.dtype, q.shape, k.shape
+    if not (q.is_cuda and k.is_cuda and v.is_cuda):
+        _check_cuda(q, k, v)
+    if k.device != dev or v.device != dev:
+        _same_device(q, k, v)
+    if len(qs) != 4 or len(ks) != 4 or v.shape != ks or ks[0] != qs[0] or ks[3] != qs[3]:
+        raise ValueError(f"q (B, Tq, H, D), k and v (B, Tk, Hk, D) expected, got {tuple(qs)}, {tuple(ks)}, "
+                         f"{tuple(v.shape)}")
+    if dt not in _DTYPES or k.dtype != dt or v.dtype != dt:
         raise TypeError("q, k and v must share one dtype of fp16, bf16, fp32")
-    B, Tk = k.shape[:2]
-    if not cross_attn_supported(q.shape[2], k.shape[2], q.shape[3], q.dtype):
-        raise ValueError(f"heads {q.shape[2]} / {k.shape[2]} of {q.shape[3]} are not supported: key heads divide query "
+    if not cross_attn_supported(qs[2], ks[2], qs[3], dt):
+        raise ValueError(f"heads {qs[2]} / {ks[2]} of {qs[3]} are not supported: key heads divide query "
                          f"heads, head size a multiple of 8 up to {CROSS_ATTN_MAX_DIM}")
     if not (_vector_ok(q) and _vector_ok(k) and _vector_ok(v)):
         raise ValueError("q, k and v need contiguous, 16-byte aligned head rows")
-    if key_lens is not None and (key_lens.dtype != torch.int32 or key_lens.shape != (B,) or not key_lens.is_contiguous()):
-        raise ValueError("key_lens must be contiguous int32 (B,)")
-    if key_mask is not None and (key_mask.dtype != torch.bool or key_mask.shape != (B, Tk)
-                                 or not key_mask.is_contiguous()):
-        raise ValueError("key_mask must be contiguous bool (B, Tk)")
-    scale = 1.0 / math.sqrt(q.shape[3]) if scale is None else float(scale)
+    if key_lens is not None:
+        _check_cuda(key_lens)
+        _same_device(q, key_lens)
+        if key_lens.dtype != torch.int32 or key_lens.shape != ks[:1] or not key_lens.is_contiguous():
+            raise ValueError("key_lens must be contiguous int32 (B,)")
+    if key_mask is not None:
+        _check_cuda(key_mask)
+        _same_device(q, key_mask)
+        if key_mask.dtype != torch.bool or key_mask.shape != ks[:2] or not key_mask.is_contiguous():
+            raise ValueError("key_mask must be contiguous bool (B, Tk)")
+    scale = 1.0 / math.sqrt(qs[3]) if scale is None else float(scale)
     if not 0.0 < scale < 3e38:
         raise ValueError(f"scale must be positive and finite, got {scale}")
     if _wants_grad(q, k, v):
