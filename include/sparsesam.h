@@ -342,8 +342,8 @@ int ssam_groupnorm_act_bwd(const void* x, const void* dout, int N, int64_t HW, i
  *   out_f32 : optional fp32 [B, Tq, heads, d] contiguous copy of the result before its
  *             rounding, and lse, optional fp32 [B, heads, Tq] (base-2 log-sum-exp of the
  *             logits): what the backward pass takes. For dtype 2 with a contiguous `out`
- *             that pass takes `out` itself; where ssam_cross_attn_bwd_uses_out_f32()
- *             is 0 (fp16 / bf16 with few keys) it takes NULL.
+ *             that pass takes `out` itself; where ssam_cross_attn_bwd_uses_stats()
+ *             is 0 (fp16 / bf16 with few keys) out_f32, lse and delta may be NULL there.
  * ssam_cross_attn_bwd: contiguous gradients dq [B, Tq, heads, d], dk, dv [B, Tk, kv_heads, d]
  * of x's dtype; dq, or dk and dv together, may be NULL (not computed). Keys that are not
  * there get zero gradients. delta: fp32 [B, heads, Tq] scratch.
@@ -354,7 +354,7 @@ int ssam_groupnorm_act_bwd(const void* x, const void* dout, int N, int64_t HW, i
 int ssam_cross_attn_fwd(const void* q, const void* k, const void* v, const int64_t* strides, int B, int Tq, int Tk,
                         int heads, int kv_heads, int d, int dtype, float scale, const int32_t* key_lens,
                         const uint8_t* key_mask, void* out, float* out_f32, float* lse, void* stream);
-int ssam_cross_attn_bwd_uses_out_f32(int Tk, int d, int dtype);
+int ssam_cross_attn_bwd_uses_stats(int Tk, int d, int dtype);
 int ssam_cross_attn_bwd(const void* q, const void* k, const void* v, const void* dout, const int64_t* strides, int B,
                         int Tq, int Tk, int heads, int kv_heads, int d, int dtype, float scale, const int32_t* key_lens,
                         const uint8_t* key_mask, const float* out_f32, const float* lse, float* delta, void* dq,

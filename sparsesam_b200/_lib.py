@@ -65,7 +65,7 @@ SIGNATURES: dict[str, tuple] = {
                                        c_int, c_ptr, c_ptr, c_ptr, c_ptr, c_size, c_ptr]),
     "ssam_cross_attn_fwd": (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_f32,
                                     c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr]),
-    "ssam_cross_attn_bwd_uses_out_f32": (c_int, [c_int, c_int, c_int]),
+    "ssam_cross_attn_bwd_uses_stats": (c_int, [c_int, c_int, c_int]),
     "ssam_cross_attn_bwd": (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                                     c_f32, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr]),
     "ssam_layernorm_rows_copy": (c_int, [c_ptr, c_int, c_int, c_ptr, c_ptr, c_f32, c_ptr, c_ptr, c_ptr]),

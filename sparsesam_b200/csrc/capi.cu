@@ -212,8 +212,8 @@ int ssam_cross_attn_fwd(const void* q, const void* k, const void* v, const int64
                               out_f32, lse, static_cast<cudaStream_t>(stream));
 }
 
-int ssam_cross_attn_bwd_uses_out_f32(int Tk, int d, int dtype) {
-  return ssam::cross_attn_bwd_uses_out_f32(Tk, d, dtype);
+int ssam_cross_attn_bwd_uses_stats(int Tk, int d, int dtype) {
+  return ssam::cross_attn_bwd_uses_stats(Tk, d, dtype);
 }
 
 int ssam_cross_attn_bwd(const void* q, const void* k, const void* v, const void* dout, const int64_t* strides, int B,

@@ -496,14 +496,15 @@ int cross_attn_fwd(const void* q, const void* k, const void* v, const int64_t* s
   return xattn_dispatch(a, dtype, false, stream);
 }
 
-int cross_attn_bwd_uses_out_f32(int Tk, int d, int dtype) { return xattn_uses_out_f32(Tk, d, dtype) ? 1 : 0; }
+int cross_attn_bwd_uses_stats(int Tk, int d, int dtype) { return xattn_uses_stats(Tk, d, dtype) ? 1 : 0; }
 
 int cross_attn_bwd(const void* q, const void* k, const void* v, const void* dout, const int64_t* strides, int B, int Tq,
                    int Tk, int heads, int kv_heads, int d, int dtype, float scale, const int32_t* key_lens,
                    const uint8_t* key_mask, const float* out_f32, const float* lse, float* delta, void* dq, void* dk,
                    void* dv, cudaStream_t stream) {
   if (q == nullptr || k == nullptr || v == nullptr || dout == nullptr || strides == nullptr ||
-      (out_f32 == nullptr && xattn_uses_out_f32(Tk, d, dtype)) || lse == nullptr || delta == nullptr || (dk == nullptr) != (dv == nullptr))
+      ((out_f32 == nullptr || lse == nullptr || delta == nullptr) && xattn_uses_stats(Tk, d, dtype)) ||
+      (dk == nullptr) != (dv == nullptr))
     return SSAM_ERR_INVALID;
   XAttn a = xattn_args(q, k, v, strides, B, Tq, Tk, heads, kv_heads, d, scale, key_lens, key_mask);
   a.dout = dout, a.out_f32 = const_cast<float*>(out_f32), a.lse = const_cast<float*>(lse), a.delta = delta;

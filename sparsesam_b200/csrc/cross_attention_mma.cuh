@@ -72,6 +72,11 @@ __device__ __forceinline__ uint32_t movm(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
+__device__ __forceinline__ float rcp_fast(float x) {   // 2^-23 relative, far below the half types' rounding
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 // x, y -> packed value and packed remainder
 template <class T>
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
@@ -403,17 +408,23 @@ __global__ void __launch_bounds__(kXmThreads) xattn_fwd_mma(const XAttn a, int s
 //
 // The reference point of the exponentials is renewed only when a logit exceeds it by
 // 2^8 (as in attention.cu), so the cross-lane maximum is not taken every step.
+//
+// HP = 2 (heads of 16 next to one another): a fragment is two heads of a token, 64 contiguous
+// bytes, because 32-byte pieces keep the L1 tags, not the DRAM, busy (tokens -> image, 64 images:
+// 35 us with HP = 1 at 72 % of L1). Lanes t < 2 hold the first head's channels, so a query
+// fragment with the other half zeroed gives one head's logits, and likewise V^T rows g < 4
+// are the first head's. Twice the tensor instructions, of which there are plenty.
 // ---------------------------------------------------------------------------
 constexpr float kXmNone = -1e30f;           // reference before the first key
 constexpr float kXmSlack = 8.f;
 
-template <class T, int DP, int NQ>
+template <class T, int DP, int NQ, int HP>
 __global__ void __launch_bounds__(kXmThreads) xattn_fwd_few_rows(const XAttn a, int) {
   constexpr int NR = DP / 8, NU = NR / 2;    // 8- and 16-channel blocks
-  constexpr int KM = DP <= 32 ? 2 : 1;       // 16-key tiles per step
+  constexpr int KM = DP <= 32 && HP * NQ <= 4 ? 2 : 1;   // 16-key tiles per step
   extern __shared__ __align__(16) float xsm[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
-  const int b = blockIdx.z, n = blockIdx.y;
+  const int b = blockIdx.z, n = blockIdx.y * HP;
   const int cl = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
   const int rows = a.group * a.Tq;
   const int r0 = static_cast<int>(blockIdx.x) / cl * 8 * NQ;
@@ -421,174 +432,201 @@ __global__ void __launch_bounds__(kXmThreads) xattn_fwd_few_rows(const XAttn a, 
   const int steps = (keys + 16 * KM - 1) / (16 * KM), ns = kXmWarps * cl;
   const int per = (steps + ns - 1) / ns * (16 * KM);
   const int j_begin = min(keys, (rank * kXmWarps + warp) * per), j_end = min(keys, j_begin + per);
-  const T* kb = static_cast<const T*>(a.k) + b * a.ks[0] + n * a.ks[2];
-  const T* vb = static_cast<const T*>(a.v) + b * a.vs[0] + n * a.vs[2];
   const uint8_t* mask = a.key_mask == nullptr ? nullptr : a.key_mask + static_cast<int64_t>(b) * a.Tk;
+  const int d = HP * a.d;                    // channels of a fragment
+  const T* kp = static_cast<const T*>(a.k) + b * a.ks[0] + n * a.ks[2] + (j_begin + g) * a.ks[1];
+  const T* vp = static_cast<const T*>(a.v) + b * a.vs[0] + n * a.vs[2] + (j_begin + g) * a.vs[1];
 
   uint32_t k[KM][2][NR], v[KM][2][NR];
   float bias[KM][2];                         // 0, or -infinity for a key that is not there
-  auto load = [&](int j0) {
+  auto load = [&](int j0) {                  // loads keys j0 + .. and moves on
+    if (mask == nullptr && j0 + 16 * KM <= j_end) {
 #pragma unroll
-    for (int i = 0; i < KM; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int j = j0 + i * 16 + h * 8 + g;
-        const bool ok = j < j_end && (mask == nullptr || __ldg(mask + j) != 0);
-        bias[i][h] = ok ? 0.f : -INFINITY;
-        load_frag<T, DP>(kb + j * a.ks[1], t, a.d, ok, k[i][h]);
-        load_frag<T, DP>(vb + j * a.vs[1], t, a.d, ok, v[i][h]);
+      for (int i = 0; i < 2 * KM; ++i) {
+        bias[i / 2][i % 2] = 0.f;
+        load_frag<T, DP>(kp + i * 8 * a.ks[1], t, d, true, k[i / 2][i % 2]);
+        load_frag<T, DP>(vp + i * 8 * a.vs[1], t, d, true, v[i / 2][i % 2]);
       }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2 * KM; ++i) {
+        const int j = j0 + i * 8 + g;
+        const bool ok = j < j_end && (mask == nullptr || __ldg(mask + j) != 0);
+        bias[i / 2][i % 2] = ok ? 0.f : -INFINITY;
+        load_frag<T, DP>(kp + i * 8 * a.ks[1], t, d, ok, k[i / 2][i % 2]);
+        load_frag<T, DP>(vp + i * 8 * a.vs[1], t, d, ok, v[i / 2][i % 2]);
+      }
+    }
+    kp += 16 * KM * a.ks[1];
+    vp += 16 * KM * a.vs[1];
   };
   load(j_begin);
-  uint32_t q[NQ][NR];
+  uint32_t q[HP][NQ][NR];
 #pragma unroll
   for (int i = 0; i < NQ; ++i) {
     const int r = r0 + i * 8 + g;
-    load_frag<T, DP>(static_cast<const T*>(a.q) + row_offset(a, a.qs, b, n, min(r, rows - 1)), t, a.d, r < rows, q[i]);
+    uint32_t x[NR];
+    load_frag<T, DP>(static_cast<const T*>(a.q) + row_offset(a, a.qs, b, n, min(r, rows - 1)), t, d, r < rows, x);
+#pragma unroll
+    for (int z = 0; z < HP; ++z)
+#pragma unroll
+      for (int c = 0; c < NR; ++c) q[z][i][c] = HP == 1 || t / 2 == z ? x[c] : 0u;
   }
-  float o[NQ][NU][4], ref[NQ][2], l[NQ][2];
+  float o[NQ][NU][4];
+  float2 ref[HP][NQ], l[HP][NQ];             // of queries 2t, 2t + 1
 #pragma unroll
   for (int i = 0; i < NQ; ++i) {
-    ref[i][0] = ref[i][1] = kXmNone, l[i][0] = l[i][1] = 0.f;
+#pragma unroll
+    for (int z = 0; z < HP; ++z) ref[z][i] = make_float2(kXmNone, kXmNone), l[z][i] = make_float2(0.f, 0.f);
 #pragma unroll
     for (int u = 0; u < NU; ++u) o[i][u][0] = o[i][u][1] = o[i][u][2] = o[i][u][3] = 0.f;
   }
+  const float2 c2 = make_float2(a.c, a.c);
 
   for (int j0 = j_begin; j0 < j_end; j0 += 16 * KM) {
-    float s[NQ][KM][4];
+    float2 s[HP][NQ][KM][2];                 // [key g | g + 8] x queries 2t, 2t + 1
     uint32_t vt[KM][2][NR];
     bool renew = false;
 #pragma unroll
     for (int x = 0; x < KM; ++x) {
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) {
-        s[i][x][0] = s[i][x][1] = s[i][x][2] = s[i][x][3] = 0.f;
+      for (int z = 0; z < HP; ++z)
 #pragma unroll
-        for (int c = 0; c < NR; c += 2)
-          Mma<T>::run(s[i][x], k[x][0][c], k[x][1][c], k[x][0][c + 1], k[x][1][c + 1], q[i][c], q[i][c + 1]);
+        for (int i = 0; i < NQ; ++i) {
+          float f[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[i][x][e] = fmaf(s[i][x][e], a.c, bias[x][e >> 1]);
-          renew |= s[i][x][e] > ref[i][e & 1] + kXmSlack;
+          for (int c = 0; c < NR; c += 2)
+            Mma<T>::run(f, k[x][0][c], k[x][1][c], k[x][0][c + 1], k[x][1][c + 1], q[z][i][c], q[z][i][c + 1]);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            s[z][i][x][h] = fma2(make_float2(f[2 * h], f[2 * h + 1]), c2, make_float2(bias[x][h], bias[x][h]));
         }
-      }
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int c = 0; c < NR; ++c) vt[x][h][c] = movm(v[x][h][c]);
     }
     if (j0 + 16 * KM < j_end) load(j0 + 16 * KM);     // the next step's, under this one's arithmetic
+#pragma unroll
+    for (int z = 0; z < HP; ++z)
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        float2 m = ref[z][i];
+#pragma unroll
+        for (int x = 0; x < KM; ++x)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) m.x = fmaxf(m.x, s[z][i][x][h].x), m.y = fmaxf(m.y, s[z][i][x][h].y);
+        renew |= m.x > ref[z][i].x + kXmSlack || m.y > ref[z][i].y + kXmSlack;
+      }
     if (__any_sync(0xffffffffu, renew)) {
 #pragma unroll
-      for (int i = 0; i < NQ; ++i)
+      for (int i = 0; i < NQ; ++i) {
+        float2 mine = make_float2(1.f, 1.f);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float m = ref[i][e];
+        for (int z = 0; z < HP; ++z) {
+          float2 m = ref[z][i];
 #pragma unroll
-          for (int x = 0; x < KM; ++x) m = fmaxf(m, fmaxf(s[i][x][e], s[i][x][e + 2]));
+          for (int x = 0; x < KM; ++x)
 #pragma unroll
-          for (int w = 4; w < 32; w <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
-          const float f = ex2f(ref[i][e] - m);
-          ref[i][e] = m;
-          l[i][e] *= f;
+            for (int h = 0; h < 2; ++h) m.x = fmaxf(m.x, s[z][i][x][h].x), m.y = fmaxf(m.y, s[z][i][x][h].y);
 #pragma unroll
-          for (int u = 0; u < NU; ++u) o[i][u][e] *= f, o[i][u][e + 2] *= f;
+          for (int w = 4; w < 32; w <<= 1) {
+            m.x = fmaxf(m.x, __shfl_xor_sync(0xffffffffu, m.x, w));
+            m.y = fmaxf(m.y, __shfl_xor_sync(0xffffffffu, m.y, w));
+          }
+          const float2 f = make_float2(ex2f(ref[z][i].x - m.x), ex2f(ref[z][i].y - m.y));
+          ref[z][i] = m;
+          l[z][i] = mul2(l[z][i], f);
+          if (HP == 1 || g / 4 == z) mine = f;         // the sums of lane g belong to head g / 4
         }
+#pragma unroll
+        for (int u = 0; u < NU; ++u) o[i][u][0] *= mine.x, o[i][u][1] *= mine.y, o[i][u][2] *= mine.x, o[i][u][3] *= mine.y;
+      }
     }
 #pragma unroll
-    for (int i = 0; i < NQ; ++i)
+    for (int z = 0; z < HP; ++z)
 #pragma unroll
       for (int x = 0; x < KM; ++x) {
+        uint32_t va[2][NR];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[i][x][e] = ex2f(s[i][x][e] - ref[i][e & 1]);
-          l[i][e & 1] += s[i][x][e];
-        }
-        uint32_t h0, l0, h1, l1;
-        split2<T>(s[i][x][0], s[i][x][1], h0, l0);
-        split2<T>(s[i][x][2], s[i][x][3], h1, l1);
-        h0 = movm(h0), h1 = movm(h1), l0 = movm(l0), l1 = movm(l1);
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int u = 0; u < NU; ++u) {
-          Mma<T>::run(o[i][u], vt[x][0][2 * u], vt[x][0][2 * u + 1], vt[x][1][2 * u], vt[x][1][2 * u + 1], h0, h1);
-          Mma<T>::run(o[i][u], vt[x][0][2 * u], vt[x][0][2 * u + 1], vt[x][1][2 * u], vt[x][1][2 * u + 1], l0, l1);
+          for (int c = 0; c < NR; ++c) va[h][c] = HP == 1 || g / 4 == z ? vt[x][h][c] : 0u;
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+          uint32_t hi[2], lo[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float2 p = add2(s[z][i][x][h], make_float2(-ref[z][i].x, -ref[z][i].y));
+            p.x = ex2f(p.x), p.y = ex2f(p.y);
+            l[z][i] = add2(l[z][i], p);
+            split2<T>(p.x, p.y, hi[h], lo[h]);
+            hi[h] = movm(hi[h]), lo[h] = movm(lo[h]);
+          }
+#pragma unroll
+          for (int u = 0; u < NU; ++u) {
+            Mma<T>::run(o[i][u], va[0][2 * u], va[0][2 * u + 1], va[1][2 * u], va[1][2 * u + 1], hi[0], hi[1]);
+            Mma<T>::run(o[i][u], va[0][2 * u], va[0][2 * u + 1], va[1][2 * u], va[1][2 * u + 1], lo[0], lo[1]);
+          }
         }
       }
   }
 
-  // Join: the highest reference of the warps, then of the cluster's blocks; every warp rescales
-  // its share to it, the shares are summed in a fixed order and divided on the way out.
-  constexpr int PER = NU * 4 + 2, NREG = NQ * PER, ROWS = 8 * NQ;
-  float* s_top = xsm;                        // [8][ROWS]
-  float* s_acc = xsm + kXmWarps * ROWS;      // [4][NREG][32]
+  // Join. Every warp leaves its references and sums; the block joins them at their highest reference, and
+  // the cluster's blocks theirs on the way out, in a fixed order.
+  constexpr int PER = NU * 4 + 2, NREG = NQ * PER, ROWS = HP * 8 * NQ;
+  float* s_ref = xsm;                        // [8][ROWS]: head z, query 8 i + x at z 8 NQ + 8 i + x
+  float* s_top = s_ref + kXmWarps * ROWS;    // [ROWS]
+  float* s_acc = s_top + ROWS;               // [8][NREG][32]; the block's sums end up in [0]
+  const int hz = HP == 1 ? 0 : g / 4;        // the head of this lane's sums
 #pragma unroll
-  for (int i = 0; i < NQ; ++i)
+  for (int i = 0; i < NQ; ++i) {
+    float* to = s_acc + (warp * NREG + i * PER) * 32 + lane;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+    for (int z = 0; z < HP; ++z) {
 #pragma unroll
-      for (int w = 4; w < 32; w <<= 1) l[i][e] += __shfl_xor_sync(0xffffffffu, l[i][e], w);
-      if (g == 0) s_top[warp * ROWS + i * 8 + 2 * t + e] = ref[i][e];
-    }
-  __syncthreads();
-  float top[NQ][2];
-#pragma unroll
-  for (int i = 0; i < NQ; ++i)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float m = kXmNone;
-#pragma unroll
-      for (int w = 0; w < kXmWarps; ++w) m = fmaxf(m, s_top[w * ROWS + i * 8 + 2 * t + e]);
-      top[i][e] = m;
-    }
-  __syncthreads();
-  if (warp == 0 && g == 0) {
-#pragma unroll
-    for (int i = 0; i < NQ; ++i) s_top[i * 8 + 2 * t] = top[i][0], s_top[i * 8 + 2 * t + 1] = top[i][1];
-  }
-  if (cl > 1) {
-    cluster_sync_all();
-#pragma unroll
-    for (int i = 0; i < NQ; ++i)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const uint32_t at = smem_u32(s_top + i * 8 + 2 * t + e);
-        for (int w = 0; w < cl; ++w) top[i][e] = fmaxf(top[i][e], ld_dsmem(mapa_shared(at, w)));
+      for (int w = 4; w < 32; w <<= 1) {
+        l[z][i].x += __shfl_xor_sync(0xffffffffu, l[z][i].x, w);
+        l[z][i].y += __shfl_xor_sync(0xffffffffu, l[z][i].y, w);
       }
-  }
-  float acc[NREG];
-#pragma unroll
-  for (int i = 0; i < NQ; ++i)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float f = ex2f(ref[i][e] - top[i][e]);
-      acc[i * PER + NU * 4 + e] = l[i][e] * f;
-#pragma unroll
-      for (int u = 0; u < NU; ++u) acc[i * PER + u * 4 + e] = o[i][u][e] * f, acc[i * PER + u * 4 + e + 2] = o[i][u][e + 2] * f;
+      if (g == 0) *reinterpret_cast<float2*>(s_ref + warp * ROWS + (z * NQ + i) * 8 + 2 * t) = ref[z][i];
+      if (HP == 1 || hz == z) to[NU * 4 * 32] = l[z][i].x, to[(NU * 4 + 1) * 32] = l[z][i].y;
     }
-  warp_tree_sum<NREG>(acc, s_acc, warp, lane);
-  __syncthreads();
-  if (warp == 0) {
 #pragma unroll
-    for (int i = 0; i < NREG; ++i) s_acc[i * 32 + lane] = acc[i];
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) to[(u * 4 + e) * 32] = o[i][u][e];
+  }
+  __syncthreads();
+  for (int w = warp; w < NREG; w += kXmWarps) {          // register w of every lane; its query is 8 i + 2t + (w & 1)
+    const int ro = (hz * NQ + w / PER) * 8 + 2 * t + (w % PER & 1);
+    float top = kXmNone, x = 0.f;
+#pragma unroll
+    for (int z = 0; z < kXmWarps; ++z) top = fmaxf(top, s_ref[z * ROWS + ro]);
+#pragma unroll
+    for (int z = 0; z < kXmWarps; ++z) x = fmaf(s_acc[(z * NREG + w) * 32 + lane], ex2f(s_ref[z * ROWS + ro] - top), x);
+    s_acc[w * 32 + lane] = x;                            // read by this lane only so far
+    if (w % PER < 2 && g % (8 / HP) == 0) s_top[ro] = top;
   }
   if (cl > 1) cluster_sync_all(); else __syncthreads();
   const uint32_t base = smem_u32(s_acc) + lane * 4;
-  const int64_t stat0 = (static_cast<int64_t>(b) * a.heads + n * a.group) * a.Tq;
+  const int64_t stat0 = (static_cast<int64_t>(b) * a.heads + (n + hz) * a.group) * a.Tq;
   for (int w = rank * kXmWarps + warp; w < 2 * NQ * NU; w += cl * kXmWarps) {
-    const int e = w % 2, u = w / 2 % NU, i = w / 2 / NU, ro = i * 8 + 2 * t + e, r = r0 + ro;
+    const int e = w % 2, u = w / 2 % NU, i = w / 2 / NU, ro = (hz * NQ + i) * 8 + 2 * t + e, r = r0 + i * 8 + 2 * t + e;
     float x = 0.f, y = 0.f, den = 0.f, m = kXmNone;
+    for (int z = 0; z < cl; ++z) m = fmaxf(m, ld_dsmem(mapa_shared(smem_u32(s_top + ro), z)));
     for (int z = 0; z < cl; ++z) {
       const uint32_t from = mapa_shared(base, z);
-      x += ld_dsmem(from + (i * PER + u * 4 + e) * 128);
-      y += ld_dsmem(from + (i * PER + u * 4 + e + 2) * 128);
-      den += ld_dsmem(from + (i * PER + NU * 4 + e) * 128);
-      m = fmaxf(m, ld_dsmem(mapa_shared(smem_u32(s_top + ro), z)));
+      const float f = ex2f(ld_dsmem(mapa_shared(smem_u32(s_top + ro), z)) - m);
+      x = fmaf(ld_dsmem(from + (i * PER + u * 4 + e) * 128), f, x);
+      y = fmaf(ld_dsmem(from + (i * PER + u * 4 + e + 2) * 128), f, y);
+      den = fmaf(ld_dsmem(from + (i * PER + NU * 4 + e) * 128), f, den);
     }
     if (r >= rows) continue;
     const float inv = den == 0.f ? 0.f : 1.f / den;
-    const int ch = g / 2 * (DP / 4) + 4 * u + g % 2;   // and ch + 2
-    T* to = static_cast<T*>(a.out) + row_offset(a, a.os, b, n, r);
-    float* to32 = a.out_f32 == nullptr ? nullptr : a.out_f32 + row_dense(a, b, n, r);
+    const int ch = g / 2 % (4 / HP) * (DP / 4) + 4 * u + g % 2;   // and ch + 2, of head n + hz
+    T* to = static_cast<T*>(a.out) + row_offset(a, a.os, b, n + hz, r);
+    float* to32 = a.out_f32 == nullptr ? nullptr : a.out_f32 + row_dense(a, b, n + hz, r);
     if (ch < a.d) {
       store1(to + ch, x * inv);
       if (to32 != nullptr) to32[ch] = x * inv;
@@ -597,131 +635,155 @@ __global__ void __launch_bounds__(kXmThreads) xattn_fwd_few_rows(const XAttn a, 
       store1(to + ch + 2, y * inv);
       if (to32 != nullptr) to32[ch + 2] = y * inv;
     }
-    if (a.lse != nullptr && u == 0 && g == 0) a.lse[stat0 + r] = den == 0.f ? INFINITY : m + log2f(den);
+    if (a.lse != nullptr && u == 0 && g % (8 / HP) == 0) a.lse[stat0 + r] = den == 0.f ? INFINITY : m + log2f(den);
   }
   if (cl > 1) cluster_sync_all();
 }
 
 // ---------------------------------------------------------------------------
-// Forward, many query rows on few keys (at most 8 NK): a warp keeps the K and turned V
-// fragments of one (image, key head) and walks its share of the rows 16 at a time, the
+// Forward, many queries on few keys (at most 8 NK): a warp keeps the K and turned V
+// fragments of one (image, query head) and walks its share of the queries 16 at a time, the
 // next rows in flight. Bound by the bytes of q and out; neighbouring warps hold
-// neighbouring heads, so a block touches whole rows.
+// neighbouring heads, so a block touches whole rows. HP = 2 as above.
 // ---------------------------------------------------------------------------
-template <class T, int DP, int NK>
+template <class T, int DP, int NK, int HP>
 __global__ void __launch_bounds__(kXmThreads) xattn_fwd_few_keys(const XAttn a, int chunks) {
   constexpr int NR = DP / 8;
   const int lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+  const int units = a.heads / HP;
   const int64_t w = static_cast<int64_t>(blockIdx.x) * kXmWarps + threadIdx.x / 32;
-  const int n = static_cast<int>(w % a.kv_heads), chunk = static_cast<int>(w / a.kv_heads % chunks);
-  const int64_t bb = w / a.kv_heads / chunks;
+  const int h = static_cast<int>(w % units) * HP, chunk = static_cast<int>(w / units % chunks);
+  const int64_t bb = w / units / chunks;
   if (bb >= a.B) return;
-  const int b = static_cast<int>(bb);
-  const int rows = a.group * a.Tq, tiles = (rows + 15) / 16, per = (tiles + chunks - 1) / chunks;
-  const int r_begin = min(rows, chunk * per * 16), r_end = min(rows, r_begin + per * 16);
+  const int b = static_cast<int>(bb), n = h / a.group;
+  const int tiles = (a.Tq + 15) / 16, per = (tiles + chunks - 1) / chunks;
+  const int r_begin = min(a.Tq, chunk * per * 16), r_end = min(a.Tq, r_begin + per * 16);
   if (r_begin >= r_end) return;
-  const int keys = xattn_keys(a, b);
+  const int keys = xattn_keys(a, b), d = HP * a.d;
   const T* kb = static_cast<const T*>(a.k) + b * a.ks[0] + n * a.ks[2];
   const T* vb = static_cast<const T*>(a.v) + b * a.vs[0] + n * a.vs[2];
-  const T* qb = static_cast<const T*>(a.q);
   const uint8_t* mask = a.key_mask == nullptr ? nullptr : a.key_mask + static_cast<int64_t>(b) * a.Tk;
-  const int64_t stat0 = (static_cast<int64_t>(b) * a.heads + n * a.group) * a.Tq;
+  // rows r0 + g and r0 + g + 8
+  const T* qp = static_cast<const T*>(a.q) + b * a.qs[0] + h * a.qs[2] + static_cast<int64_t>(r_begin + g) * a.qs[1];
+  T* op = static_cast<T*>(a.out) + b * a.os[0] + h * a.os[2] + static_cast<int64_t>(r_begin + g) * a.os[1];
+  const int64_t q8 = 8 * a.qs[1], o8 = 8 * a.os[1];
+  float* lse = a.lse == nullptr ? nullptr : a.lse + (static_cast<int64_t>(b) * a.heads + h) * a.Tq;
+  float* o32 = a.out_f32 == nullptr ? nullptr : a.out_f32 + (static_cast<int64_t>(b) * a.Tq * a.heads + h) * a.d + t * (DP / 4);
 
-  uint32_t k[NK][NR], v[NK][NR], q[2][NR];
-  float bias[NK][2];                         // of keys 8 i + 2t + e
+  uint32_t k[HP][NK][NR], v[HP][NK][NR], q[2][NR];
+  float2 bias[NK];                           // of keys 8 i + 2t, + 1
   auto load_q = [&](int r) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      load_frag<T, DP>(qb + row_offset(a, a.qs, b, n, min(r + h * 8 + g, rows - 1)), t, a.d, r + h * 8 + g < r_end, q[h]);
+    load_frag<T, DP>(qp, t, d, r + g < r_end, q[0]);
+    load_frag<T, DP>(qp + q8, t, d, r + g + 8 < r_end, q[1]);
+    qp += 2 * q8;
   };
   load_q(r_begin);
 #pragma unroll
   for (int i = 0; i < NK; ++i) {
     const int j = i * 8 + g;
     const bool ok = j < keys && (mask == nullptr || __ldg(mask + j) != 0);
-    load_frag<T, DP>(kb + j * a.ks[1], t, a.d, ok, k[i]);
-    load_frag<T, DP>(vb + j * a.vs[1], t, a.d, ok, v[i]);
+    uint32_t x[NR], y[NR];
+    load_frag<T, DP>(kb + j * a.ks[1], t, d, ok, x);
+    load_frag<T, DP>(vb + j * a.vs[1], t, d, ok, y);
     const float mine = ok ? 0.f : -INFINITY;
-    bias[i][0] = __shfl_sync(0xffffffffu, mine, 8 * t);
-    bias[i][1] = __shfl_sync(0xffffffffu, mine, 8 * t + 4);
+    bias[i].x = __shfl_sync(0xffffffffu, mine, 8 * t);
+    bias[i].y = __shfl_sync(0xffffffffu, mine, 8 * t + 4);
 #pragma unroll
-    for (int c = 0; c < NR; ++c) v[i][c] = movm(v[i][c]);
+    for (int c = 0; c < NR; ++c) {
+      const uint32_t turned = movm(y[c]);
+#pragma unroll
+      for (int z = 0; z < HP; ++z) {
+        k[z][i][c] = HP == 1 || t / 2 == z ? x[c] : 0u;
+        v[z][i][c] = HP == 1 || g / 4 == z ? turned : 0u;
+      }
+    }
   }
 
+  const float2 c2 = make_float2(a.c, a.c);
   for (int r0 = r_begin; r0 < r_end; r0 += 16) {
-    float s[NK][4];
+    float2 s[HP][NK][2];
 #pragma unroll
-    for (int i = 0; i < NK; ++i) {
-      s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+    for (int z = 0; z < HP; ++z)
 #pragma unroll
-      for (int c = 0; c < NR; c += 2) Mma<T>::run(s[i], q[0][c], q[1][c], q[0][c + 1], q[1][c + 1], k[i][c], k[i][c + 1]);
-    }
+      for (int i = 0; i < NK; ++i) {
+        float f[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < NR; c += 2) Mma<T>::run(f, q[0][c], q[1][c], q[0][c + 1], q[1][c + 1], k[z][i][c], k[z][i][c + 1]);
+        s[z][i][0] = fma2(make_float2(f[0], f[1]), c2, bias[i]);
+        s[z][i][1] = fma2(make_float2(f[2], f[3]), c2, bias[i]);
+      }
     if (r0 + 16 < r_end) load_q(r0 + 16);
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, inv[2];
-#pragma unroll
-    for (int i = 0; i < NK; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[i][e] = fmaf(s[i][e], a.c, bias[i][e & 1]);
-        m[e >> 1] = fmaxf(m[e >> 1], s[i][e]);
-      }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      m[h] = fmaxf(m[h], __shfl_xor_sync(0xffffffffu, m[h], 1));
-      m[h] = fmaxf(m[h], __shfl_xor_sync(0xffffffffu, m[h], 2));
-      m[h] = fmaxf(m[h], kXmNone);           // a row without keys: 2^(-inf + 1e30) = 0
-    }
-#pragma unroll
-    for (int i = 0; i < NK; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[i][e] = ex2f(s[i][e] - m[e >> 1]);
-        l[e >> 1] += s[i][e];
-      }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-      inv[h] = l[h] == 0.f ? 0.f : 1.f / l[h];
-    }
+    float m[HP][2], l[HP][2];
     float o[NR][4];
 #pragma unroll
     for (int c = 0; c < NR; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
 #pragma unroll
-    for (int i = 0; i < NK; i += 2) {
-      uint32_t hi[4], lo[4];
+    for (int z = 0; z < HP; ++z) {
+      float inv[2];
 #pragma unroll
-      for (int x = 0; x < (NK > 1 ? 2 : 1); ++x) {
-        split2<T>(s[i + x][0] * inv[0], s[i + x][1] * inv[0], hi[2 * x], lo[2 * x]);
-        split2<T>(s[i + x][2] * inv[1], s[i + x][3] * inv[1], hi[2 * x + 1], lo[2 * x + 1]);
+      for (int e = 0; e < 2; ++e) {
+        float x = kXmNone;                   // a row without keys: 2^(-inf + 1e30) = 0
+#pragma unroll
+        for (int i = 0; i < NK; ++i) x = fmaxf(x, fmaxf(s[z][i][e].x, s[z][i][e].y));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+        m[z][e] = x;
+        float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+          float2 p = add2(s[z][i][e], make_float2(-x, -x));
+          p.x = ex2f(p.x), p.y = ex2f(p.y);
+          s[z][i][e] = p;
+          sum = add2(sum, p);
+        }
+        float y = sum.x + sum.y;
+        y += __shfl_xor_sync(0xffffffffu, y, 1);
+        y += __shfl_xor_sync(0xffffffffu, y, 2);
+        l[z][e] = y;
+        inv[e] = y == 0.f ? 0.f : rcp_fast(y);
       }
 #pragma unroll
-      for (int c = 0; c < NR; ++c) {
-        if constexpr (NK == 1) {
-          Mma<T>::run8(o[c], hi[0], hi[1], v[0][c]);
-          Mma<T>::run8(o[c], lo[0], lo[1], v[0][c]);
-        } else {
-          Mma<T>::run(o[c], hi[0], hi[1], hi[2], hi[3], v[i][c], v[i + 1][c]);
-          Mma<T>::run(o[c], lo[0], lo[1], lo[2], lo[3], v[i][c], v[i + 1][c]);
+      for (int i = 0; i < NK; i += 2) {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int x = 0; x < (NK > 1 ? 2 : 1); ++x)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float2 p = mul2(s[z][i + x][e], make_float2(inv[e], inv[e]));
+            split2<T>(p.x, p.y, hi[2 * x + e], lo[2 * x + e]);
+          }
+#pragma unroll
+        for (int c = 0; c < NR; ++c) {
+          if constexpr (NK == 1) {
+            Mma<T>::run8(o[c], hi[0], hi[1], v[z][0][c]);
+            Mma<T>::run8(o[c], lo[0], lo[1], v[z][0][c]);
+          } else {
+            Mma<T>::run(o[c], hi[0], hi[1], hi[2], hi[3], v[z][i][c], v[z][i + 1][c]);
+            Mma<T>::run(o[c], lo[0], lo[1], lo[2], lo[3], v[z][i][c], v[z][i + 1][c]);
+          }
         }
       }
     }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = r0 + h * 8 + g;
+    for (int e = 0; e < 2; ++e) {
+      const int r = r0 + e * 8 + g;
       if (r >= r_end) continue;
       uint32_t y[NR];
 #pragma unroll
-      for (int c = 0; c < NR; ++c) y[c] = Mma<T>::pack(o[c][2 * h], o[c][2 * h + 1]);
-      store_frag<T, DP>(static_cast<T*>(a.out) + row_offset(a, a.os, b, n, r), t, a.d, y);
-      if (a.lse != nullptr && t == 0) a.lse[stat0 + r] = l[h] == 0.f ? INFINITY : m[h] + log2f(l[h]);
-      if (a.out_f32 != nullptr) {
-        float* f = a.out_f32 + row_dense(a, b, n, r) + t * (DP / 4);
+      for (int c = 0; c < NR; ++c) y[c] = Mma<T>::pack(o[c][2 * e], o[c][2 * e + 1]);
+      store_frag<T, DP>(op + e * o8, t, d, y);
+      if (lse != nullptr && t < HP) {
+        const float ml = HP == 2 && t == 1 ? m[HP - 1][e] : m[0][e], ll = HP == 2 && t == 1 ? l[HP - 1][e] : l[0][e];
+        lse[static_cast<int64_t>(t) * a.Tq + r] = ll == 0.f ? INFINITY : ml + log2f(ll);
+      }
+      if (o32 != nullptr) {
+        float* f = o32 + static_cast<int64_t>(r) * a.heads * a.d;
 #pragma unroll
         for (int c = 0; c < NR; ++c)
-          if (t * (DP / 4) + 2 * c < a.d) *reinterpret_cast<float2*>(f + 2 * c) = make_float2(o[c][2 * h], o[c][2 * h + 1]);
+          if (t * (DP / 4) + 2 * c < d) *reinterpret_cast<float2*>(f + 2 * c) = make_float2(o[c][2 * e], o[c][2 * e + 1]);
       }
     }
+    op += 2 * o8;
   }
 }
 
@@ -826,7 +888,7 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_few(const XAttn a, int) 
   const int steps = (total + 15) / 16, ns = kXmWarps * cl, per = (steps + ns - 1) / ns * 16;
   const int begin = min(total, (rank * kXmWarps + warp) * per), end = min(total, begin + per);
   uint32_t x1[2][NR], x2[2][NR];
-  float xs[2], xd[2];                        // long keys: bias of the key; long rows: lse (and D, found below)
+  float xs[2], xd[2];                        // long keys: bias of the key; long rows: maximum and D, found below
   auto load_long = [&](int i0) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -837,7 +899,6 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_few(const XAttn a, int) 
         xs[h] = ok ? 0.f : -INFINITY;
       } else {
         load_row(i, end, x1[h], x2[h]);
-        xs[h] = i < end ? __ldg(a.lse + stat0 + i) : INFINITY;
       }
     }
   };
@@ -895,16 +956,34 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_few(const XAttn a, int) 
         Mma<T>::run(ds[i], x2[0][c], x2[1][c], x2[0][c + 1], x2[1][c + 1], y2[i][c], y2[i][c + 1]);
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        p[i][e] = ex2f(fmaf(s[e], a.c, FEW_ROWS ? xs[e >> 1] : fs[i][e & 1]) - (FEW_ROWS ? fs[i][e & 1] : xs[e >> 1]));
+      for (int e = 0; e < 4; ++e) {
+        p[i][e] = fmaf(s[e], a.c, FEW_ROWS ? xs[e >> 1] : fs[i][e & 1]);
+        if constexpr (FEW_ROWS) p[i][e] = ex2f(p[i][e] - fs[i][e & 1]);
+      }
     }
     if constexpr (!FEW_ROWS) {
-      // all keys are here: D from p and dp themselves, so that a query with one key has dS = 0 exactly
+      // all keys are here: the whole softmax and D from these logits and dp themselves, so that a query with
+      // one key has p = 1 and dS = 0 exactly, and the forward pass leaves nothing but its inputs
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float f = 0.f;
+        float m = kXmNone, l = 0.f, f = 0.f;
 #pragma unroll
-        for (int i = 0; i < NF; ++i) f = fmaf(p[i][2 * h], ds[i][2 * h], fmaf(p[i][2 * h + 1], ds[i][2 * h + 1], f));
+        for (int i = 0; i < NF; ++i) m = fmaxf(m, fmaxf(p[i][2 * h], p[i][2 * h + 1]));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+#pragma unroll
+        for (int i = 0; i < NF; ++i) {
+          p[i][2 * h] = ex2f(p[i][2 * h] - m), p[i][2 * h + 1] = ex2f(p[i][2 * h + 1] - m);
+          l += p[i][2 * h] + p[i][2 * h + 1];
+        }
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        l = l == 0.f ? 0.f : rcp_fast(l);
+#pragma unroll
+        for (int i = 0; i < NF; ++i) {
+          p[i][2 * h] *= l, p[i][2 * h + 1] *= l;
+          f = fmaf(p[i][2 * h], ds[i][2 * h], fmaf(p[i][2 * h + 1], ds[i][2 * h + 1], f));
+        }
         f += __shfl_xor_sync(0xffffffffu, f, 1);
         xd[h] = f + __shfl_xor_sync(0xffffffffu, f, 2);
       }
@@ -1005,31 +1084,34 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_few(const XAttn a, int) 
     }
   }
 
-  // join the few side's sums of the warps and the cluster
-  auto join = [&](float* acc, void* to_v, float factor, bool first) {
-    constexpr int NREG = NF * NU * 4;
-    if (cl > 1 && !first) cluster_sync_all();          // everybody has read the previous sums
-    warp_tree_sum<NREG>(acc, xsm, warp, lane);
-    __syncthreads();
-    if (warp == 0) {
+  // join the few side's sums of the warps and the cluster, in a fixed order
+  constexpr int N1 = NF * NU * 4, NREG = FEW_ROWS ? N1 : 2 * N1;   // [8][NREG][32]; the block's sums end up in [0]
 #pragma unroll
-      for (int i = 0; i < NREG; ++i) xsm[i * 32 + lane] = acc[i];
+  for (int w = 0; w < N1; ++w) {
+    xsm[(warp * NREG + w) * 32 + lane] = acc1[w / 4 / NU][w / 4 % NU][w % 4];
+    if constexpr (!FEW_ROWS) xsm[(warp * NREG + N1 + w) * 32 + lane] = acc2[w / 4 / NU][w / 4 % NU][w % 4];
+  }
+  __syncthreads();
+  for (int w = warp; w < NREG; w += kXmWarps) {
+    float x = 0.f;
+#pragma unroll
+    for (int z = 0; z < kXmWarps; ++z) x += xsm[(z * NREG + w) * 32 + lane];
+    xsm[w * 32 + lane] = x;                                        // read by this lane only so far
+  }
+  if (cl > 1) cluster_sync_all(); else __syncthreads();
+  const uint32_t base = smem_u32(xsm) + lane * 4;
+  for (int w = rank * kXmWarps + warp; w < NREG; w += cl * kXmWarps) {
+    const bool second = w >= N1;
+    const int v = second ? w - N1 : w, e = v % 4, u = v / 4 % NU, f = v / 4 / NU * 8 + 2 * t + (e & 1);
+    float x = 0.f;
+    for (int z = 0; z < cl; ++z) x += ld_dsmem(mapa_shared(base, z) + w * 128);
+    const int ch = g / 2 * (DP / 4) + 4 * u + g % 2 + (e & 2);
+    T* to = static_cast<T*>(FEW_ROWS ? a.dq : second ? a.dv : a.dk);
+    if (f < (FEW_ROWS ? rows : a.Tk) && ch < a.d && to != nullptr) {
+      const int64_t at = FEW_ROWS ? row_dense(a, b, n, f) : ((static_cast<int64_t>(b) * a.Tk + f) * a.kv_heads + n) * a.d;
+      store1(to + at + ch, x * (second ? 1.f / kP : a.scale));
     }
-    if (cl > 1) cluster_sync_all(); else __syncthreads();
-    const uint32_t base = smem_u32(xsm) + lane * 4;
-    for (int w = rank * kXmWarps + warp; w < NREG; w += cl * kXmWarps) {
-      const int e = w % 4, u = w / 4 % NU, f = w / 4 / NU * 8 + 2 * t + (e & 1);
-      float x = 0.f;
-      for (int z = 0; z < cl; ++z) x += ld_dsmem(mapa_shared(base, z) + w * 128);
-      const int ch = g / 2 * (DP / 4) + 4 * u + g % 2 + (e & 2);
-      if (f < (FEW_ROWS ? rows : a.Tk) && ch < a.d && to_v != nullptr) {
-        const int64_t to = FEW_ROWS ? row_dense(a, b, n, f) : ((static_cast<int64_t>(b) * a.Tk + f) * a.kv_heads + n) * a.d;
-        store1(static_cast<T*>(to_v) + to + ch, x * factor);
-      }
-    }
-  };
-  join(&acc1[0][0][0], FEW_ROWS ? a.dq : a.dk, a.scale, true);
-  if constexpr (!FEW_ROWS) join(&acc2[0][0][0], a.dv, 1.f / kP, false);
+  }
   if (cl > 1) cluster_sync_all();
 }
 
@@ -1214,13 +1296,14 @@ constexpr int kXmFewTiles = 128 / DP;
 template <int DP>
 constexpr int kXmKeyTiles = DP <= 32 ? 8 : 256 / DP;
 
-// Blocks per cluster: enough blocks for two per SM, each warp with at least one step.
+// Blocks per cluster: blocks are added along the long side until every SM has one, while each warp
+// keeps at least one step. (Two per SM measured slower: 64 pairs of 4096 keys forward 17 us against 12,
+// the join outweighs the shorter walks.)
 static int xattn_cluster(int64_t blocks, int other, int step) {
   int c = 1;
-  while (c < 8 && blocks * c < 2 * 148 && other > c * kXmWarps * step) c *= 2;
+  while (c < 8 && blocks * c < 148 && other > c * kXmWarps * step) c *= 2;
   return c;
 }
-
 template <class T, int DP, int MT>
 static int xattn_fwd_mma_launch(const XAttn& a, cudaStream_t stream) {
   const int rows = a.group * a.Tq, tiles = (rows + 16 * MT - 1) / (16 * MT);
@@ -1236,32 +1319,44 @@ static int xattn_fwd_mma_launch(const XAttn& a, cudaStream_t stream) {
                         1);
 }
 
-template <class T, int DP, int NQ>
+template <class T, int DP, int NQ, int HP = 1>
 static int xattn_few_rows_launch(const XAttn& a, cudaStream_t stream) {
   const int rows = a.group * a.Tq, tiles = (rows + 8 * NQ - 1) / (8 * NQ);
-  const int cl = xattn_cluster(static_cast<int64_t>(a.B) * a.kv_heads * tiles, a.Tk, DP <= 32 ? 32 : 16);
-  const size_t smem = (kXmWarps * 8 * NQ + 4 * NQ * (DP / 4 + 2) * 32) * sizeof(float);
-  return launch_cluster(xattn_fwd_few_rows<T, DP, NQ>, dim3(tiles * cl, a.kv_heads, a.B), kXmThreads, smem, cl, stream,
-                        a, 0);
+  const int cl = xattn_cluster(static_cast<int64_t>(a.B) * (a.kv_heads / HP) * tiles, a.Tk, DP <= 32 ? 32 : 16);
+  constexpr size_t smem = (kXmWarps * HP * 8 * NQ + HP * 8 * NQ + kXmWarps * NQ * (DP / 4 + 2) * 32) * sizeof(float);
+  static PerDeviceOnce once;
+  const int st = allow_smem(once, xattn_fwd_few_rows<T, DP, NQ, HP>, smem);
+  if (st != SSAM_OK) return st;
+  return launch_cluster(xattn_fwd_few_rows<T, DP, NQ, HP>, dim3(tiles * cl, a.kv_heads / HP, a.B), kXmThreads, smem, cl,
+                        stream, a, 0);
 }
 
-template <class T, int DP, int NK>
+template <class T, int DP, int NK, int HP = 1>
 static int xattn_few_keys_launch(const XAttn& a, cudaStream_t stream) {
-  const int rows = a.group * a.Tq, tiles = (rows + 15) / 16;
-  const int64_t pairs = static_cast<int64_t>(a.B) * a.kv_heads;
+  const int tiles = (a.Tq + 15) / 16;
+  const int64_t pairs = static_cast<int64_t>(a.B) * (a.heads / HP);
   // row shares: at least 4 tiles each (the K, V fragments are loaded once per share), about 64 warps per SM
   const int64_t want = (148 * 64 + pairs - 1) / pairs;
   const int chunks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, (tiles + 3) / 4)));
   const int64_t blocks = (pairs * chunks + kXmWarps - 1) / kXmWarps;
-  return launch_cluster(xattn_fwd_few_keys<T, DP, NK>, dim3(static_cast<unsigned>(blocks)), kXmThreads, 0, 1, stream, a,
-                        chunks);
+  return launch_cluster(xattn_fwd_few_keys<T, DP, NK, HP>, dim3(static_cast<unsigned>(blocks)), kXmThreads, 0, 1, stream,
+                        a, chunks);
+}
+
+// Heads of 16 that lie side by side in every tensor can be read two at a time.
+static bool xattn_paired(const XAttn& a) {
+  return a.d == 16 && a.group == 1 && a.heads % 2 == 0 && a.qs[2] == 16 && a.ks[2] == 16 && a.vs[2] == 16 && a.os[2] == 16;
 }
 
 template <class T, int DP, int NF, bool FEW_ROWS>
 static int xattn_bwd_few_launch(const XAttn& a, cudaStream_t stream) {
   const int cl = xattn_cluster(static_cast<int64_t>(a.B) * a.kv_heads, FEW_ROWS ? a.Tk : a.group * a.Tq, 16);
-  return launch_cluster(xattn_bwd_few<T, DP, NF, FEW_ROWS>, dim3(cl, a.kv_heads, a.B), kXmThreads,
-                        4 * NF * (DP / 4) * 32 * sizeof(float), cl, stream, a, 0);
+  constexpr size_t smem = kXmWarps * (FEW_ROWS ? 1 : 2) * NF * (DP / 4) * 32 * sizeof(float);
+  static PerDeviceOnce once;
+  const int st = allow_smem(once, xattn_bwd_few<T, DP, NF, FEW_ROWS>, smem);
+  if (st != SSAM_OK) return st;
+  return launch_cluster(xattn_bwd_few<T, DP, NF, FEW_ROWS>, dim3(cl, a.kv_heads, a.B), kXmThreads, smem, cl, stream, a,
+                        0);
 }
 // the smallest instance that holds `few` entries
 template <class T, int DP, bool FEW_ROWS>
@@ -1292,6 +1387,16 @@ template <class T, int DP>
 static int xattn_mma_dp(const XAttn& a, bool backward, cudaStream_t stream) {
   const int rows = a.group * a.Tq;
   if (!backward) {
+    if constexpr (DP == 16) {
+      // two heads to a warp where that leaves every SM a block (and every row 16-byte pieces)
+      if (xattn_paired(a)) {
+        const int64_t pairs = static_cast<int64_t>(a.B) * a.heads;
+        if (a.Tk <= 8) return xattn_few_keys_launch<T, 32, 1, 2>(a, stream);
+        if (a.Tk <= 16) return xattn_few_keys_launch<T, 32, 2, 2>(a, stream);
+        if (a.Tk > 64 && pairs >= 2 * 148 && rows <= 8) return xattn_few_rows_launch<T, 32, 1, 2>(a, stream);
+        if (a.Tk > 64 && pairs >= 2 * 148 && rows <= 16) return xattn_few_rows_launch<T, 32, 2, 2>(a, stream);
+      }
+    }
     if (a.Tk <= 8) return xattn_few_keys_launch<T, DP, 1>(a, stream);
     if (a.Tk <= 16) return xattn_few_keys_launch<T, DP, 2>(a, stream);
     if constexpr (kXmKeyTiles<DP> >= 4) {
@@ -1326,8 +1431,8 @@ static int xattn_mma(const XAttn& a, bool backward, cudaStream_t stream) {
   return xattn_mma_dp<T, 128>(a, backward, stream);
 }
 
-// Whether the backward pass reads out_f32 (else D comes from P and dP, see xattn_bwd_few).
-static bool xattn_uses_out_f32(int Tk, int d, int dtype) {
+// Whether the backward pass reads out_f32 and lse (else it finds them itself, see xattn_bwd_few).
+static bool xattn_uses_stats(int Tk, int d, int dtype) {
   const int dp = d <= 16 ? 16 : d <= 32 ? 32 : d <= 64 ? 64 : 128;
   return dtype == 2 || Tk > 8 * (128 / dp);
 }

@@ -45,6 +45,17 @@ inline int current_device() {
   return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < kMaxDevices ? dev : -1;
 }
 
+// Lets `kernel` be launched with up to `bytes` of dynamic shared memory (once per device).
+template <class K>
+int allow_smem(PerDeviceOnce& once, K kernel, int64_t bytes) {
+  return once.run(current_device(), [&]() -> int {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) ==
+                   cudaSuccess
+               ? SSAM_OK
+               : SSAM_ERR_CUDA;
+  });
+}
+
 // Multiprocessor count of `dev` (cached; 148 on B200).
 int num_sms(int dev);
 
@@ -105,7 +116,7 @@ int patch_im2col_split3(const float* img, int B, int Cin, int H, int W, int p, v
 int cross_attn_fwd(const void* q, const void* k, const void* v, const int64_t* strides, int B, int Tq, int Tk,
                    int heads, int kv_heads, int d, int dtype, float scale, const int32_t* key_lens,
                    const uint8_t* key_mask, void* out, float* out_f32, float* lse, cudaStream_t stream);
-int cross_attn_bwd_uses_out_f32(int Tk, int d, int dtype);
+int cross_attn_bwd_uses_stats(int Tk, int d, int dtype);
 int cross_attn_bwd(const void* q, const void* k, const void* v, const void* dout, const int64_t* strides, int B, int Tq,
                    int Tk, int heads, int kv_heads, int d, int dtype, float scale, const int32_t* key_lens,
                    const uint8_t* key_mask, const float* out_f32, const float* lse, float* delta, void* dq, void* dk,

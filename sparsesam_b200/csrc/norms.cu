@@ -800,13 +800,6 @@ static int groupnorm_check(int N, int64_t HW, int C, int G, int act, int dtype, 
 }
 
 template <class K>
-static int allow_smem(PerDeviceOnce& once, K kernel, int64_t bytes) {
-  return once.run(current_device(), [&] {
-    return status_from_cuda(
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
-  });
-}
-template <class K>
 static int launch_gn(K kernel, PerDeviceOnce& once, dim3 grid, size_t smem, int cluster, cudaStream_t stream,
                      const GnArgs& a) {
   const int st = allow_smem(once, kernel, kGnResident);

@@ -631,7 +631,7 @@ def _strides(a: torch.Tensor, b: torch.Tensor, c: torch.Tensor, d: torch.Tensor)
 
 
 def _cross_attn(q, k, v, scale, key_lens, key_mask, train):
-    """(out, out in fp32 or None, [lse, D] statistics); the last two only for training."""
+    """(out, out in fp32, [lse, D] statistics); the last two only where the backward pass reads them."""
     B, Tq, H, D = q.shape
     Tk, Hk = k.shape[1], k.shape[2]
     out = torch.empty(B, Tq, H, D, dtype=q.dtype, device=q.device)
@@ -639,12 +639,9 @@ def _cross_attn(q, k, v, scale, key_lens, key_mask, train):
         return out.zero_(), None, None
     dt = _DTYPES[q.dtype]
     stats = out32 = None
-    if train:
+    if train and _lib.load().ssam_cross_attn_bwd_uses_stats(Tk, D, dt):
         stats = torch.empty(2, B, H, Tq, dtype=torch.float32, device=q.device)
-        if dt == 2:
-            out32 = out
-        elif _lib.load().ssam_cross_attn_bwd_uses_out_f32(Tk, D, dt):
-            out32 = torch.empty(B, Tq, H, D, dtype=torch.float32, device=q.device)
+        out32 = out if dt == 2 else torch.empty(B, Tq, H, D, dtype=torch.float32, device=q.device)
     _launch("ssam_cross_attn_fwd", q, q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v, out), B, Tq, Tk, H, Hk,
             D, dt, scale, _ptr(key_lens), _ptr(key_mask), out.data_ptr(), None if out32 is out else _ptr(out32),
             _ptr(stats))
@@ -670,16 +667,16 @@ class _CrossAttn(torch.autograd.Function):
         if need[1] or need[2]:
             dk = torch.empty(B, Tk, Hk, D, dtype=q.dtype, device=q.device)
             dv = torch.empty(B, Tk, Hk, D, dtype=q.dtype, device=q.device)
-        if stats is None:     # no queries or no keys: nothing depends on anything
+        if Tk == 0 or q.numel() == 0:     # no keys or no queries: nothing depends on anything
             for g in (dq, dk, dv):
                 if g is not None:
                     g.zero_()
             return dq, dk, dv, None, None, None
         dout = _vector_rows(dout)
-        lse = stats.data_ptr()
+        lse = _ptr(stats)
         _launch("ssam_cross_attn_bwd", q, q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(),
                 _strides(q, k, v, dout), B, Tq, Tk, H, Hk, D, _DTYPES[q.dtype], ctx.scale, _ptr(key_lens), _ptr(key_mask),
-                _ptr(out32), lse, lse + 4 * B * H * Tq, _ptr(dq), _ptr(dk), _ptr(dv))
+                _ptr(out32), lse, None if lse is None else lse + 4 * B * H * Tq, _ptr(dq), _ptr(dk), _ptr(dv))
         return dq, dk, dv, None, None, None
 
 

@@ -36,10 +36,10 @@ def test_cross_attention_abi():
     assert fwd(B=65536) == UNSUP
     assert fwd(q=8) == ALIGN and fwd(out=24) == ALIGN and fwd(out32=20) == ALIGN
     assert fwd(st=strides(12)) == ALIGN and fwd(st=strides(6), dtype=2) == ALIGN
-    assert bwd(q=None) == INV and bwd(dout=None) == INV and bwd(o32=None, dtype=2) == INV and bwd(lse=None) == INV
-    assert bwd(delta=None) == INV and bwd(dk=None) == INV and bwd(dv=None) == INV
+    assert bwd(q=None) == INV and bwd(dout=None) == INV and bwd(o32=None, dtype=2) == INV and bwd(lse=None, dtype=2) == INV
+    assert bwd(delta=None, dtype=2) == INV and bwd(dk=None) == INV and bwd(dv=None) == INV
     assert bwd(dout=8) == ALIGN and bwd(dq=8) == ALIGN and bwd(d=20) == UNSUP and bwd(st=strides(4)) == ALIGN
-    uses = _lib.load().ssam_cross_attn_bwd_uses_out_f32
+    uses = _lib.load().ssam_cross_attn_bwd_uses_stats
     assert uses(64, 16, 0) == 0 and uses(65, 16, 1) == 1 and uses(1, 16, 2) == 1 and uses(9, 72, 0) == 1 and uses(8, 128, 1) == 0
     assert bwd(dq=None, dk=None, dv=None) == 0          # nothing asked for: nothing launched
 
