@@ -1,8 +1,8 @@
 """Builds libsparsesam_b200.so in-tree with nvcc for sm_100a.
 
-The library is a plain C-ABI shared object (no torch headers), compiled from the
-single translation unit csrc/lib.cu. It is rebuilt when any csrc/ or include/
-file is newer than the .so.
+The library is a plain C-ABI shared object (no torch headers), linked from the
+translation units UNITS, which are compiled at the same time. It is rebuilt when
+any csrc/ or include/ file is newer than the .so.
 """
 from __future__ import annotations
 
@@ -10,6 +10,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PKG_DIR)
@@ -18,11 +20,13 @@ INCLUDE = os.path.join(REPO_DIR, "include")
 LIB_NAME = "libsparsesam_b200.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 
+UNITS = ["lib.cu", "cross_attention.cu", "cross_attention_fp16.cu", "cross_attention_bf16.cu", "norms.cu"]
+
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
-    "-shared", "-Xcompiler", "-fPIC",
-    "--expt-relaxed-constexpr", "--split-compile", "0",
+    "-Xcompiler", "-fPIC",
+    "--expt-relaxed-constexpr",
 ]
 
 
@@ -53,16 +57,22 @@ def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | N
     """Compile the library if it is missing or stale; return its path."""
     if not force and not needs_build():
         return LIB_PATH
+    def run(cmd: list[str]) -> None:
+        if verbose:
+            print(" ".join(cmd), file=sys.stderr)
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+        if verbose and (res.stdout or res.stderr):
+            print(res.stdout, res.stderr, file=sys.stderr)
+
     tmp = LIB_PATH + ".tmp"
-    cmd = [_nvcc(), *NVCC_FLAGS, *(extra_flags or []), "-I", INCLUDE,
-           "-o", tmp, os.path.join(CSRC, "lib.cu")]
-    if verbose:
-        print(" ".join(cmd), file=sys.stderr)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
-    if verbose and (res.stdout or res.stderr):
-        print(res.stdout, res.stderr, file=sys.stderr)
+    with tempfile.TemporaryDirectory(prefix="ssam_build_") as work:
+        objects = [os.path.join(work, unit + ".o") for unit in UNITS]
+        with ThreadPoolExecutor(len(UNITS)) as pool:
+            list(pool.map(run, [[_nvcc(), *NVCC_FLAGS, *(extra_flags or []), "-I", INCLUDE, "-c", "-o", obj,
+                                 os.path.join(CSRC, unit)] for unit, obj in zip(UNITS, objects)]))
+        run([_nvcc(), *NVCC_FLAGS, "-shared", "-o", tmp, *objects])
     os.replace(tmp, LIB_PATH)
     return LIB_PATH
 

@@ -14,16 +14,19 @@
 
 namespace ssam {
 
+#ifndef SSAM_NO_WAITS   // translation units whose kernels wait on no barrier leave the flag to lib.cu
 // ---------------------------------------------------------------------------
 // Device error flag. A kernel whose bounded wait runs out writes a non-zero
 // SSAM_ERR_* code here and returns; the host reads it via ssam_device_error().
 // ---------------------------------------------------------------------------
-// Defined here: the library is built as one translation unit (csrc/lib.cu).
+// Defined here: every kernel that waits is in one translation unit (csrc/lib.cu).
 __device__ int g_device_error = 0;
 
 __device__ __forceinline__ void set_device_error(int code) {
   atomicCAS(&g_device_error, 0, code);
 }
+
+#endif
 
 // Upper bound on any spin-wait: about two seconds of GPU time.
 constexpr uint64_t kWaitTimeoutNs = 2000000000ull;
@@ -95,6 +98,7 @@ __device__ __forceinline__ bool mbar_try_wait_sleep(uint64_t* bar, uint32_t pari
   return ok != 0;
 }
 
+#ifndef SSAM_NO_WAITS
 // Bounded wait: suspended try_waits of at most 100 us each, abandoned after 2 s
 // (globaltimer) or 4e9 SM cycles, whichever comes first. Kept out of line; the
 // common case (phase already complete) is tested inline by mbar_wait below.
@@ -114,6 +118,12 @@ __device__ __noinline__ bool mbar_wait_slow(uint64_t* bar, uint32_t parity) {
 // back-to-back tcgen05.mma blocks cost the pair GEMM ~10 % (qkv 2.20 -> 1.96 ms).
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
   return mbar_try_wait(bar, parity) || mbar_wait_slow(bar, parity);
+}
+#endif
+
+// Asynchronous 16-byte copy to shared memory; bytes past src_bytes (0 or 16) are zeros.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t src_bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
 }
 
 // ---------------------------------------------------------------------------
@@ -255,6 +265,18 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
+__device__ __forceinline__ uint32_t cluster_nctarank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+// A float of another CTA's shared memory (shared::cluster address).
+__device__ __forceinline__ float ld_dsmem(uint32_t cluster_addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+  return v;
+}
+
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -318,6 +340,17 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t* bar, uint16_t cta_mas
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
+}
+
+__device__ __forceinline__ float ex2f(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {   // within 1 ulp: for results that are rounded to a half type
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // Packed fp32 pair arithmetic (sm_100: one instruction for two lanes of work).

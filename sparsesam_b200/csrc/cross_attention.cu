@@ -1,90 +1,5 @@
-// Cross attention between two token sets of different lengths (prompt tokens <->
-// image tokens in the mask decoder), forward and backward.
-//
-//   S[r, j] = scale <q_r, k_j>,  P = softmax over the keys that are there,  O = P V
-//   dV = P^T dO,  dP = dO V^T,  D_r = sum_j P dP = <dO_r, O_r>,
-//   dS = P (dP - D),  dQ = scale dS K,  dK = scale dS^T Q
-//
-// q (B, Tq, heads, d), k and v (B, Tk, kv_heads, d): kv_heads divides heads, and
-// query head h reads key head h / (heads / kv_heads). The query heads of one key
-// head are handled as further query rows: row r = g Tq + t of key head n is token t
-// of head n * group + g. Keys at or behind key_lens[b], and keys whose key_mask
-// byte is 0, are not there: their logits are never used and their K and V rows are
-// read as zeros, so whatever they hold (infinities, NaN) reaches no result. A query
-// without keys gives a zero row and zero gradients.
-//
-// Softmax statistics are kept in base 2: m = max of scale log2(e) s, and
-// lse = m + log2(sum 2^(.. - m)), +infinity for a row without keys, which makes
-// every probability of that row 2^-inf = 0 in the backward pass.
-//
-// Work along the long axis is split over the slices of a block and over the blocks
-// of a cluster; the partial results meet in (distributed) shared memory in a fixed
-// order, so results do not depend on scheduling and no workspace is needed.
-#include <cuda_fp16.h>
-
-#include <algorithm>
-
-#include "common.cuh"
-#include "host_util.h"
-
-namespace ssam {
-
-struct XAttn {
-  const void *q, *k, *v, *dout;
-  int64_t qs[3], ks[3], vs[3], os[3];  // element strides (batch, token, head); os: out / dout
-  int B, Tq, Tk, heads, kv_heads, group, d;
-  float scale, c;                      // c = scale * log2(e)
-  const int32_t* key_lens;
-  const uint8_t* key_mask;             // [B, Tk]
-  void* out;
-  float* out_f32;                      // [B, Tq, heads, d]
-  float* lse;                          // [B, heads, Tq]
-  float* delta;                        // [B, heads, Tq]
-  void *dq, *dk, *dv;                  // contiguous
-};
-
-__device__ __forceinline__ int xattn_keys(const XAttn& a, int b) {
-  return a.key_lens == nullptr ? a.Tk : min(max(__ldg(a.key_lens + b), 0), a.Tk);
-}
-
-// cluster-wide helpers
-__device__ __forceinline__ uint32_t cluster_nctarank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ float ld_dsmem(uint32_t cluster_addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
-  return v;
-}
-
-__device__ __forceinline__ float ex2f(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-template <class K>
-static int launch_cluster(K kernel, dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream,
-                          const XAttn& a, int arg) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = cluster;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return status_from_cuda(cudaLaunchKernelEx(&cfg, kernel, a, arg));
-}
-
-}  // namespace ssam
-
-#include "cross_attention_mma.cuh"
+// Cross attention: the entry points and the fp32 kernels (formulas and conventions in cross_attention.cuh).
+#include "cross_attention.cuh"
 
 namespace ssam {
 
@@ -93,55 +8,71 @@ namespace ssam {
 // a row. A block holds RB rows x KS slices of the other axis (RB * KS * TPR = 128).
 // ---------------------------------------------------------------------------
 constexpr int kXThreads = 128;
-constexpr int kXTile = 32;  // entries of the other axis staged at a time
+// entries of the other axis staged at a time (two stages, filled by cp.async)
+template <int DP>
+constexpr int kXTile = DP == 16 ? 128 : DP == 32 ? 64 : DP == 64 ? 32 : 16;
+template <int DP>
+constexpr size_t kXStages = 2 * 2 * kXTile<DP> * (DP + 4) * sizeof(float);
 
-template <int DT, int TPR>
-__device__ __forceinline__ float row_dot(const float (&a)[DT], const float* b) {
-  float s = 0.f;
+// <a, b> in two chains of packed FMAs; every dot product of these kernels has this order, so that with one
+// key dP and D are the same number.
+template <int DT, int TPR, class B>
+__device__ __forceinline__ float row_dot(const float2 (&a)[DT / 2], B b) {
+  float2 s0 = make_float2(0.f, 0.f), s1 = s0;
 #pragma unroll
-  for (int i = 0; i < DT; i += 4) {
-    const float4 v = *reinterpret_cast<const float4*>(b + i);
-    s = fmaf(a[i], v.x, s);
-    s = fmaf(a[i + 1], v.y, s);
-    s = fmaf(a[i + 2], v.z, s);
-    s = fmaf(a[i + 3], v.w, s);
+  for (int i = 0; i < DT / 2; i += 2) {
+    const float4 v = b(i / 2);
+    s0 = fma2(a[i], make_float2(v.x, v.y), s0);
+    s1 = fma2(a[i + 1], make_float2(v.z, v.w), s1);
   }
+  s0 = add2(s0, s1);
+  float s = s0.x + s0.y;
 #pragma unroll
   for (int o = 1; o < TPR; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   return s;
 }
+template <int DT, int TPR>
+__device__ __forceinline__ float row_dot(const float2 (&a)[DT / 2], const float* b) {
+  return row_dot<DT, TPR>(a, [b](int i) { return *reinterpret_cast<const float4*>(b + 4 * i); });
+}
 template <int DT>
-__device__ __forceinline__ void row_axpy(float w, const float* b, float (&acc)[DT]) {
+__device__ __forceinline__ void row_axpy(float w, const float* b, float2 (&acc)[DT / 2]) {
+  const float2 w2 = make_float2(w, w);
 #pragma unroll
-  for (int i = 0; i < DT; i += 4) {
-    const float4 v = *reinterpret_cast<const float4*>(b + i);
-    acc[i] = fmaf(w, v.x, acc[i]);
-    acc[i + 1] = fmaf(w, v.y, acc[i + 1]);
-    acc[i + 2] = fmaf(w, v.z, acc[i + 2]);
-    acc[i + 3] = fmaf(w, v.w, acc[i + 3]);
+  for (int i = 0; i < DT / 2; i += 2) {
+    const float4 v = *reinterpret_cast<const float4*>(b + 2 * i);
+    acc[i] = fma2(w2, make_float2(v.x, v.y), acc[i]);
+    acc[i + 1] = fma2(w2, make_float2(v.z, v.w), acc[i + 1]);
   }
 }
 template <int DT>
-__device__ __forceinline__ void load_row(const float* p, int dims, bool ok, float (&r)[DT]) {
+__device__ __forceinline__ void load_row(const float* p, int dims, bool ok, float2 (&r)[DT / 2]) {
 #pragma unroll
   for (int i = 0; i < DT; i += 4) {
     const float4 v = ok && i < dims ? __ldg(reinterpret_cast<const float4*>(p + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
-    r[i] = v.x, r[i + 1] = v.y, r[i + 2] = v.z, r[i + 3] = v.w;
+    r[i / 2] = make_float2(v.x, v.y), r[i / 2 + 1] = make_float2(v.z, v.w);
   }
 }
+template <int DT>
+__device__ __forceinline__ void clear_row(float2 (&r)[DT / 2]) {
+#pragma unroll
+  for (int i = 0; i < DT / 2; ++i) r[i] = make_float2(0.f, 0.f);
+}
 
-// Copies `n` rows (<= kXTile) of width d into sm[kXTile][LD] as floats; rows for
-// which ok(i) is false, and channels past d, are zero.
+// Starts the copy of `n` rows of width d into sm[kXTile][DP + 4]; rows n .. kXTile - 1, rows for which ok(i) is
+// false, and channels past d, are zeros.
 template <int DP, class P, class O>
 __device__ __forceinline__ void stage_rows(float* sm, int n, int d, P row, O ok) {
   constexpr int V = DP / 4, LD = DP + 4;
-  for (int e = threadIdx.x; e < kXTile * V; e += kXThreads) {
-    const int i = e / V, c = (e % V) * 4;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (i < n && c < d && ok(i)) v = __ldg(reinterpret_cast<const float4*>(row(i) + c));
-    *reinterpret_cast<float4*>(sm + i * LD + c) = v;
+#pragma unroll
+  for (int e0 = 0; e0 < kXTile<DP> * V; e0 += kXThreads) {
+    const int e = e0 + threadIdx.x, i = e / V, c = (e % V) * 4;
+    const bool there = i < n && c < d && ok(i);
+    cp_async16(smem_u32(sm + i * LD + c), there ? row(i) + c : row(0), there ? 16u : 0u);
   }
 }
+__device__ __forceinline__ void stage_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void stage_wait() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
 
 // Sum over the KS slices of the block and the blocks of the cluster of part[slice][row][W]:
 // the block's slices are summed into slice 0, then the cluster's blocks each take a share
@@ -171,53 +102,95 @@ __device__ __forceinline__ void merge_sums(float* part, int KS, int RB, int W, E
   cluster_sync_all();
 }
 
+// What the two row kernels share: a block's place, and the walk over its keys. body(tile of K, tile of V, keys of
+// the tile rounded up to the slices, there) is called with the tile in shared memory.
+struct XPlace {
+  int part, lr, slice, KS, b, n, cl, rank, rows, r0, r, t, h;
+  bool row_ok;
+  __device__ __forceinline__ XPlace(const XAttn& a, int RB, int TPR) {
+    KS = kXThreads / (RB * TPR);
+    part = threadIdx.x % TPR, lr = threadIdx.x / TPR % RB, slice = threadIdx.x / (TPR * RB);
+    b = blockIdx.z, n = blockIdx.y;
+    cl = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
+    rows = a.group * a.Tq;
+    r0 = static_cast<int>(blockIdx.x) / cl * RB, r = r0 + lr;
+    const int g = r / a.Tq;
+    t = r - g * a.Tq, h = n * a.group + g;
+    row_ok = r < rows;
+  }
+};
+template <int DP, class B>
+__device__ __forceinline__ void walk_keys(const XAttn& a, const XPlace& x, float* xsm, uint8_t (&there)[2][kXTile<DP>], B body) {
+  constexpr int XT = kXTile<DP>, LD = DP + 4;
+  const int keys = xattn_keys(a, x.b);
+  const float* kb = static_cast<const float*>(a.k) + x.b * a.ks[0] + x.n * a.ks[2];
+  const float* vb = static_cast<const float*>(a.v) + x.b * a.vs[0] + x.n * a.vs[2];
+  const uint8_t* mask = a.key_mask == nullptr ? nullptr : a.key_mask + static_cast<int64_t>(x.b) * a.Tk;
+  auto stage = [&](int j0, int buf) {
+    if (j0 < keys) {
+      const int nk = min(XT, keys - j0);
+      auto ok = [&](int i) { return mask == nullptr || __ldg(mask + j0 + i) != 0; };
+      float* to = xsm + buf * 2 * XT * LD;
+      stage_rows<DP>(to, nk, a.d, [&](int i) { return kb + (j0 + i) * a.ks[1]; }, ok);
+      stage_rows<DP>(to + XT * LD, nk, a.d, [&](int i) { return vb + (j0 + i) * a.vs[1]; }, ok);
+      if (threadIdx.x < XT) there[buf][threadIdx.x] = threadIdx.x < nk && ok(threadIdx.x);
+    }
+    stage_commit();
+  };
+  stage(x.rank * XT, 0);
+  int buf = 0;
+  for (int j0 = x.rank * XT; j0 < keys; j0 += x.cl * XT, buf ^= 1) {
+    stage(j0 + x.cl * XT, buf ^ 1);
+    stage_wait();
+    __syncthreads();
+    const float* sk = xsm + buf * 2 * XT * LD;
+    body(sk, sk + XT * LD, (min(XT, keys - j0) + x.KS - 1) / x.KS * x.KS, there[buf]);
+    __syncthreads();                         // the other buffer is filled next
+  }
+}
+
 template <int DT, int TPR>
 __global__ void __launch_bounds__(kXThreads) xattn_fwd_scalar(const XAttn a, int RB) {
-  constexpr int DP = DT * TPR, LD = DP + 4;
+  constexpr int DP = DT * TPR, LD = DP + 4, U = 4;
   extern __shared__ __align__(16) float xsm[];
-  float *sk = xsm, *sv = xsm + kXTile * LD;
-  __shared__ uint8_t there[kXTile];
-  const int KS = kXThreads / (RB * TPR);
-  const int part = threadIdx.x % TPR, lr = (threadIdx.x / TPR) % RB, slice = threadIdx.x / (TPR * RB);
-  const int b = blockIdx.z, n = blockIdx.y;
-  const int cl = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
-  const int rows = a.group * a.Tq;
-  const int r0 = (blockIdx.x / cl) * RB, r = r0 + lr;
-  const int g = r / a.Tq, t = r - g * a.Tq, h = n * a.group + g;
-  const bool row_ok = r < rows;
-  const int dims = a.d - part * DT;
-  float q[DT], o[DT];
-  load_row<DT>(static_cast<const float*>(a.q) + b * a.qs[0] + t * a.qs[1] + h * a.qs[2] + part * DT, dims, row_ok, q);
-#pragma unroll
-  for (int i = 0; i < DT; ++i) o[i] = 0.f;
+  __shared__ uint8_t there[2][kXTile<DP>];
+  const XPlace x(a, RB, TPR);
+  const int part = x.part, lr = x.lr, slice = x.slice, KS = x.KS, b = x.b, n = x.n, cl = x.cl, rank = x.rank, rows = x.rows,
+            r0 = x.r0;
+  float2 q[DT / 2], o[DT / 2];
+  load_row<DT>(static_cast<const float*>(a.q) + b * a.qs[0] + x.t * a.qs[1] + x.h * a.qs[2] + part * DT, a.d - part * DT,
+               x.row_ok, q);
+  clear_row<DT>(o);
   float m = -INFINITY, l = 0.f;
-  const int keys = xattn_keys(a, b);
-  const float* kb = static_cast<const float*>(a.k) + b * a.ks[0] + n * a.ks[2];
-  const float* vb = static_cast<const float*>(a.v) + b * a.vs[0] + n * a.vs[2];
-  const uint8_t* mask = a.key_mask == nullptr ? nullptr : a.key_mask + static_cast<int64_t>(b) * a.Tk;
-  for (int j0 = rank * kXTile; j0 < keys; j0 += cl * kXTile) {
-    const int nk = min(kXTile, keys - j0);
-    auto ok = [&](int i) { return mask == nullptr || __ldg(mask + j0 + i) != 0; };
-    __syncthreads();
-    stage_rows<DP>(sk, nk, a.d, [&](int i) { return kb + (j0 + i) * a.ks[1]; }, ok);
-    stage_rows<DP>(sv, nk, a.d, [&](int i) { return vb + (j0 + i) * a.vs[1]; }, ok);
-    if (threadIdx.x < kXTile) there[threadIdx.x] = threadIdx.x < nk && ok(threadIdx.x);
-    __syncthreads();
-    for (int j = slice; j < kXTile; j += KS) {
-      const float s = row_dot<DT, TPR>(q, sk + j * LD + part * DT) * a.c;
-      if (!there[j]) continue;
-      if (s > m) {
-        const float f = ex2f(m - s);
+  walk_keys<DP>(a, x, xsm, there, [&](const float* sk, const float* sv, int nk, const uint8_t* here) {
+    for (int j = slice; j < nk; j += U * KS) {           // U keys at a time: one look at the maximum
+      float s[U], top = m;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        s[u] = -INFINITY;
+        if (j - slice + u * KS < nk) {                   // the same for all threads
+          const int i = j + u * KS;
+          const float y = row_dot<DT, TPR>(q, sk + i * LD + part * DT) * a.c;
+          if (here[i]) s[u] = y;
+        }
+        top = fmaxf(top, s[u]);
+      }
+      if (top > m) {
+        const float f = ex2f(m - top);
         l *= f;
 #pragma unroll
-        for (int i = 0; i < DT; ++i) o[i] *= f;
-        m = s;
+        for (int i = 0; i < DT / 2; ++i) o[i] = mul2(o[i], make_float2(f, f));
+        m = top;
       }
-      const float p = s == -INFINITY ? 0.f : ex2f(s - m);  // a NaN logit stays one
-      l += p;
-      row_axpy<DT>(p, sv + j * LD + part * DT, o);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (j - slice + u * KS >= nk) break;
+        const float p = s[u] == -INFINITY ? 0.f : ex2f(s[u] - m);  // a NaN logit stays one
+        l += p;
+        row_axpy<DT>(p, sv + (j + u * KS) * LD + part * DT, o);
+      }
     }
-  }
+  });
   // join the slices and blocks: rescale everybody's share to the common maximum first
   __syncthreads();
   float* ms = xsm;                       // [KS][RB]
@@ -237,7 +210,7 @@ __global__ void __launch_bounds__(kXThreads) xattn_fwd_scalar(const XAttn a, int
   const float f = m == -INFINITY ? 0.f : ex2f(m - top);
   float* mine = acc + (slice * RB + lr) * W;
 #pragma unroll
-  for (int i = 0; i < DT; ++i) mine[part * DT + i] = o[i] * f;
+  for (int i = 0; i < DT / 2; ++i) mine[part * DT + 2 * i] = o[i].x * f, mine[part * DT + 2 * i + 1] = o[i].y * f;
   if (part == 0) mine[DP] = l * f;
   // the sums, then the division: the row's denominator is summed with its entries
   __syncthreads();
@@ -287,74 +260,45 @@ template <int DT, int TPR>
 __global__ void __launch_bounds__(kXThreads) xattn_dq_scalar(const XAttn a, int RB) {
   constexpr int DP = DT * TPR, LD = DP + 4;
   extern __shared__ __align__(16) float xsm[];
-  float *sk = xsm, *sv = xsm + kXTile * LD;
-  __shared__ uint8_t there[kXTile];
-  const int KS = kXThreads / (RB * TPR);
-  const int part = threadIdx.x % TPR, lr = (threadIdx.x / TPR) % RB, slice = threadIdx.x / (TPR * RB);
-  const int b = blockIdx.z, n = blockIdx.y;
-  const int cl = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
-  const int rows = a.group * a.Tq;
-  const int r0 = (blockIdx.x / cl) * RB, r = r0 + lr;
-  const int g = r / a.Tq, t = r - g * a.Tq, h = n * a.group + g;
-  const bool row_ok = r < rows;
-  const int dims = a.d - part * DT;
-  float q[DT], dO[DT], dq[DT];
-  load_row<DT>(static_cast<const float*>(a.q) + b * a.qs[0] + t * a.qs[1] + h * a.qs[2] + part * DT, dims, row_ok, q);
-  load_row<DT>(static_cast<const float*>(a.dout) + b * a.os[0] + t * a.os[1] + h * a.os[2] + part * DT, dims, row_ok,
-                  dO);
-  const int64_t stat = (static_cast<int64_t>(b) * a.heads + h) * a.Tq + t;
-  // D in the order of dP's sum, so that a row with one key has dP - D = 0 exactly
-  load_row<DT>(a.out_f32 + ((static_cast<int64_t>(b) * a.Tq + t) * a.heads + h) * a.d + part * DT, dims, row_ok,
-                      dq);
-  float delta = 0.f;
-#pragma unroll
-  for (int i = 0; i < DT; ++i) delta = fmaf(dO[i], dq[i], delta);
-#pragma unroll
-  for (int o = 1; o < TPR; o <<= 1) delta += __shfl_xor_sync(0xffffffffu, delta, o);
-  const float lse = row_ok ? a.lse[stat] : INFINITY;
-  if (row_ok && part == 0 && slice == 0 && rank == 0) a.delta[stat] = delta;
-#pragma unroll
-  for (int i = 0; i < DT; ++i) dq[i] = 0.f;
-  if (a.dq != nullptr) {
-    const int keys = xattn_keys(a, b);
-    const float* kb = static_cast<const float*>(a.k) + b * a.ks[0] + n * a.ks[2];
-    const float* vb = static_cast<const float*>(a.v) + b * a.vs[0] + n * a.vs[2];
-    const uint8_t* mask = a.key_mask == nullptr ? nullptr : a.key_mask + static_cast<int64_t>(b) * a.Tk;
-    for (int j0 = rank * kXTile; j0 < keys; j0 += cl * kXTile) {
-      const int nk = min(kXTile, keys - j0);
-      auto ok = [&](int i) { return mask == nullptr || __ldg(mask + j0 + i) != 0; };
-      __syncthreads();
-      stage_rows<DP>(sk, nk, a.d, [&](int i) { return kb + (j0 + i) * a.ks[1]; }, ok);
-      stage_rows<DP>(sv, nk, a.d, [&](int i) { return vb + (j0 + i) * a.vs[1]; }, ok);
-      if (threadIdx.x < kXTile) there[threadIdx.x] = threadIdx.x < nk && ok(threadIdx.x);
-      __syncthreads();
-      for (int j = slice; j < kXTile; j += KS) {
-        const float s = row_dot<DT, TPR>(q, sk + j * LD + part * DT) * a.c;
-        const float dp = row_dot<DT, TPR>(dO, sv + j * LD + part * DT);
-        if (!there[j]) continue;
-        row_axpy<DT>(ex2f(s - lse) * (dp - delta), sk + j * LD + part * DT, dq);
-      }
+  __shared__ uint8_t there[2][kXTile<DP>];
+  const XPlace x(a, RB, TPR);
+  const int part = x.part, slice = x.slice, KS = x.KS, b = x.b, dims = a.d - x.part * DT;
+  float2 q[DT / 2], dO[DT / 2], dq[DT / 2];
+  load_row<DT>(static_cast<const float*>(a.q) + b * a.qs[0] + x.t * a.qs[1] + x.h * a.qs[2] + part * DT, dims, x.row_ok, q);
+  load_row<DT>(static_cast<const float*>(a.dout) + b * a.os[0] + x.t * a.os[1] + x.h * a.os[2] + part * DT, dims, x.row_ok, dO);
+  const int64_t stat = (static_cast<int64_t>(b) * a.heads + x.h) * a.Tq + x.t;
+  load_row<DT>(a.out_f32 + ((static_cast<int64_t>(b) * a.Tq + x.t) * a.heads + x.h) * a.d + part * DT, dims, x.row_ok, dq);
+  const float delta = row_dot<DT, TPR>(dO, [&](int i) { return make_float4(dq[2 * i].x, dq[2 * i].y, dq[2 * i + 1].x, dq[2 * i + 1].y); });
+  const float lse = x.row_ok ? a.lse[stat] : INFINITY;
+  if (x.row_ok && part == 0 && slice == 0 && x.rank == 0) a.delta[stat] = delta;
+  if (a.dq == nullptr) return;               // only D was wanted
+  clear_row<DT>(dq);
+  walk_keys<DP>(a, x, xsm, there, [&](const float* sk, const float* sv, int nk, const uint8_t* here) {
+#pragma unroll 1
+    for (int j = slice; j < nk; j += KS) {
+      const float s = row_dot<DT, TPR>(q, sk + j * LD + part * DT) * a.c;
+      const float dp = row_dot<DT, TPR>(dO, sv + j * LD + part * DT);
+      row_axpy<DT>(here[j] ? ex2f(s - lse) * (dp - delta) : 0.f, sk + j * LD + part * DT, dq);
     }
-    __syncthreads();
-    float* mine = xsm + (slice * RB + lr) * DP + part * DT;
+  });
+  __syncthreads();
+  float* mine = xsm + (slice * RB + x.lr) * DP + part * DT;
 #pragma unroll
-    for (int i = 0; i < DT; ++i) mine[i] = dq[i];
-    merge_sums(xsm, KS, RB, DP, [&](int er, int col, float s) {
-      const int rr = r0 + er;
-      if (rr >= rows || col >= a.d) return;
-      const int eg = rr / a.Tq, et = rr - eg * a.Tq, eh = n * a.group + eg;
-      *(static_cast<float*>(a.dq) + ((static_cast<int64_t>(b) * a.Tq + et) * a.heads + eh) * a.d + col) = s * a.scale;
-    });
-  }
+  for (int i = 0; i < DT / 2; ++i) mine[2 * i] = dq[i].x, mine[2 * i + 1] = dq[i].y;
+  merge_sums(xsm, KS, RB, DP, [&](int er, int col, float s) {
+    const int rr = x.r0 + er;
+    if (rr >= x.rows || col >= a.d) return;
+    const int eg = rr / a.Tq, et = rr - eg * a.Tq, eh = x.n * a.group + eg;
+    static_cast<float*>(a.dq)[((static_cast<int64_t>(b) * a.Tq + et) * a.heads + eh) * a.d + col] = s * a.scale;
+  });
 }
 
 // dK, dV: a thread owns (part of) one key; the block's slices walk the query rows.
 template <int DT, int TPR>
 __global__ void __launch_bounds__(kXThreads) xattn_dkv_scalar(const XAttn a, int RB) {
-  constexpr int DP = DT * TPR, LD = DP + 4;
+  constexpr int DP = DT * TPR, LD = DP + 4, XT = kXTile<DP>;
   extern __shared__ __align__(16) float xsm[];
-  float *sq = xsm, *so = xsm + kXTile * LD;
-  __shared__ float s_lse[kXTile], s_delta[kXTile];
+  __shared__ float s_lse[2][XT], s_delta[2][XT];
   const int KS = kXThreads / (RB * TPR);
   const int part = threadIdx.x % TPR, lr = (threadIdx.x / TPR) % RB, slice = threadIdx.x / (TPR * RB);
   const int b = blockIdx.z, n = blockIdx.y;
@@ -364,41 +308,55 @@ __global__ void __launch_bounds__(kXThreads) xattn_dkv_scalar(const XAttn a, int
   const bool key_ok = j < xattn_keys(a, b) &&
                       (a.key_mask == nullptr || __ldg(a.key_mask + static_cast<int64_t>(b) * a.Tk + j) != 0);
   const int dims = a.d - part * DT;
-  float k[DT], v[DT], dk[DT], dv[DT];
+  float2 k[DT / 2], v[DT / 2], dk[DT / 2], dv[DT / 2];
   load_row<DT>(static_cast<const float*>(a.k) + b * a.ks[0] + j * a.ks[1] + n * a.ks[2] + part * DT, dims, key_ok, k);
   load_row<DT>(static_cast<const float*>(a.v) + b * a.vs[0] + j * a.vs[1] + n * a.vs[2] + part * DT, dims, key_ok, v);
-#pragma unroll
-  for (int i = 0; i < DT; ++i) dk[i] = 0.f, dv[i] = 0.f;
-  for (int r0 = rank * kXTile; r0 < rows; r0 += cl * kXTile) {
-    const int nr = min(kXTile, rows - r0);
-    auto at = [&](int i, const int64_t (&st)[3]) {
-      const int r = r0 + i, g = r / a.Tq, t = r - g * a.Tq;
-      return b * st[0] + t * st[1] + (n * a.group + g) * st[2];
-    };
-    auto ok = [](int) { return true; };
-    __syncthreads();
-    stage_rows<DP>(sq, nr, a.d, [&](int i) { return static_cast<const float*>(a.q) + at(i, a.qs); }, ok);
-    stage_rows<DP>(so, nr, a.d, [&](int i) { return static_cast<const float*>(a.dout) + at(i, a.os); }, ok);
-    if (threadIdx.x < kXTile) {
-      const int i = threadIdx.x, r = r0 + i, g = r / a.Tq, t = r - g * a.Tq;
-      const int64_t stat = (static_cast<int64_t>(b) * a.heads + n * a.group + g) * a.Tq + t;
-      s_lse[i] = i < nr ? a.lse[stat] : INFINITY;
-      s_delta[i] = i < nr ? a.delta[stat] : 0.f;
+  clear_row<DT>(dk);
+  clear_row<DT>(dv);
+  auto stage = [&](int r0, int buf) {
+    if (r0 < rows) {
+      const int nr = min(XT, rows - r0);
+      auto at = [&](int i, const int64_t (&st)[3]) {
+        const int r = r0 + i, g = a.group == 1 ? 0 : r / a.Tq, t = r - g * a.Tq;
+        return b * st[0] + t * st[1] + (n * a.group + g) * st[2];
+      };
+      auto ok = [](int) { return true; };
+      float* to = xsm + buf * 2 * XT * LD;
+      stage_rows<DP>(to, nr, a.d, [&](int i) { return static_cast<const float*>(a.q) + at(i, a.qs); }, ok);
+      stage_rows<DP>(to + XT * LD, nr, a.d, [&](int i) { return static_cast<const float*>(a.dout) + at(i, a.os); }, ok);
+      const int64_t stat = (static_cast<int64_t>(b) * a.heads + n * a.group) * a.Tq + r0;   // rows of a key head follow one another
+      if (threadIdx.x < XT) {
+        s_lse[buf][threadIdx.x] = threadIdx.x < nr ? a.lse[stat + threadIdx.x] : INFINITY;
+        s_delta[buf][threadIdx.x] = threadIdx.x < nr ? a.delta[stat + threadIdx.x] : 0.f;
+      }
     }
+    stage_commit();
+  };
+  stage(rank * XT, 0);
+  int buf = 0;
+  for (int r0 = rank * XT; r0 < rows; r0 += cl * XT, buf ^= 1) {
+    stage(r0 + cl * XT, buf ^ 1);
+    stage_wait();
     __syncthreads();
-    for (int i = slice; i < kXTile; i += KS) {
+    const float *sq = xsm + buf * 2 * XT * LD, *so = sq + XT * LD;
+    const int nr = (min(XT, rows - r0) + KS - 1) / KS * KS;      // entries behind the last have p = 2^-inf = 0
+#pragma unroll 1
+    for (int i = slice; i < nr; i += KS) {
       const float s = row_dot<DT, TPR>(k, sq + i * LD + part * DT) * a.c;
       const float dp = row_dot<DT, TPR>(v, so + i * LD + part * DT);
-      if (!key_ok || i >= nr) continue;
-      const float p = ex2f(s - s_lse[i]);
+      const float p = key_ok ? ex2f(s - s_lse[buf][i]) : 0.f;
       row_axpy<DT>(p, so + i * LD + part * DT, dv);
-      row_axpy<DT>(p * (dp - s_delta[i]), sq + i * LD + part * DT, dk);
+      row_axpy<DT>(p * (dp - s_delta[buf][i]), sq + i * LD + part * DT, dk);
     }
+    __syncthreads();
   }
   __syncthreads();
   float* mine = xsm + (slice * RB + lr) * (2 * DP) + part * DT;
 #pragma unroll
-  for (int i = 0; i < DT; ++i) mine[i] = dk[i], mine[DP + i] = dv[i];
+  for (int i = 0; i < DT / 2; ++i) {
+    mine[2 * i] = dk[i].x, mine[2 * i + 1] = dk[i].y;
+    mine[DP + 2 * i] = dv[i].x, mine[DP + 2 * i + 1] = dv[i].y;
+  }
   merge_sums(xsm, KS, RB, 2 * DP, [&](int er, int col, float s) {
     const int jj = j0 + er, c = col % DP;
     if (jj >= a.Tk || c >= a.d) return;
@@ -411,45 +369,44 @@ __global__ void __launch_bounds__(kXThreads) xattn_dkv_scalar(const XAttn a, int
 }
 
 // Launch
-// Rows per block (a power of two, at most 128 / tpr) and blocks per cluster for `own` rows that
-// each walk `other` entries: blocks are added along `other` until the device is filled.
-static void xattn_plan(int own, int other, int64_t pairs, int tpr, int* rb, int* cluster) {
+// Rows per block (a power of two, at most 128 / tpr) and blocks per cluster for `own` rows that each walk `other`
+// entries, `tile` at a time: blocks are added along `other` until the device is filled.
+static void xattn_plan(int own, int other, int64_t pairs, int tpr, int tile, int* rb, int* cluster) {
   int r = 4;
   while (r < own && r < kXThreads / tpr) r *= 2;
   const int64_t blocks = pairs * ((own + r - 1) / r);
   int c = 1;
-  while (c < 8 && blocks * c < 2 * 148 && other > c * kXTile) c *= 2;
+  while (c < 8 && blocks * c < 2 * 148 && other > c * tile) c *= 2;
   *rb = r;
   *cluster = c;
 }
 
 template <int DT, int TPR>
 static int xattn_scalar(const XAttn& a, bool backward, cudaStream_t stream) {
-  constexpr int DP = DT * TPR;
-  const size_t tiles = 2 * kXTile * (DP + 4) * sizeof(float);
+  constexpr int DP = DT * TPR, XT = kXTile<DP>;
+  constexpr size_t stages = kXStages<DP>;
   const int64_t pairs = static_cast<int64_t>(a.B) * a.kv_heads;
   const int rows = a.group * a.Tq;
   int rb, cl;
+  xattn_plan(rows, a.Tk, pairs, TPR, XT, &rb, &cl);
+  const dim3 by_rows((rows + rb - 1) / rb * cl, a.kv_heads, a.B);
   if (!backward) {
-    xattn_plan(rows, a.Tk, pairs, TPR, &rb, &cl);
-    const size_t merge = (kXThreads + kXThreads / TPR * (DP + 1)) * sizeof(float);
-    return launch_cluster(xattn_fwd_scalar<DT, TPR>, dim3((rows + rb - 1) / rb * cl, a.kv_heads, a.B), kXThreads,
-                          tiles > merge ? tiles : merge, cl, stream, a, rb);
+    constexpr size_t merge = (kXThreads + kXThreads / TPR * (DP + 1)) * sizeof(float);
+    static_assert(merge <= 48 << 10 && stages <= 48 << 10, "no opt-in needed");
+    return launch_cluster(xattn_fwd_scalar<DT, TPR>, by_rows, kXThreads, stages > merge ? stages : merge, cl, stream, a, rb);
   }
-  xattn_plan(rows, a.Tk, pairs, TPR, &rb, &cl);
-  size_t merge = kXThreads / TPR * DP * sizeof(float);
-  int st = launch_cluster(xattn_dq_scalar<DT, TPR>, dim3((rows + rb - 1) / rb * cl, a.kv_heads, a.B), kXThreads,
-                          tiles > merge ? tiles : merge, cl, stream, a, rb);
+  constexpr size_t merge = kXThreads / TPR * 2 * DP * sizeof(float);
+  static_assert(merge <= 48 << 10, "no opt-in needed");
+  const int st = launch_cluster(xattn_dq_scalar<DT, TPR>, by_rows, kXThreads, stages > merge ? stages : merge, cl, stream, a, rb);
   if (st != SSAM_OK || a.dk == nullptr) return st;
-  xattn_plan(a.Tk, rows, pairs, TPR, &rb, &cl);
-  merge = kXThreads / TPR * 2 * DP * sizeof(float);
+  xattn_plan(a.Tk, rows, pairs, TPR, XT, &rb, &cl);
   return launch_cluster(xattn_dkv_scalar<DT, TPR>, dim3((a.Tk + rb - 1) / rb * cl, a.kv_heads, a.B), kXThreads,
-                        tiles > merge ? tiles : merge, cl, stream, a, rb);
+                        stages > merge ? stages : merge, cl, stream, a, rb);
 }
 
 static int xattn_dispatch(const XAttn& a, int dtype, bool backward, cudaStream_t stream) {
-  if (dtype == 0) return xattn_mma<__half>(a, backward, stream);
-  if (dtype == 1) return xattn_mma<__nv_bfloat16>(a, backward, stream);
+  if (dtype == 0) return xattn_fp16(a, backward, stream);
+  if (dtype == 1) return xattn_bf16(a, backward, stream);
   if (a.d <= 16) return xattn_scalar<16, 1>(a, backward, stream);
   if (a.d <= 32) return xattn_scalar<32, 1>(a, backward, stream);
   if (a.d <= 64) return xattn_scalar<32, 2>(a, backward, stream);

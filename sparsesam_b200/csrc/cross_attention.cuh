@@ -1,0 +1,90 @@
+// Cross attention between two token sets of different lengths (prompt tokens <->
+// image tokens in the mask decoder), forward and backward.
+//
+//   S[r, j] = scale <q_r, k_j>,  P = softmax over the keys that are there,  O = P V
+//   dV = P^T dO,  dP = dO V^T,  D_r = sum_j P dP = <dO_r, O_r>,
+//   dS = P (dP - D),  dQ = scale dS K,  dK = scale dS^T Q
+//
+// q (B, Tq, heads, d), k and v (B, Tk, kv_heads, d): kv_heads divides heads, and
+// query head h reads key head h / (heads / kv_heads). The query heads of one key
+// head are handled as further query rows: row r = g Tq + t of key head n is token t
+// of head n * group + g. Keys at or behind key_lens[b], and keys whose key_mask
+// byte is 0, are not there: their logits are never used and their K and V rows are
+// read as zeros, so whatever they hold (infinities, NaN) reaches no result. A query
+// without keys gives a zero row and zero gradients.
+//
+// Softmax statistics are kept in base 2: m = max of scale log2(e) s, and
+// lse = m + log2(sum 2^(.. - m)), +infinity for a row without keys, which makes
+// every probability of that row 2^-inf = 0 in the backward pass.
+//
+// Work along the long axis is split over the slices of a block and over the blocks
+// of a cluster; the partial results meet in (distributed) shared memory in a fixed
+// order, so results do not depend on scheduling and no workspace is needed.
+//
+// This header: what the translation units of the operator share (cross_attention.cu: entry points and the
+// fp32 kernels; cross_attention_fp16.cu, _bf16.cu: the tensor-core kernels).
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#define SSAM_NO_WAITS
+#include "common.cuh"
+#include "host_util.h"
+
+namespace ssam {
+
+struct XAttn {
+  const void *q, *k, *v, *dout;
+  int64_t qs[3], ks[3], vs[3], os[3];  // element strides (batch, token, head); os: out / dout
+  int B, Tq, Tk, heads, kv_heads, group, d;
+  float scale, c;                      // c = scale * log2(e)
+  const int32_t* key_lens;
+  const uint8_t* key_mask;             // [B, Tk]
+  void* out;
+  float* out_f32;                      // [B, Tq, heads, d]
+  float* lse;                          // [B, heads, Tq]
+  float* delta;                        // [B, heads, Tq]
+  void *dq, *dk, *dv;                  // contiguous
+};
+
+__device__ __forceinline__ int xattn_keys(const XAttn& a, int b) {
+  return a.key_lens == nullptr ? a.Tk : min(max(__ldg(a.key_lens + b), 0), a.Tk);
+}
+
+template <class K>
+static int launch_cluster(K kernel, dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream,
+                          const XAttn& a, int arg) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return status_from_cuda(cudaLaunchKernelEx(&cfg, kernel, a, arg));
+}
+
+// The tensor-core path (cross_attention_mma.cuh), one translation unit per type.
+int xattn_fp16(const XAttn& a, bool backward, cudaStream_t stream);
+int xattn_bf16(const XAttn& a, bool backward, cudaStream_t stream);
+
+// Entries of a short side that stay in registers: 8-entry tiles of the backward kernel (about 6 DP / 8
+// registers each) and of the forward kernel's keys (2 DP / 8 registers each).
+template <int DP>
+constexpr int kXmFewTiles = 128 / DP;
+template <int DP>
+constexpr int kXmKeyTiles = DP <= 32 ? 8 : 256 / DP;
+
+// Whether the backward pass reads out_f32 and lse (else it finds them itself, see xattn_bwd_few).
+inline bool xattn_uses_stats(int Tk, int d, int dtype) {
+  const int few = d <= 16 ? kXmFewTiles<16> : d <= 32 ? kXmFewTiles<32> : d <= 64 ? kXmFewTiles<64> : kXmFewTiles<128>;
+  return dtype == 2 || Tk > 8 * few;
+}
+
+}  // namespace ssam

@@ -1,5 +1,5 @@
-// Tensor-core kernels of the cross attention for fp16 / bf16 (included by
-// cross_attention.cu, which has the formulas and the conventions).
+// Tensor-core kernels of the cross attention for fp16 / bf16 (formulas and conventions
+// in cross_attention.cuh).
 //
 // Everything is built from mma.m16n8k16 on registers: head sizes here are 16 to 128
 // and one of the two token sets is usually a handful of prompt tokens, so a warp's
@@ -19,6 +19,8 @@
 // terms (value and remainder), so that a result carries one rounding to its type instead
 // of two. A single term measured 1.4 times the error of the rounded definition.
 #pragma once
+
+#include "cross_attention.cuh"
 
 namespace ssam {
 
@@ -70,11 +72,6 @@ __device__ __forceinline__ void store1(__nv_bfloat16* p, float v) { *p = __float
 __device__ __forceinline__ uint32_t movm(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-  return y;
-}
-__device__ __forceinline__ float rcp_fast(float x) {   // 2^-23 relative, far below the half types' rounding
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 // x, y -> packed value and packed remainder
@@ -1289,13 +1286,6 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_long(const XAttn a, int)
 // ---------------------------------------------------------------------------
 // Launch rules
 // ---------------------------------------------------------------------------
-// Entries of a short side that stay in registers: 8-entry tiles of the backward kernel (about
-// 6 DP / 8 registers each) and of the forward kernel's keys (2 DP / 8 registers each).
-template <int DP>
-constexpr int kXmFewTiles = 128 / DP;
-template <int DP>
-constexpr int kXmKeyTiles = DP <= 32 ? 8 : 256 / DP;
-
 // Blocks per cluster: blocks are added along the long side until every SM has one, while each warp
 // keeps at least one step. (Two per SM measured slower: 64 pairs of 4096 keys forward 17 us against 12,
 // the join outweighs the shorter walks.)
@@ -1429,12 +1419,6 @@ static int xattn_mma(const XAttn& a, bool backward, cudaStream_t stream) {
   if (a.d <= 32) return xattn_mma_dp<T, 32>(a, backward, stream);
   if (a.d <= 64) return xattn_mma_dp<T, 64>(a, backward, stream);
   return xattn_mma_dp<T, 128>(a, backward, stream);
-}
-
-// Whether the backward pass reads out_f32 and lse (else it finds them itself, see xattn_bwd_few).
-static bool xattn_uses_stats(int Tk, int d, int dtype) {
-  const int dp = d <= 16 ? 16 : d <= 32 ? 32 : d <= 64 ? 64 : 128;
-  return dtype == 2 || Tk > 8 * (128 / dp);
 }
 
 }  // namespace ssam

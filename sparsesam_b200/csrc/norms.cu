@@ -15,6 +15,7 @@
 
 #include <algorithm>
 
+#define SSAM_NO_WAITS
 #include "common.cuh"
 #include "host_util.h"
 
@@ -28,16 +29,11 @@ enum { kActNone = 0, kActRelu = 1, kActGelu = 2, kActSilu = 3 };
 // division: a thousandth of the output's rounding, and 2 to 3 times fewer instructions,
 // which is what bounded these kernels (GELU apply of 16 x 256 x 256 x 64: 108 us exact).
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
-__device__ __forceinline__ float rcp_approx(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // 1 / (1 + p u) of a pair from one reciprocal of the product (both factors are at least 1): the
 // reciprocals and exponentials (MUFU, a quarter of the FMA rate) are what GELU waits for.
 __device__ __forceinline__ float2 erf_t2(float2 u) {
   const float2 d = fma2(both(0.3275911f), u, both(1.0f));
-  const float r = rcp_approx(d.x * d.y);
+  const float r = rcp_fast(d.x * d.y);
   return mul2(both(r), make_float2(d.y, d.x));
 }
 // h = q / 2 of 7.1.26 without its exponential, e = exp(-u^2)
@@ -82,7 +78,7 @@ __device__ __forceinline__ float2 act_value(float2 z) {
 }
 template <bool EXACT>
 __device__ __forceinline__ float silu_slope(float z) {
-  const float s = EXACT ? 1.f / (1.f + expf(-z)) : rcp_approx(1.f + __expf(-z));
+  const float s = EXACT ? 1.f / (1.f + expf(-z)) : rcp_fast(1.f + __expf(-z));
   return s * (1.f + z * (1.f - s));
 }
 __device__ __forceinline__ float gelu_slope_exact(float z) {
