@@ -191,6 +191,22 @@ __global__ void __launch_bounds__(kXThreads) xattn_fwd_scalar(const XAttn a, int
       }
     }
   });
+  if (KS == 1 && cl == 1) {                  // a row is one group of TPR threads
+    if (!x.row_ok) return;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    float* to = static_cast<float*>(a.out) + b * a.os[0] + x.t * a.os[1] + x.h * a.os[2] + part * DT;
+    float* to32 = a.out_f32 == nullptr ? nullptr : a.out_f32 + ((static_cast<int64_t>(b) * a.Tq + x.t) * a.heads + x.h) * a.d + part * DT;
+#pragma unroll
+    for (int i = 0; i < DT; i += 4) {
+      if (part * DT + i >= a.d) break;
+      const float4 y = make_float4(o[i / 2].x * inv, o[i / 2].y * inv, o[i / 2 + 1].x * inv, o[i / 2 + 1].y * inv);
+      *reinterpret_cast<float4*>(to + i) = y;
+      if (to32 != nullptr) *reinterpret_cast<float4*>(to32 + i) = y;
+    }
+    if (a.lse != nullptr && part == 0)
+      a.lse[(static_cast<int64_t>(b) * a.heads + x.h) * a.Tq + x.t] = l == 0.f ? INFINITY : m + log2f(l);
+    return;
+  }
   // join the slices and blocks: rescale everybody's share to the common maximum first
   __syncthreads();
   float* ms = xsm;                       // [KS][RB]
@@ -281,6 +297,17 @@ __global__ void __launch_bounds__(kXThreads) xattn_dq_scalar(const XAttn a, int 
       row_axpy<DT>(here[j] ? ex2f(s - lse) * (dp - delta) : 0.f, sk + j * LD + part * DT, dq);
     }
   });
+  if (KS == 1 && x.cl == 1) {
+    if (!x.row_ok) return;
+    float* to = static_cast<float*>(a.dq) + ((static_cast<int64_t>(b) * a.Tq + x.t) * a.heads + x.h) * a.d + part * DT;
+#pragma unroll
+    for (int i = 0; i < DT; i += 4) {
+      if (part * DT + i >= a.d) break;
+      *reinterpret_cast<float4*>(to + i) = make_float4(dq[i / 2].x * a.scale, dq[i / 2].y * a.scale, dq[i / 2 + 1].x * a.scale,
+                                                       dq[i / 2 + 1].y * a.scale);
+    }
+    return;
+  }
   __syncthreads();
   float* mine = xsm + (slice * RB + x.lr) * DP + part * DT;
 #pragma unroll

@@ -78,8 +78,8 @@ __device__ __forceinline__ uint32_t movm(uint32_t x) {
 template <class T>
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
   hi = Mma<T>::pack(x, y);
-  const float2 h = Mma<T>::unpack(hi);
-  lo = Mma<T>::pack(x - h.x, y - h.y);
+  const float2 h = Mma<T>::unpack(hi), r = add2(make_float2(x, y), make_float2(-h.x, -h.y));
+  lo = Mma<T>::pack(r.x, r.y);
 }
 
 // This lane's DP / 4 channels of a token row (DP / 8 registers); zeros past channel d and when !ok.
@@ -148,12 +148,16 @@ __device__ __forceinline__ void warp_tree_sum(float* acc, float* sm, int warp, i
 }
 
 // ---------------------------------------------------------------------------
-// Forward. A warp holds 16 MT query rows of one key head and walks keys CK at a time.
+// Forward, two long sides. A warp holds 16 MT query rows of one key head and walks keys CK at a time.
 // split = false: the block's 8 warps hold 8 row tiles and each walks all keys.
 // split = true: one row tile per block, its keys shared by the 8 warps and the cluster.
+// The reference point of the exponentials is renewed only when a logit exceeds it by 2^8.
 // ---------------------------------------------------------------------------
+constexpr float kXmNone = -1e30f;           // reference before the first key
+constexpr float kXmSlack = 8.f;
+
 template <class T, int DP, int MT>
-__global__ void __launch_bounds__(kXmThreads) xattn_fwd_mma(const XAttn a, int split) {
+__global__ void __launch_bounds__(kXmThreads) xattn_fwd_long(const XAttn a, int split) {
   constexpr int NR = DP / 8;                 // registers of a row fragment = 8-channel blocks
   constexpr int CK = DP <= 32 ? 32 : 16;     // keys per step
   constexpr int NT = CK / 8;
@@ -172,10 +176,35 @@ __global__ void __launch_bounds__(kXmThreads) xattn_fwd_mma(const XAttn a, int s
     j_begin = min(keys, (rank * kXmWarps + warp) * per);
     j_end = min(keys, j_begin + per);
   }
-  const T* kb = static_cast<const T*>(a.k) + b * a.ks[0] + n * a.ks[2];
-  const T* vb = static_cast<const T*>(a.v) + b * a.vs[0] + n * a.vs[2];
   const uint8_t* mask = a.key_mask == nullptr ? nullptr : a.key_mask + static_cast<int64_t>(b) * a.Tk;
+  const T* kp = static_cast<const T*>(a.k) + b * a.ks[0] + n * a.ks[2] + (j_begin + g) * a.ks[1];
+  const T* vp = static_cast<const T*>(a.v) + b * a.vs[0] + n * a.vs[2] + (j_begin + g) * a.vs[1];
 
+  uint32_t k[NT][NR], v[NT][NR];
+  float2 bias[NT];                           // of keys 8 i + 2t, + 1: 0, or -infinity where there is none
+  auto load = [&](int j0) {                  // loads keys j0 + .. and moves on
+    if (mask == nullptr && j0 + CK <= j_end) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        bias[i] = make_float2(0.f, 0.f);
+        load_frag<T, DP>(kp + i * 8 * a.ks[1], t, a.d, true, k[i]);
+        load_frag<T, DP>(vp + i * 8 * a.vs[1], t, a.d, true, v[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const int j = j0 + i * 8 + g;
+        const bool ok = j < j_end && (mask == nullptr || __ldg(mask + j) != 0);
+        const float mine = ok ? 0.f : -INFINITY;
+        bias[i] = make_float2(__shfl_sync(0xffffffffu, mine, 8 * t), __shfl_sync(0xffffffffu, mine, 8 * t + 4));
+        load_frag<T, DP>(kp + i * 8 * a.ks[1], t, a.d, ok, k[i]);
+        load_frag<T, DP>(vp + i * 8 * a.vs[1], t, a.d, ok, v[i]);
+      }
+    }
+    kp += CK * a.ks[1];
+    vp += CK * a.vs[1];
+  };
+  load(j_begin);
   uint32_t q[MT][2][NR];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
@@ -185,99 +214,91 @@ __global__ void __launch_bounds__(kXmThreads) xattn_fwd_mma(const XAttn a, int s
       load_frag<T, DP>(static_cast<const T*>(a.q) + row_offset(a, a.qs, b, n, min(r, rows - 1)), t, a.d, r < rows,
                        q[mt][h]);
     }
-  float o[MT][NR][4], m[MT][2], l[MT][2];
+  float o[MT][NR][4], m[MT][2];
+  float2 l2[MT][2];                          // the lane's sums over keys 2t and 2t + 1
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
-    m[mt][0] = m[mt][1] = -INFINITY, l[mt][0] = l[mt][1] = 0.f;
+    m[mt][0] = m[mt][1] = kXmNone, l2[mt][0] = l2[mt][1] = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < NR; ++i) o[mt][i][0] = o[mt][i][1] = o[mt][i][2] = o[mt][i][3] = 0.f;
   }
+  const float2 c2 = make_float2(a.c, a.c);
 
   for (int j0 = j_begin; j0 < j_end; j0 += CK) {
-    uint32_t k[NT][NR], v[NT][NR];
+    float2 s[MT][NT][2];
+    uint32_t vt[NT][NR];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const int j = j0 + i * 8 + g;
-      const bool ok = j < j_end && (mask == nullptr || __ldg(mask + j) != 0);
-      load_frag<T, DP>(kb + j * a.ks[1], t, a.d, ok, k[i]);
-      load_frag<T, DP>(vb + j * a.vs[1], t, a.d, ok, v[i]);
-    }
-    const bool edge = j0 + CK > j_end || mask != nullptr;
-    uint32_t there = 0xffffffffu;            // bit 2i + e: key j0 + 8i + 2t + e
-    if (edge) {
-      there = 0;
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
+      for (int i = 0; i < NT; ++i) {
+        float f[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int j = j0 + i * 8 + 2 * t + e;
-          if (j < j_end && (mask == nullptr || __ldg(mask + j) != 0)) there |= 1u << (2 * i + e);
-        }
-    }
+        for (int c = 0; c < NR; c += 2)
+          Mma<T>::run(f, q[mt][0][c], q[mt][1][c], q[mt][0][c + 1], q[mt][1][c + 1], k[i][c], k[i][c + 1]);
+        s[mt][i][0] = fma2(make_float2(f[0], f[1]), c2, bias[i]);
+        s[mt][i][1] = fma2(make_float2(f[2], f[3]), c2, bias[i]);
+      }
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int c = 0; c < NR; ++c) v[i][c] = movm(v[i][c]);
+      for (int c = 0; c < NR; ++c) vt[i][c] = movm(v[i][c]);
+    if (j0 + CK < j_end) load(j0 + CK);      // the next step's, under this one's arithmetic
+    bool renew = false;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      float s[NT][4];
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
-#pragma unroll
-        for (int c = 0; c < NR; c += 2)
-          Mma<T>::run(s[i], q[mt][0][c], q[mt][1][c], q[mt][0][c + 1], q[mt][1][c + 1], k[i][c], k[i][c + 1]);
-      }
-      float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[i][e] = __fmul_rn(s[i][e], a.c);
-          if (edge && !(there >> (2 * i + (e & 1)) & 1u)) s[i][e] = -INFINITY;
-          mx[e >> 1] = fmaxf(mx[e >> 1], s[i][e]);
-        }
-      float use[2];
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-        mx[h] = fmaxf(mx[h], m[mt][h]);
-        use[h] = mx[h] == -INFINITY ? 0.f : mx[h];   // no key so far: 2^(-inf - 0) = 0
-        const float f = ex2f(m[mt][h] - use[h]);
-        m[mt][h] = mx[h];
-        l[mt][h] *= f;
+        float x = m[mt][h];
 #pragma unroll
-        for (int c = 0; c < NR; ++c) o[mt][c][2 * h] *= f, o[mt][c][2 * h + 1] *= f;
+        for (int i = 0; i < NT; ++i) x = fmaxf(x, fmaxf(s[mt][i][h].x, s[mt][i][h].y));
+        renew |= x > m[mt][h] + kXmSlack;
       }
+    if (__any_sync(0xffffffffu, renew)) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[i][e] = ex2f(__fsub_rn(s[i][e], use[e >> 1]));
-          l[mt][e >> 1] += s[i][e];
+        for (int h = 0; h < 2; ++h) {
+          float x = m[mt][h];
+#pragma unroll
+          for (int i = 0; i < NT; ++i) x = fmaxf(x, fmaxf(s[mt][i][h].x, s[mt][i][h].y));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+          const float f = ex2f(m[mt][h] - x);
+          m[mt][h] = x;
+          l2[mt][h] = mul2(l2[mt][h], make_float2(f, f));
+#pragma unroll
+          for (int c = 0; c < NR; ++c) o[mt][c][2 * h] *= f, o[mt][c][2 * h + 1] *= f;
         }
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int i = 0; i < NT; i += 2) {
         uint32_t hi[4], lo[4];
-        split2<T>(s[i][0], s[i][1], hi[0], lo[0]);
-        split2<T>(s[i][2], s[i][3], hi[1], lo[1]);
-        split2<T>(s[i + 1][0], s[i + 1][1], hi[2], lo[2]);
-        split2<T>(s[i + 1][2], s[i + 1][3], hi[3], lo[3]);
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float2 p = add2(s[mt][i + x][h], make_float2(-m[mt][h], -m[mt][h]));
+            p.x = ex2f(p.x), p.y = ex2f(p.y);
+            l2[mt][h] = add2(l2[mt][h], p);
+            split2<T>(p.x, p.y, hi[2 * x + h], lo[2 * x + h]);
+          }
 #pragma unroll
         for (int c = 0; c < NR; ++c) {
-          Mma<T>::run(o[mt][c], hi[0], hi[1], hi[2], hi[3], v[i][c], v[i + 1][c]);
-          Mma<T>::run(o[mt][c], lo[0], lo[1], lo[2], lo[3], v[i][c], v[i + 1][c]);
+          Mma<T>::run(o[mt][c], hi[0], hi[1], hi[2], hi[3], vt[i][c], vt[i + 1][c]);
+          Mma<T>::run(o[mt][c], lo[0], lo[1], lo[2], lo[3], vt[i][c], vt[i + 1][c]);
         }
       }
-    }
   }
 
   // the lanes of a quad share a row
+  float l[MT][2];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
+      l[mt][h] = l2[mt][h].x + l2[mt][h].y;
       l[mt][h] += __shfl_xor_sync(0xffffffffu, l[mt][h], 1);
       l[mt][h] += __shfl_xor_sync(0xffffffffu, l[mt][h], 2);
     }
@@ -323,7 +344,7 @@ __global__ void __launch_bounds__(kXmThreads) xattn_fwd_mma(const XAttn a, int s
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float x = -INFINITY;
+      float x = kXmNone;
 #pragma unroll
       for (int w = 0; w < kXmWarps; ++w) x = fmaxf(x, s_top[w * ROWS + mt * 16 + h * 8 + g]);
       top[mt][h] = x;
@@ -349,7 +370,7 @@ __global__ void __launch_bounds__(kXmThreads) xattn_fwd_mma(const XAttn a, int s
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float f = m[mt][h] == -INFINITY && !(l[mt][h] != l[mt][h]) ? 0.f : ex2f(m[mt][h] - top[mt][h]);
+      const float f = ex2f(m[mt][h] - top[mt][h]);
       acc[mt * (NR * 4 + 2) + NR * 4 + h] = l[mt][h] * f;
 #pragma unroll
       for (int c = 0; c < NR; ++c) {
@@ -369,7 +390,7 @@ __global__ void __launch_bounds__(kXmThreads) xattn_fwd_mma(const XAttn a, int s
     const int mt = u / (2 * NR), h = u / NR % 2, c = u % NR;
     const int ro = mt * 16 + h * 8 + g, r = r0 + ro;
     const int i0 = mt * (NR * 4 + 2) + c * 4 + 2 * h, il = mt * (NR * 4 + 2) + NR * 4 + h;
-    float x = 0.f, y = 0.f, den = 0.f, mm = -INFINITY;
+    float x = 0.f, y = 0.f, den = 0.f, mm = kXmNone;
     for (int i = 0; i < cl; ++i) {
       const uint32_t from = mapa_shared(base, i);
       x += ld_dsmem(from + i0 * 128);
@@ -377,7 +398,6 @@ __global__ void __launch_bounds__(kXmThreads) xattn_fwd_mma(const XAttn a, int s
       den += ld_dsmem(from + il * 128);
       if (cl > 1) mm = fmaxf(mm, ld_dsmem(mapa_shared(smem_u32(s_top + ro), i)));
     }
-    if (cl == 1) mm = -INFINITY;
     if (r < rows) {
       const float inv = den == 0.f ? 0.f : 1.f / den;
       const int ch = t * (DP / 4) + 2 * c;
@@ -412,9 +432,6 @@ __global__ void __launch_bounds__(kXmThreads) xattn_fwd_mma(const XAttn a, int s
 // fragment with the other half zeroed gives one head's logits, and likewise V^T rows g < 4
 // are the first head's. Twice the tensor instructions, of which there are plenty.
 // ---------------------------------------------------------------------------
-constexpr float kXmNone = -1e30f;           // reference before the first key
-constexpr float kXmSlack = 8.f;
-
 template <class T, int DP, int NQ, int HP>
 __global__ void __launch_bounds__(kXmThreads) xattn_fwd_few_rows(const XAttn a, int) {
   constexpr int NR = DP / 8, NU = NR / 2;    // 8- and 16-channel blocks
@@ -1146,7 +1163,7 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_long(const XAttn a, int)
   };
 
   uint32_t x1[M][2][NR], x2[M][2][NR];
-  float own_s[M][2], own_d[M][2];            // own rows: lse, D; own keys: bias
+  float own_s[M][2], own_d[M][2];            // own rows: -lse, -D; own keys: bias
 #pragma unroll
   for (int mt = 0; mt < M; ++mt)
 #pragma unroll
@@ -1154,9 +1171,9 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_long(const XAttn a, int)
       const int i = own0 + mt * 16 + h * 8 + g;
       if constexpr (OWN_ROWS) {
         load_row(i, x1[mt][h], x2[mt][h]);
-        own_s[mt][h] = i < rows ? __ldg(a.lse + stat0 + i) : INFINITY;
-        own_d[mt][h] = row_delta<T, DP>(a.out_f32 + row_dense(a, b, n, min(i, rows - 1)), x2[mt][h], t, a.d, i < rows);
-        if (rank == 0 && warp == 0 && t == 0 && i < rows) a.delta[stat0 + i] = own_d[mt][h];
+        own_s[mt][h] = i < rows ? -__ldg(a.lse + stat0 + i) : -INFINITY;
+        own_d[mt][h] = -row_delta<T, DP>(a.out_f32 + row_dense(a, b, n, min(i, rows - 1)), x2[mt][h], t, a.d, i < rows);
+        if (rank == 0 && warp == 0 && t == 0 && i < rows) a.delta[stat0 + i] = -own_d[mt][h];
       } else {
         load_key(i, x1[mt][h], x2[mt][h]);
         own_s[mt][h] = key_ok(i) ? 0.f : -INFINITY;
@@ -1179,28 +1196,50 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_long(const XAttn a, int)
   const int steps = (total + 15) / 16, ns = kXmWarps * cl;
   const int per = (steps + ns - 1) / ns * 16;
   const int begin = min(total, (rank * kXmWarps + warp) * per), end = min(total, begin + per);
-  for (int i0 = begin; i0 < end; i0 += 16) {
-    uint32_t y1[2][NR], y2[2][NR];
+  uint32_t y1[2][NR], y2[2][NR];
+  float2 ys[2], yd[2];                       // of entries i0 + 8 nt + 2t, + 1: bias of keys; -lse, -D of rows
+  // rows of one query head follow one another in memory, and so do keys
+  const bool straight = OWN_ROWS || a.group == 1;
+  const T* p1 = OWN_ROWS ? kb + (begin + g) * a.ks[1] : qb + b * a.qs[0] + n * a.qs[2] + (begin + g) * a.qs[1];
+  const T* p2 = OWN_ROWS ? vb + (begin + g) * a.vs[1] : ob + b * a.os[0] + n * a.os[2] + (begin + g) * a.os[1];
+  const int64_t st1 = OWN_ROWS ? a.ks[1] : a.qs[1], st2 = OWN_ROWS ? a.vs[1] : a.os[1];
+  auto load = [&](int i0) {
+    if (straight && i0 + 16 <= end && (!OWN_ROWS || mask == nullptr)) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if constexpr (OWN_ROWS)
-        load_key(i0 + h * 8 + g, y1[h], y2[h]);
-      else
-        load_row(i0 + h * 8 + g, y1[h], y2[h]);
-    }
-    float ys[2][2], yd[2][2];                // of entries i0 + 8 nt + 2t + e: bias of keys; lse, D of rows
-#pragma unroll
-    for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int i = i0 + nt * 8 + 2 * t + e;
+      for (int h = 0; h < 2; ++h) {
+        load_frag<T, DP>(p1 + h * 8 * st1, t, a.d, true, y1[h]);
+        load_frag<T, DP>(p2 + h * 8 * st2, t, a.d, true, y2[h]);
         if constexpr (OWN_ROWS) {
-          ys[nt][e] = key_ok(i) ? 0.f : -INFINITY;
+          ys[h] = make_float2(0.f, 0.f);
         } else {
-          ys[nt][e] = i < rows ? __ldg(a.lse + stat0 + i) : INFINITY;
-          yd[nt][e] = i < rows ? __ldg(a.delta + stat0 + i) : 0.f;
+          const float *ls = a.lse + stat0 + i0 + h * 8 + 2 * t, *dl = a.delta + stat0 + i0 + h * 8 + 2 * t;
+          ys[h] = make_float2(-__ldg(ls), -__ldg(ls + 1));
+          yd[h] = make_float2(-__ldg(dl), -__ldg(dl + 1));
         }
       }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int i = i0 + h * 8 + g;
+        float one, two = 0.f;
+        if constexpr (OWN_ROWS) {
+          load_key(i, y1[h], y2[h]);
+          one = key_ok(i) ? 0.f : -INFINITY;
+        } else {
+          load_row(i, y1[h], y2[h]);
+          one = i < rows ? -__ldg(a.lse + stat0 + i) : -INFINITY;
+          two = i < rows ? -__ldg(a.delta + stat0 + i) : 0.f;
+        }
+        ys[h] = make_float2(__shfl_sync(0xffffffffu, one, 8 * t), __shfl_sync(0xffffffffu, one, 8 * t + 4));
+        yd[h] = make_float2(__shfl_sync(0xffffffffu, two, 8 * t), __shfl_sync(0xffffffffu, two, 8 * t + 4));
+      }
+    }
+    p1 += 16 * st1;
+    p2 += 16 * st2;
+  };
+  load(begin);
+  const float2 c2 = make_float2(a.c, a.c);
+  for (int i0 = begin; i0 < end; i0 += 16) {
     Turned<T, 2, NR> y1t;
     uint32_t y2t[OWN_ROWS ? 1 : 2][NR];
     y1t.make(y1);
@@ -1210,36 +1249,42 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_long(const XAttn a, int)
 #pragma unroll
         for (int c = 0; c < NR; ++c) y2t[h][c] = movm(y2[h][c]);
     }
+    float2 p[M][2][2], ds[M][2][2];          // [own tile][other 8][own g | g + 8] x other 2t, 2t + 1
 #pragma unroll
-    for (int mt = 0; mt < M; ++mt) {
-      float p[2][4], ds[2][4];
-      uint32_t hi[4], lo[4];
+    for (int mt = 0; mt < M; ++mt)
 #pragma unroll
       for (int nt = 0; nt < 2; ++nt) {
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
-        ds[nt][0] = ds[nt][1] = ds[nt][2] = ds[nt][3] = 0.f;
+        float s[4] = {0.f, 0.f, 0.f, 0.f}, d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < NR; c += 2) {
           Mma<T>::run(s, x1[mt][0][c], x1[mt][1][c], x1[mt][0][c + 1], x1[mt][1][c + 1], y1[nt][c], y1[nt][c + 1]);
-          Mma<T>::run(ds[nt], x2[mt][0][c], x2[mt][1][c], x2[mt][0][c + 1], x2[mt][1][c + 1], y2[nt][c], y2[nt][c + 1]);
+          Mma<T>::run(d, x2[mt][0][c], x2[mt][1][c], x2[mt][0][c + 1], x2[mt][1][c + 1], y2[nt][c], y2[nt][c + 1]);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float bias = OWN_ROWS ? ys[nt][e & 1] : own_s[mt][e >> 1];
-          const float lse = OWN_ROWS ? own_s[mt][e >> 1] : ys[nt][e & 1];
-          p[nt][e] = ex2f(fmaf(s[e], a.c, bias) - lse);
-          ds[nt][e] = p[nt][e] * (ds[nt][e] - (OWN_ROWS ? own_d[mt][e >> 1] : yd[nt][e & 1]));
+        for (int h = 0; h < 2; ++h) {
+          const float2 own = make_float2(own_s[mt][h], own_s[mt][h]);      // -lse of rows, bias of keys
+          float2 f = fma2(make_float2(s[2 * h], s[2 * h + 1]), c2, OWN_ROWS ? ys[nt] : own);
+          f = add2(f, OWN_ROWS ? own : ys[nt]);
+          f.x = ex2f(f.x), f.y = ex2f(f.y);
+          p[mt][nt][h] = f;
+          ds[mt][nt][h] = mul2(f, add2(make_float2(d[2 * h], d[2 * h + 1]),
+                                       OWN_ROWS ? make_float2(own_d[mt][h], own_d[mt][h]) : yd[nt]));
         }
-        split2<__nv_bfloat16>(ds[nt][0], ds[nt][1], hi[2 * nt], lo[2 * nt]);
-        split2<__nv_bfloat16>(ds[nt][2], ds[nt][3], hi[2 * nt + 1], lo[2 * nt + 1]);
       }
+    if (i0 + 16 < end) load(i0 + 16);        // the next step's, under this one's arithmetic
+#pragma unroll
+    for (int mt = 0; mt < M; ++mt) {
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) split2<__nv_bfloat16>(ds[mt][nt][h].x, ds[mt][nt][h].y, hi[2 * nt + h], lo[2 * nt + h]);
       ds_product<T, 2, NR>(acc1[mt], hi, lo, y1t, 0);
       if constexpr (!OWN_ROWS) {
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          split2<T>(p[nt][0] * kP, p[nt][1] * kP, hi[2 * nt], lo[2 * nt]);
-          split2<T>(p[nt][2] * kP, p[nt][3] * kP, hi[2 * nt + 1], lo[2 * nt + 1]);
-        }
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) split2<T>(p[mt][nt][h].x * kP, p[mt][nt][h].y * kP, hi[2 * nt + h], lo[2 * nt + h]);
 #pragma unroll
         for (int c = 0; c < NR; ++c) {
           Mma<T>::run(acc2[mt][c], hi[0], hi[1], hi[2], hi[3], y2t[0][c], y2t[1][c]);
@@ -1295,17 +1340,17 @@ static int xattn_cluster(int64_t blocks, int other, int step) {
   return c;
 }
 template <class T, int DP, int MT>
-static int xattn_fwd_mma_launch(const XAttn& a, cudaStream_t stream) {
+static int xattn_fwd_long_launch(const XAttn& a, cudaStream_t stream) {
   const int rows = a.group * a.Tq, tiles = (rows + 16 * MT - 1) / (16 * MT);
   const int64_t pairs = static_cast<int64_t>(a.B) * a.kv_heads;
   constexpr int CK = DP <= 32 ? 32 : 16;
   const int64_t whole = pairs * ((tiles + kXmWarps - 1) / kXmWarps);
   if (a.Tk <= 2 * CK || (tiles >= kXmWarps && whole >= 2 * 148))
-    return launch_cluster(xattn_fwd_mma<T, DP, MT>, dim3((tiles + kXmWarps - 1) / kXmWarps, a.kv_heads, a.B),
+    return launch_cluster(xattn_fwd_long<T, DP, MT>, dim3((tiles + kXmWarps - 1) / kXmWarps, a.kv_heads, a.B),
                           kXmThreads, 0, 1, stream, a, 0);
   const int cl = xattn_cluster(pairs * tiles, a.Tk, CK);
   const size_t smem = (kXmWarps * 16 * MT + 4 * MT * (DP / 2 + 2) * 32) * sizeof(float);
-  return launch_cluster(xattn_fwd_mma<T, DP, MT>, dim3(tiles * cl, a.kv_heads, a.B), kXmThreads, smem, cl, stream, a,
+  return launch_cluster(xattn_fwd_long<T, DP, MT>, dim3(tiles * cl, a.kv_heads, a.B), kXmThreads, smem, cl, stream, a,
                         1);
 }
 
@@ -1400,9 +1445,9 @@ static int xattn_mma_dp(const XAttn& a, bool backward, cudaStream_t stream) {
     if constexpr (DP <= 64) {
       if (rows <= 24 || (rows > 32 && rows <= 48)) return xattn_few_rows_launch<T, DP, 3>(a, stream);
       if (rows <= 64) return xattn_few_rows_launch<T, DP, 4>(a, stream);
-      return xattn_fwd_mma_launch<T, DP, 2>(a, stream);
+      return xattn_fwd_long_launch<T, DP, 2>(a, stream);
     } else {
-      return xattn_fwd_mma_launch<T, DP, 1>(a, stream);
+      return xattn_fwd_long_launch<T, DP, 1>(a, stream);
     }
   }
   if (a.Tk <= 8 * kXmFewTiles<DP>) return xattn_bwd_few_pick<T, DP, false>(a, a.Tk, stream);
