@@ -1132,10 +1132,11 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_few(const XAttn a, int) 
 // Two long sides, one kernel per side. A warp owns 16 M entries of one (OWN_ROWS: query rows, x = q, dout;
 // else keys, x = k, v) and walks the other 16 entries at a time (y):
 //   own rows:  dq += ds k              own keys:  dk += ds q,  dv += p dout
-// The other side is shared by the block's warps and the cluster. The rows' kernel comes first and
-// leaves D for the keys'.
+// split = false: the block's 8 warps own 8 tiles and each walks all of the other side. split = true: one tile per
+// block, the other side shared by its warps and the cluster (the join takes about as long as ten steps).
+// The rows' kernel comes first and leaves D for the keys'.
 template <class T, int DP, int M, bool OWN_ROWS>
-__global__ void __launch_bounds__(kXmThreads) xattn_bwd_long(const XAttn a, int) {
+__global__ void __launch_bounds__(kXmThreads) xattn_bwd_long(const XAttn a, int split) {
   constexpr int NR = DP / 8;
   constexpr float kP = kPScale<T>;
   extern __shared__ __align__(16) float xsm[];
@@ -1143,7 +1144,8 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_long(const XAttn a, int)
   const int b = blockIdx.z, n = blockIdx.y;
   const int cl = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
   const int rows = a.group * a.Tq, keys = xattn_keys(a, b);
-  const int own0 = static_cast<int>(blockIdx.x) / cl * 16 * M;
+  const int own0 = (split ? static_cast<int>(blockIdx.x) / cl : static_cast<int>(blockIdx.x) * kXmWarps + warp) * 16 * M;
+  if (!split && own0 >= (OWN_ROWS ? rows : a.Tk)) return;
   const T* qb = static_cast<const T*>(a.q);
   const T* ob = static_cast<const T*>(a.dout);
   const T* kb = static_cast<const T*>(a.k) + b * a.ks[0] + n * a.ks[2];
@@ -1173,7 +1175,7 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_long(const XAttn a, int)
         load_row(i, x1[mt][h], x2[mt][h]);
         own_s[mt][h] = i < rows ? -__ldg(a.lse + stat0 + i) : -INFINITY;
         own_d[mt][h] = -row_delta<T, DP>(a.out_f32 + row_dense(a, b, n, min(i, rows - 1)), x2[mt][h], t, a.d, i < rows);
-        if (rank == 0 && warp == 0 && t == 0 && i < rows) a.delta[stat0 + i] = -own_d[mt][h];
+        if ((!split || (rank == 0 && warp == 0)) && t == 0 && i < rows) a.delta[stat0 + i] = -own_d[mt][h];
       } else {
         load_key(i, x1[mt][h], x2[mt][h]);
         own_s[mt][h] = key_ok(i) ? 0.f : -INFINITY;
@@ -1193,9 +1195,9 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_long(const XAttn a, int)
         if constexpr (!OWN_ROWS) acc2[mt][c][e] = 0.f;
       }
   const int total = OWN_ROWS ? keys : (own0 < keys ? rows : 0);
-  const int steps = (total + 15) / 16, ns = kXmWarps * cl;
+  const int steps = (total + 15) / 16, ns = split ? kXmWarps * cl : 1;
   const int per = (steps + ns - 1) / ns * 16;
-  const int begin = min(total, (rank * kXmWarps + warp) * per), end = min(total, begin + per);
+  const int begin = split ? min(total, (rank * kXmWarps + warp) * per) : 0, end = min(total, begin + per);
   uint32_t y1[2][NR], y2[2][NR];
   float2 ys[2], yd[2];                       // of entries i0 + 8 nt + 2t, + 1: bias of keys; -lse, -D of rows
   // rows of one query head follow one another in memory, and so do keys
@@ -1294,6 +1296,26 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_long(const XAttn a, int)
     }
   }
 
+  if (!split) {
+#pragma unroll
+    for (int mt = 0; mt < M; ++mt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int i = own0 + mt * 16 + h * 8 + g;
+        if (i >= (OWN_ROWS ? rows : a.Tk)) continue;
+        const int64_t to = OWN_ROWS ? row_dense(a, b, n, i) : ((static_cast<int64_t>(b) * a.Tk + i) * a.kv_heads + n) * a.d;
+        uint32_t y[NR];
+#pragma unroll
+        for (int c = 0; c < NR; ++c) y[c] = Mma<T>::pack(acc1[mt][c][2 * h] * a.scale, acc1[mt][c][2 * h + 1] * a.scale);
+        store_frag<T, DP>(static_cast<T*>(OWN_ROWS ? a.dq : a.dk) + to, t, a.d, y);
+        if constexpr (!OWN_ROWS) {
+#pragma unroll
+          for (int c = 0; c < NR; ++c) y[c] = Mma<T>::pack(acc2[mt][c][2 * h] * (1.f / kP), acc2[mt][c][2 * h + 1] * (1.f / kP));
+          store_frag<T, DP>(static_cast<T*>(a.dv) + to, t, a.d, y);
+        }
+      }
+    return;
+  }
   // join the owned sums of the warps and the cluster
   auto join = [&](float* acc, void* to_v, float factor, bool first) {
     constexpr int NREG = M * NR * 4;
@@ -1345,7 +1367,7 @@ static int xattn_fwd_long_launch(const XAttn& a, cudaStream_t stream) {
   const int64_t pairs = static_cast<int64_t>(a.B) * a.kv_heads;
   constexpr int CK = DP <= 32 ? 32 : 16;
   const int64_t whole = pairs * ((tiles + kXmWarps - 1) / kXmWarps);
-  if (a.Tk <= 2 * CK || (tiles >= kXmWarps && whole >= 2 * 148))
+  if (a.Tk <= 2 * CK || (tiles >= kXmWarps && whole >= 148))
     return launch_cluster(xattn_fwd_long<T, DP, MT>, dim3((tiles + kXmWarps - 1) / kXmWarps, a.kv_heads, a.B),
                           kXmThreads, 0, 1, stream, a, 0);
   const int cl = xattn_cluster(pairs * tiles, a.Tk, CK);
@@ -1412,10 +1434,15 @@ template <class T, int DP, int M, bool OWN_ROWS>
 static int xattn_bwd_long_launch(const XAttn& a, cudaStream_t stream) {
   const int rows = a.group * a.Tq, own = OWN_ROWS ? rows : a.Tk, other = OWN_ROWS ? a.Tk : rows;
   const int tiles = (own + 16 * M - 1) / (16 * M);
-  const int cl = xattn_cluster(static_cast<int64_t>(a.B) * a.kv_heads * tiles, other, 16);
-  const size_t smem = 4 * M * (DP / 2) * 32 * sizeof(float);
+  const int64_t pairs = static_cast<int64_t>(a.B) * a.kv_heads;
+  const int groups = (tiles + kXmWarps - 1) / kXmWarps;
+  if (tiles >= kXmWarps && pairs * groups >= 148)
+    return launch_cluster(xattn_bwd_long<T, DP, M, OWN_ROWS>, dim3(groups, a.kv_heads, a.B), kXmThreads, 0, 1, stream, a, 0);
+  const int cl = xattn_cluster(pairs * tiles, other, 16);
+  constexpr size_t smem = 4 * M * (DP / 2) * 32 * sizeof(float);
+  static_assert(smem <= 48 << 10, "no opt-in needed");
   return launch_cluster(xattn_bwd_long<T, DP, M, OWN_ROWS>, dim3(tiles * cl, a.kv_heads, a.B), kXmThreads, smem, cl,
-                        stream, a, 0);
+                        stream, a, 1);
 }
 
 template <class T, int DP>
@@ -1452,10 +1479,9 @@ static int xattn_mma_dp(const XAttn& a, bool backward, cudaStream_t stream) {
   }
   if (a.Tk <= 8 * kXmFewTiles<DP>) return xattn_bwd_few_pick<T, DP, false>(a, a.Tk, stream);
   if (rows <= 8 * kXmFewTiles<DP>) return xattn_bwd_few_pick<T, DP, true>(a, rows, stream);
-  constexpr int M = DP <= 32 ? 2 : 1;
-  const int st = xattn_bwd_long_launch<T, DP, M, true>(a, stream);
+  const int st = xattn_bwd_long_launch<T, DP, DP <= 64 ? 2 : 1, true>(a, stream);
   if (st != SSAM_OK || a.dk == nullptr) return st;
-  return xattn_bwd_long_launch<T, DP, M, false>(a, stream);
+  return xattn_bwd_long_launch<T, DP, DP <= 32 ? 2 : 1, false>(a, stream);
 }
 
 template <class T>
