@@ -90,6 +90,27 @@ class RowLayerNorm(nn.LayerNorm):
         return super().forward(x)
 
 
+class GroupNormAct2d(nn.GroupNorm):
+    """nn.GroupNorm of an NCHW map (same parameters) with an activation of ops.ACTIVATIONS
+    after it, the normalisation of convolutional segmentation heads. On CUDA
+    channels-last maps of one dtype with the parameters computed by
+    ssam_groupnorm_act (differentiable), elsewhere by torch."""
+
+    def __init__(self, num_groups: int, num_channels: int, eps: float = 1e-5, act: str = "none"):
+        super().__init__(num_groups, num_channels, eps=eps, affine=True)
+        if act not in ops.ACTIVATIONS:
+            raise ValueError(f"act must be one of {tuple(ops.ACTIVATIONS)}, got {act!r}")
+        self.act = act
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        nhwc = x.permute(0, 2, 3, 1)
+        if x.is_cuda and self.weight.dtype == x.dtype and nhwc.is_contiguous() and ops.groupnorm_act_supported(
+                x.shape[1], self.num_groups, x.dtype):
+            return ops.groupnorm_act(nhwc, self.num_groups, self.weight, self.bias, self.eps, self.act).permute(0, 3, 1, 2)
+        y = super().forward(x)
+        return {"none": lambda t: t, "relu": F.relu, "gelu": F.gelu, "silu": F.silu}[self.act](y)
+
+
 def _ln_gelu(c: int):
     """LayerNorm2d with the GELU fused, and the Identity that holds the GELU's slot."""
     return LayerNorm2d(c, gelu=True), nn.Identity()
@@ -224,7 +245,9 @@ class PromptEncoder(nn.Module):
 # ---------------------------------------------------------------------------
 class DecoderAttention(nn.Module):
     """Multi-head attention whose q / k / v projections go down to
-    embedding_dim / downsample_rate channels (the cross-attention layers use 2)."""
+    embedding_dim / downsample_rate channels (the cross-attention layers use 2). On
+    CUDA tensors computed by ssam_cross_attn (fp16, bf16, fp32; differentiable),
+    elsewhere by torch."""
 
     def __init__(self, embedding_dim: int, num_heads: int, downsample_rate: int = 1):
         super().__init__()
@@ -240,13 +263,28 @@ class DecoderAttention(nn.Module):
 
     def _split(self, x: torch.Tensor) -> torch.Tensor:
         b, n, c = x.shape
-        return x.view(b, n, self.num_heads, c // self.num_heads).transpose(1, 2)
+        return x.view(b, n, self.num_heads, c // self.num_heads)
 
-    def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
+    def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                key_lens: Optional[torch.Tensor] = None, key_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """key_lens (int32 (B,)) and key_mask (bool (B, Tk), True: attend) say which keys are
+        there (a padded batch of prompts); a query without keys gives out_proj's bias."""
         qh, kh, vh = self._split(self.q_proj(q)), self._split(self.k_proj(k)), self._split(self.v_proj(v))
-        o = F.scaled_dot_product_attention(qh, kh, vh)       # softmax(q k^T / sqrt(c)) v
-        b, h, n, c = o.shape
-        return self.out_proj(o.transpose(1, 2).reshape(b, n, h * c))
+        h, c = qh.shape[2:]
+        if qh.is_cuda and ops.cross_attn_supported(h, h, c, qh.dtype):
+            o = ops.cross_attn(qh, kh, vh, key_lens=key_lens, key_mask=key_mask)
+        else:
+            mask = key_mask
+            if key_lens is not None:
+                there = torch.arange(kh.shape[1], device=kh.device) < key_lens.view(-1, 1)
+                mask = there if mask is None else mask & there
+            if mask is not None:
+                mask = mask[:, None, None, :]
+            o = F.scaled_dot_product_attention(qh.transpose(1, 2), kh.transpose(1, 2), vh.transpose(1, 2),
+                                               attn_mask=mask).transpose(1, 2)      # softmax(q k^T / sqrt(c)) v
+            if mask is not None:
+                o = torch.where(mask.any(-1)[..., None], o, torch.zeros((), dtype=o.dtype, device=o.device))
+        return self.out_proj(o.reshape(o.shape[0], o.shape[1], h * c))
 
 
 class DecoderMLPBlock(nn.Module):

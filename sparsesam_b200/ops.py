@@ -596,6 +596,12 @@ class _GroupNormAct(torch.autograd.Function):
         return dx, dw, db, None, None, None
 
 
+def groupnorm_act_supported(channels: int, groups: int, dtype: torch.dtype) -> bool:
+    """Whether groupnorm_act takes these channels."""
+    unit = 4 if dtype == torch.float32 else 8
+    return dtype in _DTYPES and groups > 0 and channels % groups == 0 and channels % unit == 0 and channels <= 256 * unit
+
+
 def groupnorm_act(x: torch.Tensor, groups: int, w: torch.Tensor, b: torch.Tensor, eps: float = 1e-5,
                   act: str = "none") -> torch.Tensor:
     """act(GroupNorm(x) * w + b) of channels-last maps x (N, ..., C): statistics over all
@@ -611,8 +617,9 @@ def groupnorm_act(x: torch.Tensor, groups: int, w: torch.Tensor, b: torch.Tensor
         raise ValueError("x must be (N, ..., C), w and b (C,)")
     if not x.is_contiguous() or not w.is_contiguous() or not b.is_contiguous():
         raise ValueError("x, w and b must be contiguous (x channels-last)")
-    if groups <= 0 or x.shape[-1] % groups:
-        raise ValueError(f"groups must divide the {x.shape[-1]} channels, got {groups}")
+    if not groupnorm_act_supported(x.shape[-1], groups, x.dtype):
+        raise ValueError(f"{groups} groups of {x.shape[-1]} channels are not supported: groups divide the channels, a "
+                         f"multiple of 8 up to 2048 (fp32: of 4 up to 1024)")
     if act not in ACTIVATIONS:
         raise ValueError(f"act must be one of {tuple(ACTIVATIONS)}, got {act!r}")
     if _wants_grad(x, w, b):
