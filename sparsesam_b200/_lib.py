@@ -135,7 +135,7 @@ def load() -> ctypes.CDLL:
                 raise RuntimeError(
                     f"{path} is missing: build it with `python -m sparsesam_b200.build` "
                     "(or __graft_entry__.build()); there is no fallback implementation")
-            handle = ctypes.CDLL(path)
+            handle = ctypes.CDLL(path, mode=ctypes.RTLD_GLOBAL)   # _torch_ops finds the entry points here
             for name, (res, args) in SIGNATURES.items():
                 fn = getattr(handle, name, None)
                 if fn is None:
@@ -144,6 +144,18 @@ def load() -> ctypes.CDLL:
                 fn.argtypes = args
             _lib = handle
     return _lib
+
+
+def torch_ops():
+    """The extension module of the decoder's operators (csrc/torch_ops.cpp); raise if it has not been built."""
+    load()
+    import torch  # noqa: F401, PLC0415 (its libraries come first; the C ABI itself needs no torch)
+    try:
+        from . import _torch_ops  # noqa: PLC0415
+    except ImportError as e:
+        raise RuntimeError(f"{_build.TORCH_OPS_PATH} is missing or does not fit this torch ({e}): build it with `python -m "
+                           "sparsesam_b200.build` (or __graft_entry__.build()); there is no fallback implementation") from e
+    return _torch_ops
 
 
 def missing_symbols() -> list[str]:

@@ -1,8 +1,10 @@
 """Builds libsparsesam_b200.so in-tree with nvcc for sm_100a.
 
 The library is a plain C-ABI shared object (no torch headers), linked from the
-translation units UNITS, which are compiled at the same time. It is rebuilt when
-any csrc/ or include/ file is newer than the .so.
+translation units UNITS, which are compiled at the same time. Beside it the Python
+extension module _torch_ops (csrc/torch_ops.cpp, torch headers, no device code) gives
+the decoder's operators their torch form. Both are rebuilt when any csrc/ or include/
+file is newer than they are.
 """
 from __future__ import annotations
 
@@ -19,6 +21,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 INCLUDE = os.path.join(REPO_DIR, "include")
 LIB_NAME = "libsparsesam_b200.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
+TORCH_OPS_PATH = os.path.join(PKG_DIR, "_torch_ops.so")
 
 UNITS = ["lib.cu", "cross_attention.cu", "cross_attention_fp16.cu", "cross_attention_bf16.cu", "norms.cu"]
 
@@ -41,15 +44,30 @@ def _sources() -> list[str]:
     out = []
     for d in (CSRC, INCLUDE):
         for name in sorted(os.listdir(d)):
-            if name.endswith((".cu", ".cuh", ".h")):
+            if name.endswith((".cu", ".cuh", ".h", ".cpp")):
                 out.append(os.path.join(d, name))
     return out
 
 
+def _torch_ops_command(out: str) -> list[str]:
+    """Compile and link _torch_ops against this interpreter's torch and, found beside it, the library."""
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=_torch_ops",
+            "-I", os.path.join(root, "include"), "-I", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+            "-I", os.path.join(cuda, "include"), "-I", sysconfig.get_paths()["include"], "-I", INCLUDE,
+            "-o", out, os.path.join(CSRC, "torch_ops.cpp"),
+            "-L", os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+
+
 def needs_build() -> bool:
-    if not os.path.exists(LIB_PATH):
+    if not (os.path.exists(LIB_PATH) and os.path.exists(TORCH_OPS_PATH)):
         return True
-    t = os.path.getmtime(LIB_PATH)
+    t = min(os.path.getmtime(LIB_PATH), os.path.getmtime(TORCH_OPS_PATH))
     return any(os.path.getmtime(s) > t for s in _sources())
 
 
@@ -66,14 +84,18 @@ def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | N
         if verbose and (res.stdout or res.stderr):
             print(res.stdout, res.stderr, file=sys.stderr)
 
-    tmp = LIB_PATH + ".tmp"
+    tmp, tmp_ops = LIB_PATH + ".tmp", TORCH_OPS_PATH + ".tmp"
     with tempfile.TemporaryDirectory(prefix="ssam_build_") as work:
         objects = [os.path.join(work, unit + ".o") for unit in UNITS]
-        with ThreadPoolExecutor(len(UNITS)) as pool:
-            list(pool.map(run, [[_nvcc(), *NVCC_FLAGS, *(extra_flags or []), "-I", INCLUDE, "-c", "-o", obj,
-                                 os.path.join(CSRC, unit)] for unit, obj in zip(UNITS, objects)]))
+        units = [[_nvcc(), *NVCC_FLAGS, *(extra_flags or []), "-I", INCLUDE, "-c", "-o", obj, os.path.join(CSRC, unit)]
+                 for unit, obj in zip(UNITS, objects)]
+        # the module's references to the library are resolved when it is loaded, after the library
+        units.append(_torch_ops_command(tmp_ops))
+        with ThreadPoolExecutor(len(units)) as pool:
+            list(pool.map(run, units))
         run([_nvcc(), *NVCC_FLAGS, "-shared", "-o", tmp, *objects])
     os.replace(tmp, LIB_PATH)
+    os.replace(tmp_ops, TORCH_OPS_PATH)
     return LIB_PATH
 
 

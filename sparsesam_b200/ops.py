@@ -7,9 +7,6 @@ a CUDA device is rejected.
 """
 from __future__ import annotations
 
-import ctypes
-import math
-
 import torch
 
 from . import _lib
@@ -50,34 +47,15 @@ def _check_cuda(*ts: torch.Tensor) -> None:
             raise ValueError("sparsesam_b200 ops run on CUDA tensors only (no CPU fallback)")
 
 
-def _launch(name: str, t: torch.Tensor, *args) -> None:
-    """Call an entry point on t's device and that device's current torch stream (the last argument)."""
-    dev = t.get_device()
-    if dev == torch._C._cuda_getDevice():
-        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
-    else:
-        with torch.cuda.device(dev):
-            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+_native = None
 
 
-def _twice_guarded(backward):
-    """A Function's backward that autograd may differentiate no further. The guard of once_differentiable costs
-    a few microseconds and matters only where a graph of the backward pass is recorded."""
-    guarded = torch.autograd.function.once_differentiable(backward)
-
-    def run(ctx, dout):
-        return (guarded if torch.is_grad_enabled() else backward)(ctx, dout)
-
-    return staticmethod(run)
-
-
-def _same_device(*ts: torch.Tensor) -> None:
-    if any(t is not None and t.device != ts[0].device for t in ts):
-        raise ValueError("all tensors of a call must be on one device")
-
-
-def _wants_grad(*ts: torch.Tensor) -> bool:
-    return torch.is_grad_enabled() and any(t.requires_grad for t in ts)
+def _torch_ops():
+    """csrc/torch_ops.cpp: checks, outputs and autograd nodes of the decoder's operators."""
+    global _native
+    if _native is None:
+        _native = _lib.torch_ops()
+    return _native
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
@@ -492,114 +470,30 @@ def layernorm_nchw(x: torch.Tensor, B: int, H: int, W: int, w: torch.Tensor, b: 
     return out
 
 
+# ---------------------------------------------------------------------------
+# The decoder's operators (differentiable once; csrc/torch_ops.cpp)
+# ---------------------------------------------------------------------------
 LN_HALF_CHANNELS = (32, 64, 128, 256)
-_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
-
-
-def _layernorm_gelu_half(x, w, b, eps, gelu):
-    out = torch.empty_like(x)
-    C = x.shape[-1]
-    if x.numel():
-        _launch("ssam_layernorm_gelu_half", x, x.data_ptr(), x.numel() // C, C, w.data_ptr(), b.data_ptr(), eps, gelu,
-                _DTYPES[x.dtype], out.data_ptr())
-    return out
-
-
-class _LayerNormGeluHalf(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w, b, eps, gelu):
-        ctx.save_for_backward(x, w, b)
-        ctx.eps, ctx.gelu = eps, gelu
-        return _layernorm_gelu_half(x, w, b, eps, gelu)
-
-    @_twice_guarded
-    def backward(ctx, dout):
-        x, w, b = ctx.saved_tensors
-        C = x.shape[-1]
-        rows = x.numel() // C
-        if rows == 0:
-            return torch.zeros_like(x), torch.zeros_like(w), torch.zeros_like(b), None, None
-        dout = _dense(dout)
-        dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty_like(b)
-        n = _lib.load().ssam_layernorm_gelu_half_bwd_workspace_size(rows, C)
-        ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-        _launch("ssam_layernorm_gelu_half_bwd", x, x.data_ptr(), dout.data_ptr(), rows, C, w.data_ptr(), b.data_ptr(),
-                ctx.eps, ctx.gelu, _DTYPES[x.dtype], dx.data_ptr(), dw.data_ptr(), db.data_ptr(), ws.data_ptr(), n)
-        return dx, dw, db, None, None
-
-
-def _dense(t: torch.Tensor) -> torch.Tensor:
-    """t in row-major memory that vector loads can read (an incoming gradient may have any layout)."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+_OPERATOR_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 
 
 def layernorm_gelu_half(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor, eps: float,
                         gelu: bool) -> torch.Tensor:
     """Channel LayerNorm (+ exact GELU) of fp16 / bf16 channels-last rows (..., C),
     C in LN_HALF_CHANNELS; w, b of x's dtype. Returns a new tensor of x's shape.
-    Differentiable in x, w and b (once)."""
-    _check_cuda(x, w, b)
-    if x.dtype not in (torch.float16, torch.bfloat16) or w.dtype != x.dtype or b.dtype != x.dtype:
-        raise ValueError("x, w and b must share one half-precision dtype")
-    if not x.is_contiguous() or not w.is_contiguous() or not b.is_contiguous():
-        raise ValueError("x, w and b must be contiguous")
-    if _wants_grad(x, w, b):
-        return _LayerNormGeluHalf.apply(x, w, b, float(eps), int(bool(gelu)))
-    return _layernorm_gelu_half(x, w, b, float(eps), int(bool(gelu)))
+    Differentiable in x, w and b."""
+    _lib.launch_count += 1
+    return _torch_ops().layernorm_gelu_half(x, w, b, eps, gelu)
 
 
-# ---------------------------------------------------------------------------
-# GroupNorm + activation
-# ---------------------------------------------------------------------------
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
-
-
-def _groupnorm_act(x, groups, w, b, eps, act, stats):
-    N, C = x.shape[0], x.shape[-1]
-    out = torch.empty_like(x)
-    if x.numel() == 0:
-        return out, None
-    HW = x.numel() // (N * C)
-    st = torch.empty(2, N, groups, dtype=torch.float32, device=x.device) if stats else None    # mean, rstd
-    n = _lib.load().ssam_groupnorm_act_workspace_size(N, HW, C, groups, _DTYPES[x.dtype], 0)
-    ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-    mean = st.data_ptr() if stats else None
-    _launch("ssam_groupnorm_act_fwd", x, x.data_ptr(), N, HW, C, groups, w.data_ptr(), b.data_ptr(), eps, act,
-            _DTYPES[x.dtype], out.data_ptr(), mean, mean + 4 * N * groups if stats else None, _ptr(ws), n)
-    return out, st
-
-
-class _GroupNormAct(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w, b, groups, eps, act):
-        out, st = _groupnorm_act(x, groups, w, b, eps, act, True)
-        ctx.save_for_backward(x, w, b, st)
-        ctx.groups, ctx.act = groups, act
-        return out
-
-    @_twice_guarded
-    def backward(ctx, dout):
-        x, w, b, st = ctx.saved_tensors
-        if x.numel() == 0:
-            return torch.zeros_like(x), torch.zeros_like(w), torch.zeros_like(b), None, None, None
-        N, C = x.shape[0], x.shape[-1]
-        HW = x.numel() // (N * C)
-        dout = _dense(dout)
-        dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty_like(b)
-        n = _lib.load().ssam_groupnorm_act_workspace_size(N, HW, C, ctx.groups, _DTYPES[x.dtype], 1)
-        ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-        mean = st.data_ptr()
-        _launch("ssam_groupnorm_act_bwd", x, x.data_ptr(), dout.data_ptr(), N, HW, C, ctx.groups, w.data_ptr(),
-                b.data_ptr(), mean, mean + 4 * N * ctx.groups, ctx.act, _DTYPES[x.dtype], dx.data_ptr(), dw.data_ptr(),
-                db.data_ptr(), ws.data_ptr(), n)
-        return dx, dw, db, None, None, None
 
 
 def groupnorm_act_supported(channels: int, groups: int, dtype: torch.dtype) -> bool:
     """Whether groupnorm_act takes these channels."""
     unit = 4 if dtype == torch.float32 else 8
-    return dtype in _DTYPES and groups > 0 and channels % groups == 0 and channels % unit == 0 and channels <= 256 * unit
+    return (dtype in _OPERATOR_DTYPES and groups > 0 and channels % groups == 0 and channels % unit == 0
+            and channels <= 256 * unit)
 
 
 def groupnorm_act(x: torch.Tensor, groups: int, w: torch.Tensor, b: torch.Tensor, eps: float = 1e-5,
@@ -608,97 +502,12 @@ def groupnorm_act(x: torch.Tensor, groups: int, w: torch.Tensor, b: torch.Tensor
     positions and the C / groups channels of a group, per sample. act in ACTIVATIONS (gelu is
     the erf form). fp16, bf16 or fp32, one dtype for x, w (C,) and b (C,); C a multiple of 8
     (fp32: 4) and of groups, at most 2048 (fp32: 1024). Returns a new tensor of x's shape.
-    Differentiable in x, w and b (once)."""
-    _check_cuda(x, w, b)
-    _same_device(x, w, b)
-    if x.dtype not in _DTYPES or w.dtype != x.dtype or b.dtype != x.dtype:
-        raise TypeError("x, w and b must share one dtype of fp16, bf16, fp32")
-    if x.dim() < 2 or w.shape != x.shape[-1:] or b.shape != x.shape[-1:]:
-        raise ValueError("x must be (N, ..., C), w and b (C,)")
-    if not x.is_contiguous() or not w.is_contiguous() or not b.is_contiguous():
-        raise ValueError("x, w and b must be contiguous (x channels-last)")
-    if not groupnorm_act_supported(x.shape[-1], groups, x.dtype):
-        raise ValueError(f"{groups} groups of {x.shape[-1]} channels are not supported: groups divide the channels, a "
-                         f"multiple of 8 up to 2048 (fp32: of 4 up to 1024)")
-    if act not in ACTIVATIONS:
+    Differentiable in x, w and b."""
+    code = ACTIVATIONS.get(act)
+    if code is None:
         raise ValueError(f"act must be one of {tuple(ACTIVATIONS)}, got {act!r}")
-    if _wants_grad(x, w, b):
-        return _GroupNormAct.apply(x, w, b, int(groups), float(eps), ACTIVATIONS[act])
-    return _groupnorm_act(x, int(groups), w, b, float(eps), ACTIVATIONS[act], False)[0]
-
-
-# ---------------------------------------------------------------------------
-# Cross attention
-# ---------------------------------------------------------------------------
-_I64x12 = ctypes.c_int64 * 12
-
-
-def _strides(a: torch.Tensor, b: torch.Tensor, c: torch.Tensor, d: torch.Tensor):
-    return _I64x12(*a.stride()[:3], *b.stride()[:3], *c.stride()[:3], *d.stride()[:3])
-
-
-def _cross_attn(q, k, v, scale, key_lens, key_mask, train):
-    """(out, out in fp32, [lse, D] statistics); the last two only where the backward pass reads them."""
-    B, Tq, H, D = q.shape
-    Tk, Hk = k.shape[1], k.shape[2]
-    out = torch.empty(B, Tq, H, D, dtype=q.dtype, device=q.device)
-    if out.numel() == 0 or Tk == 0:
-        return out.zero_(), None, None
-    dt = _DTYPES[q.dtype]
-    stats = out32 = None
-    if train and _lib.load().ssam_cross_attn_bwd_uses_stats(Tk, D, dt):
-        stats = torch.empty(2, B, H, Tq, dtype=torch.float32, device=q.device)
-        out32 = out if dt == 2 else torch.empty(B, Tq, H, D, dtype=torch.float32, device=q.device)
-    _launch("ssam_cross_attn_fwd", q, q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v, out), B, Tq, Tk, H, Hk,
-            D, dt, scale, _ptr(key_lens), _ptr(key_mask), out.data_ptr(), None if out32 is out else _ptr(out32),
-            _ptr(stats))
-    return out, out32, stats
-
-
-class _CrossAttn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, scale, key_lens, key_mask):
-        out, out32, stats = _cross_attn(q, k, v, scale, key_lens, key_mask, True)
-        ctx.save_for_backward(q, k, v, out32, stats, key_lens, key_mask)
-        ctx.scale = scale
-        return out
-
-    @_twice_guarded
-    def backward(ctx, dout):
-        q, k, v, out32, stats, key_lens, key_mask = ctx.saved_tensors
-        B, Tq, H, D = q.shape
-        Tk, Hk = k.shape[1], k.shape[2]
-        need = ctx.needs_input_grad
-        dq = torch.empty(B, Tq, H, D, dtype=q.dtype, device=q.device) if need[0] else None
-        dk = dv = None
-        if need[1] or need[2]:
-            dk = torch.empty(B, Tk, Hk, D, dtype=q.dtype, device=q.device)
-            dv = torch.empty(B, Tk, Hk, D, dtype=q.dtype, device=q.device)
-        if Tk == 0 or q.numel() == 0:     # no keys or no queries: nothing depends on anything
-            for g in (dq, dk, dv):
-                if g is not None:
-                    g.zero_()
-            return dq, dk, dv, None, None, None
-        dout = _vector_rows(dout)
-        lse = _ptr(stats)
-        _launch("ssam_cross_attn_bwd", q, q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(),
-                _strides(q, k, v, dout), B, Tq, Tk, H, Hk, D, _DTYPES[q.dtype], ctx.scale, _ptr(key_lens), _ptr(key_mask),
-                _ptr(out32), lse, None if lse is None else lse + 4 * B * H * Tq, _ptr(dq), _ptr(dk), _ptr(dv))
-        return dq, dk, dv, None, None, None
-
-
-def _vector_ok(t: torch.Tensor) -> bool:
-    """Whether every (batch, token, head) row of t is contiguous and starts on a 16-byte boundary."""
-    if t.data_ptr() % 16:
-        return False
-    if t.is_contiguous():
-        return t.shape[3] * t.element_size() % 16 == 0
-    unit = 16 // t.element_size()
-    return t.stride(3) == 1 and all(s % unit == 0 for s, n in zip(t.stride()[:3], t.shape) if n > 1)
-
-
-def _vector_rows(t: torch.Tensor) -> torch.Tensor:
-    return t if _vector_ok(t) else t.clone(memory_format=torch.contiguous_format)
+    _lib.launch_count += 1
+    return _torch_ops().groupnorm_act(x, groups, w, b, eps, code)
 
 
 CROSS_ATTN_MAX_DIM = 128
@@ -706,7 +515,8 @@ CROSS_ATTN_MAX_DIM = 128
 
 def cross_attn_supported(heads: int, kv_heads: int, d: int, dtype: torch.dtype) -> bool:
     """Whether cross_attn takes these heads."""
-    return dtype in _DTYPES and 0 < d <= CROSS_ATTN_MAX_DIM and d % 8 == 0 and kv_heads > 0 and heads % kv_heads == 0
+    return (dtype in _OPERATOR_DTYPES and 0 < d <= CROSS_ATTN_MAX_DIM and d % 8 == 0 and kv_heads > 0
+            and heads % kv_heads == 0)
 
 
 def cross_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float | None = None,
@@ -718,38 +528,9 @@ def cross_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: floa
     D and 16-byte aligned rows (a stride of 0 broadcasts). scale defaults to 1 / sqrt(D).
     key_lens (int32 (B,)) and key_mask (bool (B, Tk), True: attend) say which keys are
     there: what the others hold does not matter, and a query without keys gives zeros.
-    Differentiable in q, k and v (once)."""
-    dev, dt, qs, ks = q.device, q.dtype, q.shape, k.shape
-    if not (q.is_cuda and k.is_cuda and v.is_cuda):
-        _check_cuda(q, k, v)
-    if k.device != dev or v.device != dev:
-        _same_device(q, k, v)
-    if len(qs) != 4 or len(ks) != 4 or v.shape != ks or ks[0] != qs[0] or ks[3] != qs[3]:
-        raise ValueError(f"q (B, Tq, H, D), k and v (B, Tk, Hk, D) expected, got {tuple(qs)}, {tuple(ks)}, "
-                         f"{tuple(v.shape)}")
-    if dt not in _DTYPES or k.dtype != dt or v.dtype != dt:
-        raise TypeError("q, k and v must share one dtype of fp16, bf16, fp32")
-    if not cross_attn_supported(qs[2], ks[2], qs[3], dt):
-        raise ValueError(f"heads {qs[2]} / {ks[2]} of {qs[3]} are not supported: key heads divide query "
-                         f"heads, head size a multiple of 8 up to {CROSS_ATTN_MAX_DIM}")
-    if not (_vector_ok(q) and _vector_ok(k) and _vector_ok(v)):
-        raise ValueError("q, k and v need contiguous, 16-byte aligned head rows")
-    if key_lens is not None:
-        _check_cuda(key_lens)
-        _same_device(q, key_lens)
-        if key_lens.dtype != torch.int32 or key_lens.shape != ks[:1] or not key_lens.is_contiguous():
-            raise ValueError("key_lens must be contiguous int32 (B,)")
-    if key_mask is not None:
-        _check_cuda(key_mask)
-        _same_device(q, key_mask)
-        if key_mask.dtype != torch.bool or key_mask.shape != ks[:2] or not key_mask.is_contiguous():
-            raise ValueError("key_mask must be contiguous bool (B, Tk)")
-    scale = 1.0 / math.sqrt(qs[3]) if scale is None else float(scale)
-    if not 0.0 < scale < 3e38:
-        raise ValueError(f"scale must be positive and finite, got {scale}")
-    if _wants_grad(q, k, v):
-        return _CrossAttn.apply(q, k, v, scale, key_lens, key_mask)
-    return _cross_attn(q, k, v, scale, key_lens, key_mask, False)[0]
+    Differentiable in q, k and v."""
+    _lib.launch_count += 1
+    return _torch_ops().cross_attn(q, k, v, scale, key_lens, key_mask)
 
 
 def split_bf16x2(x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:

@@ -14,7 +14,7 @@ import math
 import pytest
 import torch
 
-from sparsesam_b200 import ops
+from sparsesam_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -182,6 +182,25 @@ def test_partial_gradients(cuda_device):
         ins = [t.detach().requires_grad_(j == i) for j, t in enumerate((q, k, v))]
         (g,) = torch.autograd.grad(ops.cross_attn(*ins), ins[i], do)
         assert torch.equal(g, full[i + 1])
+
+
+def test_status_becomes_the_library_error(cuda_device):
+    """A refusal of the C entry that the wrapper does not foresee (a 65536th batch entry)."""
+    q = torch.zeros(65536, 1, 1, 8, dtype=torch.float16, device=cuda_device)
+    with pytest.raises(_lib.SparseSAMError) as e:
+        ops.cross_attn(q, q, q)
+    assert e.value.status == _lib.SSAM_ERR_UNSUPPORTED and e.value.fn == "ssam_cross_attn_fwd"
+
+
+def test_gradients_are_not_differentiated_again(cuda_device):
+    """Asking for a graph of the backward pass is fine; differentiating it is an error, not a silent zero."""
+    q, k, v, do = make(cuda_device, 1, 4, 9, 1, 1, 16, "fp32")
+    q.requires_grad_(True)
+    (g,) = torch.autograd.grad(ops.cross_attn(q, k, v), q, do, create_graph=True)
+    assert torch.equal(g.detach(), run(q.detach(), k, v, do)[1])
+    with pytest.raises(RuntimeError, match="cannot be differentiated"):
+        g.sum().backward()
+    assert q.grad is None
 
 
 def test_empty_sets(cuda_device):

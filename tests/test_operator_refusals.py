@@ -82,21 +82,17 @@ def test_layernorm_gradient_abi():
 
 def test_cpu_tensors_are_refused():
     t = torch.zeros(1, 4, 2, 16)
-    with pytest.raises(ValueError):
+    with pytest.raises(ValueError, match="CUDA"):
         ops.cross_attn(t, t, t)
-    with pytest.raises(ValueError):
+    with pytest.raises(ValueError, match="CUDA"):
         ops.groupnorm_act(torch.zeros(1, 4, 16), 2, torch.ones(16), torch.zeros(16))
-    with pytest.raises(ValueError):
+    with pytest.raises(ValueError, match="CUDA"):
         ops.layernorm_gelu_half(torch.zeros(4, 32).half(), torch.ones(32).half(), torch.zeros(32).half(), 1e-6, False)
 
 
-class FakeCuda(torch.Tensor):
-    """A CPU tensor that says it is on a GPU: the wrappers' own checks come before any launch."""
-    is_cuda = property(lambda self: True)
-
-
+# the device is checked last: these CPU tensors get as far as the fault that each case names
 def fake(*shape, dtype=torch.float16):
-    return torch.zeros(*shape, dtype=dtype).as_subclass(FakeCuda)
+    return torch.zeros(*shape, dtype=dtype)
 
 
 @pytest.mark.parametrize("kwargs,error", [
@@ -109,8 +105,9 @@ def fake(*shape, dtype=torch.float16):
 ])
 def test_cross_attention_wrapper(kwargs, error):
     args = {"q": fake(1, 4, 2, 16), "k": fake(1, 6, 2, 16), "v": fake(1, 6, 2, 16), **kwargs}
-    with pytest.raises(error):
+    with pytest.raises(error) as e:
         ops.cross_attn(**args)
+    assert "CUDA" not in str(e.value)
 
 
 @pytest.mark.parametrize("kwargs,error", [
@@ -120,5 +117,6 @@ def test_cross_attention_wrapper(kwargs, error):
 ])
 def test_groupnorm_wrapper(kwargs, error):
     args = {"x": fake(2, 5, 16), "groups": 2, "w": fake(16), "b": fake(16), **kwargs}
-    with pytest.raises(error):
+    with pytest.raises(error) as e:
         ops.groupnorm_act(**args)
+    assert "CUDA" not in str(e.value)
