@@ -102,11 +102,44 @@ __device__ __forceinline__ void merge_sums(float* part, int KS, int RB, int W, E
   cluster_sync_all();
 }
 
+// The block's own rows, which lie heads * d apart, through shared memory: four lanes fetch a row's 64 bytes and more
+// together, where a thread that reads its own row by itself touches 32 lines per load (image -> tokens, fp32, 64
+// images: 144 us that way). row(i) is row i's address, nullptr behind the last.
+template <int DP, class R>
+__device__ __forceinline__ void fetch_own(float* sm, int RB, int d, R row) {
+  constexpr int V = DP / 4, LD = DP + 4;
+  for (int e = threadIdx.x; e < RB * V; e += kXThreads) {
+    const int i = e / V, c = e % V * 4;
+    const float* p = row(i);
+    const bool there = p != nullptr && c < d;
+    cp_async16(smem_u32(sm + i * LD + c), there ? p + c : row(0), there ? 16u : 0u);
+  }
+}
+template <int DT>
+__device__ __forceinline__ void own_row(const float* p, float2 (&r)[DT / 2]) {
+#pragma unroll
+  for (int i = 0; i < DT; i += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(p + i);
+    r[i / 2] = make_float2(v.x, v.y), r[i / 2 + 1] = make_float2(v.z, v.w);
+  }
+}
+template <int DT>
+__device__ __forceinline__ void put_row(float* p, const float2 (&r)[DT / 2], float f) {
+#pragma unroll
+  for (int i = 0; i < DT; i += 4)
+    *reinterpret_cast<float4*>(p + i) = make_float4(r[i / 2].x * f, r[i / 2].y * f, r[i / 2 + 1].x * f, r[i / 2 + 1].y * f);
+}
+
 // What the two row kernels share: a block's place, and the walk over its keys. body(tile of K, tile of V, keys of
 // the tile rounded up to the slices, there) is called with the tile in shared memory.
 struct XPlace {
   int part, lr, slice, KS, b, n, cl, rank, rows, r0, r, t, h;
   bool row_ok;
+  // address of the block's row i in a tensor of queries, nullptr behind the last
+  __device__ __forceinline__ const float* row_of(const XAttn& a, const float* p, const int64_t (&st)[3], int i) const {
+    const int rr = r0 + i, gg = a.group == 1 ? 0 : rr / a.Tq, tt = rr - gg * a.Tq;
+    return rr < rows ? p + b * st[0] + tt * st[1] + (n * a.group + gg) * st[2] : nullptr;
+  }
   __device__ __forceinline__ XPlace(const XAttn& a, int RB, int TPR) {
     KS = kXThreads / (RB * TPR);
     part = threadIdx.x % TPR, lr = threadIdx.x / TPR % RB, slice = threadIdx.x / (TPR * RB);
@@ -158,8 +191,11 @@ __global__ void __launch_bounds__(kXThreads) xattn_fwd_scalar(const XAttn a, int
   const int part = x.part, lr = x.lr, slice = x.slice, KS = x.KS, b = x.b, n = x.n, cl = x.cl, rank = x.rank, rows = x.rows,
             r0 = x.r0;
   float2 q[DT / 2], o[DT / 2];
-  load_row<DT>(static_cast<const float*>(a.q) + b * a.qs[0] + x.t * a.qs[1] + x.h * a.qs[2] + part * DT, a.d - part * DT,
-               x.row_ok, q);
+  fetch_own<DP>(xsm, RB, a.d, [&](int i) { return x.row_of(a, static_cast<const float*>(a.q), a.qs, i); });
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
+  own_row<DT>(xsm + lr * LD + part * DT, q);
+  __syncthreads();
   clear_row<DT>(o);
   float m = -INFINITY, l = 0.f;
   walk_keys<DP>(a, x, xsm, there, [&](const float* sk, const float* sv, int nk, const uint8_t* here) {
@@ -191,20 +227,23 @@ __global__ void __launch_bounds__(kXThreads) xattn_fwd_scalar(const XAttn a, int
       }
     }
   });
-  if (KS == 1 && cl == 1) {                  // a row is one group of TPR threads
-    if (!x.row_ok) return;
+  if (KS == 1 && cl == 1) {                  // a row is one group of TPR threads: out through shared memory, as it came
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    float* to = static_cast<float*>(a.out) + b * a.os[0] + x.t * a.os[1] + x.h * a.os[2] + part * DT;
-    float* to32 = a.out_f32 == nullptr ? nullptr : a.out_f32 + ((static_cast<int64_t>(b) * a.Tq + x.t) * a.heads + x.h) * a.d + part * DT;
-#pragma unroll
-    for (int i = 0; i < DT; i += 4) {
-      if (part * DT + i >= a.d) break;
-      const float4 y = make_float4(o[i / 2].x * inv, o[i / 2].y * inv, o[i / 2 + 1].x * inv, o[i / 2 + 1].y * inv);
-      *reinterpret_cast<float4*>(to + i) = y;
-      if (to32 != nullptr) *reinterpret_cast<float4*>(to32 + i) = y;
-    }
-    if (a.lse != nullptr && part == 0)
+    put_row<DT>(xsm + lr * LD + part * DT, o, inv);
+    if (a.lse != nullptr && part == 0 && x.row_ok)
       a.lse[(static_cast<int64_t>(b) * a.heads + x.h) * a.Tq + x.t] = l == 0.f ? INFINITY : m + log2f(l);
+    __syncthreads();
+    for (int e = threadIdx.x; e < RB * (DP / 4); e += kXThreads) {
+      const int i = e / (DP / 4), col = e % (DP / 4) * 4;
+      float* to = const_cast<float*>(x.row_of(a, static_cast<const float*>(a.out), a.os, i));
+      if (to == nullptr || col >= a.d) continue;
+      const float4 y = *reinterpret_cast<const float4*>(xsm + i * LD + col);
+      *reinterpret_cast<float4*>(to + col) = y;
+      if (a.out_f32 != nullptr) {
+        const int64_t dense[3] = {static_cast<int64_t>(a.Tq) * a.heads * a.d, static_cast<int64_t>(a.heads) * a.d, a.d};
+        *reinterpret_cast<float4*>(const_cast<float*>(x.row_of(a, a.out_f32, dense, i)) + col) = y;
+      }
+    }
     return;
   }
   // join the slices and blocks: rescale everybody's share to the common maximum first
@@ -278,12 +317,23 @@ __global__ void __launch_bounds__(kXThreads) xattn_dq_scalar(const XAttn a, int 
   extern __shared__ __align__(16) float xsm[];
   __shared__ uint8_t there[2][kXTile<DP>];
   const XPlace x(a, RB, TPR);
-  const int part = x.part, slice = x.slice, KS = x.KS, b = x.b, dims = a.d - x.part * DT;
+  const int part = x.part, slice = x.slice, KS = x.KS, b = x.b;
   float2 q[DT / 2], dO[DT / 2], dq[DT / 2];
-  load_row<DT>(static_cast<const float*>(a.q) + b * a.qs[0] + x.t * a.qs[1] + x.h * a.qs[2] + part * DT, dims, x.row_ok, q);
-  load_row<DT>(static_cast<const float*>(a.dout) + b * a.os[0] + x.t * a.os[1] + x.h * a.os[2] + part * DT, dims, x.row_ok, dO);
   const int64_t stat = (static_cast<int64_t>(b) * a.heads + x.h) * a.Tq + x.t;
-  load_row<DT>(a.out_f32 + ((static_cast<int64_t>(b) * a.Tq + x.t) * a.heads + x.h) * a.d + part * DT, dims, x.row_ok, dq);
+  const int64_t dense[3] = {static_cast<int64_t>(a.Tq) * a.heads * a.d, static_cast<int64_t>(a.heads) * a.d, a.d};
+  const int own = RB * LD;
+  fetch_own<DP>(xsm, RB, a.d, [&](int i) { return x.row_of(a, static_cast<const float*>(a.q), a.qs, i); });
+  fetch_own<DP>(xsm + own, RB, a.d, [&](int i) { return x.row_of(a, static_cast<const float*>(a.dout), a.os, i); });
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
+  own_row<DT>(xsm + x.lr * LD + part * DT, q);
+  own_row<DT>(xsm + own + x.lr * LD + part * DT, dO);
+  __syncthreads();
+  fetch_own<DP>(xsm, RB, a.d, [&](int i) { return x.row_of(a, a.out_f32, dense, i); });
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
+  own_row<DT>(xsm + x.lr * LD + part * DT, dq);
+  __syncthreads();
   const float delta = row_dot<DT, TPR>(dO, [&](int i) { return make_float4(dq[2 * i].x, dq[2 * i].y, dq[2 * i + 1].x, dq[2 * i + 1].y); });
   const float lse = x.row_ok ? a.lse[stat] : INFINITY;
   if (x.row_ok && part == 0 && slice == 0 && x.rank == 0) a.delta[stat] = delta;
@@ -298,13 +348,12 @@ __global__ void __launch_bounds__(kXThreads) xattn_dq_scalar(const XAttn a, int 
     }
   });
   if (KS == 1 && x.cl == 1) {
-    if (!x.row_ok) return;
-    float* to = static_cast<float*>(a.dq) + ((static_cast<int64_t>(b) * a.Tq + x.t) * a.heads + x.h) * a.d + part * DT;
-#pragma unroll
-    for (int i = 0; i < DT; i += 4) {
-      if (part * DT + i >= a.d) break;
-      *reinterpret_cast<float4*>(to + i) = make_float4(dq[i / 2].x * a.scale, dq[i / 2].y * a.scale, dq[i / 2 + 1].x * a.scale,
-                                                       dq[i / 2 + 1].y * a.scale);
+    put_row<DT>(xsm + x.lr * LD + part * DT, dq, a.scale);
+    __syncthreads();
+    for (int e = threadIdx.x; e < RB * (DP / 4); e += kXThreads) {
+      const int i = e / (DP / 4), col = e % (DP / 4) * 4;
+      float* to = const_cast<float*>(x.row_of(a, static_cast<const float*>(a.dq), dense, i));
+      if (to != nullptr && col < a.d) *reinterpret_cast<float4*>(to + col) = *reinterpret_cast<const float4*>(xsm + i * LD + col);
     }
     return;
   }
@@ -396,14 +445,16 @@ __global__ void __launch_bounds__(kXThreads) xattn_dkv_scalar(const XAttn a, int
 }
 
 // Launch
-// Rows per block (a power of two, at most 128 / tpr) and blocks per cluster for `own` rows that each walk `other`
-// entries, `tile` at a time: blocks are added along `other` until the device is filled.
+// Rows per block (a power of two, at most 128 / tpr: few rows left empty, and a block costs as much as 16 rows) and
+// blocks per cluster for `own` rows that each walk `other` entries, `tile` at a time: blocks are added along `other`
+// until the device has four of these small blocks per SM.
 static void xattn_plan(int own, int other, int64_t pairs, int tpr, int tile, int* rb, int* cluster) {
-  int r = 4;
-  while (r < own && r < kXThreads / tpr) r *= 2;
+  int r = kXThreads / tpr;
+  for (int x = r / 2; x >= 4; x /= 2)
+    if ((own + x - 1) / x * (x + 16) < (own + r - 1) / r * (r + 16)) r = x;
   const int64_t blocks = pairs * ((own + r - 1) / r);
   int c = 1;
-  while (c < 8 && blocks * c < 2 * 148 && other > c * tile) c *= 2;
+  while (c < 8 && blocks * c < 4 * 148 && other > c * tile) c *= 2;
   *rb = r;
   *cluster = c;
 }

@@ -1356,9 +1356,11 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_long(const XAttn a, int 
 // Blocks per cluster: blocks are added along the long side until every SM has one, while each warp
 // keeps at least one step. (Two per SM measured slower: 64 pairs of 4096 keys forward 17 us against 12,
 // the join outweighs the shorter walks.)
-static int xattn_cluster(int64_t blocks, int other, int step) {
+static int xattn_cluster(int64_t blocks, int other, int step, int most = 8) {
   int c = 1;
-  while (c < 8 && blocks * c < 148 && other > c * kXmWarps * step) c *= 2;
+  // 16 only where the warps of 8 blocks would walk four steps or more (4096 keys: 4.95 us with 8, 5.4 with 16;
+  // 16384 keys: 8.8 and 7.4)
+  while (c < most && (c < 8 || (blocks * 16 <= 148 && other >= 32 * kXmWarps * step)) && blocks * c < 148 && other > c * kXmWarps * step) c *= 2;
   return c;
 }
 template <class T, int DP, int MT>
@@ -1379,11 +1381,13 @@ static int xattn_fwd_long_launch(const XAttn& a, cudaStream_t stream) {
 template <class T, int DP, int NQ, int HP = 1>
 static int xattn_few_rows_launch(const XAttn& a, cudaStream_t stream) {
   const int rows = a.group * a.Tq, tiles = (rows + 8 * NQ - 1) / (8 * NQ);
-  const int cl = xattn_cluster(static_cast<int64_t>(a.B) * (a.kv_heads / HP) * tiles, a.Tk, DP <= 32 ? 32 : 16);
   constexpr size_t smem = (kXmWarps * HP * 8 * NQ + HP * 8 * NQ + kXmWarps * NQ * (DP / 4 + 2) * 32) * sizeof(float);
   static PerDeviceOnce once;
+  static ClusterLimit limit;
   const int st = allow_smem(once, xattn_fwd_few_rows<T, DP, NQ, HP>, smem);
   if (st != SSAM_OK) return st;
+  const int cl = xattn_cluster(static_cast<int64_t>(a.B) * (a.kv_heads / HP) * tiles, a.Tk, DP <= 32 ? 32 : 16,
+                               limit.get(xattn_fwd_few_rows<T, DP, NQ, HP>, kXmThreads, smem));
   return launch_cluster(xattn_fwd_few_rows<T, DP, NQ, HP>, dim3(tiles * cl, a.kv_heads / HP, a.B), kXmThreads, smem, cl,
                         stream, a, 0);
 }
@@ -1407,11 +1411,13 @@ static bool xattn_paired(const XAttn& a) {
 
 template <class T, int DP, int NF, bool FEW_ROWS>
 static int xattn_bwd_few_launch(const XAttn& a, cudaStream_t stream) {
-  const int cl = xattn_cluster(static_cast<int64_t>(a.B) * a.kv_heads, FEW_ROWS ? a.Tk : a.group * a.Tq, 16);
   constexpr size_t smem = kXmWarps * (FEW_ROWS ? 1 : 2) * NF * (DP / 4) * 32 * sizeof(float);
   static PerDeviceOnce once;
+  static ClusterLimit limit;
   const int st = allow_smem(once, xattn_bwd_few<T, DP, NF, FEW_ROWS>, smem);
   if (st != SSAM_OK) return st;
+  const int cl = xattn_cluster(static_cast<int64_t>(a.B) * a.kv_heads, FEW_ROWS ? a.Tk : a.group * a.Tq, 16,
+                               limit.get(xattn_bwd_few<T, DP, NF, FEW_ROWS>, kXmThreads, smem));
   return launch_cluster(xattn_bwd_few<T, DP, NF, FEW_ROWS>, dim3(cl, a.kv_heads, a.B), kXmThreads, smem, cl, stream, a,
                         0);
 }

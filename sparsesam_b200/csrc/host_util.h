@@ -56,6 +56,41 @@ int allow_smem(PerDeviceOnce& once, K kernel, int64_t bytes) {
   });
 }
 
+// Blocks per cluster that a kernel may use: 16 where the device holds such a cluster of its blocks (the size is not
+// portable), else 8. Allows `bytes` of dynamic shared memory as well. Found once per device.
+class ClusterLimit {
+ public:
+  template <class K>
+  int get(K kernel, int threads, int64_t bytes) {
+    const int dev = current_device();
+    if (dev < 0) return 8;
+    int v = most_[dev].load(std::memory_order_acquire);
+    if (v != 0) return v;
+    v = 8;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) == cudaSuccess &&
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(16);
+      cfg.blockDim = dim3(threads);
+      cfg.dynamicSmemBytes = static_cast<size_t>(bytes);
+      cudaLaunchAttribute at[1];
+      at[0].id = cudaLaunchAttributeClusterDimension;
+      at[0].val.clusterDim.x = 16;
+      at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+      cfg.attrs = at;
+      cfg.numAttrs = 1;
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess && n > 0) v = 16;
+    }
+    cudaGetLastError();                      // a refusal above is an answer, not an error of the call
+    most_[dev].store(v, std::memory_order_release);
+    return v;
+  }
+
+ private:
+  std::atomic<int> most_[kMaxDevices] = {};
+};
+
 // Multiprocessor count of `dev` (cached; 148 on B200).
 int num_sms(int dev);
 

@@ -335,6 +335,19 @@ __device__ __forceinline__ void block_moments(const Running<V>& r, bool active, 
   __syncthreads();
 }
 
+// Sum over the block, for every thread; red: [2][8], used in turn by the parity of `round`.
+__device__ __forceinline__ float block_sum(float v, float* red, int round) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  float* to = red + (round & 1) * kGnWarps;
+  if (threadIdx.x % 32 == 0) to[threadIdx.x / 32] = v;
+  __syncthreads();
+  v = 0.f;
+#pragma unroll
+  for (int i = 0; i < kGnWarps; ++i) v += to[i];
+  return v;
+}
+
 struct GnArgs {
   const void *x, *dout, *w, *b;
   int64_t HW;
@@ -368,6 +381,15 @@ struct Apply {
       A[i] = mul2(A[i], make_float2(s_rs[g1], s_rs[g2]));
     }
   }
+  __device__ __forceinline__ Apply(const GnArgs& a, int ch, float mean, float rstd) {
+    load_pairs(static_cast<const T*>(a.w) + ch, A);
+    load_pairs(static_cast<const T*>(a.b) + ch, b);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      mu[i] = both(-mean);
+      A[i] = mul2(A[i], both(rstd));
+    }
+  }
   __device__ __forceinline__ void operator()(const uint4& u, T* to) const {
     float2 f[P];
     Vec<T>::unpack(u, f);
@@ -389,13 +411,62 @@ __global__ void __launch_bounds__(kGnThreads) groupnorm_resident_kernel(const Gn
   const int64_t p0 = min(a.HW, static_cast<int64_t>(rank) * a.span), p1 = min(a.HW, p0 + a.span);
   uint4* keep = reinterpret_cast<uint4*>(gsm);                       // [span][cols]
   float* vals = gsm + static_cast<int64_t>(a.span) * cols * 4;       // [lanes][slab]
-  float* red = vals + lanes * a.slab;                                // [max(G, 8)]
-  float* s_mean = red + max(G, kGnWarps);                            // [G], m2 behind it
+  float* red = vals + lanes * a.slab;                                // [max(G, 16)]
+  float* s_mean = red + max(G, 2 * kGnWarps);                            // [G], m2 behind it
   const int64_t base = (static_cast<int64_t>(n) * a.HW + p0) * a.C + c0 + col * V;
   const T* x = static_cast<const T*>(a.x) + base;
   const int len = static_cast<int>(p1 - p0);
   Running<V> r;
   if (active) r.walk(x, lane, lanes, len, a.C, [&](int p, const uint4& u) { keep[p * cols + col] = u; });
+  T* out = static_cast<T*>(a.out) + base;
+  if (G == 1) {
+    // one group: block sums of scalars, and every warp joins the cluster's moments by itself
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) m += r.mean[i].x + r.mean[i].y;
+    const float here = static_cast<float>(max(len, 1)) * a.cg;
+    const float mu_here = block_sum(r.n * m, red, 0) / here;
+    float q = 0.f;
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      const float dx = r.mean[i].x - mu_here, dy = r.mean[i].y - mu_here;
+      q += fmaf(r.n * dx, dx, r.m2[i].x) + fmaf(r.n * dy, dy, r.m2[i].y);
+    }
+    const float q_here = block_sum(q, red, 1);
+    float mu = mu_here, m2 = q_here;
+    if (cl > 1) {
+      if (threadIdx.x == 0) s_mean[0] = mu_here, s_mean[1] = q_here;
+      cluster_sync_all();
+      const int i = static_cast<int>(threadIdx.x) % 32;
+      float ni = 0.f, mi = 0.f, qi = 0.f;
+      if (i < cl) {
+        ni = static_cast<float>(min(a.HW, static_cast<int64_t>(i + 1) * a.span) - min(a.HW, static_cast<int64_t>(i) * a.span)) * a.cg;
+        const uint32_t at = mapa_shared(smem_u32(s_mean), i);
+        mi = ld_dsmem(at), qi = ld_dsmem(at + 4);
+      }
+      __syncwarp();
+      cluster_arrive();                      // this block has read its peers
+      auto warp_sum = [](float v) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+      };
+      mu = warp_sum(ni * mi) / (static_cast<float>(a.HW) * a.cg);
+      m2 = warp_sum(fmaf(ni * (mi - mu), mi - mu, qi));
+    }
+    const float rs = rsqrtf(m2 / (static_cast<float>(a.HW) * a.cg) + a.eps);
+    if (rank == 0 && threadIdx.x == 0 && a.mean != nullptr) {
+      const int64_t to = static_cast<int64_t>(n) * (a.C / a.cg) + c0 / a.cg;
+      a.mean[to] = mu, a.rstd[to] = rs;
+    }
+    if (active) {
+      const Apply<T, ACT> apply(a, c0 + col * V, mu, rs);
+      for (int p = lane; p < len; p += lanes) apply(keep[p * cols + col], out + static_cast<int64_t>(p) * a.C);
+    }
+    __syncwarp();
+    if (cl > 1) cluster_wait();              // no block leaves while its peers may read it
+    return;
+  }
   block_moments<V>(r, active, lane, col, lanes, a.slab, a.cg, static_cast<float>(max(len, 1)), vals, red, s_mean,
                    s_mean + G);
   if (cl > 1) cluster_sync_all();
@@ -424,7 +495,6 @@ __global__ void __launch_bounds__(kGnThreads) groupnorm_resident_kernel(const Gn
   if (cl > 1) cluster_sync_all(); else __syncthreads();
   if (!active) return;
   const Apply<T, ACT> apply(a, c0 + col * V, s_out, s_out + G, c0 / a.cg);
-  T* out = static_cast<T*>(a.out) + base;
   for (int p = lane; p < len; p += lanes) apply(keep[p * cols + col], out + static_cast<int64_t>(p) * a.C);
 }
 
@@ -740,10 +810,10 @@ static size_t gn_resident_smem(int64_t span, int slab, int cg, int elem, bool ba
   const int V = 16 / elem, lanes = kGnThreads / (slab / V), G = slab / cg;
   const size_t keep = static_cast<size_t>(span) * slab * elem * (backward ? 2 : 1);
   return backward ? keep + (2 * static_cast<size_t>(lanes) * slab + 2 * slab) * 4
-                  : keep + (static_cast<size_t>(lanes) * slab + std::max(G, kGnWarps) + 2 * G) * 4;
+                  : keep + (static_cast<size_t>(lanes) * slab + std::max(G, 2 * kGnWarps) + 2 * G) * 4;
 }
 
-static GnPlan groupnorm_plan(int N, int64_t HW, int C, int groups, int elem, bool backward) {
+static GnPlan groupnorm_plan(int N, int64_t HW, int C, int groups, int elem, bool backward, int most = 8) {
   GnPlan p = {};
   const int V = 16 / elem, cg = C / groups;
   // the narrowest slab of whole groups and whole vectors that is at least 64 bytes wide and divides C
@@ -760,14 +830,17 @@ static GnPlan groupnorm_plan(int N, int64_t HW, int C, int groups, int elem, boo
   while (cl < 8 && HW > cl * 64 &&
          (clusters * cl < 148 || gn_resident_smem((HW + cl - 1) / cl, slab, cg, elem, backward) > kGnResident / 2))
     cl *= 2;
+  const int64_t span0 = (HW + cl - 1) / cl;
+  // 16 blocks (not portable) only shorten the walk: they change neither what fits nor the workspace
+  if (most >= 16 && cl == 8 && clusters * 16 <= 148 && HW > 16 * 64) cl = 16;
   const int64_t span = (HW + cl - 1) / cl;
-  if (room && span < (1 << 20) && gn_resident_smem(span, slab, cg, elem, backward) <= static_cast<size_t>(kGnResident)) {
+  if (room && span0 < (1 << 20) && gn_resident_smem(span0, slab, cg, elem, backward) <= static_cast<size_t>(kGnResident)) {
     p.slab = slab, p.cluster = cl, p.span = static_cast<int>(span);
     p.smem = gn_resident_smem(span, slab, cg, elem, backward);
     return p;
   }
   const int64_t sample = HW * C * elem * (backward ? 2 : 1);
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(N, kGnL2 / sample)), launches = (N + most - 1) / most;
+  const int64_t fit = std::max<int64_t>(1, std::min<int64_t>(N, kGnL2 / sample)), launches = (N + fit - 1) / fit;
   p.batch = static_cast<int>((N + launches - 1) / launches);             // launches of about equal size
   const int per_sm = backward ? 2 : 4;
   const int64_t want = std::max<int64_t>(1, 148 * per_sm / p.batch);   // one wave: a block more would be a second
@@ -818,7 +891,9 @@ static size_t gn_floats(size_t n) { return (n + 3) / 4 * 16; }
 template <class T, int ACT>
 static int groupnorm_fwd_t(GnArgs a, int N, int G, float* ws, cudaStream_t stream) {
   static PerDeviceOnce resident, moments, apply;
-  const GnPlan p = groupnorm_plan(N, a.HW, a.C, G, sizeof(T), false);
+  static ClusterLimit limit;
+  const GnPlan p = groupnorm_plan(N, a.HW, a.C, G, sizeof(T), false,
+                                  limit.get(groupnorm_resident_kernel<T, ACT>, kGnThreads, kGnResident));
   a.span = p.span, a.slab = p.slab, a.part = ws;
   if (p.cluster)
     return launch_gn(groupnorm_resident_kernel<T, ACT>, resident, dim3(p.cluster, a.C / p.slab, N), p.smem, p.cluster,
@@ -838,7 +913,9 @@ static int groupnorm_fwd_t(GnArgs a, int N, int G, float* ws, cudaStream_t strea
 template <class T, int ACT>
 static int groupnorm_bwd_t(GnArgs a, int N, int G, void* dw, void* db, float* ws, cudaStream_t stream) {
   static PerDeviceOnce resident, sums, dx;
-  const GnPlan p = groupnorm_plan(N, a.HW, a.C, G, sizeof(T), true);
+  static ClusterLimit limit;
+  const GnPlan p = groupnorm_plan(N, a.HW, a.C, G, sizeof(T), true,
+                                  limit.get(groupnorm_bwd_resident_kernel<T, ACT>, kGnThreads, kGnResident));
   a.span = p.span, a.slab = p.slab, a.sums = ws;
   a.part = ws + gn_align(static_cast<size_t>(N) * 2 * a.C * sizeof(float)) / sizeof(float);
   int st;
