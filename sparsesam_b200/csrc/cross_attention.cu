@@ -59,13 +59,14 @@ __device__ __forceinline__ void clear_row(float2 (&r)[DT / 2]) {
   for (int i = 0; i < DT / 2; ++i) r[i] = make_float2(0.f, 0.f);
 }
 
-// Starts the copy of `n` rows of width d into sm[kXTile][DP + 4]; rows n .. kXTile - 1, rows for which ok(i) is
+// Starts the copy of `n` rows of width d into sm[kXTile][DP + 4]; rows n .. upto - 1, rows for which ok(i) is
 // false, and channels past d, are zeros.
 template <int DP, class P, class O>
-__device__ __forceinline__ void stage_rows(float* sm, int n, int d, P row, O ok) {
+__device__ __forceinline__ void stage_rows(float* sm, int n, int upto, int d, P row, O ok) {
   constexpr int V = DP / 4, LD = DP + 4;
 #pragma unroll
   for (int e0 = 0; e0 < kXTile<DP> * V; e0 += kXThreads) {
+    if (e0 >= upto * V) break;
     const int e = e0 + threadIdx.x, i = e / V, c = (e % V) * 4;
     const bool there = i < n && c < d && ok(i);
     cp_async16(smem_u32(sm + i * LD + c), there ? row(i) + c : row(0), there ? 16u : 0u);
@@ -131,7 +132,8 @@ __device__ __forceinline__ void put_row(float* p, const float2 (&r)[DT / 2], flo
 }
 
 // What the two row kernels share: a block's place, and the walk over its keys. body(tile of K, tile of V, keys of
-// the tile rounded up to the slices, there) is called with the tile in shared memory.
+// the tile rounded up to the slices, their biases: 0, or -infinity where there is no key) is called with the tile in
+// shared memory.
 struct XPlace {
   int part, lr, slice, KS, b, n, cl, rank, rows, r0, r, t, h;
   bool row_ok;
@@ -153,7 +155,7 @@ struct XPlace {
   }
 };
 template <int DP, class B>
-__device__ __forceinline__ void walk_keys(const XAttn& a, const XPlace& x, float* xsm, uint8_t (&there)[2][kXTile<DP>], B body) {
+__device__ __forceinline__ void walk_keys(const XAttn& a, const XPlace& x, float* xsm, float (&bias)[2][kXTile<DP>], B body) {
   constexpr int XT = kXTile<DP>, LD = DP + 4;
   const int keys = xattn_keys(a, x.b);
   const float* kb = static_cast<const float*>(a.k) + x.b * a.ks[0] + x.n * a.ks[2];
@@ -161,12 +163,12 @@ __device__ __forceinline__ void walk_keys(const XAttn& a, const XPlace& x, float
   const uint8_t* mask = a.key_mask == nullptr ? nullptr : a.key_mask + static_cast<int64_t>(x.b) * a.Tk;
   auto stage = [&](int j0, int buf) {
     if (j0 < keys) {
-      const int nk = min(XT, keys - j0);
+      const int nk = min(XT, keys - j0), upto = (nk + x.KS - 1) / x.KS * x.KS;
       auto ok = [&](int i) { return mask == nullptr || __ldg(mask + j0 + i) != 0; };
       float* to = xsm + buf * 2 * XT * LD;
-      stage_rows<DP>(to, nk, a.d, [&](int i) { return kb + (j0 + i) * a.ks[1]; }, ok);
-      stage_rows<DP>(to + XT * LD, nk, a.d, [&](int i) { return vb + (j0 + i) * a.vs[1]; }, ok);
-      if (threadIdx.x < XT) there[buf][threadIdx.x] = threadIdx.x < nk && ok(threadIdx.x);
+      stage_rows<DP>(to, nk, upto, a.d, [&](int i) { return kb + (j0 + i) * a.ks[1]; }, ok);
+      stage_rows<DP>(to + XT * LD, nk, upto, a.d, [&](int i) { return vb + (j0 + i) * a.vs[1]; }, ok);
+      if (threadIdx.x < XT) bias[buf][threadIdx.x] = threadIdx.x < nk && ok(threadIdx.x) ? 0.f : -INFINITY;
     }
     stage_commit();
   };
@@ -177,7 +179,7 @@ __device__ __forceinline__ void walk_keys(const XAttn& a, const XPlace& x, float
     stage_wait();
     __syncthreads();
     const float* sk = xsm + buf * 2 * XT * LD;
-    body(sk, sk + XT * LD, (min(XT, keys - j0) + x.KS - 1) / x.KS * x.KS, there[buf]);
+    body(sk, sk + XT * LD, (min(XT, keys - j0) + x.KS - 1) / x.KS * x.KS, bias[buf]);
     __syncthreads();                         // the other buffer is filled next
   }
 }
@@ -186,7 +188,7 @@ template <int DT, int TPR>
 __global__ void __launch_bounds__(kXThreads) xattn_fwd_scalar(const XAttn a, int RB) {
   constexpr int DP = DT * TPR, LD = DP + 4, U = 4;
   extern __shared__ __align__(16) float xsm[];
-  __shared__ uint8_t there[2][kXTile<DP>];
+  __shared__ float bias[2][kXTile<DP>];
   const XPlace x(a, RB, TPR);
   const int part = x.part, lr = x.lr, slice = x.slice, KS = x.KS, b = x.b, n = x.n, cl = x.cl, rank = x.rank, rows = x.rows,
             r0 = x.r0;
@@ -198,7 +200,7 @@ __global__ void __launch_bounds__(kXThreads) xattn_fwd_scalar(const XAttn a, int
   __syncthreads();
   clear_row<DT>(o);
   float m = -INFINITY, l = 0.f;
-  walk_keys<DP>(a, x, xsm, there, [&](const float* sk, const float* sv, int nk, const uint8_t* here) {
+  walk_keys<DP>(a, x, xsm, bias, [&](const float* sk, const float* sv, int nk, const float* here) {
     for (int j = slice; j < nk; j += U * KS) {           // U keys at a time: one look at the maximum
       float s[U], top = m;
 #pragma unroll
@@ -206,8 +208,7 @@ __global__ void __launch_bounds__(kXThreads) xattn_fwd_scalar(const XAttn a, int
         s[u] = -INFINITY;
         if (j - slice + u * KS < nk) {                   // the same for all threads
           const int i = j + u * KS;
-          const float y = row_dot<DT, TPR>(q, sk + i * LD + part * DT) * a.c;
-          if (here[i]) s[u] = y;
+          s[u] = fmaf(row_dot<DT, TPR>(q, sk + i * LD + part * DT), a.c, here[i]);   // -infinity: no such key
         }
         top = fmaxf(top, s[u]);
       }
@@ -315,7 +316,7 @@ template <int DT, int TPR>
 __global__ void __launch_bounds__(kXThreads) xattn_dq_scalar(const XAttn a, int RB) {
   constexpr int DP = DT * TPR, LD = DP + 4;
   extern __shared__ __align__(16) float xsm[];
-  __shared__ uint8_t there[2][kXTile<DP>];
+  __shared__ float bias[2][kXTile<DP>];
   const XPlace x(a, RB, TPR);
   const int part = x.part, slice = x.slice, KS = x.KS, b = x.b;
   float2 q[DT / 2], dO[DT / 2], dq[DT / 2];
@@ -339,12 +340,12 @@ __global__ void __launch_bounds__(kXThreads) xattn_dq_scalar(const XAttn a, int 
   if (x.row_ok && part == 0 && slice == 0 && x.rank == 0) a.delta[stat] = delta;
   if (a.dq == nullptr) return;               // only D was wanted
   clear_row<DT>(dq);
-  walk_keys<DP>(a, x, xsm, there, [&](const float* sk, const float* sv, int nk, const uint8_t* here) {
+  walk_keys<DP>(a, x, xsm, bias, [&](const float* sk, const float* sv, int nk, const float* here) {
 #pragma unroll 1
     for (int j = slice; j < nk; j += KS) {
-      const float s = row_dot<DT, TPR>(q, sk + j * LD + part * DT) * a.c;
+      const float s = fmaf(row_dot<DT, TPR>(q, sk + j * LD + part * DT), a.c, here[j]);
       const float dp = row_dot<DT, TPR>(dO, sv + j * LD + part * DT);
-      row_axpy<DT>(here[j] ? ex2f(s - lse) * (dp - delta) : 0.f, sk + j * LD + part * DT, dq);
+      row_axpy<DT>(ex2f(s - lse) * (dp - delta), sk + j * LD + part * DT, dq);
     }
   });
   if (KS == 1 && x.cl == 1) {
@@ -398,8 +399,9 @@ __global__ void __launch_bounds__(kXThreads) xattn_dkv_scalar(const XAttn a, int
       };
       auto ok = [](int) { return true; };
       float* to = xsm + buf * 2 * XT * LD;
-      stage_rows<DP>(to, nr, a.d, [&](int i) { return static_cast<const float*>(a.q) + at(i, a.qs); }, ok);
-      stage_rows<DP>(to + XT * LD, nr, a.d, [&](int i) { return static_cast<const float*>(a.dout) + at(i, a.os); }, ok);
+      const int upto = (nr + KS - 1) / KS * KS;
+      stage_rows<DP>(to, nr, upto, a.d, [&](int i) { return static_cast<const float*>(a.q) + at(i, a.qs); }, ok);
+      stage_rows<DP>(to + XT * LD, nr, upto, a.d, [&](int i) { return static_cast<const float*>(a.dout) + at(i, a.os); }, ok);
       const int64_t stat = (static_cast<int64_t>(b) * a.heads + n * a.group) * a.Tq + r0;   // rows of a key head follow one another
       if (threadIdx.x < XT) {
         s_lse[buf][threadIdx.x] = threadIdx.x < nr ? a.lse[stat + threadIdx.x] : INFINITY;

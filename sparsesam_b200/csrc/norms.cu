@@ -862,7 +862,7 @@ static int groupnorm_check(int N, int64_t HW, int C, int G, int act, int dtype, 
   if (N <= 0 || HW <= 0 || C <= 0 || G <= 0 || C % G || act < 0 || act > 3 || dtype < 0 || dtype > 2)
     return SSAM_ERR_INVALID;
   const int V = dtype == 2 ? 4 : 8;
-  if (C % V || C / V > kGnThreads || N > 65535 || HW > (1ll << 31)) return SSAM_ERR_UNSUPPORTED;
+  if (C % V || C / V > kGnThreads || N > 65535 || HW >= (1ll << 31)) return SSAM_ERR_UNSUPPORTED;
   const size_t need = groupnorm_workspace_size(N, HW, C, G, dtype, backward);
   if (workspace_bytes < need || (need > 0 && workspace == nullptr)) return SSAM_ERR_INVALID;
   return SSAM_OK;
