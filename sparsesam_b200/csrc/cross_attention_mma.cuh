@@ -1478,6 +1478,7 @@ static int xattn_mma_dp(const XAttn& a, bool backward, cudaStream_t stream) {
     if constexpr (DP <= 64) {
       if (rows <= 24 || (rows > 32 && rows <= 48)) return xattn_few_rows_launch<T, DP, 3>(a, stream);
       if (rows <= 64) return xattn_few_rows_launch<T, DP, 4>(a, stream);
+      if (a.d >= kTcMinDim && a.d <= kTcMaxDim && a.heads <= 65535) return xattn_tc_fwd(a, kIsHalf<T> ? 0 : 1, stream);
       return xattn_fwd_long_launch<T, DP, 2>(a, stream);
     } else {
       return xattn_fwd_long_launch<T, DP, 1>(a, stream);
@@ -1485,6 +1486,8 @@ static int xattn_mma_dp(const XAttn& a, bool backward, cudaStream_t stream) {
   }
   if (a.Tk <= 8 * kXmFewTiles<DP>) return xattn_bwd_few_pick<T, DP, false>(a, a.Tk, stream);
   if (rows <= 8 * kXmFewTiles<DP>) return xattn_bwd_few_pick<T, DP, true>(a, rows, stream);
+  if (!kIsHalf<T> && rows > 64 && a.Tk > 64 && a.d >= kTcMinDim && a.d <= kTcMaxDim && a.heads <= 65535)
+    return xattn_tc_bwd(a, stream);
   const int st = xattn_bwd_long_launch<T, DP, DP <= 64 ? 2 : 1, true>(a, stream);
   if (st != SSAM_OK || a.dk == nullptr) return st;
   return xattn_bwd_long_launch<T, DP, DP <= 32 ? 2 : 1, false>(a, stream);

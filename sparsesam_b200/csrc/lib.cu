@@ -6,5 +6,6 @@
 #include "perm.cu"
 #include "rows.cu"
 #include "attention.cu"
+#include "cross_attention_tc.cu"
 #include "capi.cu"
 #include "noalloc.cu"

@@ -89,7 +89,8 @@ SHAPES = [  # B, Tq, Tk, H, Hk, D
     (1, 1, 1, 1, 1, 16), (2, 1, 7, 2, 2, 16), (1, 8, 4096, 8, 8, 16), (3, 5, 65, 4, 2, 32), (2, 17, 1, 2, 2, 32),
     (2, 129, 9, 8, 8, 16), (1, 300, 64, 2, 1, 64), (2, 65, 130, 6, 2, 64), (1, 33, 257, 2, 2, 128),
     (2, 16, 16, 1, 1, 8), (1, 40, 100, 3, 1, 24), (1, 7, 515, 2, 2, 40), (2, 70, 31, 2, 2, 80), (1, 1, 3000, 4, 1, 32),
-    (2, 1000, 3, 2, 2, 16), (1, 50, 70, 2, 2, 112),
+    (2, 1000, 3, 2, 2, 16), (1, 50, 70, 2, 2, 112), (2, 150, 200, 2, 2, 40), (1, 300, 260, 4, 2, 64), (1, 129, 1030, 1, 1, 56),
+    (8, 128, 128, 8, 8, 64), (1, 1000, 65, 2, 1, 64),
 ]
 
 
@@ -102,7 +103,8 @@ def test_forward_and_gradients(cuda_device, shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
-@pytest.mark.parametrize("shape", [(4, 9, 70, 2, 2, 16), (4, 100, 20, 4, 2, 32), (4, 3, 700, 2, 1, 64), (4, 70, 90, 2, 2, 16)],
+@pytest.mark.parametrize("shape", [(4, 9, 70, 2, 2, 16), (4, 100, 20, 4, 2, 32), (4, 3, 700, 2, 1, 64), (4, 70, 90, 2, 2, 16),
+                                   (4, 130, 300, 2, 1, 64)],
                          ids=lambda s: "x".join(map(str, s)))
 @pytest.mark.parametrize("kind", ["lens", "mask", "both"])
 def test_masks(cuda_device, shape, dtype, kind):
