@@ -74,10 +74,8 @@ static int launch_cluster(K kernel, dim3 grid, int threads, size_t smem, int clu
 int xattn_fp16(const XAttn& a, bool backward, cudaStream_t stream);
 int xattn_bf16(const XAttn& a, bool backward, cudaStream_t stream);
 
-// Two long sides on the 5th-generation tensor cores (cross_attention_tc.cu): dtype 0 / 1; backward bf16.
-int xattn_tc_fwd(const XAttn& a, int dtype, cudaStream_t stream);
-int xattn_tc_bwd(const XAttn& a, cudaStream_t stream);
-constexpr int kTcMaxDim = 64, kTcMinDim = 40;   // smaller heads are bound by the exponentials either way
+// Two long sides on the 5th-generation tensor cores (cross_attention_tc.cu): dtype 0 / 1.
+int xattn_tc(const XAttn& a, int dtype, bool backward, cudaStream_t stream);
 
 // Entries of a short side that stay in registers: 8-entry tiles of the backward kernel (about 6 DP / 8
 // registers each) and of the forward kernel's keys (2 DP / 8 registers each).

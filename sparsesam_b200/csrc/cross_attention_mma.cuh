@@ -1,8 +1,8 @@
 // Tensor-core kernels of the cross attention for fp16 / bf16 (formulas and conventions
 // in cross_attention.cuh).
 //
-// Everything is built from mma.m16n8k16 on registers: head sizes here are 16 to 128
-// and one of the two token sets is usually a handful of prompt tokens, so a warp's
+// Here: one short side (the other case is cross_attention_tc.cu). Everything is built from
+// mma.m16n8k16 on registers: the short side is a handful of prompt tokens, so a warp's
 // 16-row tile is the whole problem of one head, there is nothing for a 128-row
 // tcgen05 tile to share, and DRAM or the exponentials set the pace.
 //
@@ -128,294 +128,8 @@ __device__ __forceinline__ int64_t row_dense(const XAttn& a, int b, int n, int r
   return ((static_cast<int64_t>(b) * a.Tq + t) * a.heads + n * a.group + g) * a.d;
 }
 
-// Sums acc over the block's warps into warp 0 (pairwise, a fixed order), through
-// sm[4][NREG][32]. All threads call it.
-template <int NREG>
-__device__ __forceinline__ void warp_tree_sum(float* acc, float* sm, int warp, int lane) {
-#pragma unroll
-  for (int off = kXmWarps / 2; off >= 1; off >>= 1) {
-    __syncthreads();
-    if (warp >= off && warp < 2 * off) {
-#pragma unroll
-      for (int i = 0; i < NREG; ++i) sm[((warp - off) * NREG + i) * 32 + lane] = acc[i];
-    }
-    __syncthreads();
-    if (warp < off) {
-#pragma unroll
-      for (int i = 0; i < NREG; ++i) acc[i] += sm[(warp * NREG + i) * 32 + lane];
-    }
-  }
-}
-
-// ---------------------------------------------------------------------------
-// Forward, two long sides. A warp holds 16 MT query rows of one key head and walks keys CK at a time.
-// split = false: the block's 8 warps hold 8 row tiles and each walks all keys.
-// split = true: one row tile per block, its keys shared by the 8 warps and the cluster.
-// The reference point of the exponentials is renewed only when a logit exceeds it by 2^8.
-// ---------------------------------------------------------------------------
 constexpr float kXmNone = -1e30f;           // reference before the first key
 constexpr float kXmSlack = 8.f;
-
-template <class T, int DP, int MT>
-__global__ void __launch_bounds__(kXmThreads) xattn_fwd_long(const XAttn a, int split) {
-  constexpr int NR = DP / 8;                 // registers of a row fragment = 8-channel blocks
-  constexpr int CK = DP <= 32 ? 32 : 16;     // keys per step
-  constexpr int NT = CK / 8;
-  extern __shared__ __align__(16) float xsm[];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
-  const int b = blockIdx.z, n = blockIdx.y;
-  const int cl = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
-  const int rows = a.group * a.Tq;
-  const int r0 = (split ? static_cast<int>(blockIdx.x) / cl : static_cast<int>(blockIdx.x) * kXmWarps + warp) * 16 * MT;
-  if (!split && r0 >= rows) return;
-  const int keys = xattn_keys(a, b);
-  int j_begin = 0, j_end = keys;
-  if (split) {
-    const int steps = (keys + CK - 1) / CK, ns = kXmWarps * cl;
-    const int per = (steps + ns - 1) / ns * CK;
-    j_begin = min(keys, (rank * kXmWarps + warp) * per);
-    j_end = min(keys, j_begin + per);
-  }
-  const uint8_t* mask = a.key_mask == nullptr ? nullptr : a.key_mask + static_cast<int64_t>(b) * a.Tk;
-  const T* kp = static_cast<const T*>(a.k) + b * a.ks[0] + n * a.ks[2] + (j_begin + g) * a.ks[1];
-  const T* vp = static_cast<const T*>(a.v) + b * a.vs[0] + n * a.vs[2] + (j_begin + g) * a.vs[1];
-
-  uint32_t k[NT][NR], v[NT][NR];
-  float2 bias[NT];                           // of keys 8 i + 2t, + 1: 0, or -infinity where there is none
-  auto load = [&](int j0) {                  // loads keys j0 + .. and moves on
-    if (mask == nullptr && j0 + CK <= j_end) {
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        bias[i] = make_float2(0.f, 0.f);
-        load_frag<T, DP>(kp + i * 8 * a.ks[1], t, a.d, true, k[i]);
-        load_frag<T, DP>(vp + i * 8 * a.vs[1], t, a.d, true, v[i]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        const int j = j0 + i * 8 + g;
-        const bool ok = j < j_end && (mask == nullptr || __ldg(mask + j) != 0);
-        const float mine = ok ? 0.f : -INFINITY;
-        bias[i] = make_float2(__shfl_sync(0xffffffffu, mine, 8 * t), __shfl_sync(0xffffffffu, mine, 8 * t + 4));
-        load_frag<T, DP>(kp + i * 8 * a.ks[1], t, a.d, ok, k[i]);
-        load_frag<T, DP>(vp + i * 8 * a.vs[1], t, a.d, ok, v[i]);
-      }
-    }
-    kp += CK * a.ks[1];
-    vp += CK * a.vs[1];
-  };
-  load(j_begin);
-  uint32_t q[MT][2][NR];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = r0 + mt * 16 + h * 8 + g;
-      load_frag<T, DP>(static_cast<const T*>(a.q) + row_offset(a, a.qs, b, n, min(r, rows - 1)), t, a.d, r < rows,
-                       q[mt][h]);
-    }
-  float o[MT][NR][4], m[MT][2];
-  float2 l2[MT][2];                          // the lane's sums over keys 2t and 2t + 1
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    m[mt][0] = m[mt][1] = kXmNone, l2[mt][0] = l2[mt][1] = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int i = 0; i < NR; ++i) o[mt][i][0] = o[mt][i][1] = o[mt][i][2] = o[mt][i][3] = 0.f;
-  }
-  const float2 c2 = make_float2(a.c, a.c);
-
-  for (int j0 = j_begin; j0 < j_end; j0 += CK) {
-    float2 s[MT][NT][2];
-    uint32_t vt[NT][NR];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        float f[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < NR; c += 2)
-          Mma<T>::run(f, q[mt][0][c], q[mt][1][c], q[mt][0][c + 1], q[mt][1][c + 1], k[i][c], k[i][c + 1]);
-        s[mt][i][0] = fma2(make_float2(f[0], f[1]), c2, bias[i]);
-        s[mt][i][1] = fma2(make_float2(f[2], f[3]), c2, bias[i]);
-      }
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int c = 0; c < NR; ++c) vt[i][c] = movm(v[i][c]);
-    if (j0 + CK < j_end) load(j0 + CK);      // the next step's, under this one's arithmetic
-    bool renew = false;
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float x = m[mt][h];
-#pragma unroll
-        for (int i = 0; i < NT; ++i) x = fmaxf(x, fmaxf(s[mt][i][h].x, s[mt][i][h].y));
-        renew |= x > m[mt][h] + kXmSlack;
-      }
-    if (__any_sync(0xffffffffu, renew)) {
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float x = m[mt][h];
-#pragma unroll
-          for (int i = 0; i < NT; ++i) x = fmaxf(x, fmaxf(s[mt][i][h].x, s[mt][i][h].y));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-          const float f = ex2f(m[mt][h] - x);
-          m[mt][h] = x;
-          l2[mt][h] = mul2(l2[mt][h], make_float2(f, f));
-#pragma unroll
-          for (int c = 0; c < NR; ++c) o[mt][c][2 * h] *= f, o[mt][c][2 * h + 1] *= f;
-        }
-    }
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int i = 0; i < NT; i += 2) {
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float2 p = add2(s[mt][i + x][h], make_float2(-m[mt][h], -m[mt][h]));
-            p.x = ex2f(p.x), p.y = ex2f(p.y);
-            l2[mt][h] = add2(l2[mt][h], p);
-            split2<T>(p.x, p.y, hi[2 * x + h], lo[2 * x + h]);
-          }
-#pragma unroll
-        for (int c = 0; c < NR; ++c) {
-          Mma<T>::run(o[mt][c], hi[0], hi[1], hi[2], hi[3], vt[i][c], vt[i + 1][c]);
-          Mma<T>::run(o[mt][c], lo[0], lo[1], lo[2], lo[3], vt[i][c], vt[i + 1][c]);
-        }
-      }
-  }
-
-  // the lanes of a quad share a row
-  float l[MT][2];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      l[mt][h] = l2[mt][h].x + l2[mt][h].y;
-      l[mt][h] += __shfl_xor_sync(0xffffffffu, l[mt][h], 1);
-      l[mt][h] += __shfl_xor_sync(0xffffffffu, l[mt][h], 2);
-    }
-  const int64_t stat0 = (static_cast<int64_t>(b) * a.heads + n * a.group) * a.Tq;
-  if (!split) {
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = r0 + mt * 16 + h * 8 + g;
-        if (r >= rows) continue;
-        const float inv = l[mt][h] == 0.f ? 0.f : 1.f / l[mt][h];
-        uint32_t y[NR];
-#pragma unroll
-        for (int c = 0; c < NR; ++c) y[c] = Mma<T>::pack(o[mt][c][2 * h] * inv, o[mt][c][2 * h + 1] * inv);
-        store_frag<T, DP>(static_cast<T*>(a.out) + row_offset(a, a.os, b, n, r), t, a.d, y);
-        if (a.lse != nullptr && t == 0) a.lse[stat0 + r] = l[mt][h] == 0.f ? INFINITY : m[mt][h] + log2f(l[mt][h]);
-        if (a.out_f32 != nullptr) {
-          float* f = a.out_f32 + row_dense(a, b, n, r) + t * (DP / 4);
-#pragma unroll
-          for (int c = 0; c < NR; ++c)
-            if (t * (DP / 4) + 2 * c < a.d)
-              *reinterpret_cast<float2*>(f + 2 * c) = make_float2(o[mt][c][2 * h] * inv, o[mt][c][2 * h + 1] * inv);
-        }
-      }
-    return;
-  }
-  // Join: the common maximum of the block's warps, then of the cluster's blocks; every warp
-  // rescales its share to it, the shares are summed, and the sums divided on the way out.
-  constexpr int NREG = MT * (NR * 4 + 2), ROWS = 16 * MT;
-  float* s_top = xsm;                        // [8][ROWS]
-  float* s_acc = xsm + kXmWarps * ROWS;      // [4][NREG][32]
-  float acc[NREG];
-  if (t == 0) {
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) s_top[warp * ROWS + mt * 16 + h * 8 + g] = m[mt][h];
-  }
-  __syncthreads();
-  float top[MT][2];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float x = kXmNone;
-#pragma unroll
-      for (int w = 0; w < kXmWarps; ++w) x = fmaxf(x, s_top[w * ROWS + mt * 16 + h * 8 + g]);
-      top[mt][h] = x;
-    }
-  if (cl > 1) {
-    __syncthreads();
-    if (warp == 0 && t == 0) {
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) s_top[mt * 16 + h * 8 + g] = top[mt][h];
-    }
-    cluster_sync_all();
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t at = smem_u32(s_top + mt * 16 + h * 8 + g);
-        for (int i = 0; i < cl; ++i) top[mt][h] = fmaxf(top[mt][h], ld_dsmem(mapa_shared(at, i)));
-      }
-  }
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float f = ex2f(m[mt][h] - top[mt][h]);
-      acc[mt * (NR * 4 + 2) + NR * 4 + h] = l[mt][h] * f;
-#pragma unroll
-      for (int c = 0; c < NR; ++c) {
-        acc[mt * (NR * 4 + 2) + c * 4 + 2 * h] = o[mt][c][2 * h] * f;
-        acc[mt * (NR * 4 + 2) + c * 4 + 2 * h + 1] = o[mt][c][2 * h + 1] * f;
-      }
-    }
-  warp_tree_sum<NREG>(acc, s_acc, warp, lane);
-  __syncthreads();
-  if (warp == 0) {
-#pragma unroll
-    for (int i = 0; i < NREG; ++i) s_acc[i * 32 + lane] = acc[i];
-  }
-  if (cl > 1) cluster_sync_all(); else __syncthreads();
-  const uint32_t base = smem_u32(s_acc) + lane * 4;
-  for (int u = rank * kXmWarps + warp; u < MT * 2 * NR; u += cl * kXmWarps) {
-    const int mt = u / (2 * NR), h = u / NR % 2, c = u % NR;
-    const int ro = mt * 16 + h * 8 + g, r = r0 + ro;
-    const int i0 = mt * (NR * 4 + 2) + c * 4 + 2 * h, il = mt * (NR * 4 + 2) + NR * 4 + h;
-    float x = 0.f, y = 0.f, den = 0.f, mm = kXmNone;
-    for (int i = 0; i < cl; ++i) {
-      const uint32_t from = mapa_shared(base, i);
-      x += ld_dsmem(from + i0 * 128);
-      y += ld_dsmem(from + (i0 + 1) * 128);
-      den += ld_dsmem(from + il * 128);
-      if (cl > 1) mm = fmaxf(mm, ld_dsmem(mapa_shared(smem_u32(s_top + ro), i)));
-    }
-    if (r < rows) {
-      const float inv = den == 0.f ? 0.f : 1.f / den;
-      const int ch = t * (DP / 4) + 2 * c;
-      if (ch < a.d) {
-        *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + row_offset(a, a.os, b, n, r) + ch) =
-            Mma<T>::pack(x * inv, y * inv);
-        if (a.out_f32 != nullptr)
-          *reinterpret_cast<float2*>(a.out_f32 + row_dense(a, b, n, r) + ch) = make_float2(x * inv, y * inv);
-      }
-      if (a.lse != nullptr && c == 0 && t == 0) {
-        if (cl == 1)
-          for (int w = 0; w < kXmWarps; ++w) mm = fmaxf(mm, s_top[w * ROWS + ro]);
-        a.lse[stat0 + r] = den == 0.f ? INFINITY : mm + log2f(den);
-      }
-    }
-  }
-  if (cl > 1) cluster_sync_all();
-}
 
 // ---------------------------------------------------------------------------
 // Forward, few query rows (8 NQ per block) on many keys. The short side is the column
@@ -1129,227 +843,6 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_few(const XAttn a, int) 
   if (cl > 1) cluster_sync_all();
 }
 
-// Two long sides, one kernel per side. A warp owns 16 M entries of one (OWN_ROWS: query rows, x = q, dout;
-// else keys, x = k, v) and walks the other 16 entries at a time (y):
-//   own rows:  dq += ds k              own keys:  dk += ds q,  dv += p dout
-// split = false: the block's 8 warps own 8 tiles and each walks all of the other side. split = true: one tile per
-// block, the other side shared by its warps and the cluster (the join takes about as long as ten steps).
-// The rows' kernel comes first and leaves D for the keys'.
-template <class T, int DP, int M, bool OWN_ROWS>
-__global__ void __launch_bounds__(kXmThreads) xattn_bwd_long(const XAttn a, int split) {
-  constexpr int NR = DP / 8;
-  constexpr float kP = kPScale<T>;
-  extern __shared__ __align__(16) float xsm[];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
-  const int b = blockIdx.z, n = blockIdx.y;
-  const int cl = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
-  const int rows = a.group * a.Tq, keys = xattn_keys(a, b);
-  const int own0 = (split ? static_cast<int>(blockIdx.x) / cl : static_cast<int>(blockIdx.x) * kXmWarps + warp) * 16 * M;
-  if (!split && own0 >= (OWN_ROWS ? rows : a.Tk)) return;
-  const T* qb = static_cast<const T*>(a.q);
-  const T* ob = static_cast<const T*>(a.dout);
-  const T* kb = static_cast<const T*>(a.k) + b * a.ks[0] + n * a.ks[2];
-  const T* vb = static_cast<const T*>(a.v) + b * a.vs[0] + n * a.vs[2];
-  const uint8_t* mask = a.key_mask == nullptr ? nullptr : a.key_mask + static_cast<int64_t>(b) * a.Tk;
-  const int64_t stat0 = (static_cast<int64_t>(b) * a.heads + n * a.group) * a.Tq;
-  auto key_ok = [&](int j) { return j < keys && (mask == nullptr || __ldg(mask + j) != 0); };
-  auto load_row = [&](int r, uint32_t(&x1)[NR], uint32_t(&x2)[NR]) {
-    const int rr = min(r, rows - 1);
-    load_frag<T, DP>(qb + row_offset(a, a.qs, b, n, rr), t, a.d, r < rows, x1);
-    load_frag<T, DP>(ob + row_offset(a, a.os, b, n, rr), t, a.d, r < rows, x2);
-  };
-  auto load_key = [&](int j, uint32_t(&x1)[NR], uint32_t(&x2)[NR]) {
-    const bool ok = key_ok(j);
-    load_frag<T, DP>(kb + j * a.ks[1], t, a.d, ok, x1);
-    load_frag<T, DP>(vb + j * a.vs[1], t, a.d, ok, x2);
-  };
-
-  uint32_t x1[M][2][NR], x2[M][2][NR];
-  float own_s[M][2], own_d[M][2];            // own rows: -lse, -D; own keys: bias
-#pragma unroll
-  for (int mt = 0; mt < M; ++mt)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int i = own0 + mt * 16 + h * 8 + g;
-      if constexpr (OWN_ROWS) {
-        load_row(i, x1[mt][h], x2[mt][h]);
-        own_s[mt][h] = i < rows ? -__ldg(a.lse + stat0 + i) : -INFINITY;
-        own_d[mt][h] = -row_delta<T, DP>(a.out_f32 + row_dense(a, b, n, min(i, rows - 1)), x2[mt][h], t, a.d, i < rows);
-        if ((!split || (rank == 0 && warp == 0)) && t == 0 && i < rows) a.delta[stat0 + i] = -own_d[mt][h];
-      } else {
-        load_key(i, x1[mt][h], x2[mt][h]);
-        own_s[mt][h] = key_ok(i) ? 0.f : -INFINITY;
-      }
-    }
-  if (OWN_ROWS && a.dq == nullptr) return;   // only D was wanted
-
-  float acc1[M][NR][4];                                // dq or dk
-  float acc2[OWN_ROWS ? 1 : M][NR][4];                 // dv
-#pragma unroll
-  for (int mt = 0; mt < M; ++mt)
-#pragma unroll
-    for (int c = 0; c < NR; ++c)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        acc1[mt][c][e] = 0.f;
-        if constexpr (!OWN_ROWS) acc2[mt][c][e] = 0.f;
-      }
-  const int total = OWN_ROWS ? keys : (own0 < keys ? rows : 0);
-  const int steps = (total + 15) / 16, ns = split ? kXmWarps * cl : 1;
-  const int per = (steps + ns - 1) / ns * 16;
-  const int begin = split ? min(total, (rank * kXmWarps + warp) * per) : 0, end = min(total, begin + per);
-  uint32_t y1[2][NR], y2[2][NR];
-  float2 ys[2], yd[2];                       // of entries i0 + 8 nt + 2t, + 1: bias of keys; -lse, -D of rows
-  // rows of one query head follow one another in memory, and so do keys
-  const bool straight = OWN_ROWS || a.group == 1;
-  const T* p1 = OWN_ROWS ? kb + (begin + g) * a.ks[1] : qb + b * a.qs[0] + n * a.qs[2] + (begin + g) * a.qs[1];
-  const T* p2 = OWN_ROWS ? vb + (begin + g) * a.vs[1] : ob + b * a.os[0] + n * a.os[2] + (begin + g) * a.os[1];
-  const int64_t st1 = OWN_ROWS ? a.ks[1] : a.qs[1], st2 = OWN_ROWS ? a.vs[1] : a.os[1];
-  auto load = [&](int i0) {
-    if (straight && i0 + 16 <= end && (!OWN_ROWS || mask == nullptr)) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        load_frag<T, DP>(p1 + h * 8 * st1, t, a.d, true, y1[h]);
-        load_frag<T, DP>(p2 + h * 8 * st2, t, a.d, true, y2[h]);
-        if constexpr (OWN_ROWS) {
-          ys[h] = make_float2(0.f, 0.f);
-        } else {
-          const float *ls = a.lse + stat0 + i0 + h * 8 + 2 * t, *dl = a.delta + stat0 + i0 + h * 8 + 2 * t;
-          ys[h] = make_float2(-__ldg(ls), -__ldg(ls + 1));
-          yd[h] = make_float2(-__ldg(dl), -__ldg(dl + 1));
-        }
-      }
-    } else {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int i = i0 + h * 8 + g;
-        float one, two = 0.f;
-        if constexpr (OWN_ROWS) {
-          load_key(i, y1[h], y2[h]);
-          one = key_ok(i) ? 0.f : -INFINITY;
-        } else {
-          load_row(i, y1[h], y2[h]);
-          one = i < rows ? -__ldg(a.lse + stat0 + i) : -INFINITY;
-          two = i < rows ? -__ldg(a.delta + stat0 + i) : 0.f;
-        }
-        ys[h] = make_float2(__shfl_sync(0xffffffffu, one, 8 * t), __shfl_sync(0xffffffffu, one, 8 * t + 4));
-        yd[h] = make_float2(__shfl_sync(0xffffffffu, two, 8 * t), __shfl_sync(0xffffffffu, two, 8 * t + 4));
-      }
-    }
-    p1 += 16 * st1;
-    p2 += 16 * st2;
-  };
-  load(begin);
-  const float2 c2 = make_float2(a.c, a.c);
-  for (int i0 = begin; i0 < end; i0 += 16) {
-    Turned<T, 2, NR> y1t;
-    uint32_t y2t[OWN_ROWS ? 1 : 2][NR];
-    y1t.make(y1);
-    if constexpr (!OWN_ROWS) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int c = 0; c < NR; ++c) y2t[h][c] = movm(y2[h][c]);
-    }
-    float2 p[M][2][2], ds[M][2][2];          // [own tile][other 8][own g | g + 8] x other 2t, 2t + 1
-#pragma unroll
-    for (int mt = 0; mt < M; ++mt)
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        float s[4] = {0.f, 0.f, 0.f, 0.f}, d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < NR; c += 2) {
-          Mma<T>::run(s, x1[mt][0][c], x1[mt][1][c], x1[mt][0][c + 1], x1[mt][1][c + 1], y1[nt][c], y1[nt][c + 1]);
-          Mma<T>::run(d, x2[mt][0][c], x2[mt][1][c], x2[mt][0][c + 1], x2[mt][1][c + 1], y2[nt][c], y2[nt][c + 1]);
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float2 own = make_float2(own_s[mt][h], own_s[mt][h]);      // -lse of rows, bias of keys
-          float2 f = fma2(make_float2(s[2 * h], s[2 * h + 1]), c2, OWN_ROWS ? ys[nt] : own);
-          f = add2(f, OWN_ROWS ? own : ys[nt]);
-          f.x = ex2f(f.x), f.y = ex2f(f.y);
-          p[mt][nt][h] = f;
-          ds[mt][nt][h] = mul2(f, add2(make_float2(d[2 * h], d[2 * h + 1]),
-                                       OWN_ROWS ? make_float2(own_d[mt][h], own_d[mt][h]) : yd[nt]));
-        }
-      }
-    if (i0 + 16 < end) load(i0 + 16);        // the next step's, under this one's arithmetic
-#pragma unroll
-    for (int mt = 0; mt < M; ++mt) {
-      uint32_t hi[4], lo[4];
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) split2<__nv_bfloat16>(ds[mt][nt][h].x, ds[mt][nt][h].y, hi[2 * nt + h], lo[2 * nt + h]);
-      ds_product<T, 2, NR>(acc1[mt], hi, lo, y1t, 0);
-      if constexpr (!OWN_ROWS) {
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) split2<T>(p[mt][nt][h].x * kP, p[mt][nt][h].y * kP, hi[2 * nt + h], lo[2 * nt + h]);
-#pragma unroll
-        for (int c = 0; c < NR; ++c) {
-          Mma<T>::run(acc2[mt][c], hi[0], hi[1], hi[2], hi[3], y2t[0][c], y2t[1][c]);
-          Mma<T>::run(acc2[mt][c], lo[0], lo[1], lo[2], lo[3], y2t[0][c], y2t[1][c]);
-        }
-      }
-    }
-  }
-
-  if (!split) {
-#pragma unroll
-    for (int mt = 0; mt < M; ++mt)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int i = own0 + mt * 16 + h * 8 + g;
-        if (i >= (OWN_ROWS ? rows : a.Tk)) continue;
-        const int64_t to = OWN_ROWS ? row_dense(a, b, n, i) : ((static_cast<int64_t>(b) * a.Tk + i) * a.kv_heads + n) * a.d;
-        uint32_t y[NR];
-#pragma unroll
-        for (int c = 0; c < NR; ++c) y[c] = Mma<T>::pack(acc1[mt][c][2 * h] * a.scale, acc1[mt][c][2 * h + 1] * a.scale);
-        store_frag<T, DP>(static_cast<T*>(OWN_ROWS ? a.dq : a.dk) + to, t, a.d, y);
-        if constexpr (!OWN_ROWS) {
-#pragma unroll
-          for (int c = 0; c < NR; ++c) y[c] = Mma<T>::pack(acc2[mt][c][2 * h] * (1.f / kP), acc2[mt][c][2 * h + 1] * (1.f / kP));
-          store_frag<T, DP>(static_cast<T*>(a.dv) + to, t, a.d, y);
-        }
-      }
-    return;
-  }
-  // join the owned sums of the warps and the cluster
-  auto join = [&](float* acc, void* to_v, float factor, bool first) {
-    constexpr int NREG = M * NR * 4;
-    if (cl > 1 && !first) cluster_sync_all();          // everybody has read the previous sums
-    warp_tree_sum<NREG>(acc, xsm, warp, lane);
-    __syncthreads();
-    if (warp == 0) {
-#pragma unroll
-      for (int i = 0; i < NREG; ++i) xsm[i * 32 + lane] = acc[i];
-    }
-    if (cl > 1) cluster_sync_all(); else __syncthreads();
-    const uint32_t base = smem_u32(xsm) + lane * 4;
-    for (int u = rank * kXmWarps + warp; u < M * 2 * NR; u += cl * kXmWarps) {
-      const int mt = u / (2 * NR), h = u / NR % 2, c = u % NR;
-      const int i = own0 + mt * 16 + h * 8 + g, i0 = (mt * NR + c) * 4 + 2 * h;
-      float x = 0.f, y = 0.f;
-      for (int k = 0; k < cl; ++k) {
-        const uint32_t from = mapa_shared(base, k);
-        x += ld_dsmem(from + i0 * 128);
-        y += ld_dsmem(from + (i0 + 1) * 128);
-      }
-      const int ch = t * (DP / 4) + 2 * c;
-      if (i < (OWN_ROWS ? rows : a.Tk) && ch < a.d && to_v != nullptr) {
-        const int64_t to = OWN_ROWS ? row_dense(a, b, n, i)
-                                    : ((static_cast<int64_t>(b) * a.Tk + i) * a.kv_heads + n) * a.d;
-        *reinterpret_cast<uint32_t*>(static_cast<T*>(to_v) + to + ch) = Mma<T>::pack(x * factor, y * factor);
-      }
-    }
-  };
-  join(&acc1[0][0][0], OWN_ROWS ? a.dq : a.dk, a.scale, true);
-  if constexpr (!OWN_ROWS) join(&acc2[0][0][0], a.dv, 1.f / kP, false);
-  if (cl > 1) cluster_sync_all();
-}
-
 // ---------------------------------------------------------------------------
 // Launch rules
 // ---------------------------------------------------------------------------
@@ -1363,21 +856,6 @@ static int xattn_cluster(int64_t blocks, int other, int step, int most = 8) {
   while (c < most && (c < 8 || (blocks * 16 <= 148 && other >= 32 * kXmWarps * step)) && blocks * c < 148 && other > c * kXmWarps * step) c *= 2;
   return c;
 }
-template <class T, int DP, int MT>
-static int xattn_fwd_long_launch(const XAttn& a, cudaStream_t stream) {
-  const int rows = a.group * a.Tq, tiles = (rows + 16 * MT - 1) / (16 * MT);
-  const int64_t pairs = static_cast<int64_t>(a.B) * a.kv_heads;
-  constexpr int CK = DP <= 32 ? 32 : 16;
-  const int64_t whole = pairs * ((tiles + kXmWarps - 1) / kXmWarps);
-  if (a.Tk <= 2 * CK || (tiles >= kXmWarps && whole >= 148))
-    return launch_cluster(xattn_fwd_long<T, DP, MT>, dim3((tiles + kXmWarps - 1) / kXmWarps, a.kv_heads, a.B),
-                          kXmThreads, 0, 1, stream, a, 0);
-  const int cl = xattn_cluster(pairs * tiles, a.Tk, CK);
-  const size_t smem = (kXmWarps * 16 * MT + 4 * MT * (DP / 2 + 2) * 32) * sizeof(float);
-  return launch_cluster(xattn_fwd_long<T, DP, MT>, dim3(tiles * cl, a.kv_heads, a.B), kXmThreads, smem, cl, stream, a,
-                        1);
-}
-
 template <class T, int DP, int NQ, int HP = 1>
 static int xattn_few_rows_launch(const XAttn& a, cudaStream_t stream) {
   const int rows = a.group * a.Tq, tiles = (rows + 8 * NQ - 1) / (8 * NQ);
@@ -1436,21 +914,6 @@ static int xattn_bwd_few_pick(const XAttn& a, int few, cudaStream_t stream) {
   return xattn_bwd_few_launch<T, DP, 1, FEW_ROWS>(a, stream);
 }
 
-template <class T, int DP, int M, bool OWN_ROWS>
-static int xattn_bwd_long_launch(const XAttn& a, cudaStream_t stream) {
-  const int rows = a.group * a.Tq, own = OWN_ROWS ? rows : a.Tk, other = OWN_ROWS ? a.Tk : rows;
-  const int tiles = (own + 16 * M - 1) / (16 * M);
-  const int64_t pairs = static_cast<int64_t>(a.B) * a.kv_heads;
-  const int groups = (tiles + kXmWarps - 1) / kXmWarps;
-  if (tiles >= kXmWarps && pairs * groups >= 148)
-    return launch_cluster(xattn_bwd_long<T, DP, M, OWN_ROWS>, dim3(groups, a.kv_heads, a.B), kXmThreads, 0, 1, stream, a, 0);
-  const int cl = xattn_cluster(pairs * tiles, other, 16);
-  constexpr size_t smem = 4 * M * (DP / 2) * 32 * sizeof(float);
-  static_assert(smem <= 48 << 10, "no opt-in needed");
-  return launch_cluster(xattn_bwd_long<T, DP, M, OWN_ROWS>, dim3(tiles * cl, a.kv_heads, a.B), kXmThreads, smem, cl,
-                        stream, a, 1);
-}
-
 template <class T, int DP>
 static int xattn_mma_dp(const XAttn& a, bool backward, cudaStream_t stream) {
   const int rows = a.group * a.Tq;
@@ -1478,19 +941,12 @@ static int xattn_mma_dp(const XAttn& a, bool backward, cudaStream_t stream) {
     if constexpr (DP <= 64) {
       if (rows <= 24 || (rows > 32 && rows <= 48)) return xattn_few_rows_launch<T, DP, 3>(a, stream);
       if (rows <= 64) return xattn_few_rows_launch<T, DP, 4>(a, stream);
-      if (a.d >= kTcMinDim && a.d <= kTcMaxDim && a.heads <= 65535) return xattn_tc_fwd(a, kIsHalf<T> ? 0 : 1, stream);
-      return xattn_fwd_long_launch<T, DP, 2>(a, stream);
-    } else {
-      return xattn_fwd_long_launch<T, DP, 1>(a, stream);
     }
+    return xattn_tc(a, kIsHalf<T> ? 0 : 1, false, stream);
   }
   if (a.Tk <= 8 * kXmFewTiles<DP>) return xattn_bwd_few_pick<T, DP, false>(a, a.Tk, stream);
   if (rows <= 8 * kXmFewTiles<DP>) return xattn_bwd_few_pick<T, DP, true>(a, rows, stream);
-  if (!kIsHalf<T> && rows > 64 && a.Tk > 64 && a.d >= kTcMinDim && a.d <= kTcMaxDim && a.heads <= 65535)
-    return xattn_tc_bwd(a, stream);
-  const int st = xattn_bwd_long_launch<T, DP, DP <= 64 ? 2 : 1, true>(a, stream);
-  if (st != SSAM_OK || a.dk == nullptr) return st;
-  return xattn_bwd_long_launch<T, DP, DP <= 32 ? 2 : 1, false>(a, stream);
+  return xattn_tc(a, kIsHalf<T> ? 0 : 1, true, stream);
 }
 
 template <class T>

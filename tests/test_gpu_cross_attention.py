@@ -276,3 +276,36 @@ def test_offsets_past_32_bits(cuda_device):
     vfar = buf.as_strided((1, 40, 1, 16), (step, step, 16, 1), 32)
     vfar.copy_(v)
     check(run(q, far, vfar), reference(q, k, v), "fp16")
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("shape", [(2, 150, 200, 2, 1, 128), (1, 130, 70, 6, 2, 96), (3, 50, 90, 6, 2, 72), (2, 1, 300, 140, 1, 64),
+                                   (2, 257, 1030, 2, 2, 128), (1, 400, 37, 3, 3, 16), (1, 20, 260, 2, 2, 128),
+                                   (1, 3, 700, 90, 3, 32)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_long_sides(cuda_device, shape, dtype):
+    """Tiles of 128 query rows that cross from one head of a group to the next, two panels of channels."""
+    q, k, v, do = make(cuda_device, *shape, dtype, seed=7)
+    B, Tk = shape[0], shape[2]
+    check(run(q, k, v, do), reference(q, k, v, do), dtype)
+    mask = torch.rand(B, Tk, generator=torch.Generator().manual_seed(8)).lt(0.7).to(cuda_device)
+    mask[0, : Tk // 2] = False
+    lens = torch.full((B,), Tk - 3, dtype=torch.int32, device=cuda_device)
+    gone = ~there(B, Tk, lens, mask, cuda_device)
+    k[gone] = math.nan
+    v[gone] = math.inf
+    got = run(q, k, v, do, key_lens=lens, key_mask=mask)
+    check(got, reference(q, k, v, do, lens=lens, mask=mask), dtype)
+    assert not got[2][gone].any() and not got[3][gone].any()
+
+
+@pytest.mark.parametrize("D", [16, 64, 128])
+@pytest.mark.parametrize("low", [-20, -6])
+def test_half_gradients_of_any_size(cuda_device, D, low):
+    """fp16: values and incoming gradients that grow by 2^10 each along the walk, so that the power of two that
+    dS enters its products with has to follow; small ones (from 2^-26) and large ones (to 2^12)."""
+    q, k, v, do = make(cuda_device, 2, 300, 400, 2, 2, D, "fp16", seed=9)
+    rise = lambda n: torch.exp2(torch.arange(n, device=cuda_device) * 10 // n).half()  # noqa: E731
+    v = v * rise(400)[None, :, None, None] * 2.0 ** -6
+    do = do * rise(300)[None, :, None, None] * 2.0 ** low
+    check(run(q, k, v, do), reference(q, k, v, do), "fp16")
