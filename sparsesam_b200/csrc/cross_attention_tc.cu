@@ -159,6 +159,13 @@ struct TcBlock {
     if (threadIdx.x < 32) tmem_dealloc(tmem, cols);
   }
 };
+// Every thread's copies (into shared memory) and TMEM stores are there for the tensor core.
+__device__ __forceinline__ bool tc_landed(bool ok) {
+  cp_async_wait_all();
+  fence_proxy_async_smem();
+  tc_fence_before();
+  return __syncthreads_and(ok);
+}
 constexpr float kTcNone = -1e30f, kTcSlack = 8.f;
 
 // Folded row r of key head n is token r % Tq of query head n group + r / Tq.
@@ -200,7 +207,6 @@ __global__ void __launch_bounds__(kTcThreads, 4 / NP) xattn_tc_fwd_kernel(const 
                                             [&](int i) { return key_ok(k0 + i) ? vb + (k0 + i) * a.vs[1] : nullptr; });
       if (tid < kTcOther) s_bias[buf][tid] = key_ok(k0 + tid) ? 0.f : -INFINITY;
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
   };
   tc_fetch<T, NP, kTcOwn, kTcThreads>(x1, a.d, qb, [&](int i) -> const T* {
     if (own0 + i >= rows) return nullptr;
@@ -212,24 +218,19 @@ __global__ void __launch_bounds__(kTcThreads, 4 / NP) xattn_tc_fwd_kernel(const 
   float ref = kTcNone;
   float2 l2 = make_float2(0.f, 0.f);
   const float2 c2 = make_float2(a.c, a.c);
-  bool ok = true;
+  bool ok = tc_landed(true);
   int it = 0;
   for (int j = j_begin; j < j_end; ++j, ++it) {
     const int buf = it & 1;
     const uint32_t y = ring + buf * kStage;
-    if (it > 0) ok = mbar_wait(&bars[1], (it - 1) & 1);      // the sums of the block before: its buffer and P are free
-    request(j + 1, buf ^ 1);
-    asm volatile("cp.async.wait_group 1;" ::: "memory");
-    fence_proxy_async_smem();
-    tc_fence_before();
-    ok = __syncthreads_and(ok);
-    if (!ok) break;
-    if (tid == 0) {
+    if (it > 0) ok = mbar_wait(&bars[1], (it - 1) & 1);      // the sums of the step before: its buffer and P are free
+    if (tid == 0 && ok) {
       tc_fence_after();
       tc_scores<T, NP>(B.tmem + tS, x1, y);
       umma_commit(&bars[0]);
     }
-    ok = __all_sync(0xffffffffu, mbar_wait(&bars[0], it & 1));
+    request(j + 1, buf ^ 1);
+    ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars[0], it & 1));
     tc_fence_after();
     if (ok) {
       float2 s[32];
@@ -276,8 +277,7 @@ __global__ void __launch_bounds__(kTcThreads, 4 / NP) xattn_tc_fwd_kernel(const 
       }
       tmem_st_wait();
     }
-    tc_fence_before();
-    ok = __syncthreads_and(ok);
+    ok = tc_landed(ok);
     if (!ok) break;
     if (tid == 0) {
       tc_fence_after();
@@ -416,7 +416,6 @@ __global__ void __launch_bounds__(kTcBwdThreads, 2 / NP) xattn_tc_bwd_kernel(con
           s_b[buf][tid - kTcOther] = r < rows ? -__ldg(a.delta + stat0 + r) : 0.f;
       }
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
   };
   float own_s, own_d = 0.f;                  // -lse and -D of the thread's query; bias of its key
   const int mine = own0 + lane_id;
@@ -448,25 +447,20 @@ __global__ void __launch_bounds__(kTcBwdThreads, 2 / NP) xattn_tc_bwd_kernel(con
 
   const float2 c2 = make_float2(a.c, a.c), os2 = make_float2(own_s, own_s), od2 = make_float2(own_d, own_d);
   int up = 253;                              // exponent field of the power of two on dS: 2^126 until one is seen
-  bool ok = true;
+  bool ok = tc_landed(true);
   int it = 0;
   for (int j = j_begin; j < j_end; ++j, ++it) {
     const int buf = it & 1;
     const uint32_t y = ring + buf * kStage, y2 = y + kHalfStage;
     if (it > 0) ok = mbar_wait(&bars[1], (it - 1) & 1);
-    request(j + 1, buf ^ 1);
-    asm volatile("cp.async.wait_group 1;" ::: "memory");
-    fence_proxy_async_smem();
-    tc_fence_before();
-    ok = __syncthreads_and(ok);
-    if (!ok) break;
-    if (tid == 0) {
+    if (tid == 0 && ok) {
       tc_fence_after();
       tc_scores<T, NP>(B.tmem + tS, x1, y);
       tc_scores<T, NP>(B.tmem + tD, x2, y2);
       umma_commit(&bars[0]);
     }
-    ok = __all_sync(0xffffffffu, mbar_wait(&bars[0], it & 1));
+    request(j + 1, buf ^ 1);
+    ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars[0], it & 1));
     tc_fence_after();
     // P and dS of columns 16 q .. 16 q + 15
     auto values = [&](int q, float2 (&p)[8], float2 (&ds)[8]) {
@@ -540,8 +534,7 @@ __global__ void __launch_bounds__(kTcBwdThreads, 2 / NP) xattn_tc_bwd_kernel(con
       }
       tmem_st_wait();
     }
-    tc_fence_before();
-    ok = __syncthreads_and(ok);
+    ok = tc_landed(ok);
     if (!ok) break;
     if (tid == 0) {
       tc_fence_after();
