@@ -11,6 +11,7 @@
 
 #include <atomic>
 #include <cmath>
+#include <cstdint>
 
 #include "../../include/sparsesam.h"
 
@@ -57,6 +58,12 @@ void check_devices(const Tensor& first, std::initializer_list<const Tensor*> oth
     if (t->defined()) cuda = cuda && t->is_cuda(), same = same && t->device() == first.device();
   if (!cuda) refuse("sparsesam_b200 ops run on CUDA tensors only (no CPU fallback)");
   if (!same) refuse("all tensors of a call must be on one device");
+}
+// the C entry points count tokens, heads and channels in 32 bits
+void check_sizes(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    for (const int64_t n : t->sizes())
+      if (n > INT32_MAX) refuse("a dimension of " + std::to_string(n) + " entries is not supported (at most 2^31 - 1)");
 }
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
@@ -112,7 +119,7 @@ struct LayerNormGelu : torch::autograd::Function<LayerNormGelu> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &b = saved[2];
     const int C = static_cast<int>(x.size(-1));
-    const int64_t rows = x.numel() / C;
+    const int64_t rows = C == 0 ? 0 : x.numel() / C;
     variable_list out(5);
     {
       at::AutoGradMode off(false);
@@ -141,6 +148,7 @@ Tensor layernorm_gelu_half(const Tensor& x, const Tensor& w, const Tensor& b, do
     refuse("x, w and b must share one half-precision dtype");
   }
   if (!x.is_contiguous() || !w.is_contiguous() || !b.is_contiguous()) refuse("x, w and b must be contiguous");
+  check_sizes({&w});
   if (x.dim() < 1 || w.numel() != x.size(-1) || b.numel() != x.size(-1)) refuse("w and b must have one entry per channel");
   check_devices(x, {&w, &b});
   if (wants_grad({&x, &w, &b})) return LayerNormGelu::apply(x, w, b, eps, static_cast<int64_t>(gelu));
@@ -217,6 +225,7 @@ Tensor groupnorm_act(const Tensor& x, int64_t groups, const Tensor& w, const Ten
   const auto dt = x.scalar_type();
   if (dtype_code(dt) < 0 || w.scalar_type() != dt || b.scalar_type() != dt)
     throw py::type_error("x, w and b must share one dtype of fp16, bf16, fp32");
+  check_sizes({&x});
   if (x.dim() < 2 || w.dim() != 1 || b.dim() != 1 || w.size(0) != x.size(-1) || b.size(0) != x.size(-1))
     refuse("x must be (N, ..., C), w and b (C,)");
   if (!x.is_contiguous() || !w.is_contiguous() || !b.is_contiguous())
@@ -332,6 +341,7 @@ Tensor cross_attn(const Tensor& q, const Tensor& k, const Tensor& v, std::option
   const Tensor lens = lens_.value_or(Tensor()), mask = mask_.value_or(Tensor());
   if (q.dim() != 4 || k.dim() != 4 || v.sizes() != k.sizes() || k.size(0) != q.size(0) || k.size(3) != q.size(3))
     refuse("q (B, Tq, H, D), k and v (B, Tk, Hk, D) expected, got " + shape(q) + ", " + shape(k) + ", " + shape(v));
+  check_sizes({&q, &k});
   const auto dt = q.scalar_type();
   if (dtype_code(dt) < 0 || k.scalar_type() != dt || v.scalar_type() != dt)
     throw py::type_error("q, k and v must share one dtype of fp16, bf16, fp32");

@@ -271,7 +271,7 @@ class DecoderAttention(nn.Module):
         there (a padded batch of prompts); a query without keys gives out_proj's bias."""
         qh, kh, vh = self._split(self.q_proj(q)), self._split(self.k_proj(k)), self._split(self.v_proj(v))
         h, c = qh.shape[2:]
-        if qh.is_cuda and ops.cross_attn_supported(h, h, c, qh.dtype):
+        if qh.is_cuda and qh.shape[0] <= ops.CROSS_ATTN_MAX_BATCH and ops.cross_attn_supported(h, h, c, qh.dtype):
             o = ops.cross_attn(qh, kh, vh, key_lens=key_lens, key_mask=key_mask)
         else:
             mask = key_mask

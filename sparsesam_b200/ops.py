@@ -513,6 +513,7 @@ def groupnorm_act(x: torch.Tensor, groups: int, w: torch.Tensor, b: torch.Tensor
 
 
 CROSS_ATTN_MAX_DIM = 128
+CROSS_ATTN_MAX_BATCH = 65535
 
 
 def cross_attn_supported(heads: int, kv_heads: int, d: int, dtype: torch.dtype) -> bool:
@@ -524,7 +525,8 @@ def cross_attn_supported(heads: int, kv_heads: int, d: int, dtype: torch.dtype) 
 def cross_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float | None = None,
                key_lens: torch.Tensor | None = None, key_mask: torch.Tensor | None = None) -> torch.Tensor:
     """softmax(scale q k^T) v of queries q (B, Tq, H, D) over another token set's k, v
-    (B, Tk, Hk, D); query head h reads key head h // (H // Hk). Returns (B, Tq, H, D).
+    (B, Tk, Hk, D), B up to CROSS_ATTN_MAX_BATCH; query head h reads key head h // (H // Hk).
+    Returns (B, Tq, H, D).
 
     fp16, bf16 or fp32 (one dtype), D a multiple of 8 up to 128; any strides with contiguous
     D and 16-byte aligned rows (a stride of 0 broadcasts). scale defaults to 1 / sqrt(D).

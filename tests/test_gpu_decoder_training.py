@@ -167,3 +167,15 @@ def test_attention_of_many_shapes_side_by_side(cuda_device):
             outs.append(ops.cross_attn(q, k, k))
     torch.cuda.synchronize()
     assert all(torch.equal(o, c[2]) for o, c in zip(outs, cases * 4))
+
+
+def test_attention_of_many_prompts(cuda_device):
+    """More prompts than one launch takes: the same rows as in two calls."""
+    torch.manual_seed(0)
+    attn = hq.DecoderAttention(16, 2).to(cuda_device)
+    x = torch.randn(65537, 2, 16, device=cuda_device)
+    with torch.no_grad():
+        whole = attn(x, x, x)
+        parts = torch.cat([attn(t, t, t) for t in x.split(40000)])
+    # fp32 of two orders of summation: unit-size logits and values, 4 eps of them
+    assert (whole - parts).abs().max() <= 4 * torch.finfo(torch.float32).eps * parts.abs().max() * 2

@@ -207,3 +207,12 @@ def test_layernorm_gradient_reaches_the_decoder_norms(cuda_device):
         mod(x).float().square().sum().backward()
         for t in (x, mod.weight, mod.bias):
             assert t.grad is not None and t.grad.abs().sum() > 0
+
+
+def test_layernorm_without_channels(cuda_device):
+    x = torch.zeros(3, 0, dtype=torch.float16, device=cuda_device, requires_grad=True)
+    w = torch.zeros(0, dtype=torch.float16, device=cuda_device)
+    out = ops.layernorm_gelu_half(x, w, w, 1e-6, False)
+    assert out.shape == (3, 0)
+    out.sum().backward()
+    assert x.grad.shape == (3, 0)

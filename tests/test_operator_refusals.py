@@ -120,3 +120,15 @@ def test_groupnorm_wrapper(kwargs, error):
     with pytest.raises(error) as e:
         ops.groupnorm_act(**args)
     assert "CUDA" not in str(e.value)
+
+
+def test_sizes_past_32_bits():
+    """More entries than the C entry points count: an error, not a size that has wrapped around."""
+    q = torch.zeros(1, 1, 1, 8, dtype=torch.float16)
+    for n in (2**31, 2**32 + 1):
+        with pytest.raises(ValueError, match="entries"):
+            ops.cross_attn(q.expand(1, n, 1, 8), q, q)
+        with pytest.raises(ValueError, match="entries"):
+            ops.cross_attn(q, q.expand(1, n, 1, 8), q.expand(1, n, 1, 8))
+        with pytest.raises(ValueError, match="entries"):
+            ops.groupnorm_act(q.expand(n, 1, 1, 8), 1, q[0, 0, 0], q[0, 0, 0])
