@@ -279,6 +279,17 @@ __device__ __forceinline__ float ld_dsmem(uint32_t cluster_addr) {
   return v;
 }
 
+// First call of every thread of a kernel that launch_following (host_util.h) starts: the kernel's blocks may be set up
+// while the kernel before it in the stream still runs, and wait here until that one is done and its writes are there.
+// Before it nothing is read or written and no TMEM taken. Returns 0, to be added to the pointers of the arguments:
+// read-only loads, which a compiler may move across the wait, then depend on it. early: the blocks of the kernel behind
+// may come once all of this one have been here, else when they are done.
+__device__ __forceinline__ int64_t follow_previous(bool early = true) {
+  int64_t zero;
+  asm volatile("griddepcontrol.wait;\n\tmov.u64 %0, 0;" : "=l"(zero)::"memory");
+  if (early) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  return zero;
+}
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }

@@ -185,7 +185,8 @@ __device__ __forceinline__ void walk_keys(const XAttn& a, const XPlace& x, float
 }
 
 template <int DT, int TPR>
-__global__ void __launch_bounds__(kXThreads) xattn_fwd_scalar(const XAttn a, int RB) {
+__global__ void __launch_bounds__(kXThreads) xattn_fwd_scalar(const XAttn args, int RB) {
+  const XAttn a = follow(args, false);
   constexpr int DP = DT * TPR, LD = DP + 4, U = 4;
   extern __shared__ __align__(16) float xsm[];
   __shared__ float bias[2][kXTile<DP>];
@@ -313,7 +314,8 @@ __global__ void __launch_bounds__(kXThreads) xattn_fwd_scalar(const XAttn a, int
 
 // dQ: the forward's loop with p from the saved statistics. Also writes D for the dK / dV kernel.
 template <int DT, int TPR>
-__global__ void __launch_bounds__(kXThreads) xattn_dq_scalar(const XAttn a, int RB) {
+__global__ void __launch_bounds__(kXThreads) xattn_dq_scalar(const XAttn args, int RB) {
+  const XAttn a = follow(args, false);
   constexpr int DP = DT * TPR, LD = DP + 4;
   extern __shared__ __align__(16) float xsm[];
   __shared__ float bias[2][kXTile<DP>];
@@ -372,7 +374,8 @@ __global__ void __launch_bounds__(kXThreads) xattn_dq_scalar(const XAttn a, int 
 
 // dK, dV: a thread owns (part of) one key; the block's slices walk the query rows.
 template <int DT, int TPR>
-__global__ void __launch_bounds__(kXThreads) xattn_dkv_scalar(const XAttn a, int RB) {
+__global__ void __launch_bounds__(kXThreads) xattn_dkv_scalar(const XAttn args, int RB) {
+  const XAttn a = follow(args, false);
   constexpr int DP = DT * TPR, LD = DP + 4, XT = kXTile<DP>;
   extern __shared__ __align__(16) float xsm[];
   __shared__ float s_lse[2][XT], s_delta[2][XT];
@@ -473,14 +476,14 @@ static int xattn_scalar(const XAttn& a, bool backward, cudaStream_t stream) {
   if (!backward) {
     constexpr size_t merge = (kXThreads + kXThreads / TPR * (DP + 1)) * sizeof(float);
     static_assert(merge <= 48 << 10 && stages <= 48 << 10, "no opt-in needed");
-    return launch_cluster(xattn_fwd_scalar<DT, TPR>, by_rows, kXThreads, stages > merge ? stages : merge, cl, stream, a, rb);
+    return launch_following(xattn_fwd_scalar<DT, TPR>, by_rows, kXThreads, stages > merge ? stages : merge, cl, stream, a, rb);
   }
   constexpr size_t merge = kXThreads / TPR * 2 * DP * sizeof(float);
   static_assert(merge <= 48 << 10, "no opt-in needed");
-  const int st = launch_cluster(xattn_dq_scalar<DT, TPR>, by_rows, kXThreads, stages > merge ? stages : merge, cl, stream, a, rb);
+  const int st = launch_following(xattn_dq_scalar<DT, TPR>, by_rows, kXThreads, stages > merge ? stages : merge, cl, stream, a, rb);
   if (st != SSAM_OK || a.dk == nullptr) return st;
   xattn_plan(a.Tk, rows, pairs, TPR, XT, &rb, &cl);
-  return launch_cluster(xattn_dkv_scalar<DT, TPR>, dim3((a.Tk + rb - 1) / rb * cl, a.kv_heads, a.B), kXThreads,
+  return launch_following(xattn_dkv_scalar<DT, TPR>, dim3((a.Tk + rb - 1) / rb * cl, a.kv_heads, a.B), kXThreads,
                         stages > merge ? stages : merge, cl, stream, a, rb);
 }
 

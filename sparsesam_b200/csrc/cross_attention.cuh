@@ -53,21 +53,15 @@ __device__ __forceinline__ int xattn_keys(const XAttn& a, int b) {
   return a.key_lens == nullptr ? a.Tk : min(max(__ldg(a.key_lens + b), 0), a.Tk);
 }
 
-template <class K>
-static int launch_cluster(K kernel, dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream,
-                          const XAttn& a, int arg) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = cluster;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return status_from_cuda(cudaLaunchKernelEx(&cfg, kernel, a, arg));
+// early where the kernels behind are small. Behind a kernel whose blocks take the whole register file (the backward pass
+// with a short side), or before one, blocks that come early are packed on the first free SMs: 23 -> 27 us for a pass
+// of 11 queries on 4096 keys, 18 -> 21 for 4096 on 8, fp32 49 -> 53.
+__device__ __forceinline__ XAttn follow(const XAttn& args, bool early) {
+  XAttn a = args;
+  const int64_t zero = follow_previous(early);
+  for (const void** p : {&a.q, &a.k, &a.v, &a.dout}) *p = static_cast<const char*>(*p) + zero;
+  a.key_lens += zero, a.key_mask += zero, a.out_f32 += zero, a.lse += zero, a.delta += zero;
+  return a;
 }
 
 // The tensor-core path (cross_attention_mma.cuh), one translation unit per type.

@@ -147,7 +147,8 @@ constexpr float kXmSlack = 8.f;
 // are the first head's. Twice the tensor instructions, of which there are plenty.
 // ---------------------------------------------------------------------------
 template <class T, int DP, int NQ, int HP>
-__global__ void __launch_bounds__(kXmThreads) xattn_fwd_few_rows(const XAttn a, int) {
+__global__ void __launch_bounds__(kXmThreads) xattn_fwd_few_rows(const XAttn args, int) {
+  const XAttn a = follow(args, args.lse == nullptr);
   constexpr int NR = DP / 8, NU = NR / 2;    // 8- and 16-channel blocks
   constexpr int KM = DP <= 32 && HP * NQ <= 4 ? 2 : 1;   // 16-key tiles per step
   extern __shared__ __align__(16) float xsm[];
@@ -375,7 +376,8 @@ __global__ void __launch_bounds__(kXmThreads) xattn_fwd_few_rows(const XAttn a, 
 // neighbouring heads, so a block touches whole rows. HP = 2 as above.
 // ---------------------------------------------------------------------------
 template <class T, int DP, int NK, int HP>
-__global__ void __launch_bounds__(kXmThreads) xattn_fwd_few_keys(const XAttn a, int chunks) {
+__global__ void __launch_bounds__(kXmThreads) xattn_fwd_few_keys(const XAttn args, int chunks) {
+  const XAttn a = follow(args, false);
   constexpr int NR = DP / 8;
   const int lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   const int units = a.heads / HP;
@@ -585,7 +587,8 @@ __device__ __forceinline__ float row_delta(const float* o32, const uint32_t (&x)
 //   few = query rows (FEW_ROWS): x = k, v;  y = q, dout.  dk = ds y1, dv = p y2 leave;  dq^T += k^T ds stays
 //   few = keys:                  x = q, dout;  y = k, v.  dq = ds y1 leaves;  dk^T += q^T ds, dv^T += dout^T p stay
 template <class T, int DP, int NF, bool FEW_ROWS>
-__global__ void __launch_bounds__(kXmThreads) xattn_bwd_few(const XAttn a, int) {
+__global__ void __launch_bounds__(kXmThreads) xattn_bwd_few(const XAttn args, int) {
+  const XAttn a = follow(args, false);
   constexpr int NR = DP / 8, NU = NR / 2;
   constexpr float kP = kPScale<T>;
   using B16 = Mma<__nv_bfloat16>;
@@ -866,7 +869,7 @@ static int xattn_few_rows_launch(const XAttn& a, cudaStream_t stream) {
   if (st != SSAM_OK) return st;
   const int cl = xattn_cluster(static_cast<int64_t>(a.B) * (a.kv_heads / HP) * tiles, a.Tk, DP <= 32 ? 32 : 16,
                                limit.get(xattn_fwd_few_rows<T, DP, NQ, HP>, kXmThreads, smem));
-  return launch_cluster(xattn_fwd_few_rows<T, DP, NQ, HP>, dim3(tiles * cl, a.kv_heads / HP, a.B), kXmThreads, smem, cl,
+  return launch_following(xattn_fwd_few_rows<T, DP, NQ, HP>, dim3(tiles * cl, a.kv_heads / HP, a.B), kXmThreads, smem, cl,
                         stream, a, 0);
 }
 
@@ -878,7 +881,7 @@ static int xattn_few_keys_launch(const XAttn& a, cudaStream_t stream) {
   const int64_t want = (148 * 64 + pairs - 1) / pairs;
   const int chunks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, (tiles + 3) / 4)));
   const int64_t blocks = (pairs * chunks + kXmWarps - 1) / kXmWarps;
-  return launch_cluster(xattn_fwd_few_keys<T, DP, NK, HP>, dim3(static_cast<unsigned>(blocks)), kXmThreads, 0, 1, stream,
+  return launch_following(xattn_fwd_few_keys<T, DP, NK, HP>, dim3(static_cast<unsigned>(blocks)), kXmThreads, 0, 1, stream,
                         a, chunks);
 }
 
@@ -896,7 +899,7 @@ static int xattn_bwd_few_launch(const XAttn& a, cudaStream_t stream) {
   if (st != SSAM_OK) return st;
   const int cl = xattn_cluster(static_cast<int64_t>(a.B) * a.kv_heads, FEW_ROWS ? a.Tk : a.group * a.Tq, 16,
                                limit.get(xattn_bwd_few<T, DP, NF, FEW_ROWS>, kXmThreads, smem));
-  return launch_cluster(xattn_bwd_few<T, DP, NF, FEW_ROWS>, dim3(cl, a.kv_heads, a.B), kXmThreads, smem, cl, stream, a,
+  return launch_following(xattn_bwd_few<T, DP, NF, FEW_ROWS>, dim3(cl, a.kv_heads, a.B), kXmThreads, smem, cl, stream, a,
                         0);
 }
 // the smallest instance that holds `few` entries

@@ -178,7 +178,8 @@ __device__ __forceinline__ TcRow tc_row(const XAttn& a, int n, int r) {
 }
 
 template <class T, int NP>
-__global__ void __launch_bounds__(kTcThreads, 4 / NP) xattn_tc_fwd_kernel(const XAttn a) {
+__global__ void __launch_bounds__(kTcThreads, 4 / NP) xattn_tc_fwd_kernel(const XAttn args) {
+  const XAttn a = follow(args, true);
   constexpr int kTile = NP * kTcTile, kHalfStage = NP * kTcHalf, kStage = 2 * kHalfStage, kCols = 128 * NP;
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) uint64_t bars[2];
@@ -366,7 +367,8 @@ constexpr int kTcBwdThreads = 256;
 constexpr float kTcPScale = 4096.f;
 
 template <class T, int NP, bool OWN_ROWS>
-__global__ void __launch_bounds__(kTcBwdThreads, 2 / NP) xattn_tc_bwd_kernel(const XAttn a) {
+__global__ void __launch_bounds__(kTcBwdThreads, 2 / NP) xattn_tc_bwd_kernel(const XAttn args) {
+  const XAttn a = follow(args, true);
   constexpr bool kScaled = std::is_same<T, __half>::value;
   constexpr int kTile = NP * kTcTile, kHalfStage = NP * kTcHalf, kStage = 2 * kHalfStage;
   constexpr int kCols = NP == 1 || OWN_ROWS ? 256 : 512;
@@ -622,18 +624,7 @@ static int xattn_tc_launch(K kernel, PerDeviceOnce& once, const XAttn& a, int ow
   if (st != SSAM_OK) return st;
   const int tiles = (own + kTcOwn - 1) / kTcOwn;
   const int cl = xattn_tc_cluster(static_cast<int64_t>(a.B) * a.kv_heads * tiles, per_sm, (other + kTcOther - 1) / kTcOther);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(tiles * cl, a.kv_heads, a.B);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = cl;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return status_from_cuda(cudaLaunchKernelEx(&cfg, kernel, a));
+  return launch_following(kernel, dim3(tiles * cl, a.kv_heads, a.B), dim3(threads), smem, cl, stream, a);
 }
 
 template <class T, int NP>

@@ -103,6 +103,27 @@ int make_tmap_2d_bf16(CUtensorMap* map, const void* base, uint64_t rows, uint64_
 
 int status_from_cuda(cudaError_t e);
 
+// Launches a kernel that begins with follow_previous (common.cuh), in clusters of `cluster` blocks along x. Its set-up
+// runs under the end of the kernel before it: calls one behind the other 6.4 -> 5.4 us (attention of one image), 9.5 ->
+// 7.3 (one long query), 8.2 -> 7.1 (GroupNorm of a map), the 13 kernels of a streamed GroupNorm's pass 264 -> 256.
+template <class... P, class... A>
+int launch_following(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t stream, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = cluster;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  return status_from_cuda(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
+}
+
 // Entry points implemented in the per-kernel translation units.
 int conv3x3_nhwc(const void* in, int B, int H, int W, int Cin, const void* w, int Cout, const float* bias, void* out,
                  cudaStream_t stream);

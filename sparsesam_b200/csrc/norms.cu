@@ -362,6 +362,14 @@ struct GnArgs {
   float* sums;         // [N][2][C] totals of g and g xh
 };
 
+__device__ __forceinline__ GnArgs follow(const GnArgs& args) {
+  GnArgs a = args;
+  const int64_t zero = follow_previous();
+  for (const void** p : {&a.x, &a.dout, &a.w, &a.b}) *p = static_cast<const char*>(*p) + zero;
+  a.mean += zero, a.rstd += zero, a.part += zero, a.sums += zero;
+  return a;
+}
+
 using GnRing1 = Ring<8, 1, kGnThreads>;    // forward: 32 KB a block, four blocks per SM
 using GnRing2 = Ring<6, 2, kGnThreads>;    // backward (x, dout): 48 KB a block, two blocks per SM
 
@@ -400,7 +408,8 @@ struct Apply {
 };
 
 template <class T, int ACT>
-__global__ void __launch_bounds__(kGnThreads) groupnorm_resident_kernel(const GnArgs a) {
+__global__ void __launch_bounds__(kGnThreads) groupnorm_resident_kernel(const GnArgs args) {
+  const GnArgs a = follow(args);
   constexpr int V = Vec<T>::V;
   extern __shared__ __align__(16) float gsm[];
   const int cols = a.slab / V, lanes = kGnThreads / cols, G = a.slab / a.cg;
@@ -581,7 +590,8 @@ __device__ __forceinline__ void put_sums(float* vals, int lane, int lanes, int C
 }
 
 template <class T, int ACT>
-__global__ void __launch_bounds__(kGnThreads) groupnorm_bwd_resident_kernel(const GnArgs a) {
+__global__ void __launch_bounds__(kGnThreads) groupnorm_bwd_resident_kernel(const GnArgs args) {
+  const GnArgs a = follow(args);
   constexpr int V = Vec<T>::V;
   extern __shared__ __align__(16) float gsm[];
   const int cols = a.slab / V, lanes = kGnThreads / cols, G = a.slab / a.cg, S = a.slab;
@@ -640,7 +650,8 @@ __global__ void __launch_bounds__(kGnThreads) groupnorm_bwd_resident_kernel(cons
 
 // part[n][chunk][g] = mean, squared deviations of the group over the chunk's positions
 template <class T>
-__global__ void __launch_bounds__(kGnThreads, 4) groupnorm_moments_kernel(const GnArgs a) {
+__global__ void __launch_bounds__(kGnThreads, 4) groupnorm_moments_kernel(const GnArgs args) {
+  const GnArgs a = follow(args);
   constexpr int V = Vec<T>::V;
   extern __shared__ __align__(16) float gsm[];
   const int cols = a.C / V, lanes = kGnThreads / cols, G = a.C / a.cg;
@@ -662,7 +673,8 @@ __global__ void __launch_bounds__(kGnThreads, 4) groupnorm_moments_kernel(const 
 
 // Every block joins its sample's chunks (a warp per group, the same order everywhere) and normalises its own.
 template <class T, int ACT>
-__global__ void __launch_bounds__(kGnThreads, 4) groupnorm_apply_kernel(const GnArgs a) {
+__global__ void __launch_bounds__(kGnThreads, 4) groupnorm_apply_kernel(const GnArgs args) {
+  const GnArgs a = follow(args);
   constexpr int V = Vec<T>::V;
   extern __shared__ __align__(16) float gsm[];  // [G] mean, [G] rstd
   const int n = a.n0 + blockIdx.y, chunks = gridDim.x, G = a.C / a.cg;
@@ -706,7 +718,8 @@ __global__ void __launch_bounds__(kGnThreads, 4) groupnorm_apply_kernel(const Gn
 
 // part[n][chunk][0 | 1][c] = sums over the chunk's positions of g and of g xh
 template <class T, int ACT>
-__global__ void __launch_bounds__(kGnThreads, 2) groupnorm_bwd_sums_kernel(const GnArgs a) {
+__global__ void __launch_bounds__(kGnThreads, 2) groupnorm_bwd_sums_kernel(const GnArgs args) {
+  const GnArgs a = follow(args);
   constexpr int V = Vec<T>::V;
   extern __shared__ __align__(16) float gsm[];  // [2][lanes][C], [2][C]
   const int cols = a.C / V, lanes = kGnThreads / cols;
@@ -734,6 +747,7 @@ __global__ void __launch_bounds__(kGnThreads, 2) groupnorm_bwd_sums_kernel(const
 
 // sums[n][..] = the sample's chunks; a warp's lanes are 32 entries, its block's warps share the chunks
 __global__ void __launch_bounds__(1024) groupnorm_bwd_totals_kernel(const float* part, int n0, int chunks, int C, float* sums) {
+  part += follow_previous();
   __shared__ float sm[32][33];
   const int n = n0 + blockIdx.y, e = blockIdx.x * 32 + threadIdx.x;
   float s = 0.f;
@@ -749,7 +763,8 @@ __global__ void __launch_bounds__(1024) groupnorm_bwd_totals_kernel(const float*
 }
 
 template <class T, int ACT>
-__global__ void __launch_bounds__(kGnThreads, 2) groupnorm_bwd_dx_kernel(const GnArgs a) {
+__global__ void __launch_bounds__(kGnThreads, 2) groupnorm_bwd_dx_kernel(const GnArgs args) {
+  const GnArgs a = follow(args);
   constexpr int V = Vec<T>::V;
   extern __shared__ __align__(16) float gsm[];  // [2][C] sums times w, [2][G] group means
   const int n = a.n0 + blockIdx.y, G = a.C / a.cg;
@@ -781,6 +796,7 @@ __global__ void __launch_bounds__(kGnThreads, 2) groupnorm_bwd_dx_kernel(const G
 template <class T>
 __global__ void __launch_bounds__(1024) norm_param_grad_kernel(const float* __restrict__ sums, int P, int C,
                                                                T* __restrict__ dw, T* __restrict__ db) {
+  sums += follow_previous();
   __shared__ float sm[32][33];
   const int e = blockIdx.x * 32 + threadIdx.x;
   float s = 0.f;
@@ -873,18 +889,7 @@ static int launch_gn(K kernel, PerDeviceOnce& once, dim3 grid, size_t smem, int 
                      const GnArgs& a) {
   const int st = allow_smem(once, kernel, kGnResident);
   if (st != SSAM_OK) return st;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(kGnThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = cluster;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return status_from_cuda(cudaLaunchKernelEx(&cfg, kernel, a));
+  return launch_following(kernel, grid, dim3(kGnThreads), smem, cluster, stream, a);
 }
 static size_t gn_floats(size_t n) { return (n + 3) / 4 * 16; }
 
@@ -930,15 +935,15 @@ static int groupnorm_bwd_t(GnArgs a, int N, int G, void* dw, void* db, float* ws
       st = launch_gn(groupnorm_bwd_sums_kernel<T, ACT>, sums, grid, gn_floats((2 * lanes + 2) * a.C) + GnRing2::bytes, 1,
                      stream, a);
       if (st != SSAM_OK) return st;
-      groupnorm_bwd_totals_kernel<<<dim3((2 * a.C + 31) / 32, grid.y), dim3(32, 32), 0, stream>>>(a.part, a.n0, p.chunks, a.C, a.sums);
-      st = status_from_cuda(cudaGetLastError());
+      st = launch_following(groupnorm_bwd_totals_kernel, dim3((2 * a.C + 31) / 32, grid.y), dim3(32, 32), 0, 1, stream, a.part, a.n0,
+                            p.chunks, a.C, a.sums);
       if (st == SSAM_OK)
         st = launch_gn(groupnorm_bwd_dx_kernel<T, ACT>, dx, grid, gn_floats(2 * (a.C + G)) + GnRing2::bytes, 1, stream, a);
       if (st != SSAM_OK) return st;
     }
   }
-  norm_param_grad_kernel<T><<<(2 * a.C + 31) / 32, dim3(32, 32), 0, stream>>>(a.sums, N, a.C, static_cast<T*>(dw), static_cast<T*>(db));
-  return status_from_cuda(cudaGetLastError());
+  return launch_following(norm_param_grad_kernel<T>, dim3((2 * a.C + 31) / 32), dim3(32, 32), 0, 1, stream, a.sums, N, a.C,
+                          static_cast<T*>(dw), static_cast<T*>(db));
 }
 
 #define SSAM_GN_ACT(T, call)                         \
@@ -1002,6 +1007,8 @@ __global__ void __launch_bounds__(256) layernorm_half_bwd_kernel(const T* __rest
                                                                  int64_t rows, const T* __restrict__ w,
                                                                  const T* __restrict__ b, float eps, T* __restrict__ dx,
                                                                  float* __restrict__ sums) {
+  const int64_t zero = follow_previous();
+  x += zero, dout += zero, w += zero, b += zero;
   constexpr int TPR = C / 8, RPB = 256 / TPR;
   __shared__ __align__(16) float part[2][RPB][C];
   const int t = threadIdx.x % TPR, lr = threadIdx.x / TPR;
@@ -1089,13 +1096,12 @@ static int layernorm_half_bwd_c(const void* x, const void* dout, int64_t rows, c
                                 int gelu, void* dx, void* dw, void* db, float* ws, cudaStream_t stream) {
   const int blocks = layernorm_bwd_blocks(rows, C);
   auto* kernel = gelu ? layernorm_half_bwd_kernel<T, C, true> : layernorm_half_bwd_kernel<T, C, false>;
-  kernel<<<blocks, 256, 0, stream>>>(static_cast<const T*>(x), static_cast<const T*>(dout), rows,
-                                     static_cast<const T*>(w), static_cast<const T*>(b), eps, static_cast<T*>(dx), ws);
-  const int st = status_from_cuda(cudaGetLastError());
+  const int st = launch_following(kernel, dim3(blocks), dim3(256), 0, 1, stream, static_cast<const T*>(x),
+                                  static_cast<const T*>(dout), rows, static_cast<const T*>(w), static_cast<const T*>(b), eps,
+                                  static_cast<T*>(dx), ws);
   if (st != SSAM_OK) return st;
-  norm_param_grad_kernel<T><<<(2 * C + 31) / 32, dim3(32, 32), 0, stream>>>(ws, blocks, C, static_cast<T*>(dw),
-                                                                           static_cast<T*>(db));
-  return status_from_cuda(cudaGetLastError());
+  return launch_following(norm_param_grad_kernel<T>, dim3((2 * C + 31) / 32), dim3(32, 32), 0, 1, stream, ws, blocks, C,
+                          static_cast<T*>(dw), static_cast<T*>(db));
 }
 
 template <class T>

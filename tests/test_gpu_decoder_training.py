@@ -179,3 +179,55 @@ def test_attention_of_many_prompts(cuda_device):
         parts = torch.cat([attn(t, t, t) for t in x.split(40000)])
     # fp32 of two orders of summation: unit-size logits and values, 4 eps of them
     assert (whole - parts).abs().max() <= 4 * torch.finfo(torch.float32).eps * parts.abs().max() * 2
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_calls_behind_one_another(cuda_device, captured):
+    """Each call reads what the one before has written, in memory that earlier calls have just given back: the same
+    bits as with a synchronisation after each. Short and long sides, resident and streamed maps, gradients."""
+    g = torch.Generator().manual_seed(11)
+    r = lambda *s: torch.randn(*s, generator=g).to(torch.bfloat16).to(cuda_device)  # noqa: E731
+    tokens, image, rows = r(8, 9, 8, 16), r(8, 4096, 8, 16), r(2, 200, 2, 64)
+    maps, w, b = r(16, 128 * 128, 64), r(64), r(64)
+
+    def chain(wait):
+        t, i, y, m = tokens, image, rows, maps
+        out = []
+        for _ in range(3):
+            t = wait(ops.cross_attn(t, i, i))
+            i = wait(ops.cross_attn(i, t, t))
+            y = wait(ops.cross_attn(y, y, y))
+            m = wait(ops.groupnorm_act(m, 8, w, b, 1e-5, "gelu"))
+            y = wait(ops.groupnorm_act(y.reshape(2, 400, 64), 4, w, b, 1e-5, "silu")).view(2, 200, 2, 64)
+            y = wait(ops.layernorm_gelu_half(y.contiguous(), w, b, 1e-6, True))
+        leaves = [x.detach().requires_grad_(True) for x in (t, i, y, m, w, b)]
+        o = wait(ops.cross_attn(leaves[0], leaves[1], leaves[1]))
+        p = wait(ops.cross_attn(leaves[2], leaves[2], leaves[2]))
+        n = wait(ops.groupnorm_act(leaves[3], 8, leaves[4], leaves[5], 1e-5, "gelu"))
+        q = wait(ops.layernorm_gelu_half(p, leaves[4], leaves[5], 1e-6, True))
+        grads = torch.autograd.grad([o, q, n], leaves, [tokens, rows, maps])
+        return [*(x.detach() for x in (t, i, y, m, o, p, n, q)), *grads]
+
+    def settle(x):
+        torch.cuda.synchronize()
+        return x
+
+    expect = [x.clone() for x in chain(settle)]
+    torch.cuda.synchronize()
+    if captured:
+        side = torch.cuda.Stream(cuda_device)
+        side.wait_stream(torch.cuda.current_stream(cuda_device))
+        with torch.cuda.stream(side):
+            chain(lambda x: x)
+            side.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                got = chain(lambda x: x)
+        for _ in range(3):
+            graph.replay()
+    else:
+        for _ in range(3):
+            got = chain(lambda x: x)
+    torch.cuda.synchronize()
+    for i, (x, y) in enumerate(zip(expect, got)):
+        assert torch.isfinite(x.float()).all() and torch.equal(x, y), i
