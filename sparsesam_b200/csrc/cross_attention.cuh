@@ -71,12 +71,20 @@ int xattn_bf16(const XAttn& a, bool backward, cudaStream_t stream);
 // Two long sides on the 5th-generation tensor cores (cross_attention_tc.cu): dtype 0 / 1.
 int xattn_tc(const XAttn& a, int dtype, bool backward, cudaStream_t stream);
 
-// Entries of a short side that stay in registers: 8-entry tiles of the backward kernel (about 6 DP / 8
-// registers each) and of the forward kernel's keys (2 DP / 8 registers each).
+// What counts as a short side, in tiles of 8 entries that stay in registers; longer ones go to the tcgen05 kernels.
+// Measured on both sides with 8 x 8 heads, 4096 entries on the long side, bf16 (mma.sync against tcgen05, us):
+//   backward (with its forward), DP 16: 64 rows 56 / 93, 64 keys 59 / 118; DP 32: 32 rows 58 / 99, 32 keys 47 / 133;
+//     DP 64: 16 rows 68 / 117, 16 keys 53 / 187; DP 128: 8 rows 132 / 246, 8 keys 106 / 439. The next tile spills.
+//   forward, keys: DP 16: 64 keys 17.5 / 22.4; DP 32: 32 keys 12.9 / 23.4, 64 keys 31.4 / 23.8; DP 64: 32 keys
+//     26.5 / 27.0; DP 128: 16 keys 40.7 / 63.9.
+//   forward, rows: DP 16: 64 rows 16.5 / 29.2; DP 32: 64 rows 26.7 / 29.5; DP 64: 32 rows 29.7 / 28.7 (one batch
+//     entry 17.6 / 19.4), 48 rows 41 / 29; DP 128: 16 rows 36.6 / 52.0.
 template <int DP>
 constexpr int kXmFewTiles = 128 / DP;
 template <int DP>
-constexpr int kXmKeyTiles = DP <= 32 ? 8 : 256 / DP;
+constexpr int kXmKeyTiles = DP <= 16 ? 8 : DP <= 64 ? 4 : 2;
+template <int DP>
+constexpr int kXmRowTiles = DP <= 32 ? 8 : DP <= 64 ? 4 : 2;
 
 // Whether the backward pass reads out_f32 and lse (else it finds them itself, see xattn_bwd_few).
 inline bool xattn_uses_stats(int Tk, int d, int dtype) {

@@ -941,9 +941,9 @@ static int xattn_mma_dp(const XAttn& a, bool backward, cudaStream_t stream) {
     }
     if (rows <= 8) return xattn_few_rows_launch<T, DP, 1>(a, stream);
     if (rows <= 16) return xattn_few_rows_launch<T, DP, 2>(a, stream);
-    if constexpr (DP <= 64) {
-      if (rows <= 24 || (rows > 32 && rows <= 48)) return xattn_few_rows_launch<T, DP, 3>(a, stream);
-      if (rows <= 64) return xattn_few_rows_launch<T, DP, 4>(a, stream);
+    if constexpr (kXmRowTiles<DP> >= 4) {        // up to 32 rows to a block: two blocks of 24 or 32 past that
+      if (rows <= 24 || (rows > 32 && rows <= 48 && kXmRowTiles<DP> == 8)) return xattn_few_rows_launch<T, DP, 3>(a, stream);
+      if (rows <= 8 * kXmRowTiles<DP>) return xattn_few_rows_launch<T, DP, 4>(a, stream);
     }
     return xattn_tc(a, kIsHalf<T> ? 0 : 1, false, stream);
   }
