@@ -376,7 +376,7 @@ __global__ void __launch_bounds__(kTcBwdThreads, 2 / NP) xattn_tc_bwd_kernel(con
   __shared__ __align__(8) uint64_t bars[2];
   __shared__ uint32_t holder;
   __shared__ __align__(16) float s_a[2][kTcOther], s_b[2][kTcOther];   // of the other side: bias; or -lse and -D
-  __shared__ float s_top[kScaled ? kTcBwdThreads : 1];
+  __shared__ float s_top[kScaled ? kTcBwdThreads : 1], s_d[OWN_ROWS ? kTcOwn : 1];
   TcBlock B;
   B.open(raw, bars, &holder, kCols);
   const uint32_t x1 = B.sm, x2 = B.sm + kTile, ring = B.sm + 2 * kTile, tS = 0, tD = 64, tA1 = 128, tA2 = 128 + 64 * NP;
@@ -419,26 +419,34 @@ __global__ void __launch_bounds__(kTcBwdThreads, 2 / NP) xattn_tc_bwd_kernel(con
       }
     }
   };
-  float own_s, own_d = 0.f;                  // -lse and -D of the thread's query; bias of its key
+  float own_s;                               // -lse of the thread's query; bias of its key
   const int mine = own0 + lane_id;
   if constexpr (OWN_ROWS) {
     tc_fetch<T, NP, kTcOwn, kTcBwdThreads>(x1, a.d, qb, [&](int i) { return row_at(qb, a.qs, own0 + i); });
     tc_fetch<T, NP, kTcOwn, kTcBwdThreads>(x2, a.d, ob, [&](int i) { return row_at(ob, a.os, own0 + i); });
     request(j_begin, 0);
-    own_s = -INFINITY;
-    if (mine < rows) {
-      own_s = -__ldg(a.lse + stat0 + mine);
-      const TcRow at = tc_row(a, n, mine);
-      const T* o = ob + at.t * a.os[1] + at.h * a.os[2];
-      const float* o32 = a.out_f32 + ((static_cast<int64_t>(b) * a.Tq + at.t) * a.heads + at.h) * a.d;
-      for (int c = 0; c < a.d; c += 8) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(o + c));
-        const float4 f0 = __ldg(reinterpret_cast<const float4*>(o32 + c)), f1 = __ldg(reinterpret_cast<const float4*>(o32 + c + 4));
+    own_s = mine < rows ? -__ldg(a.lse + stat0 + mine) : -INFINITY;
+    // D: 8 NP threads to a row, 8 channels each, so that a load covers whole lines
+    const int c = tid % (8 * NP) * 8;
+#pragma unroll
+    for (int i = tid / (8 * NP); i < kTcOwn; i += kTcBwdThreads / (8 * NP)) {
+      const int r = own0 + i;
+      float y = 0.f;
+      if (r < rows && c < a.d) {
+        const TcRow at = tc_row(a, n, r);
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(ob + at.t * a.os[1] + at.h * a.os[2] + c));
+        const float4* o32 = reinterpret_cast<const float4*>(a.out_f32 + ((static_cast<int64_t>(b) * a.Tq + at.t) * a.heads + at.h) * a.d + c);
+        const float4 f0 = __ldg(o32), f1 = __ldg(o32 + 1);
         const float2 g0 = tc_unpack<T>(u.x), g1 = tc_unpack<T>(u.y), g2 = tc_unpack<T>(u.z), g3 = tc_unpack<T>(u.w);
-        own_d = fmaf(-f0.x, g0.x, fmaf(-f0.y, g0.y, fmaf(-f0.z, g1.x, fmaf(-f0.w, g1.y, own_d))));
-        own_d = fmaf(-f1.x, g2.x, fmaf(-f1.y, g2.y, fmaf(-f1.z, g3.x, fmaf(-f1.w, g3.y, own_d))));
+        y = fmaf(f0.x, g0.x, fmaf(f0.y, g0.y, fmaf(f0.z, g1.x, f0.w * g1.y)));
+        y = fmaf(f1.x, g2.x, fmaf(f1.y, g2.y, fmaf(f1.z, g3.x, fmaf(f1.w, g3.y, y))));
       }
-      if (rank == 0 && half == 0) a.delta[stat0 + mine] = -own_d;
+#pragma unroll
+      for (int o = 4 * NP; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+      if (c == 0) {
+        s_d[i] = y;
+        if (r < rows && rank == 0) a.delta[stat0 + r] = y;
+      }
     }
   } else {
     tc_fetch<T, NP, kTcOwn, kTcBwdThreads>(x1, a.d, kb, [&](int i) { return key_at(kb, a.ks, own0 + i); });
@@ -447,9 +455,10 @@ __global__ void __launch_bounds__(kTcBwdThreads, 2 / NP) xattn_tc_bwd_kernel(con
     own_s = key_ok(mine) ? 0.f : -INFINITY;
   }
 
+  bool ok = tc_landed(true);
+  const float own_d = OWN_ROWS ? -s_d[lane_id] : 0.f;
   const float2 c2 = make_float2(a.c, a.c), os2 = make_float2(own_s, own_s), od2 = make_float2(own_d, own_d);
   int up = 253;                              // exponent field of the power of two on dS: 2^126 until one is seen
-  bool ok = tc_landed(true);
   int it = 0;
   for (int j = j_begin; j < j_end; ++j, ++it) {
     const int buf = it & 1;
