@@ -35,6 +35,41 @@ template <int DT, int TPR>
 __device__ __forceinline__ float row_dot(const float2 (&a)[DT / 2], const float* b) {
   return row_dot<DT, TPR>(a, [b](int i) { return *reinterpret_cast<const float4*>(b + 4 * i); });
 }
+// the same for NR rows: b is read once
+template <int DT, int TPR, int NR>
+__device__ __forceinline__ void rows_dot(const float2 (&a)[NR][DT / 2], const float* b, float (&y)[NR]) {
+  float2 s0[NR], s1[NR];
+#pragma unroll
+  for (int z = 0; z < NR; ++z) s0[z] = s1[z] = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < DT / 2; i += 2) {
+    const float4 v = *reinterpret_cast<const float4*>(b + 2 * i);
+#pragma unroll
+    for (int z = 0; z < NR; ++z) {
+      s0[z] = fma2(a[z][i], make_float2(v.x, v.y), s0[z]);
+      s1[z] = fma2(a[z][i + 1], make_float2(v.z, v.w), s1[z]);
+    }
+  }
+#pragma unroll
+  for (int z = 0; z < NR; ++z) {
+    s0[z] = add2(s0[z], s1[z]);
+    y[z] = s0[z].x + s0[z].y;
+#pragma unroll
+    for (int o = 1; o < TPR; o <<= 1) y[z] += __shfl_xor_sync(0xffffffffu, y[z], o);
+  }
+}
+template <int DT, int NR>
+__device__ __forceinline__ void rows_axpy(const float (&w)[NR], const float* b, float2 (&acc)[NR][DT / 2]) {
+#pragma unroll
+  for (int i = 0; i < DT / 2; i += 2) {
+    const float4 v = *reinterpret_cast<const float4*>(b + 2 * i);
+#pragma unroll
+    for (int z = 0; z < NR; ++z) {
+      acc[z][i] = fma2(make_float2(w[z], w[z]), make_float2(v.x, v.y), acc[z][i]);
+      acc[z][i + 1] = fma2(make_float2(w[z], w[z]), make_float2(v.z, v.w), acc[z][i + 1]);
+    }
+  }
+}
 template <int DT>
 __device__ __forceinline__ void row_axpy(float w, const float* b, float2 (&acc)[DT / 2]) {
   const float2 w2 = make_float2(w, w);
@@ -105,7 +140,7 @@ __device__ __forceinline__ void merge_sums(float* part, int KS, int RB, int W, E
 
 // The block's own rows, which lie heads * d apart, through shared memory: four lanes fetch a row's 64 bytes and more
 // together, where a thread that reads its own row by itself touches 32 lines per load (image -> tokens, fp32, 64
-// images: 144 us that way). row(i) is row i's address, nullptr behind the last.
+// images: 144 us that way, 128 through shared memory). row(i) is row i's address, nullptr behind the last.
 template <int DP, class R>
 __device__ __forceinline__ void fetch_own(float* sm, int RB, int d, R row) {
   constexpr int V = DP / 4, LD = DP + 4;
@@ -142,13 +177,13 @@ struct XPlace {
     const int rr = r0 + i, gg = a.group == 1 ? 0 : rr / a.Tq, tt = rr - gg * a.Tq;
     return rr < rows ? p + b * st[0] + tt * st[1] + (n * a.group + gg) * st[2] : nullptr;
   }
-  __device__ __forceinline__ XPlace(const XAttn& a, int RB, int TPR) {
+  __device__ __forceinline__ XPlace(const XAttn& a, int RB, int TPR, int NR = 1) {
     KS = kXThreads / (RB * TPR);
     part = threadIdx.x % TPR, lr = threadIdx.x / TPR % RB, slice = threadIdx.x / (TPR * RB);
     b = blockIdx.z, n = blockIdx.y;
     cl = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
     rows = a.group * a.Tq;
-    r0 = static_cast<int>(blockIdx.x) / cl * RB, r = r0 + lr;
+    r0 = static_cast<int>(blockIdx.x) / cl * RB * NR, r = r0 + lr;
     const int g = r / a.Tq;
     t = r - g * a.Tq, h = n * a.group + g;
     row_ok = r < rows;
@@ -184,71 +219,14 @@ __device__ __forceinline__ void walk_keys(const XAttn& a, const XPlace& x, float
   }
 }
 
+// Joins the slices' and blocks' shares of the rows.
 template <int DT, int TPR>
-__global__ void __launch_bounds__(kXThreads) xattn_fwd_scalar(const XAttn args, int RB) {
-  const XAttn a = follow(args, false);
-  constexpr int DP = DT * TPR, LD = DP + 4, U = 4;
-  extern __shared__ __align__(16) float xsm[];
-  __shared__ float bias[2][kXTile<DP>];
-  const XPlace x(a, RB, TPR);
+__device__ __forceinline__ void xattn_fwd_join(const XAttn& a, const XPlace& x, float* xsm, int RB, const float2 (&o)[DT / 2], float m,
+                                               float l) {
+  constexpr int DP = DT * TPR;
   const int part = x.part, lr = x.lr, slice = x.slice, KS = x.KS, b = x.b, n = x.n, cl = x.cl, rank = x.rank, rows = x.rows,
             r0 = x.r0;
-  float2 q[DT / 2], o[DT / 2];
-  fetch_own<DP>(xsm, RB, a.d, [&](int i) { return x.row_of(a, static_cast<const float*>(a.q), a.qs, i); });
-  asm volatile("cp.async.wait_all;" ::: "memory");
-  __syncthreads();
-  own_row<DT>(xsm + lr * LD + part * DT, q);
-  __syncthreads();
-  clear_row<DT>(o);
-  float m = -INFINITY, l = 0.f;
-  walk_keys<DP>(a, x, xsm, bias, [&](const float* sk, const float* sv, int nk, const float* here) {
-    for (int j = slice; j < nk; j += U * KS) {           // U keys at a time: one look at the maximum
-      float s[U], top = m;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        s[u] = -INFINITY;
-        if (j - slice + u * KS < nk) {                   // the same for all threads
-          const int i = j + u * KS;
-          s[u] = fmaf(row_dot<DT, TPR>(q, sk + i * LD + part * DT), a.c, here[i]);   // -infinity: no such key
-        }
-        top = fmaxf(top, s[u]);
-      }
-      if (top > m) {
-        const float f = ex2f(m - top);
-        l *= f;
-#pragma unroll
-        for (int i = 0; i < DT / 2; ++i) o[i] = mul2(o[i], make_float2(f, f));
-        m = top;
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (j - slice + u * KS >= nk) break;
-        const float p = s[u] == -INFINITY ? 0.f : ex2f(s[u] - m);  // a NaN logit stays one
-        l += p;
-        row_axpy<DT>(p, sv + (j + u * KS) * LD + part * DT, o);
-      }
-    }
-  });
-  if (KS == 1 && cl == 1) {                  // a row is one group of TPR threads: out through shared memory, as it came
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    put_row<DT>(xsm + lr * LD + part * DT, o, inv);
-    if (a.lse != nullptr && part == 0 && x.row_ok)
-      a.lse[(static_cast<int64_t>(b) * a.heads + x.h) * a.Tq + x.t] = l == 0.f ? INFINITY : m + log2f(l);
-    __syncthreads();
-    for (int e = threadIdx.x; e < RB * (DP / 4); e += kXThreads) {
-      const int i = e / (DP / 4), col = e % (DP / 4) * 4;
-      float* to = const_cast<float*>(x.row_of(a, static_cast<const float*>(a.out), a.os, i));
-      if (to == nullptr || col >= a.d) continue;
-      const float4 y = *reinterpret_cast<const float4*>(xsm + i * LD + col);
-      *reinterpret_cast<float4*>(to + col) = y;
-      if (a.out_f32 != nullptr) {
-        const int64_t dense[3] = {static_cast<int64_t>(a.Tq) * a.heads * a.d, static_cast<int64_t>(a.heads) * a.d, a.d};
-        *reinterpret_cast<float4*>(const_cast<float*>(x.row_of(a, a.out_f32, dense, i)) + col) = y;
-      }
-    }
-    return;
-  }
-  // join the slices and blocks: rescale everybody's share to the common maximum first
+  // rescale everybody's share to the common maximum first
   __syncthreads();
   float* ms = xsm;                       // [KS][RB]
   float* acc = xsm + kXThreads;          // [KS][RB][DP + 1]
@@ -310,6 +288,97 @@ __global__ void __launch_bounds__(kXThreads) xattn_fwd_scalar(const XAttn args, 
     }
   }
   if (cl > 1) cluster_sync_all();
+}
+
+// NR rows to a thread, RB apart: K and V come out of shared memory once for all of them, which is what the kernel waits
+// for (1024 x 1024, 16 x 8 heads of 16: 400 us with one row, 340 with two, of 64: 2040 and 1400; 4096 queries on 8
+// keys, 64 x 8 heads of 16: 128 and 106, at 2.5 TB/s). NR > 1: one slice, no cluster.
+template <int DT, int TPR, int NR>
+__global__ void __launch_bounds__(kXThreads) xattn_fwd_scalar(const XAttn args, int RB) {
+  const XAttn a = follow(args, false);
+  constexpr int DP = DT * TPR, LD = DP + 4, U = 4;
+  extern __shared__ __align__(16) float xsm[];
+  __shared__ float bias[2][kXTile<DP>];
+  const XPlace x(a, RB, TPR, NR);
+  const int part = x.part, lr = x.lr, slice = x.slice, KS = x.KS, b = x.b, n = x.n, cl = x.cl, rank = x.rank, rows = x.rows,
+            r0 = x.r0;
+  float2 q[NR][DT / 2], o[NR][DT / 2];
+  fetch_own<DP>(xsm, NR * RB, a.d, [&](int i) { return x.row_of(a, static_cast<const float*>(a.q), a.qs, i); });
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
+  float m[NR], l[NR];
+#pragma unroll
+  for (int z = 0; z < NR; ++z) {
+    own_row<DT>(xsm + (z * RB + lr) * LD + part * DT, q[z]);
+    clear_row<DT>(o[z]);
+    m[z] = -INFINITY, l[z] = 0.f;
+  }
+  __syncthreads();
+  walk_keys<DP>(a, x, xsm, bias, [&](const float* sk, const float* sv, int nk, const float* here) {
+    for (int j = slice; j < nk; j += U * KS) {           // U keys at a time: one look at the maximum
+      float s[NR][U], top[NR];
+#pragma unroll
+      for (int z = 0; z < NR; ++z) top[z] = m[z];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int z = 0; z < NR; ++z) s[z][u] = -INFINITY;
+        if (j - slice + u * KS < nk) {                   // the same for all threads
+          const int i = j + u * KS;
+          float y[NR];
+          rows_dot<DT, TPR, NR>(q, sk + i * LD + part * DT, y);
+#pragma unroll
+          for (int z = 0; z < NR; ++z) s[z][u] = fmaf(y[z], a.c, here[i]);   // -infinity: no such key
+        }
+#pragma unroll
+        for (int z = 0; z < NR; ++z) top[z] = fmaxf(top[z], s[z][u]);
+      }
+#pragma unroll
+      for (int z = 0; z < NR; ++z)
+        if (top[z] > m[z]) {
+          const float f = ex2f(m[z] - top[z]);
+          l[z] *= f;
+#pragma unroll
+          for (int i = 0; i < DT / 2; ++i) o[z][i] = mul2(o[z][i], make_float2(f, f));
+          m[z] = top[z];
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (j - slice + u * KS >= nk) break;
+        float p[NR];
+#pragma unroll
+        for (int z = 0; z < NR; ++z) {
+          p[z] = s[z][u] == -INFINITY ? 0.f : ex2f(s[z][u] - m[z]);  // a NaN logit stays one
+          l[z] += p[z];
+        }
+        rows_axpy<DT, NR>(p, sv + (j + u * KS) * LD + part * DT, o);
+      }
+    }
+  });
+  if (NR > 1 || (KS == 1 && cl == 1)) {      // a row is one group of TPR threads: out through shared memory, as it came
+#pragma unroll
+    for (int z = 0; z < NR; ++z) {
+      const float inv = l[z] == 0.f ? 0.f : 1.f / l[z];
+      put_row<DT>(xsm + (z * RB + lr) * LD + part * DT, o[z], inv);
+      const int r = x.r + z * RB;
+      if (a.lse != nullptr && part == 0 && r < rows)
+        a.lse[(static_cast<int64_t>(b) * a.heads + n * a.group) * a.Tq + r] = l[z] == 0.f ? INFINITY : m[z] + log2f(l[z]);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < NR * RB * (DP / 4); e += kXThreads) {
+      const int i = e / (DP / 4), col = e % (DP / 4) * 4;
+      float* to = const_cast<float*>(x.row_of(a, static_cast<const float*>(a.out), a.os, i));
+      if (to == nullptr || col >= a.d) continue;
+      const float4 y = *reinterpret_cast<const float4*>(xsm + i * LD + col);
+      *reinterpret_cast<float4*>(to + col) = y;
+      if (a.out_f32 != nullptr) {
+        const int64_t dense[3] = {static_cast<int64_t>(a.Tq) * a.heads * a.d, static_cast<int64_t>(a.heads) * a.d, a.d};
+        *reinterpret_cast<float4*>(const_cast<float*>(x.row_of(a, a.out_f32, dense, i)) + col) = y;
+      }
+    }
+    return;
+  }
+  if constexpr (NR == 1) xattn_fwd_join<DT, TPR>(a, x, xsm, RB, o[0], m[0], l[0]);
 }
 
 // dQ: the forward's loop with p from the saved statistics. Also writes D for the dK / dV kernel.
@@ -476,7 +545,13 @@ static int xattn_scalar(const XAttn& a, bool backward, cudaStream_t stream) {
   if (!backward) {
     constexpr size_t merge = (kXThreads + kXThreads / TPR * (DP + 1)) * sizeof(float);
     static_assert(merge <= 48 << 10 && stages <= 48 << 10, "no opt-in needed");
-    return launch_following(xattn_fwd_scalar<DT, TPR>, by_rows, kXThreads, stages > merge ? stages : merge, cl, stream, a, rb);
+    // two rows to a thread where that still leaves every SM two blocks (DT 32: four, of which three run at once; 512
+    // blocks of 32 channels took 696 us where 1024 of one row took 586)
+    const int two = (rows + 2 * rb - 1) / (2 * rb);
+    static_assert(2 * kXThreads / TPR * (DP + 4) * sizeof(float) <= stages, "the block's own rows");
+    if (rb * TPR == kXThreads && cl == 1 && rows > rb && pairs * two >= (DT == 16 ? 2 : 4) * 148)
+      return launch_following(xattn_fwd_scalar<DT, TPR, 2>, dim3(two, a.kv_heads, a.B), kXThreads, stages, 1, stream, a, rb);
+    return launch_following(xattn_fwd_scalar<DT, TPR, 1>, by_rows, kXThreads, stages > merge ? stages : merge, cl, stream, a, rb);
   }
   constexpr size_t merge = kXThreads / TPR * 2 * DP * sizeof(float);
   static_assert(merge <= 48 << 10, "no opt-in needed");

@@ -142,7 +142,7 @@ constexpr float kXmSlack = 8.f;
 //
 // HP = 2 (heads of 16 next to one another): a fragment is two heads of a token, 64 contiguous
 // bytes, because 32-byte pieces keep the L1 tags, not the DRAM, busy (tokens -> image, 64 images:
-// 35 us with HP = 1 at 72 % of L1). Lanes t < 2 hold the first head's channels, so a query
+// 35 us with HP = 1 at 72 % of L1, 26.4 with HP = 2 at 5.1 TB/s; one image 4.5 us, a launch and a join). Lanes t < 2 hold the first head's channels, so a query
 // fragment with the other half zeroed gives one head's logits, and likewise V^T rows g < 4
 // are the first head's. Twice the tensor instructions, of which there are plenty.
 // ---------------------------------------------------------------------------
@@ -372,8 +372,8 @@ __global__ void __launch_bounds__(kXmThreads) xattn_fwd_few_rows(const XAttn arg
 // ---------------------------------------------------------------------------
 // Forward, many queries on few keys (at most 8 NK): a warp keeps the K and turned V
 // fragments of one (image, query head) and walks its share of the queries 16 at a time, the
-// next rows in flight. Bound by the bytes of q and out; neighbouring warps hold
-// neighbouring heads, so a block touches whole rows. HP = 2 as above.
+// next rows in flight. Bound by the bytes of q and out (64 images, 4096 queries on 8 keys: 30 us,
+// 4.5 TB/s); neighbouring warps hold neighbouring heads, so a block touches whole rows. HP = 2 as above.
 // ---------------------------------------------------------------------------
 template <class T, int DP, int NK, int HP>
 __global__ void __launch_bounds__(kXmThreads) xattn_fwd_few_keys(const XAttn args, int chunks) {
@@ -583,7 +583,8 @@ __device__ __forceinline__ float row_delta(const float* o32, const uint32_t (&x)
 
 // One short side: its 8 NF entries ("few") are all of it, the columns of every tile, and stay in
 // registers with their gradient sums; warps and cluster share the long side, 16 entries at a time,
-// whose gradients are complete at once and leave at once. One pass over all inputs.
+// whose gradients are complete at once and leave at once. One pass over all inputs: 64 images, 8 queries on
+// 4096 keys, with the forward pass 106 us; 2.5 TB/s, one block of 255 registers per thread and SM.
 //   few = query rows (FEW_ROWS): x = k, v;  y = q, dout.  dk = ds y1, dv = p y2 leave;  dq^T += k^T ds stays
 //   few = keys:                  x = q, dout;  y = k, v.  dq = ds y1 leaves;  dk^T += q^T ds, dv^T += dout^T p stay
 template <class T, int DP, int NF, bool FEW_ROWS>

