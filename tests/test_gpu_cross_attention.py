@@ -309,3 +309,20 @@ def test_half_gradients_of_any_size(cuda_device, D, low):
     v = v * rise(400)[None, :, None, None] * 2.0 ** -6
     do = do * rise(300)[None, :, None, None] * 2.0 ** low
     check(run(q, k, v, do), reference(q, k, v, do), "fp16")
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("Tq,Tk,D", [(90, 100, 64), (90, 100, 128), (100, 9, 16), (9, 100, 16), (200, 9, 32)])
+def test_far_rows_of_every_kernel(cuda_device, dtype, Tq, Tk, D):
+    """All three inputs and the incoming gradient strided so that their offsets pass 2^31 elements."""
+    step = (1 << 31) // 80
+    step -= step % 8
+    buf = torch.empty(step * 200 + 4 * D, dtype=DTYPES[dtype], device=cuda_device)
+    q, k, v, do = make(cuda_device, 1, Tq, Tk, 1, 1, D, dtype, seed=12)
+    expect = run(q, k, v, do)
+    far = []
+    for i, t in enumerate((q, k, v, do)):
+        f = buf.as_strided(t.shape, (step, step, D, 1), i * D)
+        far.append(f.copy_(t))
+    got = run(*far)
+    assert all(torch.equal(x, y) for x, y in zip(got, expect))
