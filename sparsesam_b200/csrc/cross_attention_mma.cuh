@@ -128,7 +128,7 @@ __device__ __forceinline__ int64_t row_dense(const XAttn& a, int b, int n, int r
   return ((static_cast<int64_t>(b) * a.Tq + t) * a.heads + n * a.group + g) * a.d;
 }
 
-constexpr float kXmNone = -1e30f;           // reference before the first key
+constexpr float kXmNone = -3e38f;           // reference before the first key: below all finite logits that matter
 constexpr float kXmSlack = 8.f;
 
 // ---------------------------------------------------------------------------
@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(kXmThreads) xattn_fwd_few_keys(const XAttn arg
       float inv[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float x = kXmNone;                   // a row without keys: 2^(-inf + 1e30) = 0
+        float x = kXmNone;                   // a row without keys: 2^(-inf + 3e38) = 0
 #pragma unroll
         for (int i = 0; i < NK; ++i) x = fmaxf(x, fmaxf(s[z][i][e].x, s[z][i][e].y));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));

@@ -326,3 +326,16 @@ def test_far_rows_of_every_kernel(cuda_device, dtype, Tq, Tk, D):
         far.append(f.copy_(t))
     got = run(*far)
     assert all(torch.equal(x, y) for x, y in zip(got, expect))
+
+
+@pytest.mark.parametrize("Tq,Tk", [(3, 400), (400, 5), (100, 100)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_far_negative_logits(cuda_device, dtype, Tq, Tk):
+    """Logits of -7e36, all alike: still a softmax, of equal weights; not a row without keys."""
+    q, k, v, _ = make(cuda_device, 1, Tq, Tk, 2, 2, 16, dtype, seed=13)
+    q, k = torch.full_like(q, -(2.0 ** 60)), torch.full_like(k, 2.0 ** 60)
+    (out,) = run(q, k, v)
+    mean = v.double().mean(1, keepdim=True).expand(-1, Tq, -1, -1)
+    u = torch.finfo(DTYPES[dtype]).eps / 2
+    size = v.double().abs().mean(1, keepdim=True)
+    assert torch.all((out.double() - mean).abs() <= u * mean.abs() + (4 * u * u + NOISE) * size)
