@@ -576,7 +576,7 @@ static int xattn_dispatch(const XAttn& a, int dtype, bool backward, cudaStream_t
 static int xattn_check(const XAttn& a, int dtype) {
   if (a.B <= 0 || a.Tq <= 0 || a.Tk <= 0 || a.heads <= 0 || a.kv_heads <= 0 || a.d <= 0) return SSAM_ERR_INVALID;
   if (dtype < 0 || dtype > 2 || a.heads % a.kv_heads) return SSAM_ERR_INVALID;
-  if (!(a.scale > 0.f) || a.scale > 3.0e38f) return SSAM_ERR_INVALID;
+  if (!(a.scale > 0.f) || a.scale > 2.0e38f) return SSAM_ERR_INVALID;   // scale log2(e) is finite
   if (a.d > 128 || a.d % 8 || a.B > 65535 || a.kv_heads > 65535) return SSAM_ERR_UNSUPPORTED;
   if (static_cast<int64_t>(a.group) * a.Tq > (1 << 30) || a.Tk > (1 << 30)) return SSAM_ERR_UNSUPPORTED;
   const int64_t unit = dtype == 2 ? 4 : 8;

@@ -356,7 +356,7 @@ Tensor cross_attn(const Tensor& q, const Tensor& k, const Tensor& v, std::option
                          mask.size(1) != k.size(1) || !mask.is_contiguous()))
     refuse("key_mask must be contiguous bool (B, Tk)");
   const double scale = scale_ ? *scale_ : 1.0 / std::sqrt(static_cast<double>(D));
-  if (!(scale > 0.0 && scale < 3e38)) refuse("scale must be positive and finite, got " + std::to_string(scale));
+  if (!(scale > 0.0 && scale < 2e38)) refuse("scale must be positive and below 2e38, got " + std::to_string(scale));
   check_devices(q, {&k, &v, &lens, &mask});
   if (wants_grad({&q, &k, &v})) return CrossAttn::apply(q, k, v, scale, lens_, mask_);
   Tensor out32, stats;

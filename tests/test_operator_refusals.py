@@ -132,3 +132,10 @@ def test_sizes_past_32_bits():
             ops.cross_attn(q, q.expand(1, n, 1, 8), q.expand(1, n, 1, 8))
         with pytest.raises(ValueError, match="entries"):
             ops.groupnorm_act(q.expand(n, 1, 1, 8), 1, q[0, 0, 0], q[0, 0, 0])
+
+
+def test_scale_whose_exponent_base_change_overflows():
+    q = torch.zeros(1, 1, 1, 8, dtype=torch.float16)
+    assert fwd(scale=2.5e38) == INV
+    with pytest.raises(ValueError, match="scale"):
+        ops.cross_attn(q, q, q, scale=2.5e38)
