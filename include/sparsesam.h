@@ -338,7 +338,7 @@ int ssam_groupnorm_act_bwd(const void* x, const void* dout, int N, int64_t HW, i
  *             (backward: of dout in out's place); d is contiguous. A stride of 0
  *             broadcasts an input. Strides are multiples of 8 elements (fp32: 4).
  *   dtype   : 0 fp16, 1 bf16, 2 fp32; logits, statistics and sums are fp32.
- *   scale   : positive and finite.
+ *   scale   : positive, at most 2e38 (scale log2(e) has to be finite).
  *   out_f32 : optional fp32 [B, Tq, heads, d] contiguous copy of the result before its
  *             rounding, and lse, optional fp32 [B, heads, Tq] (base-2 log-sum-exp of the
  *             logits): what the backward pass takes. For dtype 2 with a contiguous `out`
