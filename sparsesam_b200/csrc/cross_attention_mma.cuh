@@ -17,7 +17,10 @@
 //
 // Second factors: probabilities and dS are fp32 and enter their product as two half
 // terms (value and remainder), so that a result carries one rounding to its type instead
-// of two. A single term measured 1.4 times the error of the rounded definition.
+// of two. A single term measured 1.4 times the error of the rounded definition. For fp16
+// inputs too these products run in bf16, which has fp32's exponents: a probability below
+// fp16's 2^-24 counts where the larger ones meet zeros. The fp16 factor then enters as two
+// bf16 terms (exact, 11 bits = 8 + 3), without the product of the two remainders (2^-18).
 #pragma once
 
 #include "cross_attention.cuh"
@@ -82,6 +85,24 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
   lo = Mma<T>::pack(r.x, r.y);
 }
 
+template <class T>
+constexpr bool kIsHalf = false;
+template <>
+constexpr bool kIsHalf<__half> = true;
+
+// A pair of T as bf16 terms: cut off after 8 bits, so that both terms take no rounding instructions
+template <class T>
+__device__ __forceinline__ void bf16_terms(uint32_t x, uint32_t& hi, uint32_t& lo) {
+  if constexpr (kIsHalf<T>) {
+    const float2 f = Mma<__half>::unpack(x);
+    hi = __byte_perm(__float_as_uint(f.x), __float_as_uint(f.y), 0x7632);
+    const float2 h = Mma<__nv_bfloat16>::unpack(hi), r = add2(f, make_float2(-h.x, -h.y));
+    lo = __byte_perm(__float_as_uint(r.x), __float_as_uint(r.y), 0x7632);
+  } else {
+    hi = x, lo = 0u;
+  }
+}
+
 // This lane's DP / 4 channels of a token row (DP / 8 registers); zeros past channel d and when !ok.
 template <class T, int DP>
 __device__ __forceinline__ void load_frag(const T* row, int t, int d, bool ok, uint32_t (&r)[DP / 8]) {
@@ -115,6 +136,11 @@ __device__ __forceinline__ void store_frag(T* row, int t, int d, const uint32_t 
 
 constexpr int kXmWarps = 8;
 constexpr int kXmThreads = 32 * kXmWarps;
+// Blocks per SM that the forward kernels' registers are held down to: N tiles of 8 entries of the short side in registers
+// (S = 2: keys, half the accumulators of rows), DP channels. The fp16 instances would each lose a block to their
+// remainders otherwise (60 keys of 64 images: 145 us, 102 with the bound).
+template <int DP, int N, int S>
+constexpr int kXmBlocks = DP * N <= 16 * S ? 2 + S : DP * N <= 32 * S && S == 2 && DP <= 32 ? 3 : DP * N <= 64 * S && DP <= 64 ? 2 : 1;
 
 // Query row r of key head n -> element offset
 __device__ __forceinline__ int64_t row_offset(const XAttn& a, const int64_t (&st)[3], int b, int n, int r) {
@@ -147,8 +173,9 @@ constexpr float kXmSlack = 8.f;
 // are the first head's. Twice the tensor instructions, of which there are plenty.
 // ---------------------------------------------------------------------------
 template <class T, int DP, int NQ, int HP>
-__global__ void __launch_bounds__(kXmThreads) xattn_fwd_few_rows(const XAttn args, int) {
+__global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NQ, 1>) xattn_fwd_few_rows(const XAttn args, int) {
   const XAttn a = follow(args, args.lse == nullptr);
+  using B16 = Mma<__nv_bfloat16>;
   constexpr int NR = DP / 8, NU = NR / 2;    // 8- and 16-channel blocks
   constexpr int KM = DP <= 32 && HP * NQ <= 4 ? 2 : 1;   // 16-key tiles per step
   extern __shared__ __align__(16) float xsm[];
@@ -276,26 +303,29 @@ __global__ void __launch_bounds__(kXmThreads) xattn_fwd_few_rows(const XAttn arg
     for (int z = 0; z < HP; ++z)
 #pragma unroll
       for (int x = 0; x < KM; ++x) {
-        uint32_t va[2][NR];
+        uint32_t hi[NQ][2], lo[NQ][2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int c = 0; c < NR; ++c) va[h][c] = HP == 1 || g / 4 == z ? vt[x][h][c] : 0u;
-#pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-          uint32_t hi[2], lo[2];
+        for (int i = 0; i < NQ; ++i)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             float2 p = add2(s[z][i][x][h], make_float2(-ref[z][i].x, -ref[z][i].y));
             p.x = ex2f(p.x), p.y = ex2f(p.y);
             l[z][i] = add2(l[z][i], p);
-            split2<T>(p.x, p.y, hi[h], lo[h]);
-            hi[h] = movm(hi[h]), lo[h] = movm(lo[h]);
+            split2<__nv_bfloat16>(p.x, p.y, hi[i][h], lo[i][h]);
+            hi[i][h] = movm(hi[i][h]), lo[i][h] = movm(lo[i][h]);
           }
 #pragma unroll
-          for (int u = 0; u < NU; ++u) {
-            Mma<T>::run(o[i][u], va[0][2 * u], va[0][2 * u + 1], va[1][2 * u], va[1][2 * u + 1], hi[0], hi[1]);
-            Mma<T>::run(o[i][u], va[0][2 * u], va[0][2 * u + 1], va[1][2 * u], va[1][2 * u + 1], lo[0], lo[1]);
+        for (int u = 0; u < NU; ++u) {
+          uint32_t vh[2][2], vl[2][2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) bf16_terms<T>(HP == 1 || g / 4 == z ? vt[x][h][2 * u + e] : 0u, vh[h][e], vl[h][e]);
+#pragma unroll
+          for (int i = 0; i < NQ; ++i) {
+            B16::run(o[i][u], vh[0][0], vh[0][1], vh[1][0], vh[1][1], hi[i][0], hi[i][1]);
+            B16::run(o[i][u], vh[0][0], vh[0][1], vh[1][0], vh[1][1], lo[i][0], lo[i][1]);
+            if constexpr (kIsHalf<T>) B16::run(o[i][u], vl[0][0], vl[0][1], vl[1][0], vl[1][1], hi[i][0], hi[i][1]);
           }
         }
       }
@@ -376,8 +406,9 @@ __global__ void __launch_bounds__(kXmThreads) xattn_fwd_few_rows(const XAttn arg
 // 4.5 TB/s); neighbouring warps hold neighbouring heads, so a block touches whole rows. HP = 2 as above.
 // ---------------------------------------------------------------------------
 template <class T, int DP, int NK, int HP>
-__global__ void __launch_bounds__(kXmThreads) xattn_fwd_few_keys(const XAttn args, int chunks) {
+__global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NK, 2>) xattn_fwd_few_keys(const XAttn args, int chunks) {
   const XAttn a = follow(args, false);
+  using B16 = Mma<__nv_bfloat16>;
   constexpr int NR = DP / 8;
   const int lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   const int units = a.heads / HP;
@@ -400,7 +431,7 @@ __global__ void __launch_bounds__(kXmThreads) xattn_fwd_few_keys(const XAttn arg
   float* lse = a.lse == nullptr ? nullptr : a.lse + (static_cast<int64_t>(b) * a.heads + h) * a.Tq;
   float* o32 = a.out_f32 == nullptr ? nullptr : a.out_f32 + (static_cast<int64_t>(b) * a.Tq * a.heads + h) * a.d + t * (DP / 4);
 
-  uint32_t k[HP][NK][NR], v[HP][NK][NR], q[2][NR];
+  uint32_t k[HP][NK][NR], v[HP][NK][NR], vl[kIsHalf<T> ? HP : 1][NK][NR], q[2][NR];   // vl: remainders
   float2 bias[NK];                           // of keys 8 i + 2t, + 1
   auto load_q = [&](int r) {
     load_frag<T, DP>(qp, t, d, r + g < r_end, q[0]);
@@ -424,7 +455,9 @@ __global__ void __launch_bounds__(kXmThreads) xattn_fwd_few_keys(const XAttn arg
 #pragma unroll
       for (int z = 0; z < HP; ++z) {
         k[z][i][c] = HP == 1 || t / 2 == z ? x[c] : 0u;
-        v[z][i][c] = HP == 1 || g / 4 == z ? turned : 0u;
+        uint32_t rest;
+        bf16_terms<T>(HP == 1 || g / 4 == z ? turned : 0u, v[z][i][c], rest);
+        if constexpr (kIsHalf<T>) vl[z][i][c] = rest;
       }
     }
   }
@@ -480,16 +513,18 @@ __global__ void __launch_bounds__(kXmThreads) xattn_fwd_few_keys(const XAttn arg
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float2 p = mul2(s[z][i + x][e], make_float2(inv[e], inv[e]));
-            split2<T>(p.x, p.y, hi[2 * x + e], lo[2 * x + e]);
+            split2<__nv_bfloat16>(p.x, p.y, hi[2 * x + e], lo[2 * x + e]);
           }
 #pragma unroll
         for (int c = 0; c < NR; ++c) {
           if constexpr (NK == 1) {
-            Mma<T>::run8(o[c], hi[0], hi[1], v[z][0][c]);
-            Mma<T>::run8(o[c], lo[0], lo[1], v[z][0][c]);
+            B16::run8(o[c], hi[0], hi[1], v[z][0][c]);
+            B16::run8(o[c], lo[0], lo[1], v[z][0][c]);
+            if constexpr (kIsHalf<T>) B16::run8(o[c], hi[0], hi[1], vl[z][0][c]);
           } else {
-            Mma<T>::run(o[c], hi[0], hi[1], hi[2], hi[3], v[z][i][c], v[z][i + 1][c]);
-            Mma<T>::run(o[c], lo[0], lo[1], lo[2], lo[3], v[z][i][c], v[z][i + 1][c]);
+            B16::run(o[c], hi[0], hi[1], hi[2], hi[3], v[z][i][c], v[z][i + 1][c]);
+            B16::run(o[c], lo[0], lo[1], lo[2], lo[3], v[z][i][c], v[z][i + 1][c]);
+            if constexpr (kIsHalf<T>) B16::run(o[c], hi[0], hi[1], hi[2], hi[3], vl[z][i][c], vl[z][i + 1][c]);
           }
         }
       }
@@ -524,10 +559,6 @@ __global__ void __launch_bounds__(kXmThreads) xattn_fwd_few_keys(const XAttn arg
 // product of the two remainders. P lies in [0, 1] and is scaled by 2^12, so that its fp16
 // remainder keeps digits down to 2^-36.
 // ---------------------------------------------------------------------------
-template <class T>
-constexpr bool kIsHalf = false;
-template <>
-constexpr bool kIsHalf<__half> = true;
 template <class T>
 constexpr float kPScale = kIsHalf<T> ? 4096.f : 1.f;
 

@@ -8,6 +8,8 @@
 //   sums += P Y2, dS Y1                 tcgen05.mma with the first operand in TMEM; the same shared-memory tile now
 //                                       MN-major (its rows are the k axis)
 // P and dS enter as two half terms: of every 16 fp32 columns, the first 8 take the values, the others the remainders.
+// The forward product runs in bf16 for fp16 inputs too (cross_attention_mma.cuh says why): the tile of V becomes two
+// bf16 tiles once the scores are there, its values in place and its remainders over the tile of K, which is then free.
 // The chain load -> mma -> softmax -> mma of a block is serial; 4 (forward: 128 TMEM columns) or 2 (backward: 256)
 // blocks per SM run each other's gaps. Tiles come by cp.async rather than TMA: rows of masked keys and channels past
 // d are zero-filled on the way, and any row stride will do. Where tiles leave the device empty, the other side is
@@ -56,9 +58,10 @@ __device__ __forceinline__ void tc_scores(uint32_t d_tmem, uint32_t a, uint32_t 
     umma_f16_ss(d_tmem, make_smem_desc(a + k / 4 * kTcTile + k % 4 * 32, 16, 1024, kSw128),
                 make_smem_desc(b + k / 4 * kTcHalf + k % 4 * 32, 16, 1024, kSw128), tc_idesc<T>(0), k > 0);
 }
-// D[128 x channels] (+)= P[128 x 64 entries] B[64 entries x channels], P in TMEM as [8 values | 8 remainders] four times
-template <class T, int NP>
-__device__ __forceinline__ void tc_sums(uint32_t d_tmem, uint32_t p_tmem, uint32_t b, bool accumulate) {
+// D[128 x channels] (+)= P[128 x 64 entries] B[64 entries x channels], P in TMEM as [8 values | 8 remainders] four times;
+// TERMS: B's remainders are at b_lo, and their product with the values is added
+template <class T, int NP, bool TERMS = false>
+__device__ __forceinline__ void tc_sums(uint32_t d_tmem, uint32_t p_tmem, uint32_t b, bool accumulate, uint32_t b_lo = 0) {
 #pragma unroll
   for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -66,6 +69,9 @@ __device__ __forceinline__ void tc_sums(uint32_t d_tmem, uint32_t p_tmem, uint32
       const uint64_t desc = make_smem_desc(b + p * kTcHalf + k * 2048, 16, 1024, kSw128);
       umma_f16_ts(d_tmem + 64 * p, p_tmem + k * 16, desc, tc_idesc<T>(1), accumulate || k > 0);
       umma_f16_ts(d_tmem + 64 * p, p_tmem + k * 16 + 8, desc, tc_idesc<T>(1), 1u);
+      if constexpr (TERMS)
+        umma_f16_ts(d_tmem + 64 * p, p_tmem + k * 16, make_smem_desc(b_lo + p * kTcHalf + k * 2048, 16, 1024, kSw128),
+                    tc_idesc<T>(1), 1u);
     }
 }
 
@@ -89,6 +95,26 @@ __device__ __forceinline__ void tc_split(float2 p, uint32_t (&out)[16], int i) {
   out[i] = tc_pack<T>(p.x, p.y);
   const float2 h = tc_unpack<T>(out[i]), r = add2(p, make_float2(-h.x, -h.y));
   out[8 + i] = tc_pack<T>(r.x, r.y);
+}
+// A landed fp16 tile of the other side as bf16 terms: the values in place, the remainders at `lo`, laid out alike.
+template <int NP, int THREADS>
+__device__ __forceinline__ void tc_terms(uint32_t tile, uint32_t lo) {
+  static_assert(kTcHalf % (THREADS * 16) == 0, "every thread has the same number of chunks");
+#pragma unroll
+  for (int i = 0; i < NP * kTcHalf / (THREADS * 16); ++i) {
+    const uint32_t o = (i * THREADS + threadIdx.x) * 16;
+    uint32_t h[4], l[4];
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(tile + o) : "memory");
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = tc_unpack<__half>(h[e]);
+      h[e] = pack_bf16x2(f.x, f.y);
+      const float2 v = tc_unpack<__nv_bfloat16>(h[e]), r = add2(f, make_float2(-v.x, -v.y));
+      l[e] = pack_bf16x2(r.x, r.y);
+    }
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(tile + o), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(lo + o), "r"(l[0]), "r"(l[1]), "r"(l[2]), "r"(l[3]) : "memory");
+  }
 }
 __device__ __forceinline__ float4 ld_dsmem4(uint32_t cluster_addr) {
   float4 v;
@@ -185,6 +211,7 @@ template <class T, int NP>
 __global__ void __launch_bounds__(kTcThreads, 4 / NP) xattn_tc_fwd_kernel(const XAttn args) {
   const XAttn a = follow(args, true);
   constexpr int kTile = NP * kTcTile, kHalfStage = NP * kTcHalf, kStage = 2 * kHalfStage, kCols = 128 * NP;
+  constexpr bool kTerms = std::is_same<T, __half>::value;
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) uint64_t bars[2];
   __shared__ uint32_t holder;
@@ -238,6 +265,7 @@ __global__ void __launch_bounds__(kTcThreads, 4 / NP) xattn_tc_fwd_kernel(const 
     ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars[0], it & 1));
     tc_fence_after();
     if (ok) {
+      if constexpr (kTerms) tc_terms<NP, kTcThreads>(y + kHalfStage, y);
       float2 s[32];
       tc_read64(B.t_lane + tS, s);
       const bool plain = mask == nullptr && (j + 1) * kTcOther <= keys;
@@ -276,7 +304,7 @@ __global__ void __launch_bounds__(kTcThreads, 4 / NP) xattn_tc_fwd_kernel(const 
           float2 p = add2(s[8 * q + i], m2);
           p.x = ex2f(p.x), p.y = ex2f(p.y);
           l2 = add2(l2, p);
-          tc_split<T>(p, out, i);
+          tc_split<__nv_bfloat16>(p, out, i);
         }
         tmem_st_32x32b_x16(B.t_lane + tS + 16 * q, out);
       }
@@ -286,7 +314,7 @@ __global__ void __launch_bounds__(kTcThreads, 4 / NP) xattn_tc_fwd_kernel(const 
     if (!ok) break;
     if (tid == 0) {
       tc_fence_after();
-      tc_sums<T, NP>(B.tmem + tO, B.tmem + tS, y + kHalfStage, it > 0);
+      tc_sums<__nv_bfloat16, NP, kTerms>(B.tmem + tO, B.tmem + tS, y + kHalfStage, it > 0, y);
       umma_commit(&bars[1]);
     }
   }

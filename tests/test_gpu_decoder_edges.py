@@ -1,0 +1,42 @@
+"""Calls of the decoder's operators that random inputs do not make: weights far below the largest one, values that are
+not finite beside ones that are, logits at the end of fp32. Bounds as derived in test_gpu_cross_attention.py and
+test_gpu_norms.py; where something else is allowed, the test says why."""
+import math
+
+import pytest
+import torch
+from test_gpu_cross_attention import DTYPES, NOISE, check, make, reference, run, there
+
+from sparsesam_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+
+def ids(s):
+    return "x".join(map(str, s))
+
+
+# B, Tq, Tk, H, Hk, D of every forward kernel of the half types: few rows (one head and two per fragment, three and four
+# tiles of rows, two per row of a group), few keys (the same), tcgen05 (one and two panels of channels; split and whole)
+FORWARD = [(1, 3, 4096, 2, 2, 16), (40, 8, 600, 8, 8, 16), (40, 12, 300, 8, 8, 16), (1, 20, 700, 2, 2, 64), (2, 3, 900, 4, 2, 32),
+           (1, 5, 300, 1, 1, 128), (2, 70, 64, 1, 1, 16), (3, 50, 8, 2, 2, 16), (3, 50, 15, 2, 2, 16), (1, 40, 30, 2, 1, 64),
+           (1, 200, 1000, 2, 1, 64), (1, 130, 900, 2, 2, 128), (8, 128, 128, 8, 8, 64), (1, 70, 100, 1, 1, 24)]
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("far", [17.0, 19.5, 21.75])
+@pytest.mark.parametrize("shape", FORWARD, ids=ids)
+def test_weights_far_below_the_largest(cuda_device, shape, far, dtype):
+    """One key has nearly all the weight and a value of zero: the result is what the others' weights of e^-far (2^-24 to
+    2^-31) carry, and has the digits of its own type."""
+    B, Tq, Tk, H, Hk, D = shape
+    q, k, v, _ = make(cuda_device, *shape, dtype, seed=21)
+    q[..., 0], k[..., 0] = 1.0, 0.0
+    q[..., 1:], k[..., 1:] = q[..., 1:] / 16, k[..., 1:] / 16     # the other logits differ a little
+    sink = Tk // 2
+    k[:, sink] = 0.0
+    k[:, sink, :, 0] = far
+    v = v.abs() * 512 + 512
+    v[:, sink] = 0.0
+    got = run(q, k, v, scale=1.0)
+    check(got, reference(q, k, v, scale=1.0), dtype)
