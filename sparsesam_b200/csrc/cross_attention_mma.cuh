@@ -553,15 +553,10 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NK, 2>) xattn_f
 }
 
 // ---------------------------------------------------------------------------
-// Backward. With p = 2^(c s - lse) and ds = p (dp - D), fp16 needs care: dS has no fixed
-// scale (it follows the loss), so its products run in bf16, which has fp32's range: dS as
-// two bf16 terms, the fp16 factor as two bf16 terms (exact, 11 = 8 + 3 bits), without the
-// product of the two remainders. P lies in [0, 1] and is scaled by 2^12, so that its fp16
-// remainder keeps digits down to 2^-36.
+// Backward. With p = 2^(c s - lse) and ds = p (dp - D): for fp16 the products of p and of dS run in
+// bf16 as well (dS follows the loss and p the logits, neither stays within fp16's exponents): two bf16
+// terms each, and the fp16 factor as two bf16 terms.
 // ---------------------------------------------------------------------------
-template <class T>
-constexpr float kPScale = kIsHalf<T> ? 4096.f : 1.f;
-
 // Turned blocks of N fragments of 8 tokens (tokens become the k axis), as bf16 for the dS products
 template <class T, int N, int NR>
 struct Turned {
@@ -622,7 +617,6 @@ template <class T, int DP, int NF, bool FEW_ROWS>
 __global__ void __launch_bounds__(kXmThreads) xattn_bwd_few(const XAttn args, int) {
   const XAttn a = follow(args, false);
   constexpr int NR = DP / 8, NU = NR / 2;
-  constexpr float kP = kPScale<T>;
   using B16 = Mma<__nv_bfloat16>;
   extern __shared__ __align__(16) float xsm[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
@@ -753,12 +747,12 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_few(const XAttn args, in
     }
     Turned<T, 2, NR> x1t;
     x1t.make(x1);
-    uint32_t x2t[2][FEW_ROWS ? 1 : NR];
+    uint32_t x2t[2][FEW_ROWS ? 1 : NR], x2l[2][FEW_ROWS ? 1 : NR];
     if constexpr (!FEW_ROWS) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int c = 0; c < NR; ++c) x2t[h][c] = movm(x2[h][c]);
+        for (int c = 0; c < NR; ++c) bf16_terms<T>(movm(x2[h][c]), x2t[h][c], x2l[h][c]);
     }
     if (i0 + 16 < end) load_long(i0 + 16);   // the next step's, under this one's arithmetic
     float e1[NR][4], e2[FEW_ROWS ? NR : 1][4];
@@ -801,27 +795,34 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_few(const XAttn args, in
       }
 #pragma unroll
       for (int x = 0; x < PAIR; ++x) {
-        split2<T>(p[i + x][0] * kP, p[i + x][1] * kP, hi[2 * x], lo[2 * x]);
-        split2<T>(p[i + x][2] * kP, p[i + x][3] * kP, hi[2 * x + 1], lo[2 * x + 1]);
+        split2<__nv_bfloat16>(p[i + x][0], p[i + x][1], hi[2 * x], lo[2 * x]);
+        split2<__nv_bfloat16>(p[i + x][2], p[i + x][3], hi[2 * x + 1], lo[2 * x + 1]);
         if constexpr (!FEW_ROWS) {
           const uint32_t h0 = movm(hi[2 * x]), h1 = movm(hi[2 * x + 1]), l0 = movm(lo[2 * x]), l1 = movm(lo[2 * x + 1]);
 #pragma unroll
           for (int u = 0; u < NU; ++u) {
             float(&c)[4] = acc2[i + x][u];
-            Mma<T>::run(c, x2t[0][2 * u], x2t[0][2 * u + 1], x2t[1][2 * u], x2t[1][2 * u + 1], h0, h1);
-            Mma<T>::run(c, x2t[0][2 * u], x2t[0][2 * u + 1], x2t[1][2 * u], x2t[1][2 * u + 1], l0, l1);
+            B16::run(c, x2t[0][2 * u], x2t[0][2 * u + 1], x2t[1][2 * u], x2t[1][2 * u + 1], h0, h1);
+            B16::run(c, x2t[0][2 * u], x2t[0][2 * u + 1], x2t[1][2 * u], x2t[1][2 * u + 1], l0, l1);
+            if constexpr (kIsHalf<T>)
+              B16::run(c, x2l[0][2 * u], x2l[0][2 * u + 1], x2l[1][2 * u], x2l[1][2 * u + 1], h0, h1);
           }
         }
       }
       if constexpr (FEW_ROWS) {
 #pragma unroll
         for (int c = 0; c < NR; ++c) {
+          uint32_t yh[2], yl[2];               // terms made here: kept, they would take the registers that are left
+#pragma unroll
+          for (int x = 0; x < PAIR; ++x) bf16_terms<T>(y2t[i + x][c], yh[x], yl[x]);
           if constexpr (PAIR == 2) {
-            Mma<T>::run(e2[c], hi[0], hi[1], hi[2], hi[3], y2t[i][c], y2t[i + 1][c]);
-            Mma<T>::run(e2[c], lo[0], lo[1], lo[2], lo[3], y2t[i][c], y2t[i + 1][c]);
+            B16::run(e2[c], hi[0], hi[1], hi[2], hi[3], yh[0], yh[1]);
+            B16::run(e2[c], lo[0], lo[1], lo[2], lo[3], yh[0], yh[1]);
+            if constexpr (kIsHalf<T>) B16::run(e2[c], hi[0], hi[1], hi[2], hi[3], yl[0], yl[1]);
           } else {
-            Mma<T>::run8(e2[c], hi[0], hi[1], y2t[0][c]);
-            Mma<T>::run8(e2[c], lo[0], lo[1], y2t[0][c]);
+            B16::run8(e2[c], hi[0], hi[1], yh[0]);
+            B16::run8(e2[c], lo[0], lo[1], yh[0]);
+            if constexpr (kIsHalf<T>) B16::run8(e2[c], hi[0], hi[1], yl[0]);
           }
         }
       }
@@ -838,7 +839,7 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_few(const XAttn args, in
           const int64_t to = ((static_cast<int64_t>(b) * a.Tk + i) * a.kv_heads + n) * a.d;
           store_frag<T, DP>(static_cast<T*>(a.dk) + to, t, a.d, y);
 #pragma unroll
-          for (int c = 0; c < NR; ++c) y[c] = Mma<T>::pack(e2[c][2 * h] * (1.f / kP), e2[c][2 * h + 1] * (1.f / kP));
+          for (int c = 0; c < NR; ++c) y[c] = Mma<T>::pack(e2[c][2 * h], e2[c][2 * h + 1]);
           store_frag<T, DP>(static_cast<T*>(a.dv) + to, t, a.d, y);
         }
       } else if (a.dq != nullptr) {
@@ -872,7 +873,7 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_few(const XAttn args, in
     T* to = static_cast<T*>(FEW_ROWS ? a.dq : second ? a.dv : a.dk);
     if (f < (FEW_ROWS ? rows : a.Tk) && ch < a.d && to != nullptr) {
       const int64_t at = FEW_ROWS ? row_dense(a, b, n, f) : ((static_cast<int64_t>(b) * a.Tk + f) * a.kv_heads + n) * a.d;
-      store1(to + at + ch, x * (second ? 1.f / kP : a.scale));
+      store1(to + at + ch, second ? x : x * a.scale);
     }
   }
   if (cl > 1) cluster_sync_all();

@@ -8,8 +8,9 @@
 //   sums += P Y2, dS Y1                 tcgen05.mma with the first operand in TMEM; the same shared-memory tile now
 //                                       MN-major (its rows are the k axis)
 // P and dS enter as two half terms: of every 16 fp32 columns, the first 8 take the values, the others the remainders.
-// The forward product runs in bf16 for fp16 inputs too (cross_attention_mma.cuh says why): the tile of V becomes two
-// bf16 tiles once the scores are there, its values in place and its remainders over the tile of K, which is then free.
+// These products run in bf16 for fp16 inputs too (cross_attention_mma.cuh says why): the other side's tile becomes two
+// bf16 tiles once the scores are there, its values in place and its remainders over a tile that is free by then (V's over
+// K, K's over V) or, in the keys' kernel, which needs both its tiles, behind the ring.
 // The chain load -> mma -> softmax -> mma of a block is serial; 4 (forward: 128 TMEM columns) or 2 (backward: 256)
 // blocks per SM run each other's gaps. Tiles come by cp.async rather than TMA: rows of masked keys and channels past
 // d are zero-filled on the way, and any row stride will do. Where tiles leave the device empty, the other side is
@@ -58,20 +59,20 @@ __device__ __forceinline__ void tc_scores(uint32_t d_tmem, uint32_t a, uint32_t 
     umma_f16_ss(d_tmem, make_smem_desc(a + k / 4 * kTcTile + k % 4 * 32, 16, 1024, kSw128),
                 make_smem_desc(b + k / 4 * kTcHalf + k % 4 * 32, 16, 1024, kSw128), tc_idesc<T>(0), k > 0);
 }
-// D[128 x channels] (+)= P[128 x 64 entries] B[64 entries x channels], P in TMEM as [8 values | 8 remainders] four times;
-// TERMS: B's remainders are at b_lo, and their product with the values is added
-template <class T, int NP, bool TERMS = false>
-__device__ __forceinline__ void tc_sums(uint32_t d_tmem, uint32_t p_tmem, uint32_t b, bool accumulate, uint32_t b_lo = 0) {
+// D[128 x channels] (+)= P[128 x 64 entries] B[64 entries x channels] in bf16, P in TMEM as [8 values | 8 remainders] four
+// times; TERMS: B's remainders are at b_lo, and their product with P's values is added
+template <int NP, bool TERMS>
+__device__ __forceinline__ void tc_sums(uint32_t d_tmem, uint32_t p_tmem, uint32_t b, uint32_t b_lo, bool accumulate) {
 #pragma unroll
   for (int k = 0; k < 4; ++k)
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
       const uint64_t desc = make_smem_desc(b + p * kTcHalf + k * 2048, 16, 1024, kSw128);
-      umma_f16_ts(d_tmem + 64 * p, p_tmem + k * 16, desc, tc_idesc<T>(1), accumulate || k > 0);
-      umma_f16_ts(d_tmem + 64 * p, p_tmem + k * 16 + 8, desc, tc_idesc<T>(1), 1u);
+      umma_f16_ts(d_tmem + 64 * p, p_tmem + k * 16, desc, tc_idesc<__nv_bfloat16>(1), accumulate || k > 0);
+      umma_f16_ts(d_tmem + 64 * p, p_tmem + k * 16 + 8, desc, tc_idesc<__nv_bfloat16>(1), 1u);
       if constexpr (TERMS)
         umma_f16_ts(d_tmem + 64 * p, p_tmem + k * 16, make_smem_desc(b_lo + p * kTcHalf + k * 2048, 16, 1024, kSw128),
-                    tc_idesc<T>(1), 1u);
+                    tc_idesc<__nv_bfloat16>(1), 1u);
     }
 }
 
@@ -90,11 +91,10 @@ __device__ __forceinline__ float2 tc_unpack(uint32_t u) {
   return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
 }
 // value pair i of 16 columns -> out[i] (values), out[8 + i] (remainders)
-template <class T>
 __device__ __forceinline__ void tc_split(float2 p, uint32_t (&out)[16], int i) {
-  out[i] = tc_pack<T>(p.x, p.y);
-  const float2 h = tc_unpack<T>(out[i]), r = add2(p, make_float2(-h.x, -h.y));
-  out[8 + i] = tc_pack<T>(r.x, r.y);
+  out[i] = pack_bf16x2(p.x, p.y);
+  const float2 h = tc_unpack<__nv_bfloat16>(out[i]), r = add2(p, make_float2(-h.x, -h.y));
+  out[8 + i] = pack_bf16x2(r.x, r.y);
 }
 // A landed fp16 tile of the other side as bf16 terms: the values in place, the remainders at `lo`, laid out alike.
 template <int NP, int THREADS>
@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(kTcThreads, 4 / NP) xattn_tc_fwd_kernel(const 
           float2 p = add2(s[8 * q + i], m2);
           p.x = ex2f(p.x), p.y = ex2f(p.y);
           l2 = add2(l2, p);
-          tc_split<__nv_bfloat16>(p, out, i);
+          tc_split(p, out, i);
         }
         tmem_st_32x32b_x16(B.t_lane + tS + 16 * q, out);
       }
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(kTcThreads, 4 / NP) xattn_tc_fwd_kernel(const 
     if (!ok) break;
     if (tid == 0) {
       tc_fence_after();
-      tc_sums<__nv_bfloat16, NP, kTerms>(B.tmem + tO, B.tmem + tS, y + kHalfStage, it > 0, y);
+      tc_sums<NP, kTerms>(B.tmem + tO, B.tmem + tS, y + kHalfStage, y, it > 0);
       umma_commit(&bars[1]);
     }
   }
@@ -391,24 +391,19 @@ __global__ void __launch_bounds__(kTcThreads, 4 / NP) xattn_tc_fwd_kernel(const 
 // OWN_ROWS: a tile of queries, x = q, dout, over keys, y = k, v: dq += dS k, and D is left for the keys' kernel.
 // Else a tile of keys, x = k, v, over the queries of its heads, y = q, dout: dk += dS q, dv += P dout.
 // Two threads share an entry, 32 columns each (warps w and w + 4 reach the same TMEM lanes).
-//
-// fp16 holds 2^-24 to 2^16: P enters times 2^12 (P <= 1 and the remainder then reach 2^-37), dS times a power of two
-// of its own entry, which brings the largest |dS| seen so far to 2^8 .. 2^15. When it would pass 2^15 the power is
-// renewed and the sums follow, which is exact. bf16 has the exponents of fp32 and needs neither.
 constexpr int kTcBwdThreads = 256;
-constexpr float kTcPScale = 4096.f;
 
 template <class T, int NP, bool OWN_ROWS>
 __global__ void __launch_bounds__(kTcBwdThreads, 2 / NP) xattn_tc_bwd_kernel(const XAttn args) {
   const XAttn a = follow(args, true);
-  constexpr bool kScaled = std::is_same<T, __half>::value;
+  constexpr bool kTerms = std::is_same<T, __half>::value;
   constexpr int kTile = NP * kTcTile, kHalfStage = NP * kTcHalf, kStage = 2 * kHalfStage;
   constexpr int kCols = NP == 1 || OWN_ROWS ? 256 : 512;
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) uint64_t bars[2];
   __shared__ uint32_t holder;
   __shared__ __align__(16) float s_a[2][kTcOther], s_b[2][kTcOther];   // of the other side: bias; or -lse and -D
-  __shared__ float s_top[kScaled ? kTcBwdThreads : 1], s_d[OWN_ROWS ? kTcOwn : 1];
+  __shared__ float s_d[OWN_ROWS ? kTcOwn : 1];
   TcBlock B;
   B.open(raw, bars, &holder, kCols);
   const uint32_t x1 = B.sm, x2 = B.sm + kTile, ring = B.sm + 2 * kTile, tS = 0, tD = 64, tA1 = 128, tA2 = 128 + 64 * NP;
@@ -490,7 +485,6 @@ __global__ void __launch_bounds__(kTcBwdThreads, 2 / NP) xattn_tc_bwd_kernel(con
   bool ok = tc_landed(true);
   const float own_d = OWN_ROWS ? -s_d[lane_id] : 0.f;
   const float2 c2 = make_float2(a.c, a.c), os2 = make_float2(own_s, own_s), od2 = make_float2(own_d, own_d);
-  int up = 253;                              // exponent field of the power of two on dS: 2^126 until one is seen
   int it = 0;
   for (int j = j_begin; j < j_end; ++j, ++it) {
     const int buf = it & 1;
@@ -505,75 +499,30 @@ __global__ void __launch_bounds__(kTcBwdThreads, 2 / NP) xattn_tc_bwd_kernel(con
     request(j + 1, buf ^ 1);
     ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars[0], it & 1));
     tc_fence_after();
-    // P and dS of columns 16 q .. 16 q + 15
-    auto values = [&](int q, float2 (&p)[8], float2 (&ds)[8]) {
-      uint32_t rs[16], rd[16];
-      tmem_ld_32x32b_x16(B.t_lane + tS + 16 * q, rs);
-      tmem_ld_32x32b_x16(B.t_lane + tD + 16 * q, rd);
-      tmem_ld_wait();
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2 sa = *reinterpret_cast<const float2*>(&s_a[buf][16 * q + 2 * i]);
-        p[i] = fma2(make_float2(__uint_as_float(rs[2 * i]), __uint_as_float(rs[2 * i + 1])), c2, OWN_ROWS ? sa : os2);
-        p[i] = add2(p[i], OWN_ROWS ? os2 : sa);
-        p[i].x = ex2f(p[i].x), p[i].y = ex2f(p[i].y);
-        const float2 dd = OWN_ROWS ? od2 : *reinterpret_cast<const float2*>(&s_b[buf][16 * q + 2 * i]);
-        ds[i] = mul2(p[i], add2(make_float2(__uint_as_float(rd[2 * i]), __uint_as_float(rd[2 * i + 1])), dd));
+    const uint32_t y_lo = OWN_ROWS ? y2 : ring + 2 * kStage, y2_lo = y_lo + kHalfStage;
+    if (ok) {
+      if constexpr (kTerms) {
+        tc_terms<NP, kTcBwdThreads>(y, y_lo);
+        if constexpr (!OWN_ROWS) tc_terms<NP, kTcBwdThreads>(y2, y2_lo);
       }
-    };
-    auto leave = [&](int q, const float2 (&p)[8], const float2 (&ds)[8], float f) {
-      uint32_t ps[16], pd[16];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        tc_split<T>(kScaled ? mul2(ds[i], make_float2(f, f)) : ds[i], pd, i);
-        if constexpr (!OWN_ROWS) tc_split<T>(kScaled ? mul2(p[i], make_float2(kTcPScale, kTcPScale)) : p[i], ps, i);
-      }
-      tmem_st_32x32b_x16(B.t_lane + tD + 16 * q, pd);
-      if constexpr (!OWN_ROWS) tmem_st_32x32b_x16(B.t_lane + tS + 16 * q, ps);
-    };
-    if constexpr (kScaled) {
-      float2 p[2][8], ds[2][8];
-      float top = 0.f;
-      if (ok) {
+      for (int q = 2 * half; q < 2 * half + 2; ++q) {          // columns 16 q .. 16 q + 15
+        uint32_t rs[16], rd[16], ps[16], pd[16];
+        tmem_ld_32x32b_x16(B.t_lane + tS + 16 * q, rs);
+        tmem_ld_32x32b_x16(B.t_lane + tD + 16 * q, rd);
+        tmem_ld_wait();
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          values(2 * half + q, p[q], ds[q]);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) top = fmaxf(top, fmaxf(fabsf(ds[q][i].x), fabsf(ds[q][i].y)));
+        for (int i = 0; i < 8; ++i) {
+          const float2 sa = *reinterpret_cast<const float2*>(&s_a[buf][16 * q + 2 * i]);
+          float2 p = fma2(make_float2(__uint_as_float(rs[2 * i]), __uint_as_float(rs[2 * i + 1])), c2, OWN_ROWS ? sa : os2);
+          p = add2(p, OWN_ROWS ? os2 : sa);
+          p.x = ex2f(p.x), p.y = ex2f(p.y);
+          const float2 dd = OWN_ROWS ? od2 : *reinterpret_cast<const float2*>(&s_b[buf][16 * q + 2 * i]);
+          tc_split(mul2(p, add2(make_float2(__uint_as_float(rd[2 * i]), __uint_as_float(rd[2 * i + 1])), dd)), pd, i);
+          if constexpr (!OWN_ROWS) tc_split(p, ps, i);
         }
-      }
-      s_top[tid] = top;
-      __syncthreads();
-      if (ok) {
-        const int e = static_cast<int>(__float_as_uint(fmaxf(top, s_top[tid ^ kTcOwn])) >> 23);   // 2^(e - 127) or more
-        const bool renew = e + up > 2 * 127 + 14;
-        if (__any_sync(0xffffffffu, renew)) {
-          const int next = renew ? min(253, 2 * 127 + 8 - e) : up;
-          const float f = next - up < -126 ? 0.f : __uint_as_float(static_cast<uint32_t>(next - up + 127) << 23);
-          up = next;
-          if (it > 0) {
-#pragma unroll
-            for (int i0 = 0; i0 < 32 * NP; i0 += 16) {
-              uint32_t o[16];
-              tmem_ld_32x32b_x16(B.t_lane + tA1 + 32 * NP * half + i0, o);
-              tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-              tmem_st_32x32b_x16(B.t_lane + tA1 + 32 * NP * half + i0, o);
-            }
-          }
-        }
-        const float f = __uint_as_float(static_cast<uint32_t>(up) << 23);
-#pragma unroll
-        for (int q = 0; q < 2; ++q) leave(2 * half + q, p[q], ds[q], f);
-        tmem_st_wait();
-      }
-    } else if (ok) {
-#pragma unroll
-      for (int q = 2 * half; q < 2 * half + 2; ++q) {
-        float2 p[8], ds[8];
-        values(q, p, ds);
-        leave(q, p, ds, 1.f);
+        tmem_st_32x32b_x16(B.t_lane + tD + 16 * q, pd);
+        if constexpr (!OWN_ROWS) tmem_st_32x32b_x16(B.t_lane + tS + 16 * q, ps);
       }
       tmem_st_wait();
     }
@@ -581,8 +530,8 @@ __global__ void __launch_bounds__(kTcBwdThreads, 2 / NP) xattn_tc_bwd_kernel(con
     if (!ok) break;
     if (tid == 0) {
       tc_fence_after();
-      tc_sums<T, NP>(B.tmem + tA1, B.tmem + tD, y, it > 0);
-      if constexpr (!OWN_ROWS) tc_sums<T, NP>(B.tmem + tA2, B.tmem + tS, y2, it > 0);
+      tc_sums<NP, kTerms>(B.tmem + tA1, B.tmem + tD, y, y_lo, it > 0);
+      if constexpr (!OWN_ROWS) tc_sums<NP, kTerms>(B.tmem + tA2, B.tmem + tS, y2, y2_lo, it > 0);
       umma_commit(&bars[1]);
     }
   }
@@ -602,11 +551,10 @@ __global__ void __launch_bounds__(kTcBwdThreads, 2 / NP) xattn_tc_bwd_kernel(con
     cp_async_wait_all();
     __syncthreads();
   }
-  const float down = kScaled ? __uint_as_float(static_cast<uint32_t>(254 - up) << 23) : 1.f;
 #pragma unroll
   for (int k = 0; k < (OWN_ROWS ? 1 : 2); ++k) {
     void* to = OWN_ROWS ? a.dq : k == 0 ? a.dk : a.dv;
-    const float f = k == 0 ? down * a.scale : kScaled ? 1.f / kTcPScale : 1.f;
+    const float f = k == 0 ? a.scale : 1.f;
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
       float2 v[16];                          // channels 64 p + 32 half ..
@@ -678,10 +626,11 @@ template <class T, int NP>
 static int xattn_tc_bwd_t(const XAttn& a, cudaStream_t stream) {
   static PerDeviceOnce by_rows, by_keys;
   constexpr int smem = NP * (2 * kTcTile + 4 * kTcHalf) + 1024;
+  constexpr int smem_keys = smem + (std::is_same<T, __half>::value ? NP * 2 * kTcHalf : 0);   // the two tiles of remainders
   const int rows = a.group * a.Tq;
   const int st = xattn_tc_launch(xattn_tc_bwd_kernel<T, NP, true>, by_rows, a, rows, a.Tk, kTcBwdThreads, 2 / NP, smem, stream);
   if (st != SSAM_OK || a.dk == nullptr) return st;
-  return xattn_tc_launch(xattn_tc_bwd_kernel<T, NP, false>, by_keys, a, a.Tk, rows, kTcBwdThreads, 2 / NP, smem, stream);
+  return xattn_tc_launch(xattn_tc_bwd_kernel<T, NP, false>, by_keys, a, a.Tk, rows, kTcBwdThreads, 2 / NP, smem_keys, stream);
 }
 int xattn_tc(const XAttn& a, int dtype, bool backward, cudaStream_t stream) {
   if (backward) {

@@ -40,3 +40,22 @@ def test_weights_far_below_the_largest(cuda_device, shape, far, dtype):
     v[:, sink] = 0.0
     got = run(q, k, v, scale=1.0)
     check(got, reference(q, k, v, scale=1.0), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("far", [19.5, 23.0])
+@pytest.mark.parametrize("shape", FORWARD, ids=ids)
+def test_gradients_of_weights_far_below_the_largest(cuda_device, shape, far, dtype):
+    """Keys of small weight (2^-28, 2^-33) below a large incoming gradient, and channels that only they reach: dq of those
+    channels, dk and dv of those keys keep the digits of the type."""
+    B, Tq, Tk, H, Hk, D = shape
+    q, k, v, do = make(cuda_device, *shape, dtype, seed=22)
+    q[..., 0], k[..., 0] = 1.0, 0.0
+    q[..., 1:], k[..., 1:] = q[..., 1:] / 16, k[..., 1:] / 16
+    near = min(3, Tk // 2)
+    k[:, :near] = 0.0
+    k[:, :near, :, 0] = far                                        # the near keys share the weight
+    v = v / 16                                                     # keeps dk below fp16's 65504
+    do = do.abs() * 256 + 256
+    got = run(q, k, v, do, scale=1.0)
+    check(got, reference(q, k, v, do, scale=1.0), dtype)
