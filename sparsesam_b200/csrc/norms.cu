@@ -29,24 +29,27 @@ enum { kActNone = 0, kActRelu = 1, kActGelu = 2, kActSilu = 3 };
 // division: a thousandth of the output's rounding, and 2 to 3 times fewer instructions,
 // which is what bounded these kernels (GELU apply of 16 x 256 x 256 x 64: 108 us exact).
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
-// 1 / (1 + p u) of a pair from one reciprocal of the product (both factors are at least 1): the
+// 1 / (1 + p u) of a pair from one reciprocal of the product (both factors are 1 to 6.3, see erf_terms2): the
 // reciprocals and exponentials (MUFU, a quarter of the FMA rate) are what GELU waits for.
 __device__ __forceinline__ float2 erf_t2(float2 u) {
   const float2 d = fma2(both(0.3275911f), u, both(1.0f));
   const float r = rcp_fast(d.x * d.y);
   return mul2(both(r), make_float2(d.y, d.x));
 }
-// h = q / 2 of 7.1.26 without its exponential, e = exp(-u^2)
+// h = q / 2 of 7.1.26 without its exponential, e = exp(-u^2). u goes no further than 16, where e is 0 (2^-369): what
+// meets e stays finite, and of two channels one that is not finite leaves the other's reciprocal alone (NaN comes
+// through e, from the u that was not cut).
 __device__ __forceinline__ void erf_terms2(float2 z, float2& u, float2& h, float2& e) {
   u = mul2(make_float2(fabsf(z.x), fabsf(z.y)), both(0.70710678118654752440f));
+  const float2 arg = mul2(mul2(u, u), both(-1.4426950408889634f));
+  e = make_float2(ex2f(arg.x), ex2f(arg.y));
+  u = make_float2(fminf(u.x, 16.f), fminf(u.y, 16.f));
   const float2 t = erf_t2(u);
   h = fma2(both(0.5307027145f), t, both(-0.7265760135f));
   h = fma2(h, t, both(0.7107068705f));
   h = fma2(h, t, both(-0.142248368f));
   h = fma2(h, t, both(0.127414796f));
   h = mul2(h, t);
-  const float2 arg = mul2(mul2(u, u), both(-1.4426950408889634f));
-  e = make_float2(ex2f(arg.x), ex2f(arg.y));
 }
 // GELU(z) = max(z, 0) - |z| h e
 __device__ __forceinline__ float2 gelu2(float2 z) {
