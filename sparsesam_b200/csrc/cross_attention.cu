@@ -168,7 +168,8 @@ __device__ __forceinline__ void put_row(float* p, const float2 (&r)[DT / 2], flo
 
 // What the two row kernels share: a block's place, and the walk over its keys. body(tile of K, tile of V, keys of
 // the tile rounded up to the slices, their biases: 0, or -infinity where there is no key) is called with the tile in
-// shared memory.
+// shared memory. False: every key that the block walked is masked, and its sums are to be left out (those of a query
+// that is not finite are not 0).
 struct XPlace {
   int part, lr, slice, KS, b, n, cl, rank, rows, r0, r, t, h;
   bool row_ok;
@@ -190,12 +191,13 @@ struct XPlace {
   }
 };
 template <int DP, class B>
-__device__ __forceinline__ void walk_keys(const XAttn& a, const XPlace& x, float* xsm, float (&bias)[2][kXTile<DP>], B body) {
+__device__ __forceinline__ bool walk_keys(const XAttn& a, const XPlace& x, float* xsm, float (&bias)[2][kXTile<DP>], B body) {
   constexpr int XT = kXTile<DP>, LD = DP + 4;
   const int keys = xattn_keys(a, x.b);
   const float* kb = static_cast<const float*>(a.k) + x.b * a.ks[0] + x.n * a.ks[2];
   const float* vb = static_cast<const float*>(a.v) + x.b * a.vs[0] + x.n * a.vs[2];
   const uint8_t* mask = a.key_mask == nullptr ? nullptr : a.key_mask + static_cast<int64_t>(x.b) * a.Tk;
+  bool some = false;
   auto stage = [&](int j0, int buf) {
     if (j0 < keys) {
       const int nk = min(XT, keys - j0), upto = (nk + x.KS - 1) / x.KS * x.KS;
@@ -203,7 +205,11 @@ __device__ __forceinline__ void walk_keys(const XAttn& a, const XPlace& x, float
       float* to = xsm + buf * 2 * XT * LD;
       stage_rows<DP>(to, nk, upto, a.d, [&](int i) { return kb + (j0 + i) * a.ks[1]; }, ok);
       stage_rows<DP>(to + XT * LD, nk, upto, a.d, [&](int i) { return vb + (j0 + i) * a.vs[1]; }, ok);
-      if (threadIdx.x < XT) bias[buf][threadIdx.x] = threadIdx.x < nk && ok(threadIdx.x) ? 0.f : -INFINITY;
+      if (threadIdx.x < XT) {
+        const bool there = threadIdx.x < nk && ok(threadIdx.x);
+        bias[buf][threadIdx.x] = there ? 0.f : -INFINITY;
+        some |= there;
+      }
     }
     stage_commit();
   };
@@ -217,6 +223,7 @@ __device__ __forceinline__ void walk_keys(const XAttn& a, const XPlace& x, float
     body(sk, sk + XT * LD, (min(XT, keys - j0) + x.KS - 1) / x.KS * x.KS, bias[buf]);
     __syncthreads();                         // the other buffer is filled next
   }
+  return mask == nullptr || __syncthreads_or(some);
 }
 
 // Joins the slices' and blocks' shares of the rows.
@@ -293,8 +300,10 @@ __device__ __forceinline__ void xattn_fwd_join(const XAttn& a, const XPlace& x, 
 // NR rows to a thread, RB apart: K and V come out of shared memory once for all of them, which is what the kernel waits
 // for (1024 x 1024, 16 x 8 heads of 16: 400 us with one row, 340 with two, of 64: 2040 and 1400; 4096 queries on 8
 // keys, 64 x 8 heads of 16: 128 and 106, at 2.5 TB/s). NR > 1: one slice, no cluster.
+// (The bounds are the blocks that fit anyway: 168 registers for NR 2, DT 32. Left to itself the compiler once took 196,
+// and 4096 x 30 of 32 channels 113 us instead of 97.)
 template <int DT, int TPR, int NR>
-__global__ void __launch_bounds__(kXThreads) xattn_fwd_scalar(const XAttn args, int RB) {
+__global__ void __launch_bounds__(kXThreads, DT == 16 ? (NR == 1 ? 7 : 4) : (NR == 1 ? 4 : 3)) xattn_fwd_scalar(const XAttn args, int RB) {
   const XAttn a = follow(args, false);
   constexpr int DP = DT * TPR, LD = DP + 4, U = 4;
   extern __shared__ __align__(16) float xsm[];
@@ -314,7 +323,7 @@ __global__ void __launch_bounds__(kXThreads) xattn_fwd_scalar(const XAttn args, 
     m[z] = -INFINITY, l[z] = 0.f;
   }
   __syncthreads();
-  walk_keys<DP>(a, x, xsm, bias, [&](const float* sk, const float* sv, int nk, const float* here) {
+  const bool some = walk_keys<DP>(a, x, xsm, bias, [&](const float* sk, const float* sv, int nk, const float* here) {
     for (int j = slice; j < nk; j += U * KS) {           // U keys at a time: one look at the maximum
       float s[NR][U], top[NR];
 #pragma unroll
@@ -355,6 +364,10 @@ __global__ void __launch_bounds__(kXThreads) xattn_fwd_scalar(const XAttn args, 
       }
     }
   });
+  if (!some) {
+#pragma unroll
+    for (int z = 0; z < NR; ++z) clear_row<DT>(o[z]), m[z] = -INFINITY, l[z] = 0.f;
+  }
   if (NR > 1 || (KS == 1 && cl == 1)) {      // a row is one group of TPR threads: out through shared memory, as it came
 #pragma unroll
     for (int z = 0; z < NR; ++z) {
@@ -411,7 +424,7 @@ __global__ void __launch_bounds__(kXThreads) xattn_dq_scalar(const XAttn args, i
   if (x.row_ok && part == 0 && slice == 0 && x.rank == 0) a.delta[stat] = delta;
   if (a.dq == nullptr) return;               // only D was wanted
   clear_row<DT>(dq);
-  walk_keys<DP>(a, x, xsm, bias, [&](const float* sk, const float* sv, int nk, const float* here) {
+  const bool some = walk_keys<DP>(a, x, xsm, bias, [&](const float* sk, const float* sv, int nk, const float* here) {
 #pragma unroll 1
     for (int j = slice; j < nk; j += KS) {
       const float s = fmaf(row_dot<DT, TPR>(q, sk + j * LD + part * DT), a.c, here[j]);
@@ -419,6 +432,7 @@ __global__ void __launch_bounds__(kXThreads) xattn_dq_scalar(const XAttn args, i
       row_axpy<DT>(ex2f(s - lse) * (dp - delta), sk + j * LD + part * DT, dq);
     }
   });
+  if (!some) clear_row<DT>(dq);
   if (KS == 1 && x.cl == 1) {
     put_row<DT>(xsm + x.lr * LD + part * DT, dq, a.scale);
     __syncthreads();

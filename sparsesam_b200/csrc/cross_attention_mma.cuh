@@ -195,8 +195,10 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NQ, 1>) xattn_f
 
   uint32_t k[KM][2][NR], v[KM][2][NR];
   float bias[KM][2];                         // 0, or -infinity for a key that is not there
+  bool some = false;                         // of this lane's keys one is there
   auto load = [&](int j0) {                  // loads keys j0 + .. and moves on
     if (mask == nullptr && j0 + 16 * KM <= j_end) {
+      some = true;
 #pragma unroll
       for (int i = 0; i < 2 * KM; ++i) {
         bias[i / 2][i % 2] = 0.f;
@@ -208,6 +210,7 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NQ, 1>) xattn_f
       for (int i = 0; i < 2 * KM; ++i) {
         const int j = j0 + i * 8 + g;
         const bool ok = j < j_end && (mask == nullptr || __ldg(mask + j) != 0);
+        some |= ok;
         bias[i / 2][i % 2] = ok ? 0.f : -INFINITY;
         load_frag<T, DP>(kp + i * 8 * a.ks[1], t, d, ok, k[i / 2][i % 2]);
         load_frag<T, DP>(vp + i * 8 * a.vs[1], t, d, ok, v[i / 2][i % 2]);
@@ -331,6 +334,16 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NQ, 1>) xattn_f
       }
   }
 
+  if (!__any_sync(0xffffffffu, some)) {      // a query that is not finite leaves NaN here, which is nothing's
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+#pragma unroll
+      for (int z = 0; z < HP; ++z) ref[z][i] = make_float2(kXmNone, kXmNone), l[z][i] = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int u = 0; u < NU; ++u) o[i][u][0] = o[i][u][1] = o[i][u][2] = o[i][u][3] = 0.f;
+    }
+  }
+
   // Join. Every warp leaves its references and sums; the block joins them at their highest reference, and
   // the cluster's blocks theirs on the way out, in a fixed order.
   constexpr int PER = NU * 4 + 2, NREG = NQ * PER, ROWS = HP * 8 * NQ;
@@ -433,16 +446,19 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NK, 2>) xattn_f
 
   uint32_t k[HP][NK][NR], v[HP][NK][NR], vl[kIsHalf<T> ? HP : 1][NK][NR], q[2][NR];   // vl: remainders
   float2 bias[NK];                           // of keys 8 i + 2t, + 1
+  int q_end = r_end;                         // rows past it are zeros
   auto load_q = [&](int r) {
-    load_frag<T, DP>(qp, t, d, r + g < r_end, q[0]);
-    load_frag<T, DP>(qp + q8, t, d, r + g + 8 < r_end, q[1]);
+    load_frag<T, DP>(qp, t, d, r + g < q_end, q[0]);
+    load_frag<T, DP>(qp + q8, t, d, r + g + 8 < q_end, q[1]);
     qp += 2 * q8;
   };
   load_q(r_begin);
+  bool some = false;
 #pragma unroll
   for (int i = 0; i < NK; ++i) {
     const int j = i * 8 + g;
     const bool ok = j < keys && (mask == nullptr || __ldg(mask + j) != 0);
+    some |= ok;
     uint32_t x[NR], y[NR];
     load_frag<T, DP>(kb + j * a.ks[1], t, d, ok, x);
     load_frag<T, DP>(vb + j * a.vs[1], t, d, ok, y);
@@ -460,6 +476,12 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NK, 2>) xattn_f
         if constexpr (kIsHalf<T>) vl[z][i][c] = rest;
       }
     }
+  }
+
+  if (!__any_sync(0xffffffffu, some)) {      // no keys: whatever the queries hold, their rows are zeros
+    q_end = r_begin;
+#pragma unroll
+    for (int c = 0; c < NR; ++c) q[0][c] = q[1][c] = 0u;
   }
 
   const float2 c2 = make_float2(a.c, a.c);
@@ -646,6 +668,8 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_few(const XAttn args, in
   const int begin = min(total, (rank * kXmWarps + warp) * per), end = min(total, begin + per);
   uint32_t x1[2][NR], x2[2][NR];
   float xs[2], xd[2];                        // long keys: bias of the key; long rows: maximum and D, found below
+  bool some = false;                         // of this lane's keys one is there
+  int row_end = end;                         // long rows past it are zeros
   auto load_long = [&](int i0) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -654,8 +678,9 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_few(const XAttn args, in
         const bool ok = i < end && key_ok(i);
         load_key(i, ok, x1[h], x2[h]);
         xs[h] = ok ? 0.f : -INFINITY;
+        some |= ok;
       } else {
-        load_row(i, end, x1[h], x2[h]);
+        load_row(i, row_end, x1[h], x2[h]);
       }
     }
   };
@@ -675,11 +700,21 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_few(const XAttn args, in
       const bool ok = key_ok(f);
       load_key(f, ok, y1[i], y2[i]);
       mine = ok ? 0.f : -INFINITY;
+      some |= ok;
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       fs[i][e] = __shfl_sync(0xffffffffu, mine, 8 * t + 4 * e);
       fd[i][e] = __shfl_sync(0xffffffffu, del, 8 * t + 4 * e);
+    }
+  }
+  if constexpr (!FEW_ROWS) {
+    if (!__any_sync(0xffffffffu, some)) {    // no keys: whatever the rows hold, their gradients are zeros
+      row_end = begin;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int c = 0; c < NR; ++c) x1[h][c] = x2[h][c] = 0u;
     }
   }
   Turned<T, NF, NR> y1t;
@@ -845,6 +880,15 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_few(const XAttn args, in
       } else if (a.dq != nullptr) {
         store_frag<T, DP>(static_cast<T*>(a.dq) + row_dense(a, b, n, i), t, a.d, y);
       }
+    }
+  }
+
+  if constexpr (FEW_ROWS) {
+    if (!__any_sync(0xffffffffu, some)) {    // as in the forward pass
+#pragma unroll
+      for (int i = 0; i < NF; ++i)
+#pragma unroll
+        for (int u = 0; u < NU; ++u) acc1[i][u][0] = acc1[i][u][1] = acc1[i][u][2] = acc1[i][u][3] = 0.f;
     }
   }
 

@@ -230,6 +230,7 @@ __global__ void __launch_bounds__(kTcThreads, 4 / NP) xattn_tc_fwd_kernel(const 
   const T* vb = static_cast<const T*>(a.v) + b * a.vs[0] + n * a.vs[2];
   const uint8_t* mask = a.key_mask == nullptr ? nullptr : a.key_mask + static_cast<int64_t>(b) * a.Tk;
   auto key_ok = [&](int j) { return j < keys && (mask == nullptr || __ldg(mask + j) != 0); };
+  bool some = false;                         // one of the keys that this thread looked at is there
   auto request = [&](int j, int buf) {
     if (j < j_end) {
       const uint32_t y = ring + buf * kStage;
@@ -237,7 +238,11 @@ __global__ void __launch_bounds__(kTcThreads, 4 / NP) xattn_tc_fwd_kernel(const 
       tc_fetch<T, NP, kTcOther, kTcThreads>(y, a.d, kb, [&](int i) { return key_ok(k0 + i) ? kb + (k0 + i) * a.ks[1] : nullptr; });
       tc_fetch<T, NP, kTcOther, kTcThreads>(y + kHalfStage, a.d, vb,
                                             [&](int i) { return key_ok(k0 + i) ? vb + (k0 + i) * a.vs[1] : nullptr; });
-      if (tid < kTcOther) s_bias[buf][tid] = key_ok(k0 + tid) ? 0.f : -INFINITY;
+      if (tid < kTcOther) {
+        const bool there = key_ok(k0 + tid);
+        s_bias[buf][tid] = there ? 0.f : -INFINITY;
+        some |= there;
+      }
     }
   };
   tc_fetch<T, NP, kTcOwn, kTcThreads>(x1, a.d, qb, [&](int i) -> const T* {
@@ -321,6 +326,9 @@ __global__ void __launch_bounds__(kTcThreads, 4 / NP) xattn_tc_fwd_kernel(const 
   if (ok && it > 0) ok = mbar_wait(&bars[1], (it - 1) & 1);
   tc_fence_after();
   __syncwarp();
+  // where every key that was walked is masked, a query that is not finite leaves NaN, which is nothing's
+  const bool any = it > 0 && (mask == nullptr || __syncthreads_or(some));
+  if (!any) ref = kTcNone, l2 = make_float2(0.f, 0.f);
   const float l = l2.x + l2.y;
   const float inv = cl > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
   const int64_t stat0 = (static_cast<int64_t>(b) * a.heads + n * a.group) * a.Tq;
@@ -330,7 +338,7 @@ __global__ void __launch_bounds__(kTcThreads, 4 / NP) xattn_tc_fwd_kernel(const 
 #pragma unroll
   for (int p = 0; p < NP; ++p) {
     float2 o[32];
-    if (it > 0) {
+    if (any) {
       tc_read64(B.t_lane + tO + 64 * p, o);
     } else {
 #pragma unroll
@@ -427,6 +435,7 @@ __global__ void __launch_bounds__(kTcBwdThreads, 2 / NP) xattn_tc_bwd_kernel(con
     return base + at.t * s[1] + at.h * s[2];
   };
   auto key_at = [&](const T* base, const int64_t (&s)[3], int j) { return key_ok(j) ? base + j * s[1] : nullptr; };
+  bool some = false;                         // one of the keys that this thread looked at is there
   auto request = [&](int j, int buf) {
     if (j < j_end) {
       const uint32_t y = ring + buf * kStage, y2 = y + kHalfStage;
@@ -434,7 +443,11 @@ __global__ void __launch_bounds__(kTcBwdThreads, 2 / NP) xattn_tc_bwd_kernel(con
       if constexpr (OWN_ROWS) {
         tc_fetch<T, NP, kTcOther, kTcBwdThreads>(y, a.d, kb, [&](int i) { return key_at(kb, a.ks, e0 + i); });
         tc_fetch<T, NP, kTcOther, kTcBwdThreads>(y2, a.d, vb, [&](int i) { return key_at(vb, a.vs, e0 + i); });
-        if (tid < kTcOther) s_a[buf][tid] = key_ok(e0 + tid) ? 0.f : -INFINITY;
+        if (tid < kTcOther) {
+          const bool there = key_ok(e0 + tid);
+          s_a[buf][tid] = there ? 0.f : -INFINITY;
+          some |= there;
+        }
       } else {
         tc_fetch<T, NP, kTcOther, kTcBwdThreads>(y, a.d, qb, [&](int i) { return row_at(qb, a.qs, e0 + i); });
         tc_fetch<T, NP, kTcOther, kTcBwdThreads>(y2, a.d, ob, [&](int i) { return row_at(ob, a.os, e0 + i); });
@@ -538,6 +551,7 @@ __global__ void __launch_bounds__(kTcBwdThreads, 2 / NP) xattn_tc_bwd_kernel(con
   if (ok && it > 0) ok = mbar_wait(&bars[1], (it - 1) & 1);
   tc_fence_after();
   __syncwarp();
+  const bool any = it > 0 && (!OWN_ROWS || mask == nullptr || __syncthreads_or(some));   // as in the forward kernel
   const int own_n = OWN_ROWS ? rows : a.Tk;
   auto to_row = [&](void* to, int r) {
     if constexpr (OWN_ROWS) {
@@ -558,7 +572,7 @@ __global__ void __launch_bounds__(kTcBwdThreads, 2 / NP) xattn_tc_bwd_kernel(con
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
       float2 v[16];                          // channels 64 p + 32 half ..
-      if (it > 0) {
+      if (any) {
         uint32_t u[32];
         tmem_ld_32x32b_x32(B.t_lane + (k == 0 ? tA1 : tA2) + 64 * p + 32 * half, u);
         tmem_ld_wait();

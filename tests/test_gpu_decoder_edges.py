@@ -59,3 +59,40 @@ def test_gradients_of_weights_far_below_the_largest(cuda_device, shape, far, dty
     do = do.abs() * 256 + 256
     got = run(q, k, v, do, scale=1.0)
     check(got, reference(q, k, v, do, scale=1.0), dtype)
+
+
+def close(y, ref, dtype, where=...):
+    """y against (value, size of the terms), as check(), at `where`."""
+    u = torch.finfo(DTYPES[dtype]).eps / 2
+    r, size = ref
+    allow = u * r.abs() + (NOISE + (4 * u * u if dtype != "fp32" else 0.0)) * size + 8 * torch.finfo(DTYPES[dtype]).tiny * u
+    err = (y.double() - r).abs()[where]
+    assert torch.all(err <= allow[where]), (err - allow[where]).max().item()
+
+
+BAD = [math.nan, math.inf, -math.inf]
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("kind", ["lens", "mask"])
+@pytest.mark.parametrize("shape", FORWARD, ids=ids)
+def test_queries_without_keys(cuda_device, shape, kind, dtype):
+    """Two padded entries of a batch have no keys, and queries and incoming gradients that are whatever their memory
+    held: zero rows and zero gradients there, and the other entries' as ever."""
+    shape = (4, *shape[1:])
+    q, k, v, do = make(cuda_device, *shape, dtype, seed=23)
+    lens = mask = None
+    if kind == "lens":
+        lens = torch.tensor([shape[2], 0, (shape[2] + 1) // 2, 0], dtype=torch.int32, device=cuda_device)
+    else:
+        mask = torch.rand(4, shape[2], generator=torch.Generator().manual_seed(24)).lt(0.7).to(cuda_device)
+        mask[::2, 0] = True
+        mask[1::2] = False
+    clean = q.clone(), do.clone()
+    for t in (q, do):
+        n = t[1::2].numel()
+        t[1::2] = torch.tensor(BAD, device=cuda_device).to(t.dtype)[torch.arange(n, device=cuda_device) % 3].view(2, *t.shape[1:])
+    out, dq = run(q, k, v, do, key_lens=lens, key_mask=mask)[:2]
+    ref = reference(clean[0], k, v, clean[1], lens=lens, mask=mask)
+    assert not out[1::2].any() and not dq[1::2].any()
+    check([out, dq], ref, dtype)
