@@ -514,6 +514,7 @@ __global__ void __launch_bounds__(kXThreads) xattn_dkv_scalar(const XAttn args, 
     }
     __syncthreads();
   }
+  if (!key_ok) clear_row<DT>(dk), clear_row<DT>(dv);   // also where a query or its gradient is not finite
   __syncthreads();
   float* mine = xsm + (slice * RB + lr) * (2 * DP) + part * DT;
 #pragma unroll

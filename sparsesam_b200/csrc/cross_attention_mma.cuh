@@ -789,6 +789,8 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_few(const XAttn args, in
 #pragma unroll
         for (int c = 0; c < NR; ++c) bf16_terms<T>(movm(x2[h][c]), x2t[h][c], x2l[h][c]);
     }
+    // keys that are not there leave zeros, also where a query or its gradient is not finite
+    const bool gone[2] = {FEW_ROWS && xs[0] != 0.f, FEW_ROWS && xs[1] != 0.f};
     if (i0 + 16 < end) load_long(i0 + 16);   // the next step's, under this one's arithmetic
     float e1[NR][4], e2[FEW_ROWS ? NR : 1][4];
 #pragma unroll
@@ -868,13 +870,13 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_few(const XAttn args, in
       if (i >= end) continue;
       uint32_t y[NR];
 #pragma unroll
-      for (int c = 0; c < NR; ++c) y[c] = Mma<T>::pack(e1[c][2 * h] * a.scale, e1[c][2 * h + 1] * a.scale);
+      for (int c = 0; c < NR; ++c) y[c] = gone[h] ? 0u : Mma<T>::pack(e1[c][2 * h] * a.scale, e1[c][2 * h + 1] * a.scale);
       if constexpr (FEW_ROWS) {
         if (a.dk != nullptr) {
           const int64_t to = ((static_cast<int64_t>(b) * a.Tk + i) * a.kv_heads + n) * a.d;
           store_frag<T, DP>(static_cast<T*>(a.dk) + to, t, a.d, y);
 #pragma unroll
-          for (int c = 0; c < NR; ++c) y[c] = Mma<T>::pack(e2[c][2 * h], e2[c][2 * h + 1]);
+          for (int c = 0; c < NR; ++c) y[c] = gone[h] ? 0u : Mma<T>::pack(e2[c][2 * h], e2[c][2 * h + 1]);
           store_frag<T, DP>(static_cast<T*>(a.dv) + to, t, a.d, y);
         }
       } else if (a.dq != nullptr) {
@@ -913,6 +915,7 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_few(const XAttn args, in
     const int v = second ? w - N1 : w, e = v % 4, u = v / 4 % NU, f = v / 4 / NU * 8 + 2 * t + (e & 1);
     float x = 0.f;
     for (int z = 0; z < cl; ++z) x += ld_dsmem(mapa_shared(base, z) + w * 128);
+    if (!FEW_ROWS && !key_ok(f)) x = 0.f;
     const int ch = g / 2 * (DP / 4) + 4 * u + g % 2 + (e & 2);
     T* to = static_cast<T*>(FEW_ROWS ? a.dq : second ? a.dv : a.dk);
     if (f < (FEW_ROWS ? rows : a.Tk) && ch < a.d && to != nullptr) {

@@ -552,6 +552,7 @@ __global__ void __launch_bounds__(kTcBwdThreads, 2 / NP) xattn_tc_bwd_kernel(con
   tc_fence_after();
   __syncwarp();
   const bool any = it > 0 && (!OWN_ROWS || mask == nullptr || __syncthreads_or(some));   // as in the forward kernel
+  const bool gone = !OWN_ROWS && own_s != 0.f;   // a key that is not there: zeros, whatever the queries hold
   const int own_n = OWN_ROWS ? rows : a.Tk;
   auto to_row = [&](void* to, int r) {
     if constexpr (OWN_ROWS) {
@@ -577,7 +578,8 @@ __global__ void __launch_bounds__(kTcBwdThreads, 2 / NP) xattn_tc_bwd_kernel(con
         tmem_ld_32x32b_x32(B.t_lane + (k == 0 ? tA1 : tA2) + 64 * p + 32 * half, u);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = make_float2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
+        for (int i = 0; i < 16; ++i)
+          v[i] = gone ? make_float2(0.f, 0.f) : make_float2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
       } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = make_float2(0.f, 0.f);

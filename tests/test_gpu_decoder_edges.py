@@ -96,3 +96,32 @@ def test_queries_without_keys(cuda_device, shape, kind, dtype):
     ref = reference(clean[0], k, v, clean[1], lens=lens, mask=mask)
     assert not out[1::2].any() and not dq[1::2].any()
     check([out, dq], ref, dtype)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("kind", ["lens", "mask"])
+@pytest.mark.parametrize("which", ["q", "dout"])
+@pytest.mark.parametrize("shape", FORWARD, ids=ids)
+def test_absent_keys_have_no_gradient(cuda_device, shape, which, kind, dtype):
+    """A query, or its incoming gradient, that is not finite: keys that are not there keep zero gradients, and the other
+    queries' rows are theirs."""
+    shape = (4, *shape[1:])
+    q, k, v, do = make(cuda_device, *shape, dtype, seed=25)
+    Tq, Tk = shape[1:3]
+    lens = mask = None
+    if kind == "lens":
+        lens = torch.tensor([Tk, Tk // 2, 1, 0], dtype=torch.int32, device=cuda_device)
+    else:
+        mask = torch.rand(4, Tk, generator=torch.Generator().manual_seed(26)).lt(0.6).to(cuda_device)
+        mask[:3, 1] = True
+        mask[3] = False
+    ref = reference(q, k, v, do, lens=lens, mask=mask)
+    bad = torch.zeros(q.shape[:3], dtype=torch.bool, device=cuda_device)
+    for i in range(4):
+        bad[i, (7 * i + 1) % Tq] = True
+        (q if which == "q" else do)[i, (7 * i + 1) % Tq] = BAD[i % 3]
+    out, dq, dk, dv = run(q, k, v, do, key_lens=lens, key_mask=mask)
+    gone = ~there(4, Tk, lens, mask, cuda_device)
+    assert not dk[gone].any() and not dv[gone].any()
+    close(out, ref[0], dtype, ~bad if which == "q" else ...)
+    close(dq, ref[1], dtype, ~bad)
