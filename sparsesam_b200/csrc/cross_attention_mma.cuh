@@ -168,9 +168,10 @@ constexpr float kXmSlack = 8.f;
 //
 // HP = 2 (heads of 16 next to one another): a fragment is two heads of a token, 64 contiguous
 // bytes, because 32-byte pieces keep the L1 tags, not the DRAM, busy (tokens -> image, 64 images:
-// 35 us with HP = 1 at 72 % of L1, 26.4 with HP = 2 at 5.1 TB/s; one image 4.5 us, a launch and a join). Lanes t < 2 hold the first head's channels, so a query
-// fragment with the other half zeroed gives one head's logits, and likewise V^T rows g < 4
-// are the first head's. Twice the tensor instructions, of which there are plenty.
+// 35 us with HP = 1 at 72 % of L1, 26.4 with HP = 2 at 5.1 TB/s; one image 4.5 us, a launch and a join). Lanes t < 2 hold the first head's channels, so key
+// and query fragments with the other half zeroed (both: 0 times a NaN of the other head is one) give one head's
+// logits. V^T rows g < 4 are the first head's; each head has accumulators of its own, and half of their rows count.
+// Twice the tensor instructions, of which there are plenty.
 // ---------------------------------------------------------------------------
 template <class T, int DP, int NQ, int HP>
 __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NQ, 1>) xattn_fwd_few_rows(const XAttn args, int) {
@@ -231,14 +232,16 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NQ, 1>) xattn_f
 #pragma unroll
       for (int c = 0; c < NR; ++c) q[z][i][c] = HP == 1 || t / 2 == z ? x[c] : 0u;
   }
-  float o[NQ][NU][4];
+  float o[HP][NQ][NU][4];
   float2 ref[HP][NQ], l[HP][NQ];             // of queries 2t, 2t + 1
 #pragma unroll
   for (int i = 0; i < NQ; ++i) {
 #pragma unroll
-    for (int z = 0; z < HP; ++z) ref[z][i] = make_float2(kXmNone, kXmNone), l[z][i] = make_float2(0.f, 0.f);
+    for (int z = 0; z < HP; ++z) {
+      ref[z][i] = make_float2(kXmNone, kXmNone), l[z][i] = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int u = 0; u < NU; ++u) o[i][u][0] = o[i][u][1] = o[i][u][2] = o[i][u][3] = 0.f;
+      for (int u = 0; u < NU; ++u) o[z][i][u][0] = o[z][i][u][1] = o[z][i][u][2] = o[z][i][u][3] = 0.f;
+    }
   }
   const float2 c2 = make_float2(a.c, a.c);
 
@@ -249,17 +252,23 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NQ, 1>) xattn_f
 #pragma unroll
     for (int x = 0; x < KM; ++x) {
 #pragma unroll
-      for (int z = 0; z < HP; ++z)
+      for (int z = 0; z < HP; ++z) {
+        uint32_t kz[2][NR];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int c = 0; c < NR; ++c) kz[h][c] = HP == 1 || t / 2 == z ? k[x][h][c] : 0u;
 #pragma unroll
         for (int i = 0; i < NQ; ++i) {
           float f[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int c = 0; c < NR; c += 2)
-            Mma<T>::run(f, k[x][0][c], k[x][1][c], k[x][0][c + 1], k[x][1][c + 1], q[z][i][c], q[z][i][c + 1]);
+            Mma<T>::run(f, kz[0][c], kz[1][c], kz[0][c + 1], kz[1][c + 1], q[z][i][c], q[z][i][c + 1]);
 #pragma unroll
           for (int h = 0; h < 2; ++h)
             s[z][i][x][h] = fma2(make_float2(f[2 * h], f[2 * h + 1]), c2, make_float2(bias[x][h], bias[x][h]));
         }
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -279,8 +288,7 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NQ, 1>) xattn_f
       }
     if (__any_sync(0xffffffffu, renew)) {
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) {
-        float2 mine = make_float2(1.f, 1.f);
+      for (int i = 0; i < NQ; ++i)
 #pragma unroll
         for (int z = 0; z < HP; ++z) {
           float2 m = ref[z][i];
@@ -296,17 +304,15 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NQ, 1>) xattn_f
           const float2 f = make_float2(ex2f(ref[z][i].x - m.x), ex2f(ref[z][i].y - m.y));
           ref[z][i] = m;
           l[z][i] = mul2(l[z][i], f);
-          if (HP == 1 || g / 4 == z) mine = f;         // the sums of lane g belong to head g / 4
-        }
 #pragma unroll
-        for (int u = 0; u < NU; ++u) o[i][u][0] *= mine.x, o[i][u][1] *= mine.y, o[i][u][2] *= mine.x, o[i][u][3] *= mine.y;
-      }
+          for (int u = 0; u < NU; ++u) o[z][i][u][0] *= f.x, o[z][i][u][1] *= f.y, o[z][i][u][2] *= f.x, o[z][i][u][3] *= f.y;
+        }
     }
 #pragma unroll
-    for (int z = 0; z < HP; ++z)
+    for (int x = 0; x < KM; ++x) {
+      uint32_t hi[HP][NQ][2], lo[HP][NQ][2];
 #pragma unroll
-      for (int x = 0; x < KM; ++x) {
-        uint32_t hi[NQ][2], lo[NQ][2];
+      for (int z = 0; z < HP; ++z)
 #pragma unroll
         for (int i = 0; i < NQ; ++i)
 #pragma unroll
@@ -314,33 +320,37 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NQ, 1>) xattn_f
             float2 p = add2(s[z][i][x][h], make_float2(-ref[z][i].x, -ref[z][i].y));
             p.x = ex2f(p.x), p.y = ex2f(p.y);
             l[z][i] = add2(l[z][i], p);
-            split2<__nv_bfloat16>(p.x, p.y, hi[i][h], lo[i][h]);
-            hi[i][h] = movm(hi[i][h]), lo[i][h] = movm(lo[i][h]);
+            split2<__nv_bfloat16>(p.x, p.y, hi[z][i][h], lo[z][i][h]);
+            hi[z][i][h] = movm(hi[z][i][h]), lo[z][i][h] = movm(lo[z][i][h]);
           }
 #pragma unroll
-        for (int u = 0; u < NU; ++u) {
-          uint32_t vh[2][2], vl[2][2];
+      for (int u = 0; u < NU; ++u) {
+        uint32_t vh[2][2], vl[2][2];
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) bf16_terms<T>(HP == 1 || g / 4 == z ? vt[x][h][2 * u + e] : 0u, vh[h][e], vl[h][e]);
+          for (int e = 0; e < 2; ++e) bf16_terms<T>(vt[x][h][2 * u + e], vh[h][e], vl[h][e]);
+#pragma unroll
+        for (int z = 0; z < HP; ++z)
 #pragma unroll
           for (int i = 0; i < NQ; ++i) {
-            B16::run(o[i][u], vh[0][0], vh[0][1], vh[1][0], vh[1][1], hi[i][0], hi[i][1]);
-            B16::run(o[i][u], vh[0][0], vh[0][1], vh[1][0], vh[1][1], lo[i][0], lo[i][1]);
-            if constexpr (kIsHalf<T>) B16::run(o[i][u], vl[0][0], vl[0][1], vl[1][0], vl[1][1], hi[i][0], hi[i][1]);
+            B16::run(o[z][i][u], vh[0][0], vh[0][1], vh[1][0], vh[1][1], hi[z][i][0], hi[z][i][1]);
+            B16::run(o[z][i][u], vh[0][0], vh[0][1], vh[1][0], vh[1][1], lo[z][i][0], lo[z][i][1]);
+            if constexpr (kIsHalf<T>) B16::run(o[z][i][u], vl[0][0], vl[0][1], vl[1][0], vl[1][1], hi[z][i][0], hi[z][i][1]);
           }
-        }
       }
+    }
   }
 
   if (!__any_sync(0xffffffffu, some)) {      // a query that is not finite leaves NaN here, which is nothing's
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
 #pragma unroll
-      for (int z = 0; z < HP; ++z) ref[z][i] = make_float2(kXmNone, kXmNone), l[z][i] = make_float2(0.f, 0.f);
+      for (int z = 0; z < HP; ++z) {
+        ref[z][i] = make_float2(kXmNone, kXmNone), l[z][i] = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int u = 0; u < NU; ++u) o[i][u][0] = o[i][u][1] = o[i][u][2] = o[i][u][3] = 0.f;
+        for (int u = 0; u < NU; ++u) o[z][i][u][0] = o[z][i][u][1] = o[z][i][u][2] = o[z][i][u][3] = 0.f;
+      }
     }
   }
 
@@ -367,7 +377,7 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NQ, 1>) xattn_f
 #pragma unroll
     for (int u = 0; u < NU; ++u)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) to[(u * 4 + e) * 32] = o[i][u][e];
+      for (int e = 0; e < 4; ++e) to[(u * 4 + e) * 32] = hz == 0 ? o[0][i][u][e] : o[HP - 1][i][u][e];
   }
   __syncthreads();
   for (int w = warp; w < NREG; w += kXmWarps) {          // register w of every lane; its query is 8 i + 2t + (w & 1)
@@ -444,7 +454,7 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NK, 2>) xattn_f
   float* lse = a.lse == nullptr ? nullptr : a.lse + (static_cast<int64_t>(b) * a.heads + h) * a.Tq;
   float* o32 = a.out_f32 == nullptr ? nullptr : a.out_f32 + (static_cast<int64_t>(b) * a.Tq * a.heads + h) * a.d + t * (DP / 4);
 
-  uint32_t k[HP][NK][NR], v[HP][NK][NR], vl[kIsHalf<T> ? HP : 1][NK][NR], q[2][NR];   // vl: remainders
+  uint32_t k[HP][NK][NR], v[NK][NR], vl[kIsHalf<T> ? NK : 1][NR], q[2][NR];   // vl: remainders
   float2 bias[NK];                           // of keys 8 i + 2t, + 1
   int q_end = r_end;                         // rows past it are zeros
   auto load_q = [&](int r) {
@@ -467,14 +477,11 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NK, 2>) xattn_f
     bias[i].y = __shfl_sync(0xffffffffu, mine, 8 * t + 4);
 #pragma unroll
     for (int c = 0; c < NR; ++c) {
-      const uint32_t turned = movm(y[c]);
+      uint32_t rest;
+      bf16_terms<T>(movm(y[c]), v[i][c], rest);
+      if constexpr (kIsHalf<T>) vl[i][c] = rest;
 #pragma unroll
-      for (int z = 0; z < HP; ++z) {
-        k[z][i][c] = HP == 1 || t / 2 == z ? x[c] : 0u;
-        uint32_t rest;
-        bf16_terms<T>(HP == 1 || g / 4 == z ? turned : 0u, v[z][i][c], rest);
-        if constexpr (kIsHalf<T>) vl[z][i][c] = rest;
-      }
+      for (int z = 0; z < HP; ++z) k[z][i][c] = HP == 1 || t / 2 == z ? x[c] : 0u;
     }
   }
 
@@ -488,22 +495,29 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NK, 2>) xattn_f
   for (int r0 = r_begin; r0 < r_end; r0 += 16) {
     float2 s[HP][NK][2];
 #pragma unroll
-    for (int z = 0; z < HP; ++z)
+    for (int z = 0; z < HP; ++z) {
+      uint32_t qz[2][NR];
+#pragma unroll
+      for (int c = 0; c < NR; ++c) {
+        qz[0][c] = HP == 1 || t / 2 == z ? q[0][c] : 0u;
+        qz[1][c] = HP == 1 || t / 2 == z ? q[1][c] : 0u;
+      }
 #pragma unroll
       for (int i = 0; i < NK; ++i) {
         float f[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < NR; c += 2) Mma<T>::run(f, q[0][c], q[1][c], q[0][c + 1], q[1][c + 1], k[z][i][c], k[z][i][c + 1]);
+        for (int c = 0; c < NR; c += 2) Mma<T>::run(f, qz[0][c], qz[1][c], qz[0][c + 1], qz[1][c + 1], k[z][i][c], k[z][i][c + 1]);
         s[z][i][0] = fma2(make_float2(f[0], f[1]), c2, bias[i]);
         s[z][i][1] = fma2(make_float2(f[2], f[3]), c2, bias[i]);
       }
+    }
     if (r0 + 16 < r_end) load_q(r0 + 16);
     float m[HP][2], l[HP][2];
-    float o[NR][4];
-#pragma unroll
-    for (int c = 0; c < NR; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
+    float o[HP][NR][4];
 #pragma unroll
     for (int z = 0; z < HP; ++z) {
+#pragma unroll
+      for (int c = 0; c < NR; ++c) o[z][c][0] = o[z][c][1] = o[z][c][2] = o[z][c][3] = 0.f;
       float inv[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -539,17 +553,25 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NK, 2>) xattn_f
           }
 #pragma unroll
         for (int c = 0; c < NR; ++c) {
+          float(&oc)[4] = o[z][c];
           if constexpr (NK == 1) {
-            B16::run8(o[c], hi[0], hi[1], v[z][0][c]);
-            B16::run8(o[c], lo[0], lo[1], v[z][0][c]);
-            if constexpr (kIsHalf<T>) B16::run8(o[c], hi[0], hi[1], vl[z][0][c]);
+            B16::run8(oc, hi[0], hi[1], v[0][c]);
+            B16::run8(oc, lo[0], lo[1], v[0][c]);
+            if constexpr (kIsHalf<T>) B16::run8(oc, hi[0], hi[1], vl[0][c]);
           } else {
-            B16::run(o[c], hi[0], hi[1], hi[2], hi[3], v[z][i][c], v[z][i + 1][c]);
-            B16::run(o[c], lo[0], lo[1], lo[2], lo[3], v[z][i][c], v[z][i + 1][c]);
-            if constexpr (kIsHalf<T>) B16::run(o[c], hi[0], hi[1], hi[2], hi[3], vl[z][i][c], vl[z][i + 1][c]);
+            B16::run(oc, hi[0], hi[1], hi[2], hi[3], v[i][c], v[i + 1][c]);
+            B16::run(oc, lo[0], lo[1], lo[2], lo[3], v[i][c], v[i + 1][c]);
+            if constexpr (kIsHalf<T>) B16::run(oc, hi[0], hi[1], hi[2], hi[3], vl[i][c], vl[i + 1][c]);
           }
         }
       }
+    }
+    // lane t's columns are channels of head t / 2 of a pair
+    if constexpr (HP == 2) {
+#pragma unroll
+      for (int c = 0; c < NR; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[0][c][e] = t / 2 == 0 ? o[0][c][e] : o[1][c][e];
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -557,7 +579,7 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NK, 2>) xattn_f
       if (r >= r_end) continue;
       uint32_t y[NR];
 #pragma unroll
-      for (int c = 0; c < NR; ++c) y[c] = Mma<T>::pack(o[c][2 * e], o[c][2 * e + 1]);
+      for (int c = 0; c < NR; ++c) y[c] = Mma<T>::pack(o[0][c][2 * e], o[0][c][2 * e + 1]);
       store_frag<T, DP>(op + e * o8, t, d, y);
       if (lse != nullptr && t < HP) {
         const float ml = HP == 2 && t == 1 ? m[HP - 1][e] : m[0][e], ll = HP == 2 && t == 1 ? l[HP - 1][e] : l[0][e];
@@ -567,7 +589,7 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NK, 2>) xattn_f
         float* f = o32 + static_cast<int64_t>(r) * a.heads * a.d;
 #pragma unroll
         for (int c = 0; c < NR; ++c)
-          if (t * (DP / 4) + 2 * c < d) *reinterpret_cast<float2*>(f + 2 * c) = make_float2(o[c][2 * e], o[c][2 * e + 1]);
+          if (t * (DP / 4) + 2 * c < d) *reinterpret_cast<float2*>(f + 2 * c) = make_float2(o[0][c][2 * e], o[0][c][2 * e + 1]);
       }
     }
     op += 2 * o8;

@@ -125,3 +125,25 @@ def test_absent_keys_have_no_gradient(cuda_device, shape, which, kind, dtype):
     assert not dk[gone].any() and not dv[gone].any()
     close(out, ref[0], dtype, ~bad if which == "q" else ...)
     close(dq, ref[1], dtype, ~bad)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("which", ["q", "k", "v"])
+@pytest.mark.parametrize("shape", FORWARD, ids=ids)
+def test_heads_do_not_meet(cuda_device, shape, which, dtype):
+    """Values that are not finite in one key head, or in its queries: the other heads are theirs."""
+    B, Tq, Tk, H, Hk, D = shape
+    H, Hk = max(H, 4), max(H, 4) * Hk // H
+    q, k, v, do = make(cuda_device, B, Tq, Tk, H, Hk, D, dtype, seed=27)
+    G = H // Hk
+    ref = reference(q, k, v, do)
+    for i, value in enumerate(BAD):
+        a, b, c = q.clone(), k.clone(), v.clone()
+        h = i % Hk
+        {"q": a[:, :, h * G : (h + 1) * G], "k": b[:, :, h : h + 1], "v": c[:, :, h : h + 1]}[which][:, 0, :, i] = value
+        got = run(a, b, c, do)
+        for n, (y, r) in enumerate(zip(got, ref)):
+            others = torch.arange(y.shape[2], device=cuda_device) // (G if n < 2 else 1) != h
+            close(y, r, dtype, (slice(None), slice(None), others))
+        if which == "q":                                           # and the other queries of the head itself
+            close(got[0], ref[0], dtype, (slice(None), slice(1, None)))
