@@ -154,7 +154,7 @@ __device__ __forceinline__ int64_t row_dense(const XAttn& a, int b, int n, int r
   return ((static_cast<int64_t>(b) * a.Tq + t) * a.heads + n * a.group + g) * a.d;
 }
 
-constexpr float kXmNone = -3e38f;           // reference before the first key: below all finite logits that matter
+constexpr float kXmNone = -3.402823466e38f;  // reference before the first key: no finite logit is below it
 constexpr float kXmSlack = 8.f;
 
 // ---------------------------------------------------------------------------
@@ -521,7 +521,7 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NK, 2>) xattn_f
       float inv[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float x = kXmNone;                   // a row without keys: 2^(-inf + 3e38) = 0
+        float x = kXmNone;                   // a row without keys: 2^(-inf + 3.4e38) = 0
 #pragma unroll
         for (int i = 0; i < NK; ++i) x = fmaxf(x, fmaxf(s[z][i][e].x, s[z][i][e].y));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));

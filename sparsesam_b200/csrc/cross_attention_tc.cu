@@ -196,7 +196,7 @@ __device__ __forceinline__ bool tc_landed(bool ok) {
   tc_fence_before();
   return __syncthreads_and(ok);
 }
-constexpr float kTcNone = -3e38f, kTcSlack = 8.f;
+constexpr float kTcNone = -3.402823466e38f, kTcSlack = 8.f;   // no finite logit is below the first
 
 // Folded row r of key head n is token r % Tq of query head n group + r / Tq.
 struct TcRow {

@@ -147,3 +147,16 @@ def test_heads_do_not_meet(cuda_device, shape, which, dtype):
             close(y, r, dtype, (slice(None), slice(None), others))
         if which == "q":                                           # and the other queries of the head itself
             close(got[0], ref[0], dtype, (slice(None), slice(1, None)))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("shape", FORWARD, ids=ids)
+def test_logits_at_the_end_of_fp32(cuda_device, shape, dtype):
+    """Every logit -3.2e38 (in base 2): equal weights, not a row without keys; the base-2 logit is finite down to -3.4e38."""
+    q, k, v, _ = make(cuda_device, *shape, dtype, seed=28)
+    q.zero_(), k.zero_()
+    q[..., 0], k[..., 0] = -(2.0 ** 64), 2.0 ** 63 * 1.3125         # <q, k> = -2.23e38, log2(e) times that -3.22e38
+    (out,) = run(q, k, v, scale=1.0)
+    mean = v.double().mean(1, keepdim=True).repeat_interleave(shape[3] // shape[4], 2).expand(out.shape)
+    size = v.double().abs().mean(1, keepdim=True).repeat_interleave(shape[3] // shape[4], 2).expand(out.shape)
+    close(out, (mean, size), dtype)
