@@ -268,23 +268,26 @@ class DecoderAttention(nn.Module):
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                 key_lens: Optional[torch.Tensor] = None, key_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
         """key_lens (int32 (B,)) and key_mask (bool (B, Tk), True: attend) say which keys are
-        there (a padded batch of prompts); a query without keys gives out_proj's bias."""
+        there (a padded batch of prompts): what the others hold does not matter, and a query
+        without keys gives out_proj's bias."""
         qh, kh, vh = self._split(self.q_proj(q)), self._split(self.k_proj(k)), self._split(self.v_proj(v))
         h, c = qh.shape[2:]
         if qh.is_cuda and qh.shape[0] <= ops.CROSS_ATTN_MAX_BATCH and ops.cross_attn_supported(h, h, c, qh.dtype):
-            o = ops.cross_attn(qh, kh, vh, key_lens=key_lens, key_mask=key_mask)
-        else:
-            mask = key_mask
-            if key_lens is not None:
-                there = torch.arange(kh.shape[1], device=kh.device) < key_lens.view(-1, 1)
-                mask = there if mask is None else mask & there
-            if mask is not None:
-                mask = mask[:, None, None, :]
-            o = F.scaled_dot_product_attention(qh.transpose(1, 2), kh.transpose(1, 2), vh.transpose(1, 2),
-                                               attn_mask=mask).transpose(1, 2)      # softmax(q k^T / sqrt(c)) v
-            if mask is not None:
-                o = torch.where(mask.any(-1)[..., None], o, torch.zeros((), dtype=o.dtype, device=o.device))
-        return self.out_proj(o.reshape(o.shape[0], o.shape[1], h * c))
+            return self.out_proj(ops.cross_attn(qh, kh, vh, key_lens=key_lens, key_mask=key_mask).flatten(2))
+        mask = key_mask
+        if key_lens is not None:
+            there = torch.arange(kh.shape[1], device=kh.device) < key_lens.view(-1, 1)
+            mask = there if mask is None else mask & there
+        if mask is not None:
+            # absent keys are zeros, and a query without keys is one that looks at all of them
+            some = mask.any(1, keepdim=True)
+            gone = ~mask[:, :, None, None]
+            qh = qh.masked_fill(~some[:, :, None, None], 0.0)
+            kh, vh = kh.masked_fill(gone, 0.0), vh.masked_fill(gone, 0.0)
+            mask = (mask | ~some)[:, None, None, :]
+        o = F.scaled_dot_product_attention(qh.transpose(1, 2), kh.transpose(1, 2), vh.transpose(1, 2),
+                                           attn_mask=mask)           # softmax(q k^T / sqrt(c)) v
+        return self.out_proj(o.transpose(1, 2).flatten(2))
 
 
 class DecoderMLPBlock(nn.Module):

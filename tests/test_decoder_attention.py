@@ -1,0 +1,54 @@
+"""hq.DecoderAttention where torch computes its attention (the host, dtypes and heads that the kernel does not take)."""
+import copy
+import math
+
+import pytest
+import torch
+
+from sparsesam_b200 import hq
+
+gpu = pytest.mark.gpu
+LENS = torch.tensor([25, 0, 7], dtype=torch.int32)
+
+
+def attention(device="cpu", dtype=torch.float32, dim=64, heads=4):
+    torch.manual_seed(0)
+    mod = hq.DecoderAttention(dim, heads, 2).to(device, dtype)
+    g = torch.Generator().manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=g).to(device, dtype)  # noqa: E731
+    return mod, r(3, 9, dim), r(3, 25, dim), r(3, 25, dim)
+
+
+def near(x, y, dtype=torch.float32):
+    """Two ways of computing some five rounded layers of unit size."""
+    eps = torch.finfo(dtype).eps
+    assert x.shape == y.shape and (x.double() - y.double()).abs().max() <= 16 * eps * max(1.0, y.abs().max().item())
+
+
+def test_masked_places_hold_anything_on_torchs_path():
+    """What the kernel promises holds elsewhere too: absent keys and queries without keys may be NaN or infinite."""
+    mod, q, k, v = attention()
+    gone = torch.arange(25)[None] >= LENS[:, None]
+    want = mod(q, torch.where(gone[..., None], 0.0, k), torch.where(gone[..., None], 0.0, v), key_lens=LENS)
+    k, v, q = k.clone(), v.clone(), q.clone()
+    k[gone], v[gone], q[1] = math.nan, math.inf, math.nan
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    out = mod(*leaves, key_lens=LENS)
+    near(out, want)
+    near(out[1], mod.out_proj.bias.expand(9, -1))
+    for t, there in zip(torch.autograd.grad(out.square().sum(), leaves), (torch.tensor([True, False, True]), ~gone, ~gone)):
+        assert torch.isfinite(t[there]).all() and not t[~there].any()
+
+
+@gpu
+def test_masked_places_hold_anything_where_torch_computes(cuda_device):
+    """Heads of 12 channels, which the kernel does not take."""
+    mod, q, k, v = attention(cuda_device, dim=96, heads=4)
+    lens = LENS.to(cuda_device)
+    gone = torch.arange(25, device=cuda_device)[None] >= lens[:, None]
+    want = copy.deepcopy(mod).cpu()(q.cpu(), k.cpu(), v.cpu(), key_lens=LENS)
+    k[gone], v[gone], q[1] = math.nan, math.inf, math.nan
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    out = mod(*leaves, key_lens=lens)
+    near(out.cpu(), want)
+    assert all(torch.isfinite(g).all() for g in torch.autograd.grad(out.square().sum(), leaves))
