@@ -272,7 +272,8 @@ class DecoderAttention(nn.Module):
         without keys gives out_proj's bias."""
         qh, kh, vh = self._split(self.q_proj(q)), self._split(self.k_proj(k)), self._split(self.v_proj(v))
         h, c = qh.shape[2:]
-        if qh.is_cuda and qh.shape[0] <= ops.CROSS_ATTN_MAX_BATCH and ops.cross_attn_supported(h, h, c, qh.dtype):
+        if (qh.is_cuda and qh.shape[0] == kh.shape[0] <= ops.CROSS_ATTN_MAX_BATCH and kh.shape == vh.shape
+                and ops.cross_attn_supported(h, h, c, qh.dtype)):
             return self.out_proj(ops.cross_attn(qh, kh, vh, key_lens=key_lens, key_mask=key_mask).flatten(2))
         mask = key_mask
         if key_lens is not None:

@@ -52,3 +52,15 @@ def test_masked_places_hold_anything_where_torch_computes(cuda_device):
     out = mod(*leaves, key_lens=lens)
     near(out.cpu(), want)
     assert all(torch.isfinite(g).all() for g in torch.autograd.grad(out.square().sum(), leaves))
+
+
+
+def test_one_query_set_for_a_batch():
+    mod, q, k, v = attention()
+    near(mod(q[:1], k, v), mod(q[:1].expand(3, -1, -1), k, v))
+
+
+@gpu
+def test_one_query_set_for_a_batch_on_the_gpu(cuda_device):
+    mod, q, k, v = attention(cuda_device)
+    near(mod(q[:1], k, v), mod(q[:1].expand(3, -1, -1), k, v))
