@@ -4,9 +4,11 @@
 // Why not ctypes and torch.autograd.Function, as the encoder's calls: these are training operators of microseconds,
 // and a node in Python costs the host more than the kernels (a pass with gradients of a 4096 x 256 LayerNorm: 100 us
 // of which 9 us of kernels; the forward call of one box prompt's attention 15 us, 5 us of kernel).
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <atomic>
@@ -64,6 +66,32 @@ void check_sizes(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
     for (const int64_t n : t->sizes())
       if (n > INT32_MAX) refuse("a dimension of " + std::to_string(n) + " entries is not supported (at most 2^31 - 1)");
+}
+// These calls are no operators of torch's dispatcher: what follows a program operator by operator does not see them.
+// A trace would hold uninitialised memory in their place and a tangent would be dropped, both without a word; tensors
+// that wrap others (vmap, grad and functionalize of torch.func, fake tensors, subclasses) have no memory of their own.
+bool plain(const Tensor& t) {
+  constexpr c10::DispatchKeySet wrapped(
+      {c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
+       c10::DispatchKey::Batched, c10::DispatchKey::Functionalize, c10::DispatchKey::Conjugate,
+       c10::DispatchKey::Negative, c10::DispatchKey::ZeroTensor});
+  return t.layout() == at::kStrided && !t.is_nested() && !t.key_set().has_any(wrapped) && !t._fw_grad(0).defined();
+}
+bool followed() {
+  return torch::jit::tracer::isTracing() ||
+         c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value();
+}
+bool takes(const std::vector<Tensor>& ts) {
+  for (const Tensor& t : ts)
+    if (!plain(t)) return false;
+  return !followed();
+}
+void check_plain(const char* op, std::initializer_list<const Tensor*> ts) {
+  bool ok = !followed();
+  for (const Tensor* t : ts) ok = ok && (!t->defined() || plain(*t));
+  if (!ok)
+    throw std::runtime_error(std::string(op) + " takes plain tensors outside of traces: torch.jit.trace, make_fx, torch.func "
+                             "transforms, forward-mode differentiation and tensor subclasses do not see it");
 }
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
@@ -142,6 +170,7 @@ struct LayerNormGelu : torch::autograd::Function<LayerNormGelu> {
 };
 
 Tensor layernorm_gelu_half(const Tensor& x, const Tensor& w, const Tensor& b, double eps, bool gelu) {
+  check_plain("layernorm_gelu_half", {&x, &w, &b});
   const auto dt = x.scalar_type();
   if ((dt != at::kHalf && dt != at::kBFloat16) || w.scalar_type() != dt || b.scalar_type() != dt) {
     check_devices(x, {&w, &b});
@@ -222,6 +251,7 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
 };
 
 Tensor groupnorm_act(const Tensor& x, int64_t groups, const Tensor& w, const Tensor& b, double eps, int64_t act) {
+  check_plain("groupnorm_act", {&x, &w, &b});
   const auto dt = x.scalar_type();
   if (dtype_code(dt) < 0 || w.scalar_type() != dt || b.scalar_type() != dt)
     throw py::type_error("x, w and b must share one dtype of fp16, bf16, fp32");
@@ -339,6 +369,7 @@ std::string shape(const Tensor& t) {
 Tensor cross_attn(const Tensor& q, const Tensor& k, const Tensor& v, std::optional<double> scale_, const std::optional<Tensor>& lens_,
                   const std::optional<Tensor>& mask_) {
   const Tensor lens = lens_.value_or(Tensor()), mask = mask_.value_or(Tensor());
+  check_plain("cross_attn", {&q, &k, &v, &lens, &mask});
   if (q.dim() != 4 || k.dim() != 4 || v.sizes() != k.sizes() || k.size(0) != q.size(0) || k.size(3) != q.size(3))
     refuse("q (B, Tq, H, D), k and v (B, Tk, Hk, D) expected, got " + shape(q) + ", " + shape(k) + ", " + shape(v));
   check_sizes({&q, &k});
@@ -378,5 +409,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("layernorm_gelu_half", &layernorm_gelu_half);
   m.def("groupnorm_act", &groupnorm_act);
   m.def("cross_attn", &cross_attn);
+  m.def("takes", &takes);
   m.def("launches", [] { return launches.load(); });
 }

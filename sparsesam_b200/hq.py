@@ -69,7 +69,8 @@ class LayerNorm2d(host.LayerNorm2d):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         nhwc = x.permute(0, 2, 3, 1)
         if (x.is_cuda and x.dtype in (torch.float16, torch.bfloat16) and self.weight.dtype == x.dtype
-                and x.shape[1] in ops.LN_HALF_CHANNELS and nhwc.is_contiguous()):
+                and not ops.followed(x, self.weight, self.bias) and x.shape[1] in ops.LN_HALF_CHANNELS
+                and nhwc.is_contiguous()):
             y = ops.layernorm_gelu_half(nhwc, self.weight, self.bias, self.eps, self.gelu)
         else:
             y = F.layer_norm(nhwc, (x.shape[1],), self.weight, self.bias, self.eps)
@@ -84,8 +85,9 @@ class RowLayerNorm(nn.LayerNorm):
     (the two-way transformer's norm of the 4096 image tokens per prompt)."""
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        if (x.is_cuda and x.dtype in (torch.float16, torch.bfloat16) and self.weight is not None
-                and self.weight.dtype == x.dtype and x.shape[-1] in ops.LN_HALF_CHANNELS and x.is_contiguous()):
+        if (x.is_cuda and x.dtype in (torch.float16, torch.bfloat16) and self.weight is not None and self.bias is not None
+                and self.weight.dtype == x.dtype and not ops.followed(x, self.weight, self.bias)
+                and x.shape[-1] in ops.LN_HALF_CHANNELS and x.is_contiguous()):
             return ops.layernorm_gelu_half(x, self.weight, self.bias, self.eps, False)
         return super().forward(x)
 
@@ -104,8 +106,8 @@ class GroupNormAct2d(nn.GroupNorm):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         nhwc = x.permute(0, 2, 3, 1)
-        if x.is_cuda and self.weight.dtype == x.dtype and nhwc.is_contiguous() and ops.groupnorm_act_supported(
-                x.shape[1], self.num_groups, x.dtype):
+        if (x.is_cuda and self.weight.dtype == x.dtype and not ops.followed(x, self.weight, self.bias)
+                and nhwc.is_contiguous() and ops.groupnorm_act_supported(x.shape[1], self.num_groups, x.dtype)):
             return ops.groupnorm_act(nhwc, self.num_groups, self.weight, self.bias, self.eps, self.act).permute(0, 3, 1, 2)
         y = super().forward(x)
         return {"none": lambda t: t, "relu": F.relu, "gelu": F.gelu, "silu": F.silu}[self.act](y)
@@ -247,7 +249,9 @@ class DecoderAttention(nn.Module):
     """Multi-head attention whose q / k / v projections go down to
     embedding_dim / downsample_rate channels (the cross-attention layers use 2). On
     CUDA tensors computed by ssam_cross_attn (fp16, bf16, fp32; differentiable),
-    elsewhere by torch."""
+    elsewhere by torch: on other devices and dtypes, in scripts, and wherever torch
+    follows the program through its operators (traces, compilers, dispatch modes,
+    vmap and other transforms, forward-mode differentiation)."""
 
     def __init__(self, embedding_dim: int, num_heads: int, downsample_rate: int = 1):
         super().__init__()
@@ -265,16 +269,23 @@ class DecoderAttention(nn.Module):
         b, n, c = x.shape
         return x.view(b, n, self.num_heads, c // self.num_heads)
 
+    def _by_kernel(self, qh: torch.Tensor, kh: torch.Tensor, vh: torch.Tensor) -> bool:
+        if (not qh.is_cuda or torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack()
+                or ops.followed(qh, kh, vh)):
+            return False
+        b, _, h, c = qh.shape
+        return (b == kh.shape[0] and kh.shape == vh.shape and b <= ops.CROSS_ATTN_MAX_BATCH
+                and ops.cross_attn_supported(h, h, c, qh.dtype))
+
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                 key_lens: Optional[torch.Tensor] = None, key_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
         """key_lens (int32 (B,)) and key_mask (bool (B, Tk), True: attend) say which keys are
         there (a padded batch of prompts): what the others hold does not matter, and a query
         without keys gives out_proj's bias."""
         qh, kh, vh = self._split(self.q_proj(q)), self._split(self.k_proj(k)), self._split(self.v_proj(v))
-        h, c = qh.shape[2:]
-        if (qh.is_cuda and qh.shape[0] == kh.shape[0] <= ops.CROSS_ATTN_MAX_BATCH and kh.shape == vh.shape
-                and ops.cross_attn_supported(h, h, c, qh.dtype)):
-            return self.out_proj(ops.cross_attn(qh, kh, vh, key_lens=key_lens, key_mask=key_mask).flatten(2))
+        if not torch.jit.is_scripting():
+            if self._by_kernel(qh, kh, vh):
+                return self.out_proj(ops.cross_attn(qh, kh, vh, key_lens=key_lens, key_mask=key_mask).flatten(2))
         mask = key_mask
         if key_lens is not None:
             there = torch.arange(kh.shape[1], device=kh.device) < key_lens.view(-1, 1)

@@ -471,8 +471,15 @@ def layernorm_nchw(x: torch.Tensor, B: int, H: int, W: int, w: torch.Tensor, b: 
 
 
 # ---------------------------------------------------------------------------
-# The decoder's operators (differentiable once; csrc/torch_ops.cpp)
+# The decoder's operators (differentiable once, in reverse mode; csrc/torch_ops.cpp)
 # ---------------------------------------------------------------------------
+def followed(*tensors: torch.Tensor) -> bool:
+    """Whether something follows the program through torch's operators, which these are not: torch.jit.trace, make_fx, a
+    transform of torch.func, forward-mode differentiation, a tensor subclass or fake tensor among `tensors`. The calls
+    below are errors then; the modules of hq.py go to torch."""
+    return not _torch_ops().takes(tensors)
+
+
 LN_HALF_CHANNELS = (32, 64, 128, 256)
 _OPERATOR_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 

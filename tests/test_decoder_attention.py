@@ -54,7 +54,6 @@ def test_masked_places_hold_anything_where_torch_computes(cuda_device):
     assert all(torch.isfinite(g).all() for g in torch.autograd.grad(out.square().sum(), leaves))
 
 
-
 def test_one_query_set_for_a_batch():
     mod, q, k, v = attention()
     near(mod(q[:1], k, v), mod(q[:1].expand(3, -1, -1), k, v))
