@@ -312,8 +312,8 @@ int ssam_layernorm_gelu_half_bwd(const void* x, const void* dout, int64_t rows, 
  *   mean, rstd : optional fp32 [N, groups], what the backward pass takes.
  * ssam_groupnorm_act_bwd: dx [N, HW, C], dw and db [C] for the output gradient dout;
  * dx may be dout. x, w, b, out, dout, dx and workspace are 16-byte aligned; C is a
- * multiple of 8 (fp32: 4) and of groups, at most 2048 (fp32: 1024), N at most 65535
- * (SSAM_ERR_UNSUPPORTED otherwise). workspace: ssam_groupnorm_act_workspace_size()
+ * multiple of 8 (fp32: 4) and of groups, at most 2048 (fp32: 1024), N at most 65535,
+ * HW below 2^31 (SSAM_ERR_UNSUPPORTED otherwise). workspace: ssam_groupnorm_act_workspace_size()
  * bytes (backward 0 / 1; 0 bytes: workspace may be NULL). Sums are taken in a fixed order: equal calls give equal bits.
  * No counterpart in the reference: the norm of the segmentation heads that follow
  * the SAM3 encoder (convolution -> GroupNorm -> ReLU).

@@ -96,7 +96,8 @@ class GroupNormAct2d(nn.GroupNorm):
     """nn.GroupNorm of an NCHW map (same parameters) with an activation of ops.ACTIVATIONS
     after it, the normalisation of convolutional segmentation heads. On CUDA
     channels-last maps of one dtype with the parameters computed by
-    ssam_groupnorm_act (differentiable), elsewhere by torch."""
+    ssam_groupnorm_act (differentiable), elsewhere, and for more maps or positions than
+    that takes, by torch."""
 
     def __init__(self, num_groups: int, num_channels: int, eps: float = 1e-5, act: str = "none"):
         super().__init__(num_groups, num_channels, eps=eps, affine=True)
@@ -107,7 +108,8 @@ class GroupNormAct2d(nn.GroupNorm):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         nhwc = x.permute(0, 2, 3, 1)
         if (x.is_cuda and self.weight.dtype == x.dtype and not ops.followed(x, self.weight, self.bias)
-                and nhwc.is_contiguous() and ops.groupnorm_act_supported(x.shape[1], self.num_groups, x.dtype)):
+                and nhwc.is_contiguous() and ops.groupnorm_act_supported(x.shape[1], self.num_groups, x.dtype)
+                and x.shape[0] <= ops.GROUPNORM_MAX_BATCH and x.shape[2] * x.shape[3] <= ops.GROUPNORM_MAX_POSITIONS):
             return ops.groupnorm_act(nhwc, self.num_groups, self.weight, self.bias, self.eps, self.act).permute(0, 3, 1, 2)
         y = super().forward(x)
         return {"none": lambda t: t, "relu": F.relu, "gelu": F.gelu, "silu": F.silu}[self.act](y)

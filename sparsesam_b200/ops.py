@@ -497,6 +497,10 @@ def layernorm_gelu_half(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor, eps: 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
 
 
+GROUPNORM_MAX_BATCH = 65535
+GROUPNORM_MAX_POSITIONS = 2**31 - 1
+
+
 def groupnorm_act_supported(channels: int, groups: int, dtype: torch.dtype) -> bool:
     """Whether groupnorm_act takes these channels."""
     unit = 4 if dtype == torch.float32 else 8
@@ -506,7 +510,8 @@ def groupnorm_act_supported(channels: int, groups: int, dtype: torch.dtype) -> b
 
 def groupnorm_act(x: torch.Tensor, groups: int, w: torch.Tensor, b: torch.Tensor, eps: float = 1e-5,
                   act: str = "none") -> torch.Tensor:
-    """act(GroupNorm(x) * w + b) of channels-last maps x (N, ..., C): statistics over all
+    """act(GroupNorm(x) * w + b) of channels-last maps x (N, ..., C), N up to
+    GROUPNORM_MAX_BATCH and up to GROUPNORM_MAX_POSITIONS positions each: statistics over all
     positions and the C / groups channels of a group, per sample. act in ACTIVATIONS (gelu is
     the erf form). fp16, bf16 or fp32, one dtype for x, w (C,) and b (C,); C a multiple of 8
     (fp32: 4) and of groups, at most 2048 (fp32: 1024). Returns a new tensor of x's shape.

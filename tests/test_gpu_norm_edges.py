@@ -6,7 +6,7 @@ import pytest
 import torch
 from test_gpu_norms import DTYPES, EPS24, make, off_border, reference, run
 
-from sparsesam_b200 import ops
+from sparsesam_b200 import _lib, hq, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +77,16 @@ def test_gelu_of_large_values(cuda_device, dtype):
     u = torch.finfo(x.dtype).eps / 2
     ok = torch.isinf(want)
     assert torch.all(torch.where(ok, y.double() == want, (y.double() - want).abs() <= u * want.abs() + 2e-7))
+
+
+def test_more_maps_than_one_launch_takes(cuda_device):
+    """The operator refuses them; the module goes to torch."""
+    g = torch.Generator().manual_seed(3)
+    mod = hq.GroupNormAct2d(2, 8, act="silu").to(cuda_device)
+    x = torch.randn(65537, 8, 2, 3, generator=g).to(cuda_device).contiguous(memory_format=torch.channels_last)
+    with torch.no_grad():
+        whole, parts = mod(x), torch.cat([mod(t) for t in x.split(40000)])
+    # fp32 statistics of 24 values in two orders, on values of a few units
+    assert (whole - parts).abs().max() <= 32 * torch.finfo(torch.float32).eps
+    with pytest.raises(_lib.SparseSAMError):
+        ops.groupnorm_act(x.permute(0, 2, 3, 1), 2, mod.weight, mod.bias)
