@@ -10,8 +10,8 @@
  *     exception crosses this boundary. Calls only enqueue work: device-side
  *     failures (a bounded wait that ran out) are reported by ssam_device_error().
  *   - bf16 tensors are passed as `void*` holding IEEE bfloat16 values; fp32 as float*.
- *   - Calls are re-entrant: the only library globals are the device error flag
- *     and per-process caches of immutable launch configuration.
+ *   - Calls are re-entrant: the only library globals are the device error flag,
+ *     per-process caches of immutable launch configuration and a launch counter.
  *
  * Reference paths below are relative to the hchautran/SparseSAM repository.
  */
@@ -53,6 +53,11 @@ const char* ssam_status_string(int status);
 /* Synchronises the current device and returns the device-side error flag
  * (SSAM_OK when no kernel raised one). `reset` != 0 clears it. */
 int ssam_device_error(int reset);
+
+/* Kernels that the decoder's operators (ssam_layernorm_gelu_half*, ssam_groupnorm_act_*,
+ * ssam_cross_attn_*) have enqueued in this process; a captured call counts once, a
+ * replay not. How many a call takes depends on its sizes (no counterpart in the reference). */
+int64_t ssam_operator_launches(void);
 
 /* Diagnostic for integrators (no counterpart in the reference): enqueues one
  * small kernel whose bounded wait nothing satisfies, so it gives up after about

@@ -28,6 +28,7 @@ SIGNATURES: dict[str, tuple] = {
                                       c_ptr, c_ptr, c_ptr, c_ptr, c_ptr]),
     "ssam_a_shape_n_init": (c_int, [c_int, c_int, c_f64, c_int]),
     "ssam_a_shape_mask": (c_int, [c_int, c_int, c_int, c_int, c_int, c_ptr]),
+    "ssam_operator_launches": (c_i64, []),
     "ssam_check_wait_timeout": (c_int, [c_ptr]),
     "ssam_hilbert_order": (c_int, [c_int, c_int, c_ptr, c_ptr, c_ptr]),
     "ssam_sparse_attn_workspace_size": (c_size, [c_int, c_int, c_int, c_int]),
@@ -93,7 +94,8 @@ SSAM_EPI_F32 = 3
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 
-# Kernels each entry point enqueues (for launch accounting); host-only calls are 0.
+# Kernels each entry point enqueues (for launch accounting); host-only calls are 0, and the
+# decoder's operators count for themselves (ssam_operator_launches).
 KERNELS_PER_CALL = {
     "ssam_zorder": 1, "ssam_stripe_sort_perm": 1, "ssam_sparse_attn_fwd": 1, "ssam_keep_select": 1,
     "ssam_check_wait_timeout": 1, "ssam_hilbert_order": 1,
@@ -101,12 +103,18 @@ KERNELS_PER_CALL = {
     "ssam_patch_im2col": 1, "ssam_broadcast_rows": 1, "ssam_im2col3x3_nhwc": 1, "ssam_nhwc_to_nchw": 1,
     "ssam_conv3x3_nhwc": 1, "ssam_gemm_bf16_addend": 1,
     "ssam_layernorm_rows": 1, "ssam_layernorm_nchw": 1, "ssam_layernorm_rows_copy": 1, "ssam_split_bf16x2": 1,
-    "ssam_layernorm_gelu_half": 1,
     "ssam_rc_mlp_fwd_noalloc": 3,
     "ssam_split_bf16x3": 1, "ssam_patch_im2col_split3": 1, "ssam_window_of_raster": 1, "ssam_fill_pad_rows": 1,
     "ssam_zstride_keep": 1,
 }
-launch_count = 0  # kernels enqueued through call(), and calls of the decoder's operators, since import (read by bench.py)
+_called = 0  # kernels enqueued through call() since import
+
+
+def __getattr__(name: str):
+    """launch_count: kernels that the library has enqueued since import (read by bench.py)."""
+    if name == "launch_count":
+        return _called + (0 if _lib is None else _lib.ssam_operator_launches())
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 class SparseSAMError(RuntimeError):
@@ -168,10 +176,10 @@ def call(name: str, *args, launches: int | None = None) -> int:
 
     ``launches`` overrides the entry's kernel count for calls whose count depends
     on the arguments (the global-grid attention adds its bias pre-pass)."""
-    global launch_count
+    global _called
     fn = getattr(load(), name)
     st = fn(*args)
-    launch_count += KERNELS_PER_CALL.get(name, 0) if launches is None else launches
+    _called += KERNELS_PER_CALL.get(name, 0) if launches is None else launches
     if st != SSAM_OK:
         msg = load().ssam_status_string(st).decode()
         raise SparseSAMError(name, st, msg)

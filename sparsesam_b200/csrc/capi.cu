@@ -55,6 +55,8 @@ int ssam_device_error(int reset) {
   return v;
 }
 
+int64_t ssam_operator_launches(void) { return ssam::g_operator_launches.load(std::memory_order_relaxed); }
+
 int ssam_check_wait_timeout(void* stream) {
   ssam::wait_timeout_check_kernel<<<1, 32, 0, static_cast<cudaStream_t>(stream)>>>();
   return status_from_cuda(cudaGetLastError());

@@ -103,6 +103,8 @@ int make_tmap_2d_bf16(CUtensorMap* map, const void* base, uint64_t rows, uint64_
 
 int status_from_cuda(cudaError_t e);
 
+inline std::atomic<int64_t> g_operator_launches{0};   // see ssam_operator_launches()
+
 // Launches a kernel that begins with follow_previous (common.cuh), in clusters of `cluster` blocks along x. Its set-up
 // runs under the end of the kernel before it: calls one behind the other 6.4 -> 5.4 us (attention of one image), 9.5 ->
 // 7.3 (one long query), 8.2 -> 7.1 (GroupNorm of a map), the 13 kernels of a streamed GroupNorm's pass 264 -> 256.
@@ -121,7 +123,9 @@ int launch_following(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, i
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  return status_from_cuda(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
+  const int st = status_from_cuda(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
+  if (st == SSAM_OK) g_operator_launches.fetch_add(1, std::memory_order_relaxed);
+  return st;
 }
 
 // Entry points implemented in the per-kernel translation units.

@@ -334,7 +334,9 @@ static int launch_layernorm_half(const void* x, int64_t rows, const void* w, con
     layernorm_half_kernel<T, C, true><<<grid, kLnHalfThreads, 0, stream>>>(xp, rows, wp, bp, eps, op);
   else
     layernorm_half_kernel<T, C, false><<<grid, kLnHalfThreads, 0, stream>>>(xp, rows, wp, bp, eps, op);
-  return status_from_cuda(cudaGetLastError());
+  const int st = status_from_cuda(cudaGetLastError());
+  if (st == SSAM_OK) g_operator_launches.fetch_add(1, std::memory_order_relaxed);
+  return st;
 }
 
 template <typename T>

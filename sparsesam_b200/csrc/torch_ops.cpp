@@ -11,7 +11,6 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
-#include <atomic>
 #include <cmath>
 #include <cstdint>
 
@@ -34,13 +33,10 @@ struct StatusError : std::runtime_error {
         status(s) {}
 };
 
-std::atomic<int64_t> launches{0};   // kernels enqueued through this module
-
-void done(const char* fn, int status, int kernels) {
+void done(const char* fn, int status) {
   if (status != SSAM_OK) throw StatusError(fn, status);
-  launches += kernels;
 }
-#define SSAM_CALL(kernels, fn, ...) done(#fn, fn(__VA_ARGS__), kernels)
+#define SSAM_CALL(fn, ...) done(#fn, fn(__VA_ARGS__))
 
 void refuse(const std::string& why) { throw py::value_error(why); }
 
@@ -131,7 +127,7 @@ Tensor layernorm_run(const Tensor& x, const Tensor& w, const Tensor& b, double e
   const int64_t C = x.size(-1);
   if (x.numel() == 0) return out;
   const On on(x);
-  SSAM_CALL(1, ssam_layernorm_gelu_half, x.data_ptr(), x.numel() / C, static_cast<int>(C), w.data_ptr(), b.data_ptr(),
+  SSAM_CALL(ssam_layernorm_gelu_half, x.data_ptr(), x.numel() / C, static_cast<int>(C), w.data_ptr(), b.data_ptr(),
             static_cast<float>(eps), static_cast<int>(gelu), dtype_code(x.scalar_type()), out.data_ptr(), on.stream);
   return out;
 }
@@ -159,7 +155,7 @@ struct LayerNormGelu : torch::autograd::Function<LayerNormGelu> {
         const size_t n = ssam_layernorm_gelu_half_bwd_workspace_size(rows, C);
         const Tensor ws = at::empty({static_cast<int64_t>(n)}, x.options().dtype(at::kByte));
         const On on(x);
-        SSAM_CALL(2, ssam_layernorm_gelu_half_bwd, x.data_ptr(), dout.data_ptr(), rows, C, w.data_ptr(), b.data_ptr(),
+        SSAM_CALL(ssam_layernorm_gelu_half_bwd, x.data_ptr(), dout.data_ptr(), rows, C, w.data_ptr(), b.data_ptr(),
                   static_cast<float>(ctx->saved_data["eps"].toDouble()), static_cast<int>(ctx->saved_data["gelu"].toInt()),
                   dtype_code(x.scalar_type()), out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), ws.data_ptr(), n,
                   on.stream);
@@ -208,7 +204,7 @@ Tensor groupnorm_run(const Tensor& x, int groups, const Tensor& w, const Tensor&
   Tensor ws;
   if (n) ws = at::empty({static_cast<int64_t>(n)}, x.options().dtype(at::kByte));
   const On on(x);
-  SSAM_CALL(n ? 2 : 1, ssam_groupnorm_act_fwd, x.data_ptr(), s.N, s.HW, s.C, groups, w.data_ptr(), b.data_ptr(),
+  SSAM_CALL(ssam_groupnorm_act_fwd, x.data_ptr(), s.N, s.HW, s.C, groups, w.data_ptr(), b.data_ptr(),
             static_cast<float>(eps), act, dt, out.data_ptr(), mean,
             mean == nullptr ? nullptr : mean + static_cast<int64_t>(s.N) * groups, ptr(ws), n, on.stream);
   return out;
@@ -241,7 +237,7 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
         const Tensor ws = at::empty({static_cast<int64_t>(n)}, x.options().dtype(at::kByte));
         const float* mean = saved[3].data_ptr<float>();
         const On on(x);
-        SSAM_CALL(2, ssam_groupnorm_act_bwd, x.data_ptr(), dout.data_ptr(), s.N, s.HW, s.C, groups, w.data_ptr(),
+        SSAM_CALL(ssam_groupnorm_act_bwd, x.data_ptr(), dout.data_ptr(), s.N, s.HW, s.C, groups, w.data_ptr(),
                   b.data_ptr(), mean, mean + static_cast<int64_t>(s.N) * groups, static_cast<int>(ctx->saved_data["act"].toInt()),
                   dt, out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), ws.data_ptr(), n, on.stream);
       }
@@ -308,7 +304,7 @@ Tensor attn_run(const Tensor& q, const Tensor& k, const Tensor& v, double scale,
   }
   const Strides st(q, k, v, out);
   const On on(q);
-  SSAM_CALL(1, ssam_cross_attn_fwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), st.s, s.B, s.Tq, s.Tk, s.H, s.Hk, s.D, s.dt,
+  SSAM_CALL(ssam_cross_attn_fwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), st.s, s.B, s.Tq, s.Tk, s.H, s.Hk, s.D, s.dt,
             static_cast<float>(scale), static_cast<const int32_t*>(ptr(lens)), static_cast<const uint8_t*>(ptr(mask)),
             out.data_ptr(), s.dt == 2 ? nullptr : static_cast<float*>(ptr(*out32)), static_cast<float*>(ptr(*stats)),
             on.stream);
@@ -346,7 +342,7 @@ struct CrossAttn : torch::autograd::Function<CrossAttn> {
         const Strides st(q, k, v, dout);
         float* lse = static_cast<float*>(ptr(stats));
         const On on(q);
-        SSAM_CALL(stats.defined() ? 2 : 1, ssam_cross_attn_bwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(),
+        SSAM_CALL(ssam_cross_attn_bwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(),
                   st.s, s.B, s.Tq, s.Tk, s.H, s.Hk, s.D, s.dt, static_cast<float>(ctx->saved_data["scale"].toDouble()),
                   static_cast<const int32_t*>(ptr(saved[5])), static_cast<const uint8_t*>(ptr(saved[6])),
                   static_cast<const float*>(ptr(out32)), lse,
@@ -410,5 +406,4 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("groupnorm_act", &groupnorm_act);
   m.def("cross_attn", &cross_attn);
   m.def("takes", &takes);
-  m.def("launches", [] { return launches.load(); });
 }

@@ -489,9 +489,7 @@ def layernorm_gelu_half(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor, eps: 
     """Channel LayerNorm (+ exact GELU) of fp16 / bf16 channels-last rows (..., C),
     C in LN_HALF_CHANNELS; w, b of x's dtype. Returns a new tensor of x's shape.
     Differentiable in x, w and b."""
-    out = _torch_ops().layernorm_gelu_half(x, w, b, eps, gelu)
-    _lib.launch_count += 1
-    return out
+    return _torch_ops().layernorm_gelu_half(x, w, b, eps, gelu)
 
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
@@ -519,9 +517,7 @@ def groupnorm_act(x: torch.Tensor, groups: int, w: torch.Tensor, b: torch.Tensor
     code = ACTIVATIONS.get(act)
     if code is None:
         raise ValueError(f"act must be one of {tuple(ACTIVATIONS)}, got {act!r}")
-    out = _torch_ops().groupnorm_act(x, groups, w, b, eps, code)
-    _lib.launch_count += 1
-    return out
+    return _torch_ops().groupnorm_act(x, groups, w, b, eps, code)
 
 
 CROSS_ATTN_MAX_DIM = 128
@@ -545,9 +541,7 @@ def cross_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: floa
     key_lens (int32 (B,)) and key_mask (bool (B, Tk), True: attend) say which keys are
     there: what the others hold does not matter, and a query without keys gives zeros.
     Differentiable in q, k and v."""
-    out = _torch_ops().cross_attn(q, k, v, scale, key_lens, key_mask)
-    _lib.launch_count += 1
-    return out
+    return _torch_ops().cross_attn(q, k, v, scale, key_lens, key_mask)
 
 
 def split_bf16x2(x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
