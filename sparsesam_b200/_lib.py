@@ -142,7 +142,7 @@ def load() -> ctypes.CDLL:
                 raise RuntimeError(
                     f"{path} is missing: build it with `python -m sparsesam_b200.build` "
                     "(or __graft_entry__.build()); there is no fallback implementation")
-            handle = ctypes.CDLL(path, mode=ctypes.RTLD_GLOBAL)   # _torch_ops finds the entry points here
+            handle = ctypes.CDLL(path)
             for name, (res, args) in SIGNATURES.items():
                 fn = getattr(handle, name, None)
                 if fn is None:

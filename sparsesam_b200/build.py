@@ -2,9 +2,9 @@
 
 The library is a plain C-ABI shared object (no torch headers), linked from the
 translation units UNITS, which are compiled at the same time. Beside it the Python
-extension module _torch_ops (csrc/torch_ops.cpp, torch headers, no device code) gives
-the decoder's operators their torch form. Both are rebuilt when any csrc/ or include/
-file is newer than they are.
+extension module _torch_ops (csrc/torch_ops.cpp, torch headers, no device code; linked to
+the library, which it finds beside itself) gives the decoder's operators their torch
+form. Both are rebuilt when any csrc/ or include/ file is newer than they are.
 """
 from __future__ import annotations
 
@@ -49,19 +49,20 @@ def _sources() -> list[str]:
     return out
 
 
-def _torch_ops_command(out: str) -> list[str]:
-    """Compile and link _torch_ops against this interpreter's torch and, found beside it, the library."""
+def _torch_ops_commands(obj: str, lib: str, out: str) -> tuple[list[str], list[str]]:
+    """Compile _torch_ops, and link it against this interpreter's torch and the library `lib`."""
     import sysconfig
 
     import torch
     root = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(_nvcc()))
-    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=_torch_ops",
-            "-I", os.path.join(root, "include"), "-I", os.path.join(root, "include", "torch", "csrc", "api", "include"),
-            "-I", os.path.join(cuda, "include"), "-I", sysconfig.get_paths()["include"], "-I", INCLUDE,
-            "-o", out, os.path.join(CSRC, "torch_ops.cpp"),
-            "-L", os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+    return (["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=_torch_ops",
+             "-I", os.path.join(root, "include"), "-I", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+             "-I", os.path.join(cuda, "include"), "-I", sysconfig.get_paths()["include"], "-I", INCLUDE,
+             "-c", "-o", obj, os.path.join(CSRC, "torch_ops.cpp")],
+            ["g++", "-shared", "-o", out, obj, lib, "-Wl,-rpath,$ORIGIN",
+             "-L", os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"])
 
 
 def needs_build() -> bool:
@@ -89,11 +90,12 @@ def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | N
         objects = [os.path.join(work, unit + ".o") for unit in UNITS]
         units = [[_nvcc(), *NVCC_FLAGS, *(extra_flags or []), "-I", INCLUDE, "-c", "-o", obj, os.path.join(CSRC, unit)]
                  for unit, obj in zip(UNITS, objects)]
-        # the module's references to the library are resolved when it is loaded, after the library
-        units.append(_torch_ops_command(tmp_ops))
+        compile_ops, link_ops = _torch_ops_commands(os.path.join(work, "torch_ops.o"), tmp, tmp_ops)
+        units.append(compile_ops)
         with ThreadPoolExecutor(len(units)) as pool:
             list(pool.map(run, units))
-        run([_nvcc(), *NVCC_FLAGS, "-shared", "-o", tmp, *objects])
+        run([_nvcc(), *NVCC_FLAGS, "-shared", "-Xlinker", f"-soname={LIB_NAME}", "-o", tmp, *objects])
+        run(link_ops)
     os.replace(tmp, LIB_PATH)
     os.replace(tmp_ops, TORCH_OPS_PATH)
     return LIB_PATH

@@ -91,3 +91,16 @@ def test_rc_mlp_workspace_size():
     sz = lib.ssam_rc_mlp_workspace_size(n, C, Hd)
     assert sz >= n * (C + Hd) * 2 and sz % 256 == 0
     assert lib.ssam_rc_mlp_workspace_size(0, C, Hd) == 0
+
+
+def test_loading_leaves_the_global_scope_alone():
+    """The library's names (a few hundred mangled ones beside the C ABI) resolve for nothing but itself and _torch_ops."""
+    import subprocess
+    import sys
+    code = ("import ctypes\nfrom sparsesam_b200 import _lib\n_lib.load(); _lib.torch_ops()\n"
+            "assert not hasattr(ctypes.CDLL(None), 'ssam_version')\n"
+            "maps = {l.split()[-1] for l in open('/proc/self/maps') if 'sparsesam_b200' in l}\n"
+            "assert sorted(m.rsplit('/', 1)[1] for m in maps) == ['_torch_ops.so', 'libsparsesam_b200.so'], maps\n")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    res = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=root)
+    assert res.returncode == 0, res.stderr
