@@ -81,7 +81,7 @@ def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | N
             print(" ".join(cmd), file=sys.stderr)
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
-            raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+            raise RuntimeError(f"{os.path.basename(cmd[0])} failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
         if verbose and (res.stdout or res.stderr):
             print(res.stdout, res.stderr, file=sys.stderr)
 
