@@ -1,10 +1,11 @@
 """Calls of ops.groupnorm_act and of the half LayerNorm's gradient that random inputs do not make: values that are not
-finite beside ones that are. Bounds as derived in test_gpu_norms.py."""
+finite beside ones that are, samples cut into several launches, ReLU's parameter gradients without its border. Bounds as
+derived in test_gpu_norms.py."""
 import math
 
 import pytest
 import torch
-from test_gpu_norms import DTYPES, EPS24, make, off_border, reference, run
+from test_gpu_norms import DTYPES, EPS24, check, make, off_border, reference, run
 
 from sparsesam_b200 import _lib, hq, ops
 
@@ -77,6 +78,26 @@ def test_gelu_of_large_values(cuda_device, dtype):
     u = torch.finfo(x.dtype).eps / 2
     ok = torch.isinf(want)
     assert torch.all(torch.where(ok, y.double() == want, (y.double() - want).abs() <= u * want.abs() + 2e-7))
+
+
+@pytest.mark.parametrize("act", ["none", "gelu"])
+@pytest.mark.parametrize("dtype,C", [("fp16", 512), ("bf16", 512), ("fp32", 256)])
+def test_groupnorm_in_several_launches(cuda_device, dtype, C, act):
+    """Five samples of 18 MB: two launches of up to three forward, three of up to two backward."""
+    x, w, b, do = make(cuda_device, (5, 132, 136, C), dtype)
+    x += torch.arange(5, device=cuda_device).view(5, 1, 1, 1) / 4           # every sample its own mean
+    check(run(lambda x, w, b: ops.groupnorm_act(x, 8, w, b, 1e-5, act), x, w, b, do), reference(x, 8, w, b, 1e-5, act, do), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("shape,groups", [((1, 64, 64, 256), 8), ((2, 200, 200, 64), 8), ((3, 67, 45, 96), 4)],
+                         ids=lambda s: str(s).replace(" ", ""))
+def test_relu_parameter_gradients(cuda_device, shape, groups, dtype):
+    """No gradient comes in where ReLU's input is within rounding of zero: the sums then have their ordinary bound."""
+    x, w, b, do = make(cuda_device, shape, dtype)
+    do = torch.where(off_border(x, groups, w, b, 1e-5), torch.zeros_like(do), do)
+    check(run(lambda x, w, b: ops.groupnorm_act(x, groups, w, b, 1e-5, "relu"), x, w, b, do),
+          reference(x, groups, w, b, 1e-5, "relu", do), dtype)
 
 
 def test_more_maps_than_one_launch_takes(cuda_device):
