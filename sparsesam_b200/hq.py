@@ -247,13 +247,29 @@ class PromptEncoder(nn.Module):
 # ---------------------------------------------------------------------------
 # Two-way transformer
 # ---------------------------------------------------------------------------
+def _kernel_not_slower(b: int, h: int, tq: int, tk: int, c: int, dtype: torch.dtype) -> bool:
+    """Where DecoderAttention takes ssam_cross_attn and where torch's fused attention, by measurement of both over
+    8 .. 4096 queries and keys (B200, 1 and 64 batch entries; device us, kernel / torch, with 64 entries). The kernels
+    are made for a short side next to a long one: half, 8 x 4096, heads of 16 27 / 145, 4096 x 8 31 / 311; fp32 92 / 822.
+    Two longer sides are torch's: half, 64 x 64 of 32 channels 28 / 6, 1000 x 1000 48 / 28 (8 entries); fp32, 64 x 64 of
+    64 channels three times as long. Small calls are the host's: 6 us here, 19 for torch's."""
+    short, long = min(tq, tk), max(tq, tk)
+    if b * h * tq * tk <= 1 << 15:
+        return True
+    if dtype == torch.float32:
+        return c <= 16 or short <= (32 if c <= 32 else 16 if c <= 64 else 8) or (c <= 32 and long >= 1024)
+    return (short <= (16 if c <= 64 else 8) or (c <= 64 and long <= 32)
+            or (short <= 128 and (c <= 16 or long >= (1024 if c <= 64 else 4096))))
+
+
 class DecoderAttention(nn.Module):
     """Multi-head attention whose q / k / v projections go down to
     embedding_dim / downsample_rate channels (the cross-attention layers use 2). On
     CUDA tensors computed by ssam_cross_attn (fp16, bf16, fp32; differentiable),
-    elsewhere by torch: on other devices and dtypes, in scripts, and wherever torch
-    follows the program through its operators (traces, compilers, dispatch modes,
-    vmap and other transforms, forward-mode differentiation)."""
+    elsewhere by torch: on other devices and dtypes, for sizes without a mask at which
+    torch's is faster, in scripts, and wherever torch follows the program through its
+    operators (traces, compilers, dispatch modes, vmap and other transforms,
+    forward-mode differentiation)."""
 
     def __init__(self, embedding_dim: int, num_heads: int, downsample_rate: int = 1):
         super().__init__()
@@ -271,13 +287,14 @@ class DecoderAttention(nn.Module):
         b, n, c = x.shape
         return x.view(b, n, self.num_heads, c // self.num_heads)
 
-    def _by_kernel(self, qh: torch.Tensor, kh: torch.Tensor, vh: torch.Tensor) -> bool:
+    def _by_kernel(self, qh: torch.Tensor, kh: torch.Tensor, vh: torch.Tensor, masked: bool) -> bool:
         if (not qh.is_cuda or torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack()
                 or ops.followed(qh, kh, vh)):
             return False
-        b, _, h, c = qh.shape
+        b, n, h, c = qh.shape
         return (b == kh.shape[0] and kh.shape == vh.shape and b <= ops.CROSS_ATTN_MAX_BATCH
-                and ops.cross_attn_supported(h, h, c, qh.dtype))
+                and ops.cross_attn_supported(h, h, c, qh.dtype)
+                and (masked or _kernel_not_slower(b, h, n, kh.shape[1], c, qh.dtype)))
 
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                 key_lens: Optional[torch.Tensor] = None, key_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -286,7 +303,7 @@ class DecoderAttention(nn.Module):
         without keys gives out_proj's bias."""
         qh, kh, vh = self._split(self.q_proj(q)), self._split(self.k_proj(k)), self._split(self.v_proj(v))
         if not torch.jit.is_scripting():
-            if self._by_kernel(qh, kh, vh):
+            if self._by_kernel(qh, kh, vh, key_lens is not None or key_mask is not None):
                 return self.out_proj(ops.cross_attn(qh, kh, vh, key_lens=key_lens, key_mask=key_mask).flatten(2))
         mask = key_mask
         if key_lens is not None:

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from sparsesam_b200 import hq
+from sparsesam_b200 import _lib, hq
 
 gpu = pytest.mark.gpu
 LENS = torch.tensor([25, 0, 7], dtype=torch.int32)
@@ -63,3 +63,22 @@ def test_one_query_set_for_a_batch():
 def test_one_query_set_for_a_batch_on_the_gpu(cuda_device):
     mod, q, k, v = attention(cuda_device)
     near(mod(q[:1], k, v), mod(q[:1].expand(3, -1, -1), k, v))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("tq,tk,dim,kernel", [(8, 4096, 128, True), (4096, 8, 128, True), (64, 64, 256, False), (9, 9, 256, True),
+                                              (1000, 1000, 512, False)])
+def test_sizes_go_where_they_are_faster(cuda_device, tq, tk, dim, kernel, dtype):
+    """Sizes that torch's attention took less time for before the kernels came still go there, unless there is a mask."""
+    torch.manual_seed(4)
+    mod = hq.DecoderAttention(dim, 8).to(cuda_device, dtype)
+    q, k = torch.randn(16, tq, dim, device=cuda_device, dtype=dtype), torch.randn(16, tk, dim, device=cuda_device, dtype=dtype)
+    lens = torch.full((16,), tk, dtype=torch.int32, device=cuda_device)
+    with torch.no_grad():
+        n0 = _lib.launch_count
+        plain = mod(q, k, k)
+        assert (_lib.launch_count > n0) == kernel
+        n0 = _lib.launch_count
+        near(mod(q, k, k, key_lens=lens), plain, dtype)
+        assert _lib.launch_count > n0
