@@ -122,3 +122,17 @@ def test_half_norms_are_traced_and_mapped(cuda_device, name):
     near(traced(x), want, torch.float16)
     near(traced(x * 2 - 1), mod(x * 2 - 1), torch.float16)
     near(torch.vmap(mod)(torch.stack([x, x + 1]))[0], want, torch.float16)
+
+
+@gpu
+@pytest.mark.parametrize("name", ["norm2d", "rows", "group"])
+def test_half_norms_run_under_a_compiler(cuda_device, name):
+    """Not as one graph: the operators are called between two."""
+    torch.manual_seed(0)
+    mod, x = {"norm2d": (hq.LayerNorm2d(64, gelu=True), torch.randn(2, 64, 5, 6)),
+              "rows": (hq.RowLayerNorm(64), torch.randn(2, 9, 64)),
+              "group": (hq.GroupNormAct2d(8, 64, act="silu"), torch.randn(2, 64, 5, 6))}[name]
+    mod, x = mod.to(cuda_device, torch.float16), x.to(cuda_device, torch.float16)
+    if x.dim() == 4:
+        x = x.contiguous(memory_format=torch.channels_last)
+    near(torch.compile(mod, backend="eager")(x) + 1, mod(x) + 1, torch.float16)
