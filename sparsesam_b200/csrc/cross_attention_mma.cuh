@@ -17,10 +17,14 @@
 //
 // Second factors: probabilities and dS are fp32 and enter their product as two half
 // terms (value and remainder), so that a result carries one rounding to its type instead
-// of two. A single term measured 1.4 times the error of the rounded definition. For fp16
-// inputs too these products run in bf16, which has fp32's exponents: a probability below
-// fp16's 2^-24 counts where the larger ones meet zeros. The fp16 factor then enters as two
-// bf16 terms (exact, 11 bits = 8 + 3), without the product of the two remainders (2^-18).
+// of two. A single term measured 1.4 times the error of the rounded definition.
+//
+// fp16 ends at 2^-24, and a key of small weight counts where the larger ones meet zeros.
+// So P enters times 2^12 to 2^15, its remainder times another 2^11, in a product of its
+// own that joins the first one's sums times 2^-11: 22 bits of every weight down to 2^-26,
+// and 2^-48 of the largest at the end. dS has no fixed scale at all (it follows the loss):
+// its products run in bf16, which has fp32's range: two bf16 terms of dS, the fp16 factor
+// as two bf16 terms (exact, 11 bits = 8 + 3), without the product of the two remainders.
 #pragma once
 
 #include "cross_attention.cuh"
@@ -90,16 +94,23 @@ constexpr bool kIsHalf = false;
 template <>
 constexpr bool kIsHalf<__half> = true;
 
-// A pair of T as bf16 terms: cut off after 8 bits, so that both terms take no rounding instructions
+// P, scaled, as two terms of T: the remainder of fp16 in units of 2^-11
 template <class T>
-__device__ __forceinline__ void bf16_terms(uint32_t x, uint32_t& hi, uint32_t& lo) {
+__device__ __forceinline__ void p_terms(float x, float y, uint32_t& hi, uint32_t& lo) {
   if constexpr (kIsHalf<T>) {
-    const float2 f = Mma<__half>::unpack(x);
-    hi = __byte_perm(__float_as_uint(f.x), __float_as_uint(f.y), 0x7632);
-    const float2 h = Mma<__nv_bfloat16>::unpack(hi), r = add2(f, make_float2(-h.x, -h.y));
-    lo = __byte_perm(__float_as_uint(r.x), __float_as_uint(r.y), 0x7632);
+    hi = Mma<T>::pack(x, y);
+    const float2 h = Mma<T>::unpack(hi), r = mul2(add2(make_float2(x, y), make_float2(-h.x, -h.y)), make_float2(2048.f, 2048.f));
+    lo = Mma<T>::pack(r.x, r.y);
   } else {
-    hi = x, lo = 0u;
+    split2<T>(x, y, hi, lo);
+  }
+}
+// acc (the remainders' product so far) in units of the values
+template <class T>
+__device__ __forceinline__ void lo_to_hi(float (&acc)[4]) {
+  if constexpr (kIsHalf<T>) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] *= 1.f / 2048.f;
   }
 }
 
@@ -155,7 +166,12 @@ __device__ __forceinline__ int64_t row_dense(const XAttn& a, int b, int n, int r
 }
 
 constexpr float kXmNone = -3.402823466e38f;  // reference before the first key: no finite logit is below it
-constexpr float kXmSlack = 8.f;
+// The reference is kXmBelow<T> below the maximum that it was taken at, and renewed when a logit is kXmSlack<T> above it:
+// exponentials end at 2^8, for fp16 at 2^15, of which 2^12 is the scale of its terms.
+template <class T>
+constexpr float kXmBelow = kIsHalf<T> ? 12.f : 0.f;
+template <class T>
+constexpr float kXmSlack = kIsHalf<T> ? 15.f : 8.f;
 
 // ---------------------------------------------------------------------------
 // Forward, few query rows (8 NQ per block) on many keys. The short side is the column
@@ -176,7 +192,6 @@ constexpr float kXmSlack = 8.f;
 template <class T, int DP, int NQ, int HP>
 __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NQ, 1>) xattn_fwd_few_rows(const XAttn args, int) {
   const XAttn a = follow(args, args.lse == nullptr);
-  using B16 = Mma<__nv_bfloat16>;
   constexpr int NR = DP / 8, NU = NR / 2;    // 8- and 16-channel blocks
   constexpr int KM = DP <= 32 && HP * NQ <= 4 ? 2 : 1;   // 16-key tiles per step
   extern __shared__ __align__(16) float xsm[];
@@ -284,7 +299,7 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NQ, 1>) xattn_f
         for (int x = 0; x < KM; ++x)
 #pragma unroll
           for (int h = 0; h < 2; ++h) m.x = fmaxf(m.x, s[z][i][x][h].x), m.y = fmaxf(m.y, s[z][i][x][h].y);
-        renew |= m.x > ref[z][i].x + kXmSlack || m.y > ref[z][i].y + kXmSlack;
+        renew |= m.x > ref[z][i].x + kXmSlack<T> || m.y > ref[z][i].y + kXmSlack<T>;
       }
     if (__any_sync(0xffffffffu, renew)) {
 #pragma unroll
@@ -301,6 +316,8 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NQ, 1>) xattn_f
             m.x = fmaxf(m.x, __shfl_xor_sync(0xffffffffu, m.x, w));
             m.y = fmaxf(m.y, __shfl_xor_sync(0xffffffffu, m.y, w));
           }
+          // not below the old one: the other queries' renewals must not lower it
+          m.x = fmaxf(m.x - kXmBelow<T>, ref[z][i].x), m.y = fmaxf(m.y - kXmBelow<T>, ref[z][i].y);
           const float2 f = make_float2(ex2f(ref[z][i].x - m.x), ex2f(ref[z][i].y - m.y));
           ref[z][i] = m;
           l[z][i] = mul2(l[z][i], f);
@@ -320,25 +337,27 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NQ, 1>) xattn_f
             float2 p = add2(s[z][i][x][h], make_float2(-ref[z][i].x, -ref[z][i].y));
             p.x = ex2f(p.x), p.y = ex2f(p.y);
             l[z][i] = add2(l[z][i], p);
-            split2<__nv_bfloat16>(p.x, p.y, hi[z][i][h], lo[z][i][h]);
+            p_terms<T>(p.x, p.y, hi[z][i][h], lo[z][i][h]);
             hi[z][i][h] = movm(hi[z][i][h]), lo[z][i][h] = movm(lo[z][i][h]);
           }
 #pragma unroll
-      for (int u = 0; u < NU; ++u) {
-        uint32_t vh[2][2], vl[2][2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) bf16_terms<T>(vt[x][h][2 * u + e], vh[h][e], vl[h][e]);
+      for (int u = 0; u < NU; ++u)
 #pragma unroll
         for (int z = 0; z < HP; ++z)
 #pragma unroll
           for (int i = 0; i < NQ; ++i) {
-            B16::run(o[z][i][u], vh[0][0], vh[0][1], vh[1][0], vh[1][1], hi[z][i][0], hi[z][i][1]);
-            B16::run(o[z][i][u], vh[0][0], vh[0][1], vh[1][0], vh[1][1], lo[z][i][0], lo[z][i][1]);
-            if constexpr (kIsHalf<T>) B16::run(o[z][i][u], vl[0][0], vl[0][1], vl[1][0], vl[1][1], hi[z][i][0], hi[z][i][1]);
+            float(&acc)[4] = o[z][i][u];
+            const uint32_t(&va)[2][NR] = vt[x];
+            if constexpr (kIsHalf<T>) {
+              float rest[4] = {0.f, 0.f, 0.f, 0.f};
+              Mma<T>::run(rest, va[0][2 * u], va[0][2 * u + 1], va[1][2 * u], va[1][2 * u + 1], lo[z][i][0], lo[z][i][1]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[e] = fmaf(rest[e], 1.f / 2048.f, acc[e]);
+            } else {
+              Mma<T>::run(acc, va[0][2 * u], va[0][2 * u + 1], va[1][2 * u], va[1][2 * u + 1], lo[z][i][0], lo[z][i][1]);
+            }
+            Mma<T>::run(acc, va[0][2 * u], va[0][2 * u + 1], va[1][2 * u], va[1][2 * u + 1], hi[z][i][0], hi[z][i][1]);
           }
-      }
     }
   }
 
@@ -431,8 +450,8 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NQ, 1>) xattn_f
 template <class T, int DP, int NK, int HP>
 __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NK, 2>) xattn_fwd_few_keys(const XAttn args, int chunks) {
   const XAttn a = follow(args, false);
-  using B16 = Mma<__nv_bfloat16>;
   constexpr int NR = DP / 8;
+  constexpr float kP = kIsHalf<T> ? 16384.f : 1.f;       // P is at most 1
   const int lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   const int units = a.heads / HP;
   const int64_t w = static_cast<int64_t>(blockIdx.x) * kXmWarps + threadIdx.x / 32;
@@ -454,7 +473,7 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NK, 2>) xattn_f
   float* lse = a.lse == nullptr ? nullptr : a.lse + (static_cast<int64_t>(b) * a.heads + h) * a.Tq;
   float* o32 = a.out_f32 == nullptr ? nullptr : a.out_f32 + (static_cast<int64_t>(b) * a.Tq * a.heads + h) * a.d + t * (DP / 4);
 
-  uint32_t k[HP][NK][NR], v[NK][NR], vl[kIsHalf<T> ? NK : 1][NR], q[2][NR];   // vl: remainders
+  uint32_t k[HP][NK][NR], v[NK][NR], q[2][NR];
   float2 bias[NK];                           // of keys 8 i + 2t, + 1
   int q_end = r_end;                         // rows past it are zeros
   auto load_q = [&](int r) {
@@ -477,9 +496,7 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NK, 2>) xattn_f
     bias[i].y = __shfl_sync(0xffffffffu, mine, 8 * t + 4);
 #pragma unroll
     for (int c = 0; c < NR; ++c) {
-      uint32_t rest;
-      bf16_terms<T>(movm(y[c]), v[i][c], rest);
-      if constexpr (kIsHalf<T>) vl[i][c] = rest;
+      v[i][c] = movm(y[c]);
 #pragma unroll
       for (int z = 0; z < HP; ++z) k[z][i][c] = HP == 1 || t / 2 == z ? x[c] : 0u;
     }
@@ -539,30 +556,30 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NK, 2>) xattn_f
         y += __shfl_xor_sync(0xffffffffu, y, 1);
         y += __shfl_xor_sync(0xffffffffu, y, 2);
         l[z][e] = y;
-        inv[e] = y == 0.f ? 0.f : rcp_fast(y);
+        inv[e] = y == 0.f ? 0.f : kP * rcp_fast(y);
       }
+      constexpr int PAIR = NK > 1 ? 2 : 1;
+      uint32_t hi[NK / PAIR][4], lo[NK / PAIR][4];
 #pragma unroll
-      for (int i = 0; i < NK; i += 2) {
-        uint32_t hi[4], lo[4];
+      for (int i = 0; i < NK; ++i)
 #pragma unroll
-        for (int x = 0; x < (NK > 1 ? 2 : 1); ++x)
+        for (int e = 0; e < 2; ++e) {
+          const float2 p = mul2(s[z][i][e], make_float2(inv[e], inv[e]));
+          p_terms<T>(p.x, p.y, hi[i / PAIR][2 * (i % PAIR) + e], lo[i / PAIR][2 * (i % PAIR) + e]);
+        }
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float2 p = mul2(s[z][i + x][e], make_float2(inv[e], inv[e]));
-            split2<__nv_bfloat16>(p.x, p.y, hi[2 * x + e], lo[2 * x + e]);
-          }
+      for (int c = 0; c < NR; ++c) {
+        float(&acc)[4] = o[z][c];
+        if constexpr (NK == 1) {
+          Mma<T>::run8(acc, lo[0][0], lo[0][1], v[0][c]);
+          lo_to_hi<T>(acc);
+          Mma<T>::run8(acc, hi[0][0], hi[0][1], v[0][c]);
+        } else {
 #pragma unroll
-        for (int c = 0; c < NR; ++c) {
-          float(&oc)[4] = o[z][c];
-          if constexpr (NK == 1) {
-            B16::run8(oc, hi[0], hi[1], v[0][c]);
-            B16::run8(oc, lo[0], lo[1], v[0][c]);
-            if constexpr (kIsHalf<T>) B16::run8(oc, hi[0], hi[1], vl[0][c]);
-          } else {
-            B16::run(oc, hi[0], hi[1], hi[2], hi[3], v[i][c], v[i + 1][c]);
-            B16::run(oc, lo[0], lo[1], lo[2], lo[3], v[i][c], v[i + 1][c]);
-            if constexpr (kIsHalf<T>) B16::run(oc, hi[0], hi[1], hi[2], hi[3], vl[i][c], vl[i + 1][c]);
-          }
+          for (int i = 0; i < NK / 2; ++i) Mma<T>::run(acc, lo[i][0], lo[i][1], lo[i][2], lo[i][3], v[2 * i][c], v[2 * i + 1][c]);
+          lo_to_hi<T>(acc);
+#pragma unroll
+          for (int i = 0; i < NK / 2; ++i) Mma<T>::run(acc, hi[i][0], hi[i][1], hi[i][2], hi[i][3], v[2 * i][c], v[2 * i + 1][c]);
         }
       }
     }
@@ -572,6 +589,12 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NK, 2>) xattn_f
       for (int c = 0; c < NR; ++c)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[0][c][e] = t / 2 == 0 ? o[0][c][e] : o[1][c][e];
+    }
+    if constexpr (kIsHalf<T>) {
+#pragma unroll
+      for (int c = 0; c < NR; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[0][c][e] *= 1.f / kP;
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -597,10 +620,11 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NK, 2>) xattn_f
 }
 
 // ---------------------------------------------------------------------------
-// Backward. With p = 2^(c s - lse) and ds = p (dp - D): for fp16 the products of p and of dS run in
-// bf16 as well (dS follows the loss and p the logits, neither stays within fp16's exponents): two bf16
-// terms each, and the fp16 factor as two bf16 terms.
+// Backward, with p = 2^(c s - lse) and ds = p (dp - D). P is at most 1.
 // ---------------------------------------------------------------------------
+template <class T>
+constexpr float kPScale = kIsHalf<T> ? 16384.f : 1.f;
+
 // Turned blocks of N fragments of 8 tokens (tokens become the k axis), as bf16 for the dS products
 template <class T, int N, int NR>
 struct Turned {
@@ -661,6 +685,7 @@ template <class T, int DP, int NF, bool FEW_ROWS>
 __global__ void __launch_bounds__(kXmThreads) xattn_bwd_few(const XAttn args, int) {
   const XAttn a = follow(args, false);
   constexpr int NR = DP / 8, NU = NR / 2;
+  constexpr float kP = kPScale<T>;
   using B16 = Mma<__nv_bfloat16>;
   extern __shared__ __align__(16) float xsm[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
@@ -804,12 +829,12 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_few(const XAttn args, in
     }
     Turned<T, 2, NR> x1t;
     x1t.make(x1);
-    uint32_t x2t[2][FEW_ROWS ? 1 : NR], x2l[2][FEW_ROWS ? 1 : NR];
+    uint32_t x2t[2][FEW_ROWS ? 1 : NR];
     if constexpr (!FEW_ROWS) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int c = 0; c < NR; ++c) bf16_terms<T>(movm(x2[h][c]), x2t[h][c], x2l[h][c]);
+        for (int c = 0; c < NR; ++c) x2t[h][c] = movm(x2[h][c]);
     }
     // keys that are not there leave zeros, also where a query or its gradient is not finite
     const bool gone[2] = {FEW_ROWS && xs[0] != 0.f, FEW_ROWS && xs[1] != 0.f};
@@ -854,34 +879,40 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_few(const XAttn args, in
       }
 #pragma unroll
       for (int x = 0; x < PAIR; ++x) {
-        split2<__nv_bfloat16>(p[i + x][0], p[i + x][1], hi[2 * x], lo[2 * x]);
-        split2<__nv_bfloat16>(p[i + x][2], p[i + x][3], hi[2 * x + 1], lo[2 * x + 1]);
+        p_terms<T>(p[i + x][0] * kP, p[i + x][1] * kP, hi[2 * x], lo[2 * x]);
+        p_terms<T>(p[i + x][2] * kP, p[i + x][3] * kP, hi[2 * x + 1], lo[2 * x + 1]);
         if constexpr (!FEW_ROWS) {
           const uint32_t h0 = movm(hi[2 * x]), h1 = movm(hi[2 * x + 1]), l0 = movm(lo[2 * x]), l1 = movm(lo[2 * x + 1]);
 #pragma unroll
           for (int u = 0; u < NU; ++u) {
             float(&c)[4] = acc2[i + x][u];
-            B16::run(c, x2t[0][2 * u], x2t[0][2 * u + 1], x2t[1][2 * u], x2t[1][2 * u + 1], h0, h1);
-            B16::run(c, x2t[0][2 * u], x2t[0][2 * u + 1], x2t[1][2 * u], x2t[1][2 * u + 1], l0, l1);
-            if constexpr (kIsHalf<T>)
-              B16::run(c, x2l[0][2 * u], x2l[0][2 * u + 1], x2l[1][2 * u], x2l[1][2 * u + 1], h0, h1);
+            if constexpr (kIsHalf<T>) {
+              float rest[4] = {0.f, 0.f, 0.f, 0.f};
+              Mma<T>::run(rest, x2t[0][2 * u], x2t[0][2 * u + 1], x2t[1][2 * u], x2t[1][2 * u + 1], l0, l1);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) c[e] = fmaf(rest[e], 1.f / 2048.f, c[e]);
+            } else {
+              Mma<T>::run(c, x2t[0][2 * u], x2t[0][2 * u + 1], x2t[1][2 * u], x2t[1][2 * u + 1], l0, l1);
+            }
+            Mma<T>::run(c, x2t[0][2 * u], x2t[0][2 * u + 1], x2t[1][2 * u], x2t[1][2 * u + 1], h0, h1);
           }
         }
       }
       if constexpr (FEW_ROWS) {
 #pragma unroll
         for (int c = 0; c < NR; ++c) {
-          uint32_t yh[2], yl[2];               // terms made here: kept, they would take the registers that are left
-#pragma unroll
-          for (int x = 0; x < PAIR; ++x) bf16_terms<T>(y2t[i + x][c], yh[x], yl[x]);
+          float rest[4] = {0.f, 0.f, 0.f, 0.f};
+          float(&low)[4] = kIsHalf<T> ? rest : e2[c];
           if constexpr (PAIR == 2) {
-            B16::run(e2[c], hi[0], hi[1], hi[2], hi[3], yh[0], yh[1]);
-            B16::run(e2[c], lo[0], lo[1], lo[2], lo[3], yh[0], yh[1]);
-            if constexpr (kIsHalf<T>) B16::run(e2[c], hi[0], hi[1], hi[2], hi[3], yl[0], yl[1]);
+            Mma<T>::run(low, lo[0], lo[1], lo[2], lo[3], y2t[i][c], y2t[i + 1][c]);
+            Mma<T>::run(e2[c], hi[0], hi[1], hi[2], hi[3], y2t[i][c], y2t[i + 1][c]);
           } else {
-            B16::run8(e2[c], hi[0], hi[1], yh[0]);
-            B16::run8(e2[c], lo[0], lo[1], yh[0]);
-            if constexpr (kIsHalf<T>) B16::run8(e2[c], hi[0], hi[1], yl[0]);
+            Mma<T>::run8(low, lo[0], lo[1], y2t[0][c]);
+            Mma<T>::run8(e2[c], hi[0], hi[1], y2t[0][c]);
+          }
+          if constexpr (kIsHalf<T>) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) e2[c][e] = fmaf(rest[e], 1.f / 2048.f, e2[c][e]);
           }
         }
       }
@@ -898,7 +929,7 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_few(const XAttn args, in
           const int64_t to = ((static_cast<int64_t>(b) * a.Tk + i) * a.kv_heads + n) * a.d;
           store_frag<T, DP>(static_cast<T*>(a.dk) + to, t, a.d, y);
 #pragma unroll
-          for (int c = 0; c < NR; ++c) y[c] = gone[h] ? 0u : Mma<T>::pack(e2[c][2 * h], e2[c][2 * h + 1]);
+          for (int c = 0; c < NR; ++c) y[c] = gone[h] ? 0u : Mma<T>::pack(e2[c][2 * h] * (1.f / kP), e2[c][2 * h + 1] * (1.f / kP));
           store_frag<T, DP>(static_cast<T*>(a.dv) + to, t, a.d, y);
         }
       } else if (a.dq != nullptr) {
@@ -942,7 +973,7 @@ __global__ void __launch_bounds__(kXmThreads) xattn_bwd_few(const XAttn args, in
     T* to = static_cast<T*>(FEW_ROWS ? a.dq : second ? a.dv : a.dk);
     if (f < (FEW_ROWS ? rows : a.Tk) && ch < a.d && to != nullptr) {
       const int64_t at = FEW_ROWS ? row_dense(a, b, n, f) : ((static_cast<int64_t>(b) * a.Tk + f) * a.kv_heads + n) * a.d;
-      store1(to + at + ch, second ? x : x * a.scale);
+      store1(to + at + ch, x * (second ? 1.f / kP : a.scale));
     }
   }
   if (cl > 1) cluster_sync_all();

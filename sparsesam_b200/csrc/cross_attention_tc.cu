@@ -8,9 +8,12 @@
 //   sums += P Y2, dS Y1                 tcgen05.mma with the first operand in TMEM; the same shared-memory tile now
 //                                       MN-major (its rows are the k axis)
 // P and dS enter as two half terms: of every 16 fp32 columns, the first 8 take the values, the others the remainders.
-// These products run in bf16 for fp16 inputs too (cross_attention_mma.cuh says why): the other side's tile becomes two
+// These products run in bf16 for fp16 inputs too (fp16 ends at 2^-24, and small weights count where the large ones meet
+// zeros; the sums in TMEM have no room for the scheme of cross_attention_mma.cuh): the other side's tile becomes two
 // bf16 tiles once the scores are there, its values in place and its remainders over a tile that is free by then (V's over
-// K, K's over V) or, in the keys' kernel, which needs both its tiles, behind the ring.
+// K, K's over V) or, in the keys' kernel, which needs both its tiles, behind the ring. Products with P take all four
+// pairs of terms: two terms of P are within 2^-17 of it, and the pair of the remainders is up to 2^-16 of a product.
+// Those with dS leave that pair out, next to the roundings of dP - D.
 // The chain load -> mma -> softmax -> mma of a block is serial; 4 (forward: 128 TMEM columns) or 2 (backward: 256)
 // blocks per SM run each other's gaps. Tiles come by cp.async rather than TMA: rows of masked keys and channels past
 // d are zero-filled on the way, and any row stride will do. Where tiles leave the device empty, the other side is
@@ -60,8 +63,8 @@ __device__ __forceinline__ void tc_scores(uint32_t d_tmem, uint32_t a, uint32_t 
                 make_smem_desc(b + k / 4 * kTcHalf + k % 4 * 32, 16, 1024, kSw128), tc_idesc<T>(0), k > 0);
 }
 // D[128 x channels] (+)= P[128 x 64 entries] B[64 entries x channels] in bf16, P in TMEM as [8 values | 8 remainders] four
-// times; TERMS: B's remainders are at b_lo, and their product with P's values is added
-template <int NP, bool TERMS>
+// times; TERMS: B's remainders are at b_lo, and their product with P's values (1), and remainders too (2), is added
+template <int NP, int TERMS>
 __device__ __forceinline__ void tc_sums(uint32_t d_tmem, uint32_t p_tmem, uint32_t b, uint32_t b_lo, bool accumulate) {
 #pragma unroll
   for (int k = 0; k < 4; ++k)
@@ -70,9 +73,11 @@ __device__ __forceinline__ void tc_sums(uint32_t d_tmem, uint32_t p_tmem, uint32
       const uint64_t desc = make_smem_desc(b + p * kTcHalf + k * 2048, 16, 1024, kSw128);
       umma_f16_ts(d_tmem + 64 * p, p_tmem + k * 16, desc, tc_idesc<__nv_bfloat16>(1), accumulate || k > 0);
       umma_f16_ts(d_tmem + 64 * p, p_tmem + k * 16 + 8, desc, tc_idesc<__nv_bfloat16>(1), 1u);
-      if constexpr (TERMS)
-        umma_f16_ts(d_tmem + 64 * p, p_tmem + k * 16, make_smem_desc(b_lo + p * kTcHalf + k * 2048, 16, 1024, kSw128),
-                    tc_idesc<__nv_bfloat16>(1), 1u);
+      if constexpr (TERMS > 0) {
+        const uint64_t lo = make_smem_desc(b_lo + p * kTcHalf + k * 2048, 16, 1024, kSw128);
+        umma_f16_ts(d_tmem + 64 * p, p_tmem + k * 16, lo, tc_idesc<__nv_bfloat16>(1), 1u);
+        if constexpr (TERMS > 1) umma_f16_ts(d_tmem + 64 * p, p_tmem + k * 16 + 8, lo, tc_idesc<__nv_bfloat16>(1), 1u);
+      }
     }
 }
 
@@ -319,7 +324,7 @@ __global__ void __launch_bounds__(kTcThreads, 4 / NP) xattn_tc_fwd_kernel(const 
     if (!ok) break;
     if (tid == 0) {
       tc_fence_after();
-      tc_sums<NP, kTerms>(B.tmem + tO, B.tmem + tS, y + kHalfStage, y, it > 0);
+      tc_sums<NP, kTerms ? 2 : 0>(B.tmem + tO, B.tmem + tS, y + kHalfStage, y, it > 0);
       umma_commit(&bars[1]);
     }
   }
@@ -543,8 +548,8 @@ __global__ void __launch_bounds__(kTcBwdThreads, 2 / NP) xattn_tc_bwd_kernel(con
     if (!ok) break;
     if (tid == 0) {
       tc_fence_after();
-      tc_sums<NP, kTerms>(B.tmem + tA1, B.tmem + tD, y, y_lo, it > 0);
-      if constexpr (!OWN_ROWS) tc_sums<NP, kTerms>(B.tmem + tA2, B.tmem + tS, y2, y2_lo, it > 0);
+      tc_sums<NP, kTerms ? 1 : 0>(B.tmem + tA1, B.tmem + tD, y, y_lo, it > 0);
+      if constexpr (!OWN_ROWS) tc_sums<NP, kTerms ? 2 : 0>(B.tmem + tA2, B.tmem + tS, y2, y2_lo, it > 0);
       umma_commit(&bars[1]);
     }
   }

@@ -1,13 +1,14 @@
 """Calls of the decoder's operators that random inputs do not make: weights far below the largest one, values that are
 not finite beside ones that are, logits at the end of fp32. Bounds as derived in test_gpu_cross_attention.py and
 test_gpu_norms.py; where something else is allowed, the test says why."""
+import ctypes
 import math
 
 import pytest
 import torch
 from test_gpu_cross_attention import DTYPES, NOISE, check, make, reference, run, there
 
-from sparsesam_b200 import ops
+from sparsesam_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -160,3 +161,31 @@ def test_logits_at_the_end_of_fp32(cuda_device, shape, dtype):
     mean = v.double().mean(1, keepdim=True).repeat_interleave(shape[3] // shape[4], 2).expand(out.shape)
     size = v.double().abs().mean(1, keepdim=True).repeat_interleave(shape[3] // shape[4], 2).expand(out.shape)
     close(out, (mean, size), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("shape", FORWARD, ids=ids)
+def test_results_before_they_are_rounded(cuda_device, shape, dtype):
+    """out_f32 and lse of the C entry: what the terms of P and V leave out shows here, without the result's rounding. One
+    key has a weight just above a half and a value just above one, of which a bf16 term leaves most, the others are 0."""
+    B, Tq, Tk, H, Hk, D = shape
+    q, k, v, _ = make(cuda_device, *shape, dtype, seed=29)
+    g = torch.Generator().manual_seed(30)
+    q.zero_(), k.zero_()
+    q[..., 0] = (torch.rand(B, Tq, H, generator=g) / 32 + math.log(Tk - 1)).to(q)
+    k[:, Tk // 3, :, 0] = 1.0
+    v.zero_()
+    v[:, Tk // 3] = (1 + torch.rand(B, Hk, D, generator=g) / 128).to(v)
+    out, out32 = torch.empty_like(q), torch.empty(B, Tq, H, D, device=cuda_device)
+    lse = torch.empty(B, H, Tq, device=cuda_device)
+    strides = (ctypes.c_int64 * 12)(*(x for t in (q, k, v, out) for x in t.stride()[:3]))
+    _lib.call("ssam_cross_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, B, Tq, Tk, H, Hk, D,
+              {"fp16": 0, "bf16": 1}[dtype], 1.0, None, None, out.data_ptr(), out32.data_ptr(), lse.data_ptr(),
+              torch.cuda.current_stream().cuda_stream)
+    u = torch.finfo(q.dtype).eps / 2
+    r, size = reference(q, k, v, scale=1.0)[0]
+    assert torch.all((out32.double() - r).abs() <= (NOISE + 4 * u * u) * size)
+    assert torch.equal(out, out32.to(out.dtype))
+    s = torch.einsum("bqhd,bkhd->bhqk", q.double(), k.double().repeat_interleave(H // Hk, 2))
+    want = torch.logsumexp(s, -1) / math.log(2.0)
+    assert torch.all((lse.double() - want).abs() <= NOISE + 2.0 ** -22 * want.abs())
