@@ -4,10 +4,12 @@ The library is a plain C-ABI shared object (no torch headers), linked from the
 translation units UNITS, which are compiled at the same time. Beside it the Python
 extension module _torch_ops (csrc/torch_ops.cpp, torch headers, no device code; linked to
 the library, which it finds beside itself) gives the decoder's operators their torch
-form. Both are rebuilt when any csrc/ or include/ file is newer than they are.
+form. Both are rebuilt when any csrc/ or include/ file is newer than they are. Where
+torch is not installed, the library is built alone.
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -65,10 +67,15 @@ def _torch_ops_commands(obj: str, lib: str, out: str) -> tuple[list[str], list[s
              "-L", os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"])
 
 
+def _with_torch() -> bool:
+    return importlib.util.find_spec("torch") is not None
+
+
 def needs_build() -> bool:
-    if not (os.path.exists(LIB_PATH) and os.path.exists(TORCH_OPS_PATH)):
+    targets = [LIB_PATH, TORCH_OPS_PATH] if _with_torch() else [LIB_PATH]
+    if not all(os.path.exists(t) for t in targets):
         return True
-    t = min(os.path.getmtime(LIB_PATH), os.path.getmtime(TORCH_OPS_PATH))
+    t = min(os.path.getmtime(t) for t in targets)
     return any(os.path.getmtime(s) > t for s in _sources())
 
 
@@ -90,14 +97,18 @@ def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | N
         objects = [os.path.join(work, unit + ".o") for unit in UNITS]
         units = [[_nvcc(), *NVCC_FLAGS, *(extra_flags or []), "-I", INCLUDE, "-c", "-o", obj, os.path.join(CSRC, unit)]
                  for unit, obj in zip(UNITS, objects)]
-        compile_ops, link_ops = _torch_ops_commands(os.path.join(work, "torch_ops.o"), tmp, tmp_ops)
-        units.append(compile_ops)
+        link_ops = None
+        if _with_torch():
+            compile_ops, link_ops = _torch_ops_commands(os.path.join(work, "torch_ops.o"), tmp, tmp_ops)
+            units.append(compile_ops)
         with ThreadPoolExecutor(len(units)) as pool:
             list(pool.map(run, units))
         run([_nvcc(), *NVCC_FLAGS, "-shared", "-Xlinker", f"-soname={LIB_NAME}", "-o", tmp, *objects])
-        run(link_ops)
+        if link_ops is not None:
+            run(link_ops)
     os.replace(tmp, LIB_PATH)
-    os.replace(tmp_ops, TORCH_OPS_PATH)
+    if link_ops is not None:
+        os.replace(tmp_ops, TORCH_OPS_PATH)
     return LIB_PATH
 
 
