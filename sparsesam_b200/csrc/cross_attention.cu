@@ -298,8 +298,8 @@ __device__ __forceinline__ void xattn_fwd_join(const XAttn& a, const XPlace& x, 
 }
 
 // NR rows to a thread, RB apart: K and V come out of shared memory once for all of them, which is what the kernel waits
-// for (1024 x 1024, 16 x 8 heads of 16: 400 us with one row, 340 with two, of 64: 2040 and 1400; 4096 queries on 8
-// keys, 64 x 8 heads of 16: 128 and 106, at 2.5 TB/s). NR > 1: one slice, no cluster.
+// for (1024 x 1024, 16 x 8 heads of 16: 400 us with one row, 312 with two, of 64: 2040 and 1345; 4096 queries on 8
+// keys, 64 x 8 heads of 16: 128 and 103, at 2.6 TB/s). NR > 1: one slice, no cluster.
 // (The bounds are the blocks that fit anyway: 168 registers for NR 2, DT 32. Left to itself the compiler once took 196,
 // and 4096 x 30 of 32 channels 113 us instead of 97.)
 template <int DT, int TPR, int NR>
@@ -309,8 +309,7 @@ __global__ void __launch_bounds__(kXThreads, DT == 16 ? (NR == 1 ? 7 : 4) : (NR 
   extern __shared__ __align__(16) float xsm[];
   __shared__ float bias[2][kXTile<DP>];
   const XPlace x(a, RB, TPR, NR);
-  const int part = x.part, lr = x.lr, slice = x.slice, KS = x.KS, b = x.b, n = x.n, cl = x.cl, rank = x.rank, rows = x.rows,
-            r0 = x.r0;
+  const int part = x.part, lr = x.lr, slice = x.slice, KS = x.KS, b = x.b, n = x.n, cl = x.cl, rows = x.rows;
   float2 q[NR][DT / 2], o[NR][DT / 2];
   fetch_own<DP>(xsm, NR * RB, a.d, [&](int i) { return x.row_of(a, static_cast<const float*>(a.q), a.qs, i); });
   asm volatile("cp.async.wait_all;" ::: "memory");

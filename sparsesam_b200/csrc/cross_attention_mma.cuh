@@ -147,9 +147,10 @@ __device__ __forceinline__ void store_frag(T* row, int t, int d, const uint32_t 
 
 constexpr int kXmWarps = 8;
 constexpr int kXmThreads = 32 * kXmWarps;
-// Blocks per SM that the forward kernels' registers are held down to: N tiles of 8 entries of the short side in registers
-// (S = 2: keys, half the accumulators of rows), DP channels. The fp16 instances would each lose a block to their
-// remainders otherwise (60 keys of 64 images: 145 us, 102 with the bound).
+// Blocks per SM that the forward kernels' registers are held to, and may use up to: N tiles of 8 entries of the short side
+// in registers (S = 2: keys, half the accumulators of rows), DP channels. These are the blocks that fit without a word
+// to the compiler, which then leaves registers unused (24 x 4096 of 64 channels, 64 images: 74 us, 70 so; 4096 x 13 of 16
+// 39.4 and 37.9) or, a few past the border, a block (64 x 4096 of 16, fp16).
 template <int DP, int N, int S>
 constexpr int kXmBlocks = DP * N <= 16 * S ? 2 + S : DP * N <= 32 * S && S == 2 && DP <= 32 ? 3 : DP * N <= 64 * S && DP <= 64 ? 2 : 1;
 
@@ -444,8 +445,7 @@ __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NQ, 1>) xattn_f
 // ---------------------------------------------------------------------------
 // Forward, many queries on few keys (at most 8 NK): a warp keeps the K and turned V
 // fragments of one (image, query head) and walks its share of the queries 16 at a time, the
-// next rows in flight. Bound by the bytes of q and out (64 images, 4096 queries on 8 keys: 30 us,
-// 4.5 TB/s); neighbouring warps hold neighbouring heads, so a block touches whole rows. HP = 2 as above.
+// next rows in flight. 64 images, 4096 queries on 8 keys: 32 us, 4.2 TB/s, issuing in 69 % of the cycles; neighbouring warps hold neighbouring heads, so a block touches whole rows. HP = 2 as above.
 // ---------------------------------------------------------------------------
 template <class T, int DP, int NK, int HP>
 __global__ void __launch_bounds__(kXmThreads, kXmBlocks<DP, HP * NK, 2>) xattn_fwd_few_keys(const XAttn args, int chunks) {
@@ -678,7 +678,7 @@ __device__ __forceinline__ float row_delta(const float* o32, const uint32_t (&x)
 // One short side: its 8 NF entries ("few") are all of it, the columns of every tile, and stay in
 // registers with their gradient sums; warps and cluster share the long side, 16 entries at a time,
 // whose gradients are complete at once and leave at once. One pass over all inputs: 64 images, 8 queries on
-// 4096 keys, with the forward pass 106 us; 2.5 TB/s, one block of 255 registers per thread and SM.
+// 4096 keys, with the forward pass 108 us; 2.5 TB/s.
 //   few = query rows (FEW_ROWS): x = k, v;  y = q, dout.  dk = ds y1, dv = p y2 leave;  dq^T += k^T ds stays
 //   few = keys:                  x = q, dout;  y = k, v.  dq = ds y1 leaves;  dk^T += q^T ds, dv^T += dout^T p stay
 template <class T, int DP, int NF, bool FEW_ROWS>

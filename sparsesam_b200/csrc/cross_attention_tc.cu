@@ -20,9 +20,9 @@
 // split over a cluster and joined through distributed shared memory in rank order.
 // Every wait is bounded; a block whose wait ran out raises SSAM_ERR_TIMEOUT and leaves.
 //
-// Bound by that chain: 1369 x 4096, 2 x 4 heads of 64, bf16, takes 40 us forward (290 TFLOP/s) and 148 with the
-// gradients, at 21 to 26 % of the tensor pipe, 18 to 29 % of the exponentials' and 38 to 47 % of the issue slots.
-// mma.sync on registers took 60 and 339. Two threads per row in the forward kernel (64 registers) were slower: 161.
+// Bound by that chain: 1369 x 4096, 2 x 4 heads of 64, bf16, takes 41 us forward (280 TFLOP/s) and 149 with the
+// gradients (fp16, with its further products, 48 and 180), at 20 to 28 % of the tensor pipe, 18 to 29 % of the
+// exponentials' and 41 to 47 % of the issue slots. mma.sync on registers took 60 and 339. Two threads per row in the forward kernel (64 registers) were slower: 161.
 #include <cuda_fp16.h>
 
 #include "common.cuh"

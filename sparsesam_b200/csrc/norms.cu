@@ -1000,8 +1000,8 @@ int groupnorm_act_bwd(const void* x, const void* dout, int N, int64_t HW, int C,
 // ---------------------------------------------------------------------------
 // Backward of ssam_layernorm_gelu_half: C / 8 threads per row, as the forward;
 // the row's moments are recomputed from x (it is read anyway). Each block sums its
-// rows' parameter gradients into one partial. 262144 x 64 with GELU, fp16: 50 us with the forward pass
-// (2.7 TB/s); the arithmetic of GELU's slope sets the pace, 4096 x 256 without it 8.0 us, three launches.
+// rows' parameter gradients into one partial. 262144 x 64 with GELU, fp16: 51 us with the forward pass
+// (2.6 TB/s), issuing in 58 % of the cycles at 30 % of the warps; 4096 x 256 without it 8.1 us, three launches.
 // ---------------------------------------------------------------------------
 constexpr int kLnRing = 3;
 using LnRing = Ring<kLnRing, 2, 256>;      // 24 KB a block
