@@ -292,8 +292,7 @@ class DecoderAttention(nn.Module):
                 or ops.followed(qh, kh, vh)):
             return False
         b, n, h, c = qh.shape
-        return (b == kh.shape[0] and kh.shape == vh.shape and b <= ops.CROSS_ATTN_MAX_BATCH
-                and ops.cross_attn_supported(h, h, c, qh.dtype)
+        return (b == kh.shape[0] and kh.shape == vh.shape and ops.cross_attn_supported(h, h, c, qh.dtype)
                 and (masked or _kernel_not_slower(b, h, n, kh.shape[1], c, qh.dtype)))
 
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -304,7 +303,15 @@ class DecoderAttention(nn.Module):
         qh, kh, vh = self._split(self.q_proj(q)), self._split(self.k_proj(k)), self._split(self.v_proj(v))
         if not torch.jit.is_scripting():
             if self._by_kernel(qh, kh, vh, key_lens is not None or key_mask is not None):
-                return self.out_proj(ops.cross_attn(qh, kh, vh, key_lens=key_lens, key_mask=key_mask).flatten(2))
+                most = ops.CROSS_ATTN_MAX_BATCH              # more prompts (which torch refuses in half) in several calls
+                if qh.shape[0] <= most:
+                    o = ops.cross_attn(qh, kh, vh, key_lens=key_lens, key_mask=key_mask)
+                else:
+                    o = torch.cat([ops.cross_attn(qh[i : i + most], kh[i : i + most], vh[i : i + most],
+                                                  key_lens=None if key_lens is None else key_lens[i : i + most],
+                                                  key_mask=None if key_mask is None else key_mask[i : i + most])
+                                   for i in range(0, qh.shape[0], most)])
+                return self.out_proj(o.flatten(2))
         mask = key_mask
         if key_lens is not None:
             there = torch.arange(kh.shape[1], device=kh.device) < key_lens.view(-1, 1)

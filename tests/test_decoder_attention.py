@@ -82,3 +82,30 @@ def test_sizes_go_where_they_are_faster(cuda_device, tq, tk, dim, kernel, dtype)
         n0 = _lib.launch_count
         near(mod(q, k, k, key_lens=lens), plain, dtype)
         assert _lib.launch_count > n0
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["plain", "lens", "mask"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_more_prompts_than_one_call_takes(cuda_device, dtype, kind):
+    """65,537 prompts, which torch's attention refuses in half precision: the rows and gradients of two calls."""
+    torch.manual_seed(5)
+    mod = hq.DecoderAttention(16, 2).to(cuda_device, dtype)
+    n, most = 65537, 40000
+    x, y = torch.randn(n, 2, 16, device=cuda_device).to(dtype), torch.randn(n, 5, 16, device=cuda_device).to(dtype)
+    kw = {}
+    if kind == "lens":
+        kw["key_lens"] = torch.randint(0, 6, (n,), device=cuda_device, dtype=torch.int32)
+    if kind == "mask":
+        kw["key_mask"] = torch.rand(n, 5, device=cuda_device) < 0.5
+
+    def run(at):
+        a, b = x[at].clone().requires_grad_(True), y[at].clone().requires_grad_(True)
+        out = mod(a, b, b, **{k: t[at] for k, t in kw.items()})
+        return [out.detach(), *torch.autograd.grad(out.float().square().sum(), (a, b))]
+
+    whole = run(slice(0, n))
+    parts = [torch.cat(t) for t in zip(run(slice(0, most)), run(slice(most, n)))]
+    # the attention's rows are the same; the projections' matrix products may be cut differently
+    for w, p in zip(whole, parts):
+        assert (w.double() - p.double()).abs().max() <= 8 * torch.finfo(dtype).eps * p.abs().max()
